@@ -60,7 +60,11 @@ EXPORTS = ("g4s_version", "g4s_params_set_defaults", "g4s_max_top_k", "g4s_creat
            "g4s_lmhead_sample_q4_0", "g4s_store_open", "g4s_store_close", "g4s_store_last_error",
            "g4s_store_tensor_count", "g4s_store_tensor_info", "g4s_store_find_tensor",
            "g4s_store_raw_pointer", "g4s_store_verify", "g4s_q4_0_device_bytes",
-           "g4s_store_upload_q4_0", "g4s_q4_0_repack", "g4s_embed_q4_0", "g4s_generate")
+           "g4s_store_upload_q4_0", "g4s_q4_0_repack", "g4s_embed_q4_0", "g4s_generate",
+           # gemma4_beam.h, bound in beam.py
+           "g4s_beam_create", "g4s_beam_destroy", "g4s_beam_last_error", "g4s_beam_select",
+           "g4s_beam_reorder", "g4s_pages_create", "g4s_pages_destroy", "g4s_pages_last_error",
+           "g4s_pages_advance", "g4s_pages_compact", "g4s_pages_copy", "g4s_beam_generate")
 
 FORWARD_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32),
                               ctypes.c_int32)

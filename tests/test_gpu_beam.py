@@ -1,0 +1,383 @@
+"""GPU tests of g4s_beam_select and g4s_beam_reorder against the plain forms
+of beam_oracle.py.
+
+Tolerances.  The kernel's lse is off by at most 2e-7 absolutely (the header's
+bound); a score is rounded once to binary32 (2^-24 of its magnitude).  numpy's
+binary64 sums are off by less than 1e-9 here.  Tokens and parents are equal
+wherever the oracle's neighbouring scores of different beams lie further apart
+than twice the lse bound, which the tests assert of their own inputs."""
+import numpy as np
+import pytest
+
+import beam_oracle as bo
+from gemma4_sampler import beam, hip, native
+
+pytestmark = pytest.mark.gpu
+F32 = np.float32
+LSE = 2e-7
+NONE = -np.inf
+
+
+def run_select(x, scores, beams, n, cap=30.0, stride=None, search=None, stream=None, lse=True,
+               inplace=False):
+    R, V = x.shape
+    batch = R // beams
+    esize = x.dtype.itemsize
+    per = 16 // esize
+    stride = (V + per - 1) // per * per if stride is None else stride
+    buf = np.zeros((R, stride), x.dtype)
+    buf[:, :V] = x
+    buf[:, V:] = 0x7F80 if x.dtype == np.uint16 else np.inf  # never read
+    own = search is None
+    if own:
+        search = beam.BeamSearch(V, batch, max(beams, (n + 1) // 2), cap, stream=stream)
+    d_x, d_s = hip.Buffer.from_array(buf), hip.Buffer.from_array(np.asarray(scores, F32))
+    d_p, d_t = (hip.Buffer.from_array(np.full(batch * n + 4, 77, np.int32)) for _ in range(2))
+    d_o = d_s if inplace else hip.Buffer.from_array(np.full(batch * n + 4, 77, F32))
+    d_l = hip.Buffer.from_array(np.full(R + 4, 77, F32)) if lse else None
+    search.select(d_x, batch, beams, d_s, n, d_p, d_t, d_o, d_lse=d_l,
+                  dtype=native.DTYPE_F32 if esize == 4 else native.DTYPE_BF16, row_stride=stride)
+    hip.synchronize()
+    p, t, o = d_p.download(np.int32), d_t.download(np.int32), d_o.download(F32)
+    assert (p[batch * n:] == 77).all() and (t[batch * n:] == 77).all()
+    if lse:
+        l = d_l.download(F32)
+        assert (l[R:] == 77).all()
+    if own:
+        search.close()
+    return (p[:batch * n].reshape(batch, n), t[:batch * n].reshape(batch, n),
+            o[:batch * n].reshape(batch, n), l[:R] if lse else None)
+
+
+def close(got, want):
+    same = got == want  # infinities
+    with np.errstate(invalid="ignore"):
+        return (same | (np.abs(got - want) <= LSE + np.abs(want) * 2.0 ** -24 * 1.01)).all()
+
+
+def check(x, scores, beams, n, cap=30.0, **kw):
+    p, t, s, lse = bo.select(x, scores, beams, n, cap)
+    gap = np.abs(np.diff(s, axis=1)) <= 2 * LSE
+    with np.errstate(invalid="ignore"):
+        gap &= (p[:, 1:] != p[:, :-1]) & np.isfinite(s[:, 1:]) & (np.diff(s, axis=1) != 0)
+    assert not gap.any(), "the input has scores too close to tell apart"
+    gp, gt, gs, gl = run_select(x, scores, beams, n, cap, **kw)
+    assert np.array_equal(gp, p) and np.array_equal(gt, t)
+    assert close(gs.astype(np.float64), s), np.nanmax(np.abs(gs - s))
+    if gl is not None:
+        assert close(gl.astype(np.float64), lse)
+
+
+def peaky(rng, R, V, dtype):
+    x = (rng.standard_normal((R, V)) * 3).astype(F32)
+    at = rng.integers(0, V, (R, min(16, V)))
+    np.put_along_axis(x, at, np.take_along_axis(x, at, 1) + rng.uniform(
+        6, 12, at.shape).astype(F32), 1)
+    return x if dtype == "f32" else bo.bf16(x)
+
+
+def running(rng, R):
+    return -rng.uniform(0, 3, R).cumsum().astype(F32) - F32(4)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("V, batch, beams, n", [
+    (2, 1, 1, 1), (3, 2, 2, 4), (63, 1, 4, 8), (257, 3, 5, 10), (8191, 2, 3, 6),
+    (8192, 1, 4, 8), (8193, 2, 4, 4), (16385, 1, 32, 64), (40009, 5, 2, 3),
+    (100003, 1, 8, 16), (262144, 1, 4, 8)])
+def test_select(dtype, V, batch, beams, n):
+    rng = np.random.default_rng(V + beams)
+    check(peaky(rng, batch * beams, V, dtype), running(rng, batch * beams), beams, n)
+
+
+@pytest.mark.parametrize("cap", [0.0, -1.0, 5.0, 50.0, 1000.0])
+def test_softcaps(cap):
+    rng = np.random.default_rng(5)
+    x = peaky(rng, 8, 20011, "f32") * F32(4)
+    check(x, running(rng, 8), 4, 8, cap=cap)
+    check(bo.bf16(x), running(rng, 8), 4, 8, cap=cap)
+
+
+def test_most_beams():
+    rng = np.random.default_rng(6)
+    check(peaky(rng, 128, 3001, "f32"), running(rng, 128), 64, 128)
+    check(peaky(rng, 64, 70001, "bf16"), running(rng, 64), 64, 128)
+
+
+def test_flat_rows_and_offsets():
+    """Rows whose mass lies in many tokens, far from 0 and from the cap."""
+    rng = np.random.default_rng(7)
+    for mid in (-25.0, 0.0, 18.0, 45.0):
+        x = (rng.standard_normal((4, 50021)) * 0.5 + mid).astype(F32)
+        check(x, running(rng, 4), 2, 4)
+        check(bo.bf16(x), running(rng, 4), 2, 4)
+
+
+def test_dead_beams_and_first_step():
+    rng = np.random.default_rng(8)
+    x = peaky(rng, 12, 9001, "f32")
+    s = np.full(12, NONE, F32)
+    s[[0, 4]] = 0  # the third sequence has no live beam
+    check(x, s, 4, 8)
+    s[5], s[6], s[7], s[8] = np.nan, -1e30, np.finfo(F32).min, -7.5
+    check(x, s, 4, 8)
+    x[s != s] = np.nan  # a dead row is not read
+    check(x, s, 4, 8)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fill", [NONE, "lowest", np.nan, -1e30])
+def test_masked_logits(dtype, fill):
+    rng = np.random.default_rng(9)
+    x = peaky(rng, 6, 12289, "f32")
+    if fill == "lowest":
+        fill = np.finfo(F32).min if dtype == "f32" else -3.38953139e38
+    x[0, rng.random(12289) < 0.7] = fill
+    x[1] = fill                    # nothing left
+    x[2] = fill
+    x[2, [5, 9000, 12288]] = [1, 2, 2]  # fewer than n, in two chunks
+    x[3, :8192] = fill             # a chunk without candidates
+    if dtype == "bf16":
+        finite = np.isfinite(x)
+        b = bo.bf16(np.where(finite, x, 0))
+        b[x == NONE], b[np.isnan(x)] = 0xFF80, 0x7FC1
+        if fill == -1e30:
+            assert bo.widen(b[1])[0] <= F32(-1e30)
+        x = b
+    check(x, running(rng, 6), 3, 6)
+    check(x, running(rng, 6), 1, 2)
+
+
+def test_fewer_candidates_than_asked():
+    rng = np.random.default_rng(10)
+    x = rng.standard_normal((4, 3)).astype(F32)
+    check(x, running(rng, 4), 2, 8)
+    x[:] = NONE
+    check(x, running(rng, 4), 2, 8)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_ties(dtype):
+    """Equal logits: the lowest tokens of the lowest beams, in masses too."""
+    rng = np.random.default_rng(11)
+    x = np.zeros((8, 30011), F32)       # everything equal
+    x[4:] = rng.integers(0, 3, (4, 30011))
+    x[7, 20000:20040] = 5
+    s = np.array([-1, -1, -1, -2, -3, -3.5, -4, -9], F32)
+    s[4:] += rng.uniform(0, .1, 4).astype(F32)
+    x[2, ::2] = -0.0                    # equal to +0
+    check(x if dtype == "f32" else bo.bf16(x), s, 4, 16)
+
+
+def test_equal_beams():
+    """Two beams with the same logits and score tie exactly: the lower first."""
+    rng = np.random.default_rng(12)
+    x = peaky(rng, 3, 50001, "f32")
+    x[2] = x[0]
+    check(x, np.array([-1.5, -1.75, -1.5], F32), 3, 12)
+
+
+def test_saturated_softcap():
+    """Distinct logits beyond the cap round to one score: the larger first."""
+    x = np.full((2, 5000), -1, F32)
+    x[0, 100:140] = 2000 + np.arange(40)[::-1] * F32(0.25)
+    x[0, 4000:4040] = 540 + np.arange(40) * F32(0.001)
+    x[1, 7] = 33
+    check(x, np.array([-2, -1], F32), 2, 100, cap=30.0)
+
+
+def test_infinite_logits():
+    rng = np.random.default_rng(13)
+    x = peaky(rng, 4, 20001, "f32")
+    x[0, [3, 15000]] = np.inf
+    x[2, 9000] = np.inf
+    x[3, :700] = np.inf  # more than a workgroup's list holds
+    for cap in (0.0, 30.0):
+        check(x, running(rng, 4), 4, 8, cap=cap)
+        check(x, running(rng, 4), 2, 8, cap=cap)
+
+
+def test_infinite_score():
+    rng = np.random.default_rng(14)
+    x = peaky(rng, 2, 5001, "f32")
+    check(x, np.array([-1, np.inf], F32), 2, 4)
+
+
+def test_stride_no_lse_and_scores_in_place():
+    rng = np.random.default_rng(15)
+    x = peaky(rng, 6, 10007, "bf16")
+    check(x, running(rng, 6), 3, 3, stride=16384, lse=False)
+    check(x, running(rng, 6), 3, 3, inplace=True)
+
+
+def test_calls_in_a_row_and_smaller_shapes():
+    """One handle, shapes that grow and shrink: nothing of a call is left over."""
+    rng = np.random.default_rng(16)
+    search = beam.BeamSearch(30001, 6, 8, 30.0)
+    for batch, beams, n, dtype in [(6, 8, 16, "f32"), (1, 1, 1, "bf16"), (2, 8, 16, "f32"),
+                                   (3, 5, 7, "bf16"), (6, 8, 8, "f32")]:
+        check(peaky(rng, batch * beams, 30001, dtype), running(rng, batch * beams), beams, n,
+              search=search)
+    search.close()
+
+
+def test_other_stream_and_another_handle():
+    rng = np.random.default_rng(17)
+    streams = [hip.Stream(nonblocking=True) for _ in range(2)]
+    for st in streams:
+        check(peaky(rng, 4, 9999, "f32"), running(rng, 4), 4, 8, stream=st)
+    for st in streams:
+        st.destroy()
+
+
+def test_select_refusals():
+    s = beam.BeamSearch(1000, 2, 4, 30.0)
+    d = hip.Buffer(8 * 1000 * 4)
+    o = hip.Buffer(4096)
+    good = dict(d_logits=d, batch=2, beams=4, d_scores=o, n_select=8, d_parents=o.offset(512),
+                d_tokens=o.offset(1024), d_out=o.offset(1536))
+    for change in [dict(batch=0), dict(batch=3), dict(beams=0), dict(beams=5), dict(n_select=0),
+                   dict(n_select=9), dict(dtype=2), dict(row_stride=999), dict(row_stride=1002),
+                   dict(row_stride=1 << 60), dict(d_logits=d.offset(4)), dict(d_logits=None),
+                   dict(d_scores=None), dict(d_parents=None), dict(d_tokens=None),
+                   dict(d_out=None), dict(d_out=o), dict(d_out=o.offset(28))]:
+        with pytest.raises(native.SamplerError) as e:
+            s.select(**dict(good, **change))
+        assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT, change
+    s.close()
+
+
+# ----------------------------------------------------------------- reorder
+
+
+def reordered(data, parents, beams, inplace):
+    out = data.copy()
+    for r, p in enumerate(parents):
+        b = r // beams
+        if p // beams == b and p >= 0:
+            out[:, r] = data[:, p]
+    return out
+
+
+@pytest.mark.parametrize("inplace", [True, False])
+@pytest.mark.parametrize("batch, beams, planes, row, stride, shift", [
+    (1, 1, 1, 16, 16, 0), (1, 4, 3, 4096, 4096, 0), (2, 3, 2, 5008, 5024, 0),
+    (1, 5, 2, 1000, 1004, 4), (3, 8, 1, 333, 350, 1), (1, 16, 2, 20000, 20000, 0),
+    (2, 17, 1, 4112, 4112, 0), (1, 32, 2, 1028, 1040, 0), (1, 64, 1, 7777, 7777, 3),
+    (5, 64, 2, 64, 80, 0)])
+def test_reorder(inplace, batch, beams, planes, row, stride, shift):
+    rng = np.random.default_rng(row + beams)
+    R = batch * beams
+    s = beam.BeamSearch(100, batch, beams, 30.0)
+    for kind in range(3):
+        if kind == 0:    # any parents, most of them more than once
+            par = np.repeat(np.arange(batch), beams) * beams + rng.integers(0, beams, R)
+        elif kind == 1:  # a permutation: every row is overwritten while another needs it
+            par = np.concatenate([b * beams + rng.permutation(beams) for b in range(batch)])
+        else:            # rows that stay: none, another sequence's, out of range
+            par = np.repeat(np.arange(batch), beams) * beams + rng.integers(0, beams, R)
+            par[::3] = rng.choice([-1, -5, R, R + 7, (1 << 31) - 1, -(1 << 31)], len(par[::3]))
+            if batch > 1:
+                par[1] = R - 1
+        data = rng.integers(0, 256, (planes, R, stride), dtype=np.uint8)
+        raw = np.zeros(shift + data.size + 64, np.uint8)
+        raw[shift:shift + data.size] = data.reshape(-1)
+        d = hip.Buffer.from_array(raw)
+        other = rng.integers(0, 256, raw.size, dtype=np.uint8)
+        e = d if inplace else hip.Buffer.from_array(other)
+        s.reorder(d.offset(shift), e.offset(shift), planes, R * stride, batch, beams, stride, row,
+                  hip.Buffer.from_array(par.astype(np.int32)))
+        hip.synchronize()
+        want = (raw if inplace else other).copy()
+        w = want[shift:shift + data.size].reshape(data.shape)
+        w[:, :, :row] = reordered(data, par, beams, inplace)[:, :, :row]
+        assert np.array_equal(e.download(np.uint8), want), kind
+        if not inplace:
+            assert np.array_equal(d.download(np.uint8), raw)
+    s.close()
+
+
+def test_reorder_planes_inside_rows():
+    """[row][plane][bytes]: the planes' stride is below the rows'."""
+    rng = np.random.default_rng(3)
+    data = rng.integers(0, 256, (8, 3, 48), dtype=np.uint8)
+    par = np.array([1, 0, 3, 3, 7, 6, 5, 4], np.int32)
+    s = beam.BeamSearch(100, 2, 4, 30.0)
+    d = hip.Buffer.from_array(data)
+    s.reorder(d, d, 3, 48, 2, 4, 144, 48, hip.Buffer.from_array(par))
+    hip.synchronize()
+    assert np.array_equal(d.download(np.uint8).reshape(data.shape), data[par])
+    s.close()
+
+
+def test_reorder_refusals():
+    s = beam.BeamSearch(100, 2, 4, 30.0)
+    d, e = hip.Buffer(1 << 16), hip.Buffer(4096)
+    good = dict(d_src=d, d_dst=d, planes=2, plane_stride=8192, batch=2, beams=4, row_stride=1024,
+                row_bytes=1024, d_parents=e)
+    s.reorder(**dict(good, row_bytes=0))
+    for change in [dict(batch=3), dict(beams=5), dict(planes=0), dict(planes=-1),
+                   dict(row_bytes=-1), dict(row_bytes=1025), dict(row_stride=-1024),
+                   dict(plane_stride=8191), dict(plane_stride=512), dict(planes=1 << 40),
+                   dict(d_src=None), dict(d_dst=None), dict(d_parents=None),
+                   dict(d_dst=d.offset(16384 - 16)), dict(d_dst=d.offset(16))]:
+        with pytest.raises(native.SamplerError) as err:
+            s.reorder(**dict(good, **change))
+        assert err.value.code == native.G4S_ERR_INVALID_ARGUMENT, change
+    s.close()
+
+
+def test_captured_step():
+    """Selection and reordering in one captured graph, replayed on new logits
+    with eager calls between."""
+    rng = np.random.default_rng(18)
+    st = hip.Stream(nonblocking=True)
+    V, W = 20000, 4
+    s = beam.BeamSearch(V, 2, W, 30.0, stream=st)
+    R = 2 * W
+    d_x = hip.Buffer(R * V * 4)
+    d_s, d_p, d_t = hip.Buffer(4 * R), hip.Buffer(4 * R), hip.Buffer(4 * R)
+    d_state, d_l = hip.Buffer(R * 4096), hip.Buffer(4 * R)
+    d_first = hip.Buffer(4 * R)
+    graph, run = _capture(st, lambda: (
+        s.select(d_x, 2, W, d_first, W, d_p, d_t, d_s, d_lse=d_l),
+        s.reorder(d_state, d_state, 1, 0, 2, W, 4096, 4096, d_p)))
+    for _ in range(4):
+        x, sc = peaky(rng, R, V, "f32"), running(rng, R)
+        data = rng.integers(0, 256, (R, 4096), dtype=np.uint8)
+        st.synchronize()
+        d_x.upload(x)
+        d_first.upload(sc)
+        d_state.upload(data)
+        run()
+        st.synchronize()
+        p, t, o, _ = bo.select(x, sc, W, W, 30.0)
+        assert np.array_equal(d_p.download(np.int32).reshape(2, W), p)
+        assert np.array_equal(d_t.download(np.int32).reshape(2, W), t)
+        assert close(d_s.download(F32).reshape(2, W).astype(np.float64), o)
+        assert np.array_equal(d_state.download(np.uint8).reshape(data.shape),
+                              data[p.reshape(-1)])
+        check(peaky(rng, 3, V, "f32"), running(rng, 3), 3, 3, search=s)
+    graph()
+    s.close()
+    st.destroy()
+
+
+def _capture(st, record):
+    """(destroy, launch) of a graph of the launches that record() makes on st."""
+    import ctypes
+    L = hip.lib()
+    g, x = ctypes.c_void_p(), ctypes.c_void_p()
+    hip.check(L.hipStreamBeginCapture(st.handle, ctypes.c_int(1)), "hipStreamBeginCapture")
+    try:
+        record()
+    finally:
+        rc = L.hipStreamEndCapture(st.handle, ctypes.byref(g))
+    hip.check(rc, "hipStreamEndCapture")
+    hip.check(L.hipGraphInstantiate(ctypes.byref(x), g, None, None, ctypes.c_size_t(0)),
+              "hipGraphInstantiate")
+
+    def destroy():
+        L.hipGraphExecDestroy(x)
+        L.hipGraphDestroy(g)
+    return destroy, lambda: hip.check(L.hipGraphLaunch(x, st.handle), "hipGraphLaunch")
