@@ -33,16 +33,84 @@ __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t token)
 __device__ __forceinline__ uint32_t entry_key(uint64_t e) { return (uint32_t)(e >> 32); }
 __device__ __forceinline__ uint32_t entry_token(uint64_t e) { return ~(uint32_t)e; }
 
-__device__ __forceinline__ double softcap64(float x, double cap)
+using cr::exp_fast_d;
+using cr::tanh_fast_d;
+
+constexpr double kLog2e = 0x1.71547652b82fep+0;
+
+__device__ __forceinline__ uint64_t d2u(double x) { return __builtin_bit_cast(uint64_t, x); }
+__device__ __forceinline__ double u2d(uint64_t u) { return __builtin_bit_cast(double, u); }
+
+template <int MODE>
+__device__ __forceinline__ double softcap64(float x, const BeamSoftcap& c)
 {
-    return cap > 0.0 ? cap * tanh((double)x / cap) : (double)x;
+    return MODE == kCapNone ? (double)x : (double)c.cap * tanh_fast_d((double)x / (double)c.cap);
 }
 
 /* exp(y - top) for y <= top; an infinite top (no softcap, x = +inf) counts 1
  * for itself and leaves nothing for the rest. */
 __device__ __forceinline__ double term64(double y, double top)
 {
-    return y == top ? 1.0 : exp(y - top);
+    const double d = y - top;
+    return y == top ? 1.0 : (d < -1000.0 ? 0.0 : exp_fast_d(d));
+}
+
+/* v(x) / x of BeamSoftcap, where |x| <= limit. */
+__device__ __forceinline__ double near_factor(double x, const BeamSoftcap& c)
+{
+    const double s = x * x;
+    double h = c.q[9];
+#pragma unroll
+    for (int i = 8; i >= 0; --i) h = __builtin_fma(h, s, c.q[i]);
+    return h;
+}
+template <int MODE>
+__device__ __forceinline__ double value64(float x, const BeamSoftcap& c)
+{
+    if (MODE == kCapPoly && fabsf(x) <= c.limit) return (double)x * near_factor((double)x, c);
+    return softcap64<MODE>(x, c) * kLog2e;
+}
+
+/* 2^t to binary32's accuracy, for t in [-2^20, 1]: what binary32 would round off
+ * t (a millionth where t is near -20) is kept by splitting t first. */
+__device__ __forceinline__ float pow2_of(double t)
+{
+    constexpr double kRound = 0x1.8p52; /* the sum's low word is the rounded integer */
+    const double m = t + kRound;
+    const float f = (float)(t - (m - kRound));
+    return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), (int)(uint32_t)d2u(m));
+}
+
+/* The term of one logit in its chunk's sum, 2^(v(x) - ref), ref = v(top). */
+template <int MODE, bool NEAR>
+__device__ __forceinline__ float term_of(float x, float top, double ref, const BeamSoftcap& c)
+{
+    if constexpr (MODE == kCapNone)
+        return x == top ? 1.0f : pow2_of(fmax(((double)x - (double)top) * kLog2e, -1000.0));
+    else if constexpr (MODE == kCapPoly && NEAR)
+        return pow2_of(__builtin_fma((double)x, near_factor((double)x, c), -ref));
+    else
+        return pow2_of(fmax(value64<MODE>(x, c) - ref, -1000.0));
+}
+
+/* Sum over the 64 lanes, in every lane (all lanes active). */
+__device__ __forceinline__ double wave_sum_f64(double v)
+{
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+    return v;
+}
+/* Sum over the workgroup, in thread 0. */
+__device__ __forceinline__ double block_sum_f64(double v, double* s_wave)
+{
+    v = wave_sum_f64(v);
+    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double r = 0.0;
+    if (threadIdx.x == 0)
+#pragma unroll
+        for (int w = 0; w < kB / 64; ++w) r += s_wave[w];
+    return r;
 }
 
 struct TopShared {
@@ -52,57 +120,48 @@ struct TopShared {
     int scan[kB / 64];
     double red[kB / 64];
     int count;
-    alignas(16) uint64_t list[kListCap]; /* every element at or above `bound`, any order */
-    uint64_t sorted[kNMax];              /* the n best of them, best first */
+    int flag;
+    alignas(16) uint64_t list[kListCap]; /* in any order */
+    alignas(16) uint64_t sorted[kNMax];
+    double y[kNMax];
 };
 
-template <int BLOCK>
-__device__ double block_sum_f64(double v, double* s_wave)
-{
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-    if ((threadIdx.x & 63) == 0) s_wave[threadIdx.x >> 6] = v;
-    __syncthreads();
-    double r = 0.0;
-#pragma unroll
-    for (int w = 0; w < BLOCK / 64; ++w) r += s_wave[w];
-    __syncthreads();
-    return r;
-}
+struct TopList {
+    int listed; /* entries of sh.list */
+    float top;  /* the largest candidate */
+};
 
-/* The n best (n <= kNMax) of the workgroup's candidates into sh.sorted; returns
- * how many there are (fewer than n where there are no more).  x: this thread's E logits,
- * token(e) their tokens.  On return `listed` entries of sh.list hold every
- * candidate at or above `bound`, except `more` further copies of `bound` itself.
+/* The workgroup's largest candidates into sh.list, at least the n best (n <= kNMax) or all
+ * there are.  x: this thread's E logits, token(e) their tokens.
  *
  * The n-th largest of the threads' largest keys bounds the n-th largest key
  * from below, and for n well below the threads few elements beside the n best
- * reach it: those are listed and ranked by counting.  Where more are at or above
- * the bound than the list holds (equal logits in masses), the n-th largest
- * key is selected exactly and of its copies the lowest tokens are taken, in
- * the order of (vector j, thread, element i) that `token` rises in. */
+ * reach it.  Where more reach it than the list holds (equal logits in
+ * masses), the n-th largest key is selected exactly and of its copies the
+ * lowest tokens are taken, in the order of (vector, thread, element) that
+ * `token` rises in. */
 template <int E, int VW, typename TokenF>
-__device__ int top_list(const float (&x)[E], TokenF token, int n, TopShared& sh, float& bound,
-                        int& listed, int& more)
+__device__ __forceinline__ TopList top_list(const float (&x)[E], float largest, TokenF token, int n, TopShared& sh)
 {
     const int tid = threadIdx.x, lane = tid & 63;
-    float m = x[0];
-#pragma unroll
-    for (int e = 1; e < E; ++e) m = fmaxf(m, x[e]);
-    const uint32_t mkey = cand_key(m);
+    const uint32_t mkey = cand_key(largest);
     sh.tmax[tid] = mkey;
     if (tid == 0) sh.count = 0;
     __syncthreads();
     uint32_t v[kB / 64];
+    uint32_t top = 0u;
     int nz = 0;
 #pragma unroll
     for (int q = 0; q < kB / 64; ++q) {
         v[q] = sh.tmax[lane + 64 * q];
+        top = v[q] > top ? v[q] : top;
         nz += __popcll(__ballot(v[q] != 0u));
     }
-    const uint32_t t = nz >= n ? wave_kth_bound<kB / 64>(v, n, 32) : 1u;
-    bound = t == 1u ? -__builtin_inff() : key2f(t);
-    if (mkey >= t) {
+    const uint32_t t = nz >= n ? wave_kth_bound<kB / 64>(v, n, 10) : 1u;
+    TopList r;
+    r.top = key2f(wave_max_u32(top));
+    const float bound = t <= 1u ? -__builtin_inff() : key2f(t);
+    if (mkey >= t && mkey != 0u) {
 #pragma unroll
         for (int e = 0; e < E; ++e)
             if (x[e] > kMasked && x[e] >= bound) {
@@ -112,14 +171,12 @@ __device__ int top_list(const float (&x)[E], TokenF token, int n, TopShared& sh,
     }
     __syncthreads();
     int cnt = sh.count;
-    more = 0;
     if (cnt > kListCap) {
         uint32_t keys[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) keys[e] = cand_key(x[e]);
         int gt, eq;
         const uint32_t kth = regs_radix_kth<kB, E>(keys, n, sh.hist, sh.misc, &gt, &eq);
-        bound = key2f(kth);
         if (tid == 0) sh.count = 0;
         __syncthreads();
 #pragma unroll
@@ -142,132 +199,201 @@ __device__ int top_list(const float (&x)[E], TokenF token, int n, TopShared& sh,
             taken += total;
         }
         cnt = n;
-        more = gt + eq - n;
         __syncthreads();
     }
-    listed = cnt;
-    for (int i = tid; i < cnt; i += kB) {
-        const uint64_t mine = sh.list[i];
-        int rank = 0;
-        for (int j = 0; j < cnt; ++j) rank += sh.list[j] > mine;
-        if (rank < n) sh.sorted[rank] = mine;
-    }
-    __syncthreads();
-    return cnt < n ? cnt : n;
+    r.listed = cnt;
+    return r;
+}
+
+/* How many of the list's entries are better than `mine`. */
+__device__ __forceinline__ int rank_in(const uint64_t* list, int cnt, uint64_t mine)
+{
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < cnt; ++j) rank += list[j] > mine;
+    return rank;
 }
 
 /* ------------------------------------------------------------------ chunks */
 
-template <int DT>
-__global__ __launch_bounds__(kB) void beam_chunk_kernel(BeamSelectArgs a)
+/* Sum of the terms of this thread's logits: in binary32 over four, whose
+ * sum rounds twice, then in binary64.  The polynomial and the split of its
+ * result run in binary64 because that costs what binary32 does on this
+ * machine, and binary32 would leave errors of 1e-6 in the terms of equal logits,
+ * which many rows of bf16 have thousands of. */
+template <int MODE, bool NEAR, bool MASK, int E>
+__device__ __forceinline__ double sum_terms(const float (&x)[E], const TopList& tl, double ref,
+                                            const BeamSoftcap& c)
+{
+    double s = 0.0;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+        float t[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            t[q] = term_of<MODE, NEAR>(x[e + q], tl.top, ref, c);
+            if constexpr (MASK) t[q] = x[e + q] > kMasked ? t[q] : 0.0f;
+        }
+        s += (double)((t[0] + t[1]) + (t[2] + t[3]));
+    }
+    return s;
+}
+
+template <int MODE, int E>
+__device__ __forceinline__ double sum_rest(const float (&x)[E], float least, float largest,
+                                           const TopList& tl, double ref, const BeamSoftcap& c)
+{
+    /* most waves hold no masked logit and none beyond the polynomial */
+    const bool near = MODE == kCapNone || (least >= -c.limit && largest <= c.limit);
+    if (MODE != kCapExact && __all(least > kMasked && near)) {
+        const double s = sum_terms<MODE, true, false>(x, tl, ref, c);
+        if (__all(s == s)) return s; /* a NaN is not seen by minimum and maximum */
+    }
+    return sum_terms<MODE, false, true>(x, tl, ref, c);
+}
+
+/* One workgroup per chunk of kBeamChunk logits: its n best candidates, ranked, and its part of
+ * the softmax denominator. */
+template <int MODE>
+__device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopShared& sh);
+__device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, TopShared& sh);
+
+template <int DT, int MODE>
+__global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
 {
     constexpr int VW = Elem<DT>::VW;
     constexpr int NV = kE / VW;
     __shared__ TopShared sh;
     const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x;
-    if (!(a.scores[row] > kMasked)) return;
-    const char* base = static_cast<const char*>(a.logits) + (int64_t)row * a.row_stride * Elem<DT>::SIZE;
-    const int64_t first = (int64_t)ch * kBeamChunk;
-    float x[kE];
+    const int b = row / a.beams;
+    const bool live = a.scores[row] > kMasked;
+    if (live) {
+        const char* base =
+            static_cast<const char*>(a.logits) + (int64_t)row * a.row_stride * Elem<DT>::SIZE;
+        const int64_t first = (int64_t)ch * kBeamChunk;
+        float x[kE];
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        float v[VW];
-        load_vec<DT>(base, first + (int64_t)(j * kB + tid) * VW, a.vocab, v);
+        for (int j = 0; j < NV; ++j) {
+            float v[VW];
+            load_vec<DT>(base, first + (int64_t)(j * kB + tid) * VW, a.vocab, v);
 #pragma unroll
-        for (int i = 0; i < VW; ++i) x[j * VW + i] = v[i];
+            for (int i = 0; i < VW; ++i) x[j * VW + i] = v[i];
+        }
+        auto token = [&](int e) {
+            return (uint32_t)first + (uint32_t)(((e / VW) * kB + tid) * VW + e % VW);
+        };
+        float largest = x[0], least = x[0];
+#pragma unroll
+        for (int e = 1; e < kE; ++e) {
+            largest = fmaxf(largest, x[e]);
+            least = fminf(least, x[e]);
+        }
+        const TopList tl = top_list<kE, VW>(x, largest, token, a.n, sh);
+        const int64_t at = (int64_t)row * a.chunks + ch;
+        uint64_t* cand = a.ws.cand + at * a.n;
+        for (int i = tid; i < tl.listed; i += kB) {
+            const uint64_t e = sh.list[i];
+            const int rank = rank_in(sh.list, tl.listed, e);
+            if (rank < a.n) st_dev(&cand[rank], e);
+        }
+        double s = 0.0;
+        if (tl.listed)
+            s = sum_rest<MODE, kE>(x, least, largest, tl, value64<MODE>(tl.top, a.cap), a.cap);
+        for (int i = tl.listed + tid; i < a.n; i += kB) st_dev(&cand[i], (uint64_t)0);
+        s = block_sum_f64(s, sh.red);
+        if (tid == 0) st_dev(&a.ws.sums[at], d2u(s));
+        if (a.chunks > 1 && !elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
+        if (a.chunks == 1) {
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+        }
+        merge_row<MODE>(a, row, sh);
+    } else {
+        if (ch != 0) return;
+        if (tid == 0 && a.lse) a.lse[row] = -__builtin_inff();
+        for (int i = tid; i < a.n; i += kB) st_dev(&a.ws.best[(int64_t)row * a.n + i], (uint64_t)0);
     }
-    auto token = [&](int e) {
-        return (uint32_t)first + (uint32_t)(((e / VW) * kB + tid) * VW + e % VW);
-    };
-    float bound;
-    int listed, more;
-    const int cnt = top_list<kE, VW>(x, token, a.n, sh, bound, listed, more);
-    const int64_t at = (int64_t)row * a.chunks + ch;
-    uint64_t* cand = a.ws.cand + at * a.n;
-    for (int i = tid; i < a.n; i += kB) cand[i] = i < cnt ? sh.sorted[i] : 0ull;
-
-    /* the listed candidates, the heaviest terms, and their further copies
-     * in binary64; the rest of the chunk */
-    const double cap = (double)a.softcap;
-    const double top = cnt ? softcap64(key2f(entry_key(sh.sorted[0])), cap) : -__builtin_inf();
-    double s = 0.0;
-    if (cnt) {
-        for (int i = tid; i < listed; i += kB)
-            s += term64(softcap64(key2f(entry_key(sh.list[i])), cap), top);
-        if (tid == 0 && more) s += (double)more * term64(softcap64(bound, cap), top);
-#pragma unroll
-        for (int e = 0; e < kE; ++e)
-            if (x[e] > kMasked && x[e] < bound) s += term64(softcap64(x[e], cap), top);
+    if (a.beams > 1 &&
+        !elect_last(&a.ws.tickets[a.batch * a.beams + b], (uint32_t)a.beams, &sh.flag))
+        return;
+    if (a.beams == 1) {
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
     }
-    s = block_sum_f64<kB>(s, sh.red);
-    if (tid == 0) a.ws.parts[at] = BeamPart{top, s};
+    merge_sequence(a, b, sh);
 }
 
 /* -------------------------------------------------------------------- rows */
 
 /* A row's n best and its normaliser from its chunks'. */
-__global__ __launch_bounds__(kB) void beam_row_kernel(BeamSelectArgs a)
+template <int MODE>
+__device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopShared& sh)
 {
     constexpr int E = 16;
-    __shared__ TopShared sh;
-    const int row = blockIdx.x, tid = threadIdx.x;
-    const bool live = a.scores[row] > kMasked;
-    uint64_t* best = a.ws.best + (int64_t)row * a.n;
+    const int tid = threadIdx.x;
     const uint64_t* cand = a.ws.cand + (int64_t)row * a.chunks * a.n;
-    const int64_t total = live ? (int64_t)a.chunks * a.n : 0;
+    const int64_t total = (int64_t)a.chunks * a.n;
     int cnt = 0;
     /* tiles of candidates beside the best of those before; the chunks' lists
      * lie in token order, so copies of one key do too */
     for (int64_t base = 0; base < total;) {
         float x[E];
         uint32_t tok[E];
+        float largest = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = e * kB + tid;
             uint64_t c = 0ull;
-            if (i < cnt)
-                c = sh.sorted[i];
-            else if (base + i - cnt < total)
-                c = cand[base + i - cnt];
+            if (e * kB < cnt + total - base) {
+                if (i < cnt)
+                    c = sh.sorted[i];
+                else if (base + i - cnt < total)
+                    c = ld_dev(&cand[base + i - cnt]);
+            }
             x[e] = c ? key2f(entry_key(c)) : -__builtin_inff();
             tok[e] = entry_token(c);
+            largest = fmaxf(largest, x[e]);
         }
         base += E * kB - cnt;
         __syncthreads();
-        float bound;
-        int listed, more;
-        cnt = top_list<E, 1>(x, [&](int e) { return tok[e]; }, a.n, sh, bound, listed, more);
-    }
-    __syncthreads();
-    const BeamPart* parts = a.ws.parts + (int64_t)row * a.chunks;
-    const double cap = (double)a.softcap;
-    const double top = cnt ? softcap64(key2f(entry_key(sh.sorted[0])), cap) : -__builtin_inf();
-    double s = 0.0;
-    if (cnt)
-        for (int c = tid; c < a.chunks; c += kB) {
-            const BeamPart p = parts[c];
-            if (p.sum > 0.0) s += p.sum * term64(p.top, top);
+        const TopList tl =
+            top_list<E, 1>(x, largest, [&](int e) { return tok[e]; }, a.n, sh);
+        for (int i = tid; i < tl.listed; i += kB) {
+            const uint64_t e = sh.list[i];
+            const int rank = rank_in(sh.list, tl.listed, e);
+            if (rank < a.n) sh.sorted[rank] = e;
         }
-    s = block_sum_f64<kB>(s, sh.red);
-    const double ls = log(s);
-    double* ys = a.ws.y + (int64_t)row * a.n;
+        cnt = tl.listed < a.n ? tl.listed : a.n;
+        __syncthreads();
+    }
+    /* the chunks' sums relative to their largest logit, which leads each list */
+    const double top =
+        cnt ? softcap64<MODE>(key2f(entry_key(sh.sorted[0])), a.cap) : -__builtin_inf();
+    double s = 0.0;
+    for (int c = tid; c < a.chunks; c += kB) {
+        const uint64_t first = ld_dev(&cand[(int64_t)c * a.n]);
+        const double sum = u2d(ld_dev(&a.ws.sums[(int64_t)row * a.chunks + c]));
+        if (first) s += sum * term64(softcap64<MODE>(key2f(entry_key(first)), a.cap), top);
+    }
+    for (int i = tid; i < cnt; i += kB) sh.y[i] = softcap64<MODE>(key2f(entry_key(sh.sorted[i])), a.cap);
+    s = block_sum_f64(s, sh.red); /* (a barrier: y is complete) */
     for (int i = tid; i < a.n; i += kB) {
         uint64_t e = i < cnt ? sh.sorted[i] : 0ull;
         double y = -__builtin_inf();
         if (e) {
             /* where tanh saturates its last bit may waver: the list may not rise */
             y = top;
-            for (int j = 1; j <= i; ++j)
-                y = fmin(y, softcap64(key2f(entry_key(sh.sorted[j])), cap));
+            for (int j = 1; j <= i; ++j) y = fmin(y, sh.y[j]);
             /* beside an infinite largest logit the rest have probability 0 */
             if (top == __builtin_inf() && y != top) e = 0ull;
         }
-        best[i] = e;
-        ys[i] = y;
+        st_dev(&a.ws.best[(int64_t)row * a.n + i], e);
+        st_dev(&a.ws.y[(int64_t)row * a.n + i], d2u(y));
     }
     if (tid == 0) {
-        a.ws.norm[2 * row] = top;
-        a.ws.norm[2 * row + 1] = ls;
+        const double ls = log(s);
+        st_dev(&a.ws.norm[2 * row], d2u(top));
+        st_dev(&a.ws.norm[2 * row + 1], d2u(ls));
         if (a.lse) a.lse[row] = cnt ? (float)(top + ls) : -__builtin_inff();
     }
 }
@@ -276,26 +402,26 @@ __global__ __launch_bounds__(kB) void beam_row_kernel(BeamSelectArgs a)
 
 /* The n best of the sequence's W sorted lists: a candidate's rank is the
  * number of better ones, found in each list by bisection. */
-__global__ __launch_bounds__(kB) void beam_sequence_kernel(BeamSelectArgs a)
+__device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, TopShared& sh)
 {
     extern __shared__ double sc[]; /* [W][n] scores, -inf = none */
-    __shared__ int s_wave[kB / 64];
-    const int b = blockIdx.x, tid = threadIdx.x;
+    const int tid = threadIdx.x;
     const int W = a.beams, n = a.n, total = W * n;
     const uint64_t* best = a.ws.best + (int64_t)b * total;
-    const double* ys = a.ws.y + (int64_t)b * total;
+    const uint64_t* ys = a.ws.y + (int64_t)b * total;
     int found = 0;
     for (int i = tid; i < total; i += kB) {
         const int w = i / n;
         double s = -__builtin_inf();
-        if (best[i]) {
-            const double* norm = a.ws.norm + 2 * ((int64_t)b * W + w);
-            s = (double)a.scores[b * W + w] + ((ys[i] == norm[0] ? 0.0 : ys[i] - norm[0]) - norm[1]);
+        if (ld_dev(&best[i])) {
+            const uint64_t* norm = a.ws.norm + 2 * ((int64_t)b * W + w);
+            const double top = u2d(ld_dev(&norm[0])), y = u2d(ld_dev(&ys[i]));
+            s = (double)a.scores[b * W + w] + ((y == top ? 0.0 : y - top) - u2d(ld_dev(&norm[1])));
             ++found;
         }
         sc[i] = s;
     }
-    found = block_sum_i32<kB>(found, s_wave);
+    found = block_sum_i32<kB>(found, sh.scan);
     int32_t* parents = a.parents + (int64_t)b * n;
     int32_t* tokens = a.tokens + (int64_t)b * n;
     float* out = a.out + (int64_t)b * n;
@@ -320,7 +446,7 @@ __global__ __launch_bounds__(kB) void beam_sequence_kernel(BeamSelectArgs a)
         }
         if (rank < n) {
             parents[rank] = b * W + w;
-            tokens[rank] = (int32_t)entry_token(best[i]);
+            tokens[rank] = (int32_t)entry_token(ld_dev(&best[i]));
             out[rank] = (float)s;
         }
     }
@@ -392,15 +518,52 @@ hipError_t reorder_with(const BeamReorderArgs& a, hipStream_t stream)
 
 }  // namespace
 
-hipError_t beam_select_launch(const BeamSelectArgs& a, int32_t dtype, hipStream_t stream)
+/* tanh(z) / z as a polynomial in z^2 for |z| <= 1.25: |z| times its error is below
+ * 5.4e-10 (weighted least squares at Chebyshev nodes, reweighted towards the
+ * least maximum). */
+BeamSoftcap beam_softcap(float cap)
+{
+    static const double q[10] = {0x1.ffffffbcad3ecp-1,  -0x1.555539c5a4875p-2,
+                                 0x1.110dd56c82b34p-3,  -0x1.b9c2e07c36e05p-5,
+                                 0x1.63abfe7705209p-6,  -0x1.161fef1075584p-7,
+                                 0x1.8c273d5cd2dc4p-9,  -0x1.c8e7e314ad0f9p-11,
+                                 0x1.650da776b43d8p-13, -0x1.0e9af9dea189cp-16};
+    BeamSoftcap c{};
+    c.cap = cap;
+    if (!(cap > 0.0f)) {
+        c.mode = kCapNone;
+        return c;
+    }
+    const double d = (double)cap;
+    c.mode = cap >= 1e-12f && cap <= 128.0f ? kCapPoly : kCapExact;
+    double scale = kLog2e;
+    for (int i = 0; i < 10; ++i) {
+        c.q[i] = q[i] * scale;
+        scale /= d * d;
+    }
+    c.limit = (float)(1.25 * d);
+    return c;
+}
+
+template <int DT>
+static void select_launch(const BeamSelectArgs& a, hipStream_t stream)
 {
     const dim3 grid((unsigned)a.chunks, (unsigned)(a.batch * a.beams));
-    if (dtype == G4S_DTYPE_F32)
-        beam_chunk_kernel<0><<<grid, kB, 0, stream>>>(a);
+    const size_t lds = sizeof(double) * a.beams * a.n;
+    if (a.cap.mode == kCapNone)
+        beam_select_kernel<DT, kCapNone><<<grid, kB, lds, stream>>>(a);
+    else if (a.cap.mode == kCapPoly)
+        beam_select_kernel<DT, kCapPoly><<<grid, kB, lds, stream>>>(a);
     else
-        beam_chunk_kernel<1><<<grid, kB, 0, stream>>>(a);
-    beam_row_kernel<<<(unsigned)(a.batch * a.beams), kB, 0, stream>>>(a);
-    beam_sequence_kernel<<<(unsigned)a.batch, kB, sizeof(double) * a.beams * a.n, stream>>>(a);
+        beam_select_kernel<DT, kCapExact><<<grid, kB, lds, stream>>>(a);
+}
+
+hipError_t beam_select_launch(const BeamSelectArgs& a, int32_t dtype, hipStream_t stream)
+{
+    if (dtype == G4S_DTYPE_F32)
+        select_launch<0>(a, stream);
+    else
+        select_launch<1>(a, stream);
     return hipGetLastError();
 }
 

@@ -41,7 +41,7 @@ int fail_in(char (&buf)[512], int code, const char* fmt, va_list ap)
 
 struct g4s_beam : Handle {
     int32_t vocab = 0, max_batch = 0, max_beams = 0, chunks = 0;
-    float softcap = 0.0f;
+    g4s::BeamSoftcap cap{};
     void* memory = nullptr;
     g4s::BeamWorkspace ws{};
 };
@@ -190,16 +190,17 @@ G4S_API int g4s_beam_create(g4s_beam** out, int32_t vocab, int32_t max_batch, in
     h->vocab = vocab;
     h->max_batch = max_batch;
     h->max_beams = max_beams;
-    h->softcap = softcap;
+    h->cap = g4s::beam_softcap(softcap);
     h->chunks = g4s::beam_chunks(vocab);
     const size_t rows = (size_t)max_batch * max_beams, n = 2 * (size_t)max_beams;
     Carver c;
     auto lay = [&] {
         c.add(&h->ws.cand, rows * h->chunks * n);
-        c.add(&h->ws.parts, rows * h->chunks);
+        c.add(&h->ws.sums, rows * h->chunks);
         c.add(&h->ws.best, rows * n);
         c.add(&h->ws.y, rows * n);
         c.add(&h->ws.norm, rows * 2);
+        c.add(&h->ws.tickets, rows + max_batch);
     };
     lay();
     const size_t bytes = c.used();
@@ -210,6 +211,14 @@ G4S_API int g4s_beam_create(g4s_beam** out, int32_t vocab, int32_t max_batch, in
     }
     c.start(h->memory);
     lay();
+    hipError_t e = hipMemsetAsync(h->ws.tickets, 0, (rows + max_batch) * sizeof(uint32_t),
+                                  h->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(h->memory);
+        delete h;
+        return hip_fail(none, e, "workspace initialisation");
+    }
     *out = h;
     return G4S_OK;
 }
@@ -264,7 +273,7 @@ int select(g4s_beam* h, const void* d_logits, int32_t dtype, int64_t row_stride,
     a.beams = beams;
     a.n = n;
     a.chunks = h->chunks;
-    a.softcap = h->softcap;
+    a.cap = h->cap;
     a.scores = d_scores;
     a.parents = d_parents;
     a.tokens = d_tokens;
