@@ -34,17 +34,27 @@ __device__ __forceinline__ uint32_t entry_key(uint64_t e) { return (uint32_t)(e 
 __device__ __forceinline__ uint32_t entry_token(uint64_t e) { return ~(uint32_t)e; }
 
 using cr::exp_fast_d;
-using cr::tanh_fast_d;
 
 constexpr double kLog2e = 0x1.71547652b82fep+0;
 
 __device__ __forceinline__ uint64_t d2u(double x) { return __builtin_bit_cast(uint64_t, x); }
 __device__ __forceinline__ double u2d(uint64_t u) { return __builtin_bit_cast(double, u); }
 
+/* cap * tanh(x / cap), off by some 2^-52 of the cap. */
 template <int MODE>
 __device__ __forceinline__ double softcap64(float x, const BeamSoftcap& c)
 {
-    return MODE == kCapNone ? (double)x : (double)c.cap * tanh_fast_d((double)x / (double)c.cap);
+    if constexpr (MODE == kCapNone) return (double)x;
+    const double cap = (double)c.cap;
+    const double e = exp_fast_d(fmax(-2.0 * fabs((double)x) / cap, -80.0));
+    return copysign(cap * ((1.0 - e) / (1.0 + e)), (double)x);
+}
+
+/* log(x) for x in [1, 2^60], off by less than 1e-12: one Newton step from binary32's. */
+__device__ __forceinline__ double log64(double x)
+{
+    const double l = (double)(__builtin_amdgcn_logf((float)x) * 0x1.62e43p-1f);
+    return l + (x * exp_fast_d(-l) - 1.0);
 }
 
 /* exp(y - top) for y <= top; an infinite top (no softcap, x = +inf) counts 1
@@ -132,16 +142,19 @@ struct TopList {
 };
 
 /* The workgroup's largest candidates into sh.list, at least the n best (n <= kNMax) or all
- * there are.  x: this thread's E logits, token(e) their tokens.
+ * there are.  x: this thread's E logits, token(e) their tokens; entry(i),
+ * i < count, reads all of them again, in an order that tokens of equal keys
+ * rise in.
  *
  * The n-th largest of the threads' largest keys bounds the n-th largest key
  * from below, and for n well below the threads few elements beside the n best
  * reach it.  Where more reach it than the list holds (equal logits in
  * masses), the n-th largest key is selected exactly and of its copies the
- * lowest tokens are taken, in the order of (vector, thread, element) that
- * `token` rises in. */
-template <int E, int VW, typename TokenF>
-__device__ __forceinline__ TopList top_list(const float (&x)[E], float largest, TokenF token, int n, TopShared& sh)
+ * first are taken; that way reads again what it needs, so that it costs the
+ * usual one no registers. */
+template <int E, typename TokenF, typename EntryF>
+__device__ __forceinline__ TopList top_list(const float (&x)[E], float largest, TokenF token,
+                                            int count, EntryF entry, int n, TopShared& sh)
 {
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t mkey = cand_key(largest);
@@ -172,30 +185,21 @@ __device__ __forceinline__ TopList top_list(const float (&x)[E], float largest, 
     __syncthreads();
     int cnt = sh.count;
     if (cnt > kListCap) {
-        uint32_t keys[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) keys[e] = cand_key(x[e]);
         int gt, eq;
-        const uint32_t kth = regs_radix_kth<kB, E>(keys, n, sh.hist, sh.misc, &gt, &eq);
+        auto key = [&](int i) { return entry_key(entry(i)); };
+        const uint32_t kth = block_radix_kth<kB>(
+            count, n, key, [&](int i) { return key(i) != 0u; }, sh.hist, sh.misc, &gt, &eq);
         if (tid == 0) sh.count = 0;
         __syncthreads();
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (keys[e] > kth) sh.list[atomicAdd(&sh.count, 1)] = entry_of(keys[e], token(e));
-        __syncthreads();
         int taken = gt;
-#pragma unroll
-        for (int j = 0; j < E / VW; ++j) {
-            int c = 0, total;
-#pragma unroll
-            for (int i = 0; i < VW; ++i) c += keys[j * VW + i] == kth;
-            int p = taken + block_exclusive_scan<kB>(c, sh.scan, total);
-#pragma unroll
-            for (int i = 0; i < VW; ++i)
-                if (keys[j * VW + i] == kth) {
-                    if (p < n) sh.list[p] = entry_of(kth, token(j * VW + i));
-                    ++p;
-                }
+#pragma unroll 1
+        for (int i0 = 0; i0 < count; i0 += kB) {
+            const uint64_t c = i0 + tid < count ? entry(i0 + tid) : 0ull;
+            if (entry_key(c) > kth) sh.list[atomicAdd(&sh.count, 1)] = c;
+            const int same = c != 0ull && entry_key(c) == kth;
+            int total;
+            const int p = taken + block_exclusive_scan<kB>(same, sh.scan, total);
+            if (same && p < n) sh.list[p] = c;
             taken += total;
         }
         cnt = n;
@@ -216,40 +220,49 @@ __device__ __forceinline__ int rank_in(const uint64_t* list, int cnt, uint64_t m
 
 /* ------------------------------------------------------------------ chunks */
 
-/* Sum of the terms of this thread's logits: in binary32 over four, whose
- * sum rounds twice, then in binary64.  The polynomial and the split of its
- * result run in binary64 because that costs what binary32 does on this
- * machine, and binary32 would leave errors of 1e-6 in the terms of equal logits,
- * which many rows of bf16 have thousands of. */
-template <int MODE, bool NEAR, bool MASK, int E>
-__device__ __forceinline__ double sum_terms(const float (&x)[E], const TopList& tl, double ref,
-                                            const BeamSoftcap& c)
+/* Sum of N (2 or 4) terms: in binary32, which rounds twice at most; such sums are added
+ * in binary64.  The polynomial and the split of its result run in binary64
+ * because that costs what binary32 does on this machine, and binary32 would
+ * leave errors of 1e-6 in the terms of equal logits, which many rows of bf16 have
+ * thousands of. */
+template <int MODE, bool NEAR, bool MASK, int N>
+__device__ __forceinline__ double sum_few(const float* x, float top, double ref,
+                                          const BeamSoftcap& c)
 {
-    double s = 0.0;
+    float t[N];
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
-        float t[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            t[q] = term_of<MODE, NEAR>(x[e + q], tl.top, ref, c);
-            if constexpr (MASK) t[q] = x[e + q] > kMasked ? t[q] : 0.0f;
-        }
-        s += (double)((t[0] + t[1]) + (t[2] + t[3]));
+    for (int q = 0; q < N; ++q) {
+        t[q] = term_of<MODE, NEAR>(x[q], top, ref, c);
+        if constexpr (MASK) t[q] = x[q] > kMasked ? t[q] : 0.0f;
     }
-    return s;
+    if constexpr (N == 2)
+        return (double)(t[0] + t[1]);
+    else
+        return (double)((t[0] + t[1]) + (t[2] + t[3]));
 }
 
-template <int MODE, int E>
-__device__ __forceinline__ double sum_rest(const float (&x)[E], float least, float largest,
-                                           const TopList& tl, double ref, const BeamSoftcap& c)
+/* This thread's part of the chunk's sum.  Most waves hold no masked logit and none
+ * beyond the polynomial; the others read their logits again (read(e), element
+ * e) rather than hold them through the longer way. */
+template <int MODE, int E, typename ReadF>
+__device__ __forceinline__ double sum_terms(const float (&x)[E], float least, float largest,
+                                            float top, const BeamSoftcap& c, ReadF read)
 {
-    /* most waves hold no masked logit and none beyond the polynomial */
+    const double ref = value64<MODE>(top, c);
     const bool near = MODE == kCapNone || (least >= -c.limit && largest <= c.limit);
+    double s = 0.0;
     if (MODE != kCapExact && __all(least > kMasked && near)) {
-        const double s = sum_terms<MODE, true, false>(x, tl, ref, c);
+#pragma unroll
+        for (int e = 0; e < E; e += 4) s += sum_few<MODE, true, false, 4>(&x[e], top, ref, c);
         if (__all(s == s)) return s; /* a NaN is not seen by minimum and maximum */
+        s = 0.0;
     }
-    return sum_terms<MODE, false, true>(x, tl, ref, c);
+#pragma unroll 1
+    for (int e = 0; e < E; e += 2) {
+        const float v[2] = {read(e), read(e + 1)};
+        s += sum_few<MODE, false, true, 2>(v, top, ref, c);
+    }
+    return s;
 }
 
 /* One workgroup per chunk of kBeamChunk logits: its n best candidates, ranked, and its part of
@@ -279,8 +292,18 @@ __global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
 #pragma unroll
             for (int i = 0; i < VW; ++i) x[j * VW + i] = v[i];
         }
+        const int rest = a.vocab - (int)first;
+        const int count = rest < kBeamChunk ? rest : kBeamChunk;
         auto token = [&](int e) {
             return (uint32_t)first + (uint32_t)(((e / VW) * kB + tid) * VW + e % VW);
+        };
+        auto read = [&](int e) {
+            const int64_t i = token(e);
+            return i < a.vocab ? load_elem<DT>(base, i) : -__builtin_inff();
+        };
+        auto entry = [&](int i) {
+            const uint32_t key = cand_key(load_elem<DT>(base, first + i));
+            return key ? entry_of(key, (uint32_t)first + (uint32_t)i) : 0ull;
         };
         float largest = x[0], least = x[0];
 #pragma unroll
@@ -288,7 +311,7 @@ __global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
             largest = fmaxf(largest, x[e]);
             least = fminf(least, x[e]);
         }
-        const TopList tl = top_list<kE, VW>(x, largest, token, a.n, sh);
+        const TopList tl = top_list<kE>(x, largest, token, count, entry, a.n, sh);
         const int64_t at = (int64_t)row * a.chunks + ch;
         uint64_t* cand = a.ws.cand + at * a.n;
         for (int i = tid; i < tl.listed; i += kB) {
@@ -298,7 +321,7 @@ __global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
         }
         double s = 0.0;
         if (tl.listed)
-            s = sum_rest<MODE, kE>(x, least, largest, tl, value64<MODE>(tl.top, a.cap), a.cap);
+            s = sum_terms<MODE, kE>(x, least, largest, tl.top, a.cap, read);
         for (int i = tl.listed + tid; i < a.n; i += kB) st_dev(&cand[i], (uint64_t)0);
         s = block_sum_f64(s, sh.red);
         if (tid == 0) st_dev(&a.ws.sums[at], d2u(s));
@@ -329,7 +352,7 @@ __global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
 template <int MODE>
 __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopShared& sh)
 {
-    constexpr int E = 16;
+    constexpr int E = 8;
     const int tid = threadIdx.x;
     const uint64_t* cand = a.ws.cand + (int64_t)row * a.chunks * a.n;
     const int64_t total = (int64_t)a.chunks * a.n;
@@ -337,27 +360,26 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopS
     /* tiles of candidates beside the best of those before; the chunks' lists
      * lie in token order, so copies of one key do too */
     for (int64_t base = 0; base < total;) {
+        const int64_t rest = cnt + total - base;
+        const int count = rest < E * kB ? (int)rest : E * kB;
+        auto entry = [&](int i) {
+            return i < cnt ? sh.sorted[i] : ld_dev(&cand[base + i - cnt]);
+        };
         float x[E];
         uint32_t tok[E];
         float largest = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = e * kB + tid;
-            uint64_t c = 0ull;
-            if (e * kB < cnt + total - base) {
-                if (i < cnt)
-                    c = sh.sorted[i];
-                else if (base + i - cnt < total)
-                    c = ld_dev(&cand[base + i - cnt]);
-            }
+            const uint64_t c = e * kB < count && i < count ? entry(i) : 0ull;
             x[e] = c ? key2f(entry_key(c)) : -__builtin_inff();
             tok[e] = entry_token(c);
             largest = fmaxf(largest, x[e]);
         }
-        base += E * kB - cnt;
+        const TopList tl = top_list<E>(
+            x, largest, [&](int e) { return tok[e]; }, count, entry, a.n, sh);
+        base += count - cnt;
         __syncthreads();
-        const TopList tl =
-            top_list<E, 1>(x, largest, [&](int e) { return tok[e]; }, a.n, sh);
         for (int i = tid; i < tl.listed; i += kB) {
             const uint64_t e = sh.list[i];
             const int rank = rank_in(sh.list, tl.listed, e);
@@ -391,7 +413,7 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopS
         st_dev(&a.ws.y[(int64_t)row * a.n + i], d2u(y));
     }
     if (tid == 0) {
-        const double ls = log(s);
+        const double ls = log64(s);
         st_dev(&a.ws.norm[2 * row], d2u(top));
         st_dev(&a.ws.norm[2 * row + 1], d2u(ls));
         if (a.lse) a.lse[row] = cnt ? (float)(top + ls) : -__builtin_inff();
