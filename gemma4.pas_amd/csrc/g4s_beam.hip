@@ -19,9 +19,10 @@ namespace g4s {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 
-constexpr int kB = kBeamBlock;
-constexpr int kE = kBeamItems;
+constexpr int kB = 256;
 constexpr int kListCap = 512; /* candidates of a workgroup kept for ranking */
 constexpr int kNMax = 2 * G4S_BEAM_MAX_BEAMS;
 constexpr float kMasked = -1e30f; /* a logit not above it is no candidate */
@@ -36,6 +37,7 @@ __device__ __forceinline__ uint32_t entry_token(uint64_t e) { return ~(uint32_t)
 using cr::exp_fast_d;
 
 constexpr double kLog2e = 0x1.71547652b82fep+0;
+constexpr double kLn2 = 0x1.62e42fefa39efp-1;
 
 __device__ __forceinline__ uint64_t d2u(double x) { return __builtin_bit_cast(uint64_t, x); }
 __device__ __forceinline__ double u2d(uint64_t u) { return __builtin_bit_cast(double, u); }
@@ -91,16 +93,19 @@ __device__ __forceinline__ float pow2_of(double t)
     return __builtin_amdgcn_ldexpf(__builtin_amdgcn_exp2f(f), (int)(uint32_t)d2u(m));
 }
 
-/* The term of one logit in its chunk's sum, 2^(v(x) - ref), ref = v(top). */
-template <int MODE, bool NEAR>
-__device__ __forceinline__ float term_of(float x, float top, double ref, const BeamSoftcap& c)
+/* 2^v(x): near, the term of a logit with |x| <= limit; far, of any unmasked one, relative to
+ * ref (0 but where the softcap leaves binary32's range). */
+template <int MODE>
+__device__ __forceinline__ float near_term(float x, const BeamSoftcap& c)
 {
-    if constexpr (MODE == kCapNone)
-        return x == top ? 1.0f : pow2_of(fmax(((double)x - (double)top) * kLog2e, -1000.0));
-    else if constexpr (MODE == kCapPoly && NEAR)
-        return pow2_of(__builtin_fma((double)x, near_factor((double)x, c), -ref));
-    else
-        return pow2_of(fmax(value64<MODE>(x, c) - ref, -1000.0));
+    const double xd = (double)x;
+    return pow2_of(xd * (MODE == kCapNone ? kLog2e : near_factor(xd, c)));
+}
+template <int MODE>
+__device__ __forceinline__ float far_term(float x, double ref, const BeamSoftcap& c)
+{
+    const double v = value64<MODE>(x, c);
+    return v == ref ? 1.0f : pow2_of(fmax(v - ref, -1000.0));
 }
 
 /* Sum over the 64 lanes, in every lane (all lanes active). */
@@ -111,6 +116,7 @@ __device__ __forceinline__ double wave_sum_f64(double v)
     return v;
 }
 /* Sum over the workgroup, in thread 0. */
+template <int BLOCK>
 __device__ __forceinline__ double block_sum_f64(double v, double* s_wave)
 {
     v = wave_sum_f64(v);
@@ -119,95 +125,25 @@ __device__ __forceinline__ double block_sum_f64(double v, double* s_wave)
     double r = 0.0;
     if (threadIdx.x == 0)
 #pragma unroll
-        for (int w = 0; w < kB / 64; ++w) r += s_wave[w];
+        for (int w = 0; w < BLOCK / 64; ++w) r += s_wave[w];
     return r;
 }
 
-struct TopShared {
-    uint32_t tmax[kB];
+template <int BLOCK>
+struct SelectShared {
+    uint32_t tmax[BLOCK];
     uint32_t hist[256];
     int misc[8];
-    int scan[kB / 64];
-    double red[kB / 64];
+    int scan[BLOCK / 64];
+    double red[BLOCK / 64];
     int count;
     int flag;
-    alignas(16) uint64_t list[kListCap]; /* in any order */
+    int hit[2]; /* number of the last tile, odd and even, with a candidate above the floor */
+    uint32_t far[BLOCK / 64][kBeamMaxTiles / 32]; /* tiles that a wave left for later */
+    alignas(16) uint64_t list[kListCap]; /* candidates, in any order */
     alignas(16) uint64_t sorted[kNMax];
     double y[kNMax];
 };
-
-struct TopList {
-    int listed; /* entries of sh.list */
-    float top;  /* the largest candidate */
-};
-
-/* The workgroup's largest candidates into sh.list, at least the n best (n <= kNMax) or all
- * there are.  x: this thread's E logits, token(e) their tokens; entry(i),
- * i < count, reads all of them again, in an order that tokens of equal keys
- * rise in.
- *
- * The n-th largest of the threads' largest keys bounds the n-th largest key
- * from below, and for n well below the threads few elements beside the n best
- * reach it.  Where more reach it than the list holds (equal logits in
- * masses), the n-th largest key is selected exactly and of its copies the
- * first are taken; that way reads again what it needs, so that it costs the
- * usual one no registers. */
-template <int E, typename TokenF, typename EntryF>
-__device__ __forceinline__ TopList top_list(const float (&x)[E], float largest, TokenF token,
-                                            int count, EntryF entry, int n, TopShared& sh)
-{
-    const int tid = threadIdx.x, lane = tid & 63;
-    const uint32_t mkey = cand_key(largest);
-    sh.tmax[tid] = mkey;
-    if (tid == 0) sh.count = 0;
-    __syncthreads();
-    uint32_t v[kB / 64];
-    uint32_t top = 0u;
-    int nz = 0;
-#pragma unroll
-    for (int q = 0; q < kB / 64; ++q) {
-        v[q] = sh.tmax[lane + 64 * q];
-        top = v[q] > top ? v[q] : top;
-        nz += __popcll(__ballot(v[q] != 0u));
-    }
-    const uint32_t t = nz >= n ? wave_kth_bound<kB / 64>(v, n, 10) : 1u;
-    TopList r;
-    r.top = key2f(wave_max_u32(top));
-    const float bound = t <= 1u ? -__builtin_inff() : key2f(t);
-    if (mkey >= t && mkey != 0u) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (x[e] > kMasked && x[e] >= bound) {
-                const int p = atomicAdd(&sh.count, 1);
-                if (p < kListCap) sh.list[p] = entry_of(f2key(x[e]), token(e));
-            }
-    }
-    __syncthreads();
-    int cnt = sh.count;
-    if (cnt > kListCap) {
-        int gt, eq;
-        auto key = [&](int i) { return entry_key(entry(i)); };
-        const uint32_t kth = block_radix_kth<kB>(
-            count, n, key, [&](int i) { return key(i) != 0u; }, sh.hist, sh.misc, &gt, &eq);
-        if (tid == 0) sh.count = 0;
-        __syncthreads();
-        int taken = gt;
-#pragma unroll 1
-        for (int i0 = 0; i0 < count; i0 += kB) {
-            const uint64_t c = i0 + tid < count ? entry(i0 + tid) : 0ull;
-            if (entry_key(c) > kth) sh.list[atomicAdd(&sh.count, 1)] = c;
-            const int same = c != 0ull && entry_key(c) == kth;
-            int total;
-            const int p = taken + block_exclusive_scan<kB>(same, sh.scan, total);
-            if (same && p < n) sh.list[p] = c;
-            taken += total;
-        }
-        cnt = n;
-        __syncthreads();
-    }
-    r.listed = cnt;
-    return r;
-}
 
 /* How many of the list's entries are better than `mine`. */
 __device__ __forceinline__ int rank_in(const uint64_t* list, int cnt, uint64_t mine)
@@ -218,123 +154,420 @@ __device__ __forceinline__ int rank_in(const uint64_t* list, int cnt, uint64_t m
     return rank;
 }
 
+/* A lower bound of the n-th largest logit of the workgroup's tile, from the threads'
+ * largest ones: below kMasked where fewer than n threads hold a candidate. */
+template <int BLOCK>
+__device__ __forceinline__ float tile_bound(float largest, int n, SelectShared<BLOCK>& sh)
+{
+    const int lane = threadIdx.x & 63;
+    sh.tmax[threadIdx.x] = cand_key(largest);
+    __syncthreads();
+    uint32_t v[BLOCK / 64];
+    int nz = 0;
+#pragma unroll
+    for (int q = 0; q < BLOCK / 64; ++q) {
+        v[q] = sh.tmax[lane + 64 * q];
+        nz += __popcll(__ballot(v[q] != 0u));
+    }
+    const uint32_t t = nz >= n ? wave_kth_bound<BLOCK / 64>(v, n, 10) : 0u;
+    return t == 0u ? -__builtin_inff() : key2f(t);
+}
+
+/* The workgroup's best candidates so far: `listed` entries of sh.list, among
+ * them the n best (n <= kNMax) or all there are.  No later logit that is not above `floor`
+ * can be among the n best: n listed ones are at or above it, and of equal
+ * logits the earlier come first. */
+struct Best {
+    float floor = kMasked;
+    int listed = 0;
+    int tiles = 0;
+};
+
+/* A tile's candidates join the list.  x(e), e < E: this thread's logits, token(e)
+ * their tokens, `largest` the largest; entry(i), i < count: all of the tile's, in
+ * token order, read again.
+ *
+ * The first tile lists what reaches tile_bound, few elements beside the n
+ * best for n well below the threads; later ones what is above the floor.  If
+ * that is more than the list holds, the bound is used there too; if that
+ * is still more (equal logits in masses), the tile's n-th largest key is
+ * selected exactly and of its copies the first are taken.  A list that has
+ * grown is cut down to its n best, whose last is the new floor. */
+template <int BLOCK, int E, typename ValueF, typename TokenF, typename EntryF>
+__device__ __forceinline__ void list_tile(Best& best, float largest, ValueF x, TokenF token,
+                                          int count, EntryF entry, int n,
+                                          SelectShared<BLOCK>& sh)
+{
+    const int tid = threadIdx.x;
+    /* one barrier a tile: a word is written again two tiles later, when all
+     * threads are past the barrier in between and so have read it */
+    int* hit = &sh.hit[++best.tiles & 1];
+    if (largest > best.floor) *hit = best.tiles;
+    __syncthreads();
+    if (*hit != best.tiles) return;
+    float bound = -__builtin_inff();
+    auto append = [&] {
+        if (largest > best.floor && largest >= bound) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const float v = x(e);
+                if (v > best.floor && v >= bound) {
+                    const int p = atomicAdd(&sh.count, 1);
+                    if (p < kListCap) sh.list[p] = entry_of(f2key(v), token(e));
+                }
+            }
+        }
+    };
+    const bool first = best.listed == 0;
+    if (first) {
+        if (tid == 0) sh.count = 0;
+        bound = tile_bound<BLOCK>(largest, n, sh);
+    }
+    append();
+    __syncthreads();
+    int cnt = sh.count;
+    if (cnt > kListCap && !first) {
+        __syncthreads();
+        if (tid == 0) sh.count = best.listed;
+        bound = tile_bound<BLOCK>(largest, n, sh);
+        append();
+        __syncthreads();
+        cnt = sh.count;
+    }
+    if (cnt > kListCap) {
+        __syncthreads();
+        if (tid == 0) sh.count = best.listed;
+        auto key = [&](int i) {
+            const uint64_t c = entry(i);
+            return c && key2f(entry_key(c)) > best.floor ? entry_key(c) : 0u;
+        };
+        int gt, eq;
+        bound = key2f(block_radix_kth<BLOCK>(
+            count, n, key, [&](int i) { return key(i) != 0u; }, sh.hist, sh.misc, &gt, &eq));
+        const uint32_t kth = f2key(bound);
+        int taken = gt;
+#pragma unroll 1
+        for (int i0 = 0; i0 < count; i0 += BLOCK) {
+            const uint64_t c = i0 + tid < count ? entry(i0 + tid) : 0ull;
+            const uint32_t k = entry_key(c);
+            if (k > kth) sh.list[atomicAdd(&sh.count, 1)] = c;
+            const int same = c != 0ull && k == kth;
+            int total;
+            const int p = taken + block_exclusive_scan<BLOCK>(same, sh.scan, total);
+            if (same && p < n) sh.list[best.listed + p] = c;
+            taken += total;
+        }
+        __syncthreads();
+        if (tid == 0) sh.count = best.listed + n;
+        cnt = best.listed + n;
+    }
+    if (bound > best.floor) best.floor = bound;
+    if (cnt >= 2 * n + 32 || cnt > kListCap - kNMax) {
+        for (int i = tid; i < cnt; i += BLOCK) {
+            const uint64_t e = sh.list[i];
+            const int rank = rank_in(sh.list, cnt, e);
+            if (rank < n) sh.sorted[rank] = e;
+        }
+        __syncthreads();
+        cnt = n;
+        for (int i = tid; i < n; i += BLOCK) sh.list[i] = sh.sorted[i];
+        best.floor = key2f(entry_key(sh.sorted[n - 1]));
+        if (tid == 0) sh.count = n;
+    }
+    best.listed = cnt;
+}
+
 /* ------------------------------------------------------------------ chunks */
 
-/* Sum of N (2 or 4) terms: in binary32, which rounds twice at most; such sums are added
- * in binary64.  The polynomial and the split of its result run in binary64
- * because that costs what binary32 does on this machine, and binary32 would
- * leave errors of 1e-6 in the terms of equal logits, which many rows of bf16 have
- * thousands of. */
-template <int MODE, bool NEAR, bool MASK, int N>
-__device__ __forceinline__ double sum_few(const float* x, float top, double ref,
-                                          const BeamSoftcap& c)
+template <int MODE, int BLOCK>
+__device__ void merge_row(const BeamSelectArgs& a, int row, SelectShared<BLOCK>& sh);
+template <int BLOCK>
+__device__ void merge_sequence(const BeamSelectArgs& a, int b, SelectShared<BLOCK>& sh,
+                               double* sc);
+
+template <int DT>
+__device__ __forceinline__ u32x4 load_raw(const char* row, int64_t e0, int vocab)
 {
-    float t[N];
+    if (e0 + Elem<DT>::VW <= vocab)
+        return *reinterpret_cast<const u32x4*>(row + e0 * Elem<DT>::SIZE);
+    float v[Elem<DT>::VW];
 #pragma unroll
-    for (int q = 0; q < N; ++q) {
-        t[q] = term_of<MODE, NEAR>(x[q], top, ref, c);
-        if constexpr (MASK) t[q] = x[q] > kMasked ? t[q] : 0.0f;
-    }
-    if constexpr (N == 2)
-        return (double)(t[0] + t[1]);
-    else
-        return (double)((t[0] + t[1]) + (t[2] + t[3]));
+    for (int i = 0; i < Elem<DT>::VW; ++i)
+        v[i] = e0 + i < vocab ? load_elem<DT>(row, e0 + i) : -__builtin_inff();
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = DT == 0 ? __float_as_uint(v[i])
+                       : (__float_as_uint(v[2 * i % Elem<DT>::VW]) >> 16) |
+                             (__float_as_uint(v[(2 * i + 1) % Elem<DT>::VW]) & 0xFFFF0000u);
+    return r;
+}
+/* Element e of the vectors r. */
+template <int DT, int NV>
+__device__ __forceinline__ float raw_value(const u32x4 (&r)[NV], int e)
+{
+    if constexpr (DT == 0) return __uint_as_float(r[e / 4][e % 4]);
+    const uint32_t w = r[e / 8][e % 8 / 2];
+    return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
 }
 
-/* This thread's part of the chunk's sum.  Most waves hold no masked logit and none
- * beyond the polynomial; the others read their logits again (read(e), element
- * e) rather than hold them through the longer way. */
-template <int MODE, int E, typename ReadF>
-__device__ __forceinline__ double sum_terms(const float (&x)[E], float least, float largest,
-                                            float top, const BeamSoftcap& c, ReadF read)
+/* Sum of four terms: in binary32, which rounds twice; such sums are added in
+ * binary64. */
+__device__ __forceinline__ double sum_four(const float (&t)[4])
 {
-    const double ref = value64<MODE>(top, c);
-    const bool near = MODE == kCapNone || (least >= -c.limit && largest <= c.limit);
-    double s = 0.0;
-    if (MODE != kCapExact && __all(least > kMasked && near)) {
-#pragma unroll
-        for (int e = 0; e < E; e += 4) s += sum_few<MODE, true, false, 4>(&x[e], top, ref, c);
-        if (__all(s == s)) return s; /* a NaN is not seen by minimum and maximum */
-        s = 0.0;
-    }
-#pragma unroll 1
-    for (int e = 0; e < E; e += 2) {
-        const float v[2] = {read(e), read(e + 1)};
-        s += sum_few<MODE, false, true, 2>(v, top, ref, c);
-    }
-    return s;
+    return (double)((t[0] + t[1]) + (t[2] + t[3]));
 }
 
-/* One workgroup per chunk of kBeamChunk logits: its n best candidates, ranked, and its part of
- * the softmax denominator. */
-template <int MODE>
-__device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopShared& sh);
-__device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, TopShared& sh);
-
-template <int DT, int MODE>
-__global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
+/* One workgroup per chunk of a row, which it takes tile by tile, the next one
+ * loading while one is worked on: its n best candidates, ranked, and its part of the softmax
+ * denominator.
+ *
+ * A term is 2^v(x), v(x) = log2(e) cap tanh(x/cap), without a reference: the
+ * softcap keeps it within binary32 (so do logits within +-80 where there is
+ * no cap).  v is a polynomial evaluated in binary64, whose instructions
+ * issue as binary32's other than multiply-add do on this machine (4.7 against 2.7
+ * cycles measured), and its fraction alone goes through binary32's exponential:
+ * binary32 throughout leaves errors of 1e-6 in the terms of equal logits, and rows of
+ * bf16 have thousands of those.  bf16 logits of large batches need no
+ * arithmetic: their terms are looked up (TABLE), 30 KiB in LDS that hold the
+ * terms of all values from 2^-24 to 64.
+ *
+ * The workgroup that ends last in a row merges its chunks, the one that ends
+ * last in a sequence its rows. */
+template <int DT, int MODE, bool TABLE, int BLOCK>
+__global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamSelectArgs a)
 {
     constexpr int VW = Elem<DT>::VW;
-    constexpr int NV = kE / VW;
-    __shared__ TopShared sh;
+    constexpr int TILE = TABLE ? kBeamTableTile : kBeamTile;
+    constexpr int NV = TILE / BLOCK / VW;
+    constexpr int E = NV * VW;
+    extern __shared__ double dyn[]; /* terms; then the sequence's scores */
+    __shared__ SelectShared<BLOCK> sh;
     const int row = blockIdx.y, ch = blockIdx.x, tid = threadIdx.x;
     const int b = row / a.beams;
     const bool live = a.scores[row] > kMasked;
     if (live) {
         const char* base =
             static_cast<const char*>(a.logits) + (int64_t)row * a.row_stride * Elem<DT>::SIZE;
-        const int64_t first = (int64_t)ch * kBeamChunk;
-        float x[kE];
+        int first = ch * a.tiles * TILE; /* of the tile; chunks start within the row */
+        const int64_t stop = (int64_t)first + (int64_t)a.tiles * TILE;
+        const int end = stop < a.vocab ? (int)stop : a.vocab;
+        u32x4 r[NV];
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            float v[VW];
-            load_vec<DT>(base, first + (int64_t)(j * kB + tid) * VW, a.vocab, v);
-#pragma unroll
-            for (int i = 0; i < VW; ++i) x[j * VW + i] = v[i];
+        for (int j = 0; j < NV; ++j)
+            r[j] = load_raw<DT>(base, (int64_t)first + (j * BLOCK + tid) * VW, a.vocab);
+        if constexpr (TABLE) {
+            float* table = reinterpret_cast<float*>(dyn);
+            for (int i = tid; i < 2 * kBeamTableHalf / 4; i += BLOCK)
+                reinterpret_cast<u32x4*>(table)[i] = reinterpret_cast<const u32x4*>(a.ws.table)[i];
+            /* (complete behind the first tile's barrier) */
         }
-        const int rest = a.vocab - (int)first;
-        const int count = rest < kBeamChunk ? rest : kBeamChunk;
-        auto token = [&](int e) {
-            return (uint32_t)first + (uint32_t)(((e / VW) * kB + tid) * VW + e % VW);
-        };
-        auto read = [&](int e) {
-            const int64_t i = token(e);
-            return i < a.vocab ? load_elem<DT>(base, i) : -__builtin_inff();
-        };
-        auto entry = [&](int i) {
-            const uint32_t key = cand_key(load_elem<DT>(base, first + i));
-            return key ? entry_of(key, (uint32_t)first + (uint32_t)i) : 0ull;
-        };
-        float largest = x[0], least = x[0];
+        for (int i = tid & 63; i < kBeamMaxTiles / 32; i += 64) sh.far[tid / 64][i] = 0u;
+        if (tid < 2) sh.hit[tid] = 0;
+        __syncthreads();
+        Best best;
+        double s = 0.0;
+        bool redo = MODE == kCapExact;
+        for (int tile = 0; first < end; first += TILE, ++tile) {
+            u32x4 next[NV];
+            if (first + TILE < end) {
 #pragma unroll
-        for (int e = 1; e < kE; ++e) {
-            largest = fmaxf(largest, x[e]);
-            least = fminf(least, x[e]);
+                for (int j = 0; j < NV; ++j)
+                    next[j] = load_raw<DT>(base, (int64_t)first + TILE + (j * BLOCK + tid) * VW,
+                                           a.vocab);
+            }
+            auto value = [&](int e) { return raw_value<DT, NV>(r, e); };
+            auto offset = [&](int e) { return ((e / VW) * BLOCK + tid) * VW + e % VW; };
+            auto entry = [&](int i) {
+                const uint32_t key = cand_key(load_elem<DT>(base, (int64_t)first + i));
+                return key ? entry_of(key, (uint32_t)(first + i)) : 0ull;
+            };
+            float largest, least;
+            bool plain; /* every logit unmasked and within the way's limit */
+            if constexpr (TABLE) {
+                /* as 16-bit integers: the largest of the positive ones, the smallest
+                 * magnitude of negative ones alone, the largest magnitude */
+                i16x2 up = __builtin_bit_cast(i16x2, r[0][0]);
+                u16x2 low = __builtin_bit_cast(u16x2, r[0][0]), wide = low;
+#pragma unroll
+                for (int i = 1; i < 4 * NV; ++i) {
+                    const uint32_t w = r[i / 4][i % 4];
+                    up = __builtin_elementwise_max(up, __builtin_bit_cast(i16x2, w));
+                    low = __builtin_elementwise_min(low, __builtin_bit_cast(u16x2, w));
+                    wide = __builtin_elementwise_max(wide, __builtin_bit_cast(u16x2, w));
+                }
+                const int u = up.x > up.y ? up.x : up.y;
+                const uint32_t l = low.x < low.y ? low.x : low.y;
+                const uint32_t m = wide.x > wide.y ? wide.x : wide.y;
+                const uint32_t negative = m >> 15 ? m & 0x7FFFu : 0u;
+                const uint32_t most = u > (int)negative ? (uint32_t)u : negative;
+                largest = __uint_as_float((u >= 0 ? (uint32_t)u : l) << 16);
+                if (__any(most > 0x7F80u)) { /* NaNs */
+                    largest = value(0);
+#pragma unroll
+                    for (int e = 1; e < E; ++e) largest = fmaxf(largest, value(e));
+                }
+                plain = __all(most < (uint32_t)kBeamTableHigh);
+            } else {
+                largest = least = value(0);
+#pragma unroll
+                for (int e = 1; e < E; ++e) {
+                    largest = fmaxf(largest, value(e));
+                    least = fminf(least, value(e));
+                }
+                plain = __all(least >= -a.cap.limit && largest <= a.cap.limit);
+            }
+            const int count = a.vocab - first < TILE ? a.vocab - first : TILE;
+            list_tile<BLOCK, E>(
+                best, largest, value, [&](int e) { return (uint32_t)(first + offset(e)); }, count,
+                entry, a.n, sh);
+
+            if constexpr (MODE != kCapExact) {
+                /* most waves; then those with masked logits or NaNs (which minimum
+                 * and maximum do not see); then, behind the loop, so that
+                 * it costs the others no registers, those with logits beyond the limit */
+                double part = 0.0;
+                if constexpr (TABLE) {
+                    const char* table = reinterpret_cast<const char*>(dyn);
+                    if (plain) {
+#pragma unroll
+                        for (int i = 0; i < 4 * NV; i += 2) {
+                            float t[4];
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const uint32_t w = r[(i + q) / 4][(i + q) % 4];
+                                u16x2 m = __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu);
+                                const u16x2 neg =
+                                    __builtin_bit_cast(u16x2, (w >> 15) & 0x00010001u);
+                                m = __builtin_elementwise_max(m, (u16x2)kBeamTableLow);
+                                m = (m - (u16x2)kBeamTableLow + neg * (u16x2)kBeamTableHalf) << 2;
+                                const uint32_t at = __builtin_bit_cast(uint32_t, m);
+                                t[2 * q] = *reinterpret_cast<const float*>(table + (at & 0xFFFFu));
+                                t[2 * q + 1] = *reinterpret_cast<const float*>(table + (at >> 16));
+                            }
+                            part += sum_four(t);
+                        }
+                    } else {
+                        bool far = false;
+#pragma unroll
+                        for (int e = 0; e < E; e += 4) {
+                            float t[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) {
+                                const float v = value(e + q);
+                                const uint32_t bits = __float_as_uint(v) >> 16;
+                                uint32_t m = bits & 0x7FFFu;
+                                far |= v > kMasked && m >= (uint32_t)kBeamTableHigh;
+                                m = m < (uint32_t)kBeamTableLow ? kBeamTableLow : m;
+                                m = m >= (uint32_t)kBeamTableHigh ? kBeamTableHigh - 1 : m;
+                                m += (bits >> 15) * kBeamTableHalf - kBeamTableLow;
+                                const float u = *reinterpret_cast<const float*>(table + 4 * m);
+                                t[q] = v > kMasked ? u : 0.0f;
+                            }
+                            part += sum_four(t);
+                        }
+                        if (__any(far)) {
+                            part = 0.0;
+                            redo = true;
+                            if ((tid & 63) == 0) sh.far[tid / 64][tile / 32] |= 1u << (tile & 31);
+                        }
+                    }
+                } else {
+                    bool done = plain;
+                    if (done) {
+#pragma unroll
+                        for (int e = 0; e < E; e += 4) {
+                            float t[4];
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+                                t[q] = near_term<MODE>(value(e + q), a.cap);
+                            part += sum_four(t);
+                        }
+                        done = __all(part == part);
+                    }
+                    if (!done) {
+                        part = 0.0;
+                        least = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            least = fminf(least, value(e) > kMasked ? value(e) : 0.0f);
+                        if (__all(least >= -a.cap.limit && largest <= a.cap.limit)) {
+#pragma unroll
+                            for (int e = 0; e < E; e += 4) {
+                                float t[4];
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const float v = value(e + q);
+                                    t[q] = near_term<MODE>(v, a.cap);
+                                    t[q] = v > kMasked ? t[q] : 0.0f;
+                                }
+                                part += sum_four(t);
+                            }
+                        } else {
+                            redo = true;
+                            if ((tid & 63) == 0) sh.far[tid / 64][tile / 32] |= 1u << (tile & 31);
+                        }
+                    }
+                }
+                s += part;
+            }
+#pragma unroll
+            for (int j = 0; j < NV; ++j) r[j] = next[j];
         }
-        const TopList tl = top_list<kE>(x, largest, token, count, entry, a.n, sh);
+        if constexpr (MODE == kCapPoly) {
+            __syncthreads();
+#pragma unroll 1
+            for (int t = 0; t < a.tiles; ++t) {
+                if (!(sh.far[tid / 64][t / 32] >> (t & 31) & 1u)) continue;
+                const int64_t from = ((int64_t)ch * a.tiles + t) * TILE;
+#pragma unroll 1
+                for (int e = 0; e < E; ++e) {
+                    const int64_t i = from + ((e / VW) * BLOCK + tid) * VW + e % VW;
+                    const float v = i < a.vocab ? load_elem<DT>(base, i) : -__builtin_inff();
+                    if (v > kMasked) s += (double)far_term<MODE>(v, 0.0, a.cap);
+                }
+            }
+        }
+        __syncthreads();
         const int64_t at = (int64_t)row * a.chunks + ch;
         uint64_t* cand = a.ws.cand + at * a.n;
-        for (int i = tid; i < tl.listed; i += kB) {
+        const int listed = best.listed;
+        for (int i = tid; i < listed; i += BLOCK) {
             const uint64_t e = sh.list[i];
-            const int rank = rank_in(sh.list, tl.listed, e);
+            const int rank = rank_in(sh.list, listed, e);
             if (rank < a.n) st_dev(&cand[rank], e);
+            if (rank == 0) sh.sorted[0] = e;
         }
-        double s = 0.0;
-        if (tl.listed)
-            s = sum_terms<MODE, kE>(x, least, largest, tl.top, a.cap, read);
-        for (int i = tl.listed + tid; i < a.n; i += kB) st_dev(&cand[i], (uint64_t)0);
-        s = block_sum_f64(s, sh.red);
-        if (tid == 0) st_dev(&a.ws.sums[at], d2u(s));
+        for (int i = listed + tid; i < a.n; i += BLOCK) st_dev(&cand[i], (uint64_t)0);
+        double ref = 0.0;
+        if (MODE != kCapPoly && __syncthreads_or(redo && listed)) {
+            /* relative to the chunk's largest logit, in a second pass */
+            const float top = key2f(entry_key(sh.sorted[0]));
+            ref = value64<MODE>(top, a.cap);
+            s = 0.0;
+#pragma unroll 1
+            for (int i = ch * a.tiles * TILE + tid; i < end; i += BLOCK) {
+                const float v = load_elem<DT>(base, i);
+                if (v > kMasked)
+                    s += v == top ? 1.0 : (double)far_term<MODE>(v, ref, a.cap);
+            }
+        }
+        s = block_sum_f64<BLOCK>(s, sh.red);
+        if (tid == 0) {
+            st_dev(&a.ws.sums[2 * at], d2u(s));
+            st_dev(&a.ws.sums[2 * at + 1], d2u(ref));
+        }
         if (a.chunks > 1 && !elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
         if (a.chunks == 1) {
             __builtin_amdgcn_s_waitcnt(0);
             __syncthreads();
         }
-        merge_row<MODE>(a, row, sh);
+        merge_row<MODE, BLOCK>(a, row, sh);
     } else {
         if (ch != 0) return;
         if (tid == 0 && a.lse) a.lse[row] = -__builtin_inff();
-        for (int i = tid; i < a.n; i += kB) st_dev(&a.ws.best[(int64_t)row * a.n + i], (uint64_t)0);
+        for (int i = tid; i < a.n; i += BLOCK)
+            st_dev(&a.ws.best[(int64_t)row * a.n + i], (uint64_t)0);
     }
     if (a.beams > 1 &&
         !elect_last(&a.ws.tickets[a.batch * a.beams + b], (uint32_t)a.beams, &sh.flag))
@@ -343,63 +576,65 @@ __global__ __launch_bounds__(kB) void beam_select_kernel(BeamSelectArgs a)
         __builtin_amdgcn_s_waitcnt(0);
         __syncthreads();
     }
-    merge_sequence(a, b, sh);
+    merge_sequence<BLOCK>(a, b, sh, dyn);
 }
 
 /* -------------------------------------------------------------------- rows */
 
 /* A row's n best and its normaliser from its chunks'. */
-template <int MODE>
-__device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopShared& sh)
+template <int MODE, int BLOCK>
+__device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
+                                          SelectShared<BLOCK>& sh)
 {
     constexpr int E = 8;
     const int tid = threadIdx.x;
     const uint64_t* cand = a.ws.cand + (int64_t)row * a.chunks * a.n;
-    const int64_t total = (int64_t)a.chunks * a.n;
-    int cnt = 0;
-    /* tiles of candidates beside the best of those before; the chunks' lists
-     * lie in token order, so copies of one key do too */
-    for (int64_t base = 0; base < total;) {
-        const int64_t rest = cnt + total - base;
-        const int count = rest < E * kB ? (int)rest : E * kB;
-        auto entry = [&](int i) {
-            return i < cnt ? sh.sorted[i] : ld_dev(&cand[base + i - cnt]);
-        };
+    const int total = a.chunks * a.n;
+    if (tid < 2) sh.hit[tid] = 0;
+    __syncthreads();
+    Best best;
+    /* the chunks' lists lie in token order, so copies of one key do too */
+    for (int base = 0; base < total; base += E * BLOCK) {
+        const int count = total - base < E * BLOCK ? total - base : E * BLOCK;
+        auto entry = [&](int i) { return ld_dev(&cand[base + i]); };
         float x[E];
         uint32_t tok[E];
         float largest = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int i = e * kB + tid;
-            const uint64_t c = e * kB < count && i < count ? entry(i) : 0ull;
+            const int i = e * BLOCK + tid;
+            const uint64_t c = e * BLOCK < count && i < count ? entry(i) : 0ull;
             x[e] = c ? key2f(entry_key(c)) : -__builtin_inff();
             tok[e] = entry_token(c);
             largest = fmaxf(largest, x[e]);
         }
-        const TopList tl = top_list<E>(
-            x, largest, [&](int e) { return tok[e]; }, count, entry, a.n, sh);
-        base += count - cnt;
-        __syncthreads();
-        for (int i = tid; i < tl.listed; i += kB) {
-            const uint64_t e = sh.list[i];
-            const int rank = rank_in(sh.list, tl.listed, e);
-            if (rank < a.n) sh.sorted[rank] = e;
-        }
-        cnt = tl.listed < a.n ? tl.listed : a.n;
-        __syncthreads();
+        list_tile<BLOCK, E>(
+            best, largest, [&](int e) { return x[e]; }, [&](int e) { return tok[e]; }, count,
+            entry, a.n, sh);
     }
-    /* the chunks' sums relative to their largest logit, which leads each list */
-    const double top =
-        cnt ? softcap64<MODE>(key2f(entry_key(sh.sorted[0])), a.cap) : -__builtin_inf();
+    __syncthreads();
+    for (int i = tid; i < best.listed; i += BLOCK) {
+        const uint64_t e = sh.list[i];
+        const int rank = rank_in(sh.list, best.listed, e);
+        if (rank < a.n) sh.sorted[rank] = e;
+    }
+    const int cnt = best.listed < a.n ? best.listed : a.n;
+    __syncthreads();
+    /* the chunks' sums relative to the row's largest logit */
+    const float first = cnt ? key2f(entry_key(sh.sorted[0])) : 0.0f;
+    const double top = cnt ? softcap64<MODE>(first, a.cap) : -__builtin_inf();
+    const double vtop = value64<MODE>(first, a.cap);
     double s = 0.0;
-    for (int c = tid; c < a.chunks; c += kB) {
-        const uint64_t first = ld_dev(&cand[(int64_t)c * a.n]);
-        const double sum = u2d(ld_dev(&a.ws.sums[(int64_t)row * a.chunks + c]));
-        if (first) s += sum * term64(softcap64<MODE>(key2f(entry_key(first)), a.cap), top);
+    for (int c = tid; c < a.chunks; c += BLOCK) {
+        const int64_t at = (int64_t)row * a.chunks + c;
+        const double sum = u2d(ld_dev(&a.ws.sums[2 * at]));
+        const double ref = u2d(ld_dev(&a.ws.sums[2 * at + 1]));
+        if (sum > 0.0) s += sum * term64(ref * kLn2, vtop * kLn2);
     }
-    for (int i = tid; i < cnt; i += kB) sh.y[i] = softcap64<MODE>(key2f(entry_key(sh.sorted[i])), a.cap);
-    s = block_sum_f64(s, sh.red); /* (a barrier: y is complete) */
-    for (int i = tid; i < a.n; i += kB) {
+    for (int i = tid; i < cnt; i += BLOCK)
+        sh.y[i] = softcap64<MODE>(key2f(entry_key(sh.sorted[i])), a.cap);
+    s = block_sum_f64<BLOCK>(s, sh.red); /* (a barrier: y is complete) */
+    for (int i = tid; i < a.n; i += BLOCK) {
         uint64_t e = i < cnt ? sh.sorted[i] : 0ull;
         double y = -__builtin_inf();
         if (e) {
@@ -424,15 +659,17 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row, TopS
 
 /* The n best of the sequence's W sorted lists: a candidate's rank is the
  * number of better ones, found in each list by bisection. */
-__device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, TopShared& sh)
+template <int BLOCK>
+__device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b,
+                                               SelectShared<BLOCK>& sh, double* sc)
 {
-    extern __shared__ double sc[]; /* [W][n] scores, -inf = none */
+    /* sc: [W][n] scores, -inf = none */
     const int tid = threadIdx.x;
     const int W = a.beams, n = a.n, total = W * n;
     const uint64_t* best = a.ws.best + (int64_t)b * total;
     const uint64_t* ys = a.ws.y + (int64_t)b * total;
     int found = 0;
-    for (int i = tid; i < total; i += kB) {
+    for (int i = tid; i < total; i += BLOCK) {
         const int w = i / n;
         double s = -__builtin_inf();
         if (ld_dev(&best[i])) {
@@ -443,11 +680,11 @@ __device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, T
         }
         sc[i] = s;
     }
-    found = block_sum_i32<kB>(found, sh.scan);
+    found = block_sum_i32<BLOCK>(found, sh.scan);
     int32_t* parents = a.parents + (int64_t)b * n;
     int32_t* tokens = a.tokens + (int64_t)b * n;
     float* out = a.out + (int64_t)b * n;
-    for (int i = tid; i < total; i += kB) {
+    for (int i = tid; i < total; i += BLOCK) {
         const double s = sc[i];
         if (s == -__builtin_inf()) continue;
         const int w = i / n;
@@ -472,7 +709,7 @@ __device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b, T
             out[rank] = (float)s;
         }
     }
-    for (int i = found + tid; i < n; i += kB) {
+    for (int i = found + tid; i < n; i += BLOCK) {
         parents[i] = -1;
         tokens[i] = -1;
         out[i] = -__builtin_inff();
@@ -554,10 +791,11 @@ BeamSoftcap beam_softcap(float cap)
     c.cap = cap;
     if (!(cap > 0.0f)) {
         c.mode = kCapNone;
+        c.limit = 80.0f;
         return c;
     }
     const double d = (double)cap;
-    c.mode = cap >= 1e-12f && cap <= 128.0f ? kCapPoly : kCapExact;
+    c.mode = cap >= 1e-12f && cap <= 80.0f ? kCapPoly : kCapExact;
     double scale = kLog2e;
     for (int i = 0; i < 10; ++i) {
         c.q[i] = q[i] * scale;
@@ -567,25 +805,94 @@ BeamSoftcap beam_softcap(float cap)
     return c;
 }
 
-template <int DT>
-static void select_launch(const BeamSelectArgs& a, hipStream_t stream)
+namespace {
+
+template <int MODE>
+__global__ __launch_bounds__(kB) void beam_init_kernel(BeamWorkspace ws, BeamSoftcap cap,
+                                                       int tickets)
 {
-    const dim3 grid((unsigned)a.chunks, (unsigned)(a.batch * a.beams));
-    const size_t lds = sizeof(double) * a.beams * a.n;
-    if (a.cap.mode == kCapNone)
-        beam_select_kernel<DT, kCapNone><<<grid, kB, lds, stream>>>(a);
-    else if (a.cap.mode == kCapPoly)
-        beam_select_kernel<DT, kCapPoly><<<grid, kB, lds, stream>>>(a);
-    else
-        beam_select_kernel<DT, kCapExact><<<grid, kB, lds, stream>>>(a);
+    const int at = blockIdx.x * kB + threadIdx.x;
+    for (int i = at; i < tickets; i += gridDim.x * kB) ws.tickets[i] = 0u;
+    for (int i = at; i < 2 * kBeamTableHalf; i += gridDim.x * kB) {
+        const uint32_t mag = i % kBeamTableHalf;
+        const float x = mag ? __uint_as_float((mag + kBeamTableLow) << 16) : 0.0f;
+        const double y = softcap64<MODE>(i < kBeamTableHalf ? x : -x, cap);
+        ws.table[i] = (float)exp_fast_d(y);
+    }
 }
 
-hipError_t beam_select_launch(const BeamSelectArgs& a, int32_t dtype, hipStream_t stream)
+template <int DT, int MODE>
+void select_launch(const BeamSelectArgs& a, const BeamPlan& plan, hipStream_t stream)
 {
-    if (dtype == G4S_DTYPE_F32)
-        select_launch<0>(a, stream);
+    const dim3 grid((unsigned)a.chunks, (unsigned)(a.batch * a.beams));
+    const size_t scores = sizeof(double) * a.beams * a.n;
+    if constexpr (DT == 1 && MODE != kCapExact) {
+        if (plan.table) {
+            const size_t table = sizeof(float) * 2 * kBeamTableHalf;
+            beam_select_kernel<DT, MODE, true, 512>
+                <<<grid, 512, table > scores ? table : scores, stream>>>(a);
+            return;
+        }
+    }
+    beam_select_kernel<DT, MODE, false, kB><<<grid, kB, scores, stream>>>(a);
+}
+
+}  // namespace
+
+BeamPlan beam_plan(int32_t vocab, int32_t rows, int32_t dtype, int32_t mode, int32_t ncu)
+{
+    BeamPlan p{};
+    const int64_t big = (vocab + kBeamTableTile - 1) / kBeamTableTile;
+    p.table = dtype == G4S_DTYPE_BF16 && mode != kCapExact && rows * big >= 4 * (int64_t)ncu;
+    const int32_t tile = p.table ? kBeamTableTile : kBeamTile;
+    const int32_t all = (vocab + tile - 1) / tile;
+    /* a row's workgroups: the fewest tiles that some CU takes one after another, its workgroups
+     * side by side counted as if in turn from `full` on, where they fill it; the
+     * start and end of a workgroup cost about a tile */
+    const int64_t full = p.table ? 2 : 3;
+    int64_t least = INT64_MAX;
+    for (int32_t tiles = 1; tiles <= all; ++tiles) {
+        const int32_t chunks = (all + tiles - 1) / tiles;
+        if (chunks > 1 && (int64_t)rows * chunks > beam_max_chunks(vocab, rows, ncu)) continue;
+        int64_t each = ((int64_t)rows * chunks + ncu - 1) / ncu;
+        if (each < full) each = full;
+        const int64_t cost = each * (tiles + 1);
+        if (cost < least) {
+            least = cost;
+            p.chunks = chunks;
+            p.tiles = tiles;
+        }
+    }
+    return p;
+}
+
+int64_t beam_max_chunks(int32_t vocab, int32_t rows, int32_t ncu)
+{
+    const int64_t every = (int64_t)((vocab + kBeamTile - 1) / kBeamTile) * rows;
+    const int64_t most = (int64_t)8 * ncu > rows ? (int64_t)8 * ncu : rows;
+    return most < every ? most : every;
+}
+
+hipError_t beam_init_launch(const BeamWorkspace& ws, const BeamSoftcap& cap, int32_t tickets,
+                            hipStream_t stream)
+{
+    if (cap.mode == kCapNone)
+        beam_init_kernel<kCapNone><<<64, kB, 0, stream>>>(ws, cap, tickets);
     else
-        select_launch<1>(a, stream);
+        beam_init_kernel<kCapPoly><<<64, kB, 0, stream>>>(ws, cap, tickets);
+    return hipGetLastError();
+}
+
+hipError_t beam_select_launch(const BeamSelectArgs& a, const BeamPlan& plan, int32_t dtype,
+                              hipStream_t stream)
+{
+    const bool f32 = dtype == G4S_DTYPE_F32;
+    if (a.cap.mode == kCapNone)
+        f32 ? select_launch<0, kCapNone>(a, plan, stream) : select_launch<1, kCapNone>(a, plan, stream);
+    else if (a.cap.mode == kCapPoly)
+        f32 ? select_launch<0, kCapPoly>(a, plan, stream) : select_launch<1, kCapPoly>(a, plan, stream);
+    else
+        f32 ? select_launch<0, kCapExact>(a, plan, stream) : select_launch<1, kCapExact>(a, plan, stream);
     return hipGetLastError();
 }
 

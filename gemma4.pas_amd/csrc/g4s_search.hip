@@ -40,8 +40,10 @@ int fail_in(char (&buf)[512], int code, const char* fmt, va_list ap)
 }  // namespace
 
 struct g4s_beam : Handle {
-    int32_t vocab = 0, max_batch = 0, max_beams = 0, chunks = 0;
+    int32_t vocab = 0, max_batch = 0, max_beams = 0, ncu = 0;
     g4s::BeamSoftcap cap{};
+    int32_t plan_rows = 0, plan_dtype = 0; /* the last call's */
+    g4s::BeamPlan plan{};
     void* memory = nullptr;
     g4s::BeamWorkspace ws{};
 };
@@ -103,7 +105,7 @@ private:
 
 /* The current device, if the library runs on it. */
 template <typename H>
-int pick_device(H* none, int* device)
+int pick_device(H* none, int* device, int* ncu = nullptr)
 {
     int n = 0;
     if (hipGetDeviceCount(&n) != hipSuccess || n < 1)
@@ -115,6 +117,7 @@ int pick_device(H* none, int* device)
     if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0)
         return fail(none, G4S_ERR_NO_DEVICE, "device %d is %s; this library targets gfx950",
                     *device, prop.gcnArchName);
+    if (ncu) *ncu = prop.multiProcessorCount;
     return G4S_OK;
 }
 
@@ -180,27 +183,29 @@ G4S_API int g4s_beam_create(g4s_beam** out, int32_t vocab, int32_t max_batch, in
                     max_batch, max_beams, G4S_BEAM_MAX_ROWS);
     if (!std::isfinite(softcap))
         return fail(none, G4S_ERR_INVALID_ARGUMENT, "softcap %g is not finite", softcap);
-    int device = 0;
-    const int rc = pick_device(none, &device);
+    int device = 0, ncu = 0;
+    const int rc = pick_device(none, &device, &ncu);
     if (rc) return rc;
     g4s_beam* h = new (std::nothrow) g4s_beam();
     if (!h) return fail(none, G4S_ERR_OUT_OF_MEMORY, "host memory");
     h->device = device;
     h->stream = (hipStream_t)hip_stream;
+    h->ncu = ncu;
     h->vocab = vocab;
     h->max_batch = max_batch;
     h->max_beams = max_beams;
     h->cap = g4s::beam_softcap(softcap);
-    h->chunks = g4s::beam_chunks(vocab);
     const size_t rows = (size_t)max_batch * max_beams, n = 2 * (size_t)max_beams;
+    const size_t chunks = (size_t)g4s::beam_max_chunks(vocab, (int32_t)rows, ncu);
     Carver c;
     auto lay = [&] {
-        c.add(&h->ws.cand, rows * h->chunks * n);
-        c.add(&h->ws.sums, rows * h->chunks);
+        c.add(&h->ws.cand, chunks * n);
+        c.add(&h->ws.sums, chunks * 2);
         c.add(&h->ws.best, rows * n);
         c.add(&h->ws.y, rows * n);
         c.add(&h->ws.norm, rows * 2);
         c.add(&h->ws.tickets, rows + max_batch);
+        c.add(&h->ws.table, (size_t)2 * g4s::kBeamTableHalf);
     };
     lay();
     const size_t bytes = c.used();
@@ -211,8 +216,8 @@ G4S_API int g4s_beam_create(g4s_beam** out, int32_t vocab, int32_t max_batch, in
     }
     c.start(h->memory);
     lay();
-    hipError_t e = hipMemsetAsync(h->ws.tickets, 0, (rows + max_batch) * sizeof(uint32_t),
-                                  h->stream);
+    hipError_t e =
+        g4s::beam_init_launch(h->ws, h->cap, (int32_t)(rows + max_batch), h->stream);
     if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
     if (e != hipSuccess) {
         (void)hipFree(h->memory);
@@ -272,7 +277,13 @@ int select(g4s_beam* h, const void* d_logits, int32_t dtype, int64_t row_stride,
     a.batch = batch;
     a.beams = beams;
     a.n = n;
-    a.chunks = h->chunks;
+    if (h->plan_rows != batch * beams || h->plan_dtype != dtype) {
+        h->plan_rows = batch * beams;
+        h->plan_dtype = dtype;
+        h->plan = g4s::beam_plan(h->vocab, batch * beams, dtype, h->cap.mode, h->ncu);
+    }
+    a.chunks = h->plan.chunks;
+    a.tiles = h->plan.tiles;
     a.cap = h->cap;
     a.scores = d_scores;
     a.parents = d_parents;
@@ -280,7 +291,7 @@ int select(g4s_beam* h, const void* d_logits, int32_t dtype, int64_t row_stride,
     a.out = d_out;
     a.lse = d_lse;
     a.ws = h->ws;
-    const hipError_t e = g4s::beam_select_launch(a, dtype, h->stream);
+    const hipError_t e = g4s::beam_select_launch(a, h->plan, dtype, h->stream);
     return e == hipSuccess ? G4S_OK : hip_fail(h, e, "beam selection launch");
 }
 
