@@ -184,8 +184,8 @@ struct Best {
 };
 
 /* A tile's candidates join the list.  x(e), e < E: this thread's logits, token(e)
- * their tokens, `largest` the largest; entry(i), i < count: all of the tile's, in
- * token order, read again.
+ * their tokens; none is above `largest`, and one is `sure` or larger unless that is -inf;
+ * entry(i), i < count: all of the tile's, in token order, read again.
  *
  * The first tile lists what reaches tile_bound, few elements beside the n
  * best for n well below the threads; later ones what is above the floor.  If
@@ -194,7 +194,8 @@ struct Best {
  * selected exactly and of its copies the first are taken.  A list that has
  * grown is cut down to its n best, whose last is the new floor. */
 template <int BLOCK, int E, typename ValueF, typename TokenF, typename EntryF>
-__device__ __forceinline__ void list_tile(Best& best, float largest, ValueF x, TokenF token,
+__device__ __forceinline__ void list_tile(Best& best, float largest, float sure, ValueF x,
+                                          TokenF token,
                                           int count, EntryF entry, int n,
                                           SelectShared<BLOCK>& sh)
 {
@@ -207,21 +208,31 @@ __device__ __forceinline__ void list_tile(Best& best, float largest, ValueF x, T
     if (*hit != best.tiles) return;
     float bound = -__builtin_inff();
     auto append = [&] {
-        if (largest > best.floor && largest >= bound) {
+        if (!__any(largest > best.floor && largest >= bound)) return;
+        /* few elements pass: by eights, most of which no lane takes further (and
+         * one after another, or they would hold registers together) */
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const float v = x(e);
-                if (v > best.floor && v >= bound) {
-                    const int p = atomicAdd(&sh.count, 1);
-                    if (p < kListCap) sh.list[p] = entry_of(f2key(v), token(e));
+        for (int e0 = 0; e0 < E; e0 += 8) {
+            float m = x(e0);
+#pragma unroll
+            for (int e = e0 + 1; e < e0 + 8; ++e) m = fmaxf(m, x(e));
+            if (__any(m > best.floor && m >= bound)) {
+#pragma unroll
+                for (int e = e0; e < e0 + 8; ++e) {
+                    const float v = x(e);
+                    if (v > best.floor && v >= bound) {
+                        const int p = atomicAdd(&sh.count, 1);
+                        if (p < kListCap) sh.list[p] = entry_of(f2key(v), token(e));
+                    }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     const bool first = best.listed == 0;
     if (first) {
         if (tid == 0) sh.count = 0;
-        bound = tile_bound<BLOCK>(largest, n, sh);
+        bound = tile_bound<BLOCK>(sure, n, sh);
     }
     append();
     __syncthreads();
@@ -229,7 +240,7 @@ __device__ __forceinline__ void list_tile(Best& best, float largest, ValueF x, T
     if (cnt > kListCap && !first) {
         __syncthreads();
         if (tid == 0) sh.count = best.listed;
-        bound = tile_bound<BLOCK>(largest, n, sh);
+        bound = tile_bound<BLOCK>(sure, n, sh);
         append();
         __syncthreads();
         cnt = sh.count;
@@ -311,6 +322,17 @@ __device__ __forceinline__ float raw_value(const u32x4 (&r)[NV], int e)
     return __uint_as_float(e & 1 ? w & 0xFFFF0000u : w << 16);
 }
 
+typedef __attribute__((address_space(3))) const float LdsFloat;
+
+/* The vectors as new values: what was unpacked from them before is unpacked
+ * again rather than held in registers. */
+template <int NV>
+__device__ __forceinline__ void forget(u32x4 (&r)[NV])
+{
+#pragma unroll
+    for (int j = 0; j < NV; ++j) __asm__ volatile("" : "+v"(r[j]));
+}
+
 /* Sum of four terms: in binary32, which rounds twice; such sums are added in
  * binary64. */
 __device__ __forceinline__ double sum_four(const float (&t)[4])
@@ -382,7 +404,7 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                 const uint32_t key = cand_key(load_elem<DT>(base, (int64_t)first + i));
                 return key ? entry_of(key, (uint32_t)(first + i)) : 0ull;
             };
-            float largest, least;
+            float largest, sure, least;
             bool plain; /* every logit unmasked and within the way's limit */
             if constexpr (TABLE) {
                 /* as 16-bit integers: the largest of the positive ones, the smallest
@@ -401,11 +423,10 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                 const uint32_t m = wide.x > wide.y ? wide.x : wide.y;
                 const uint32_t negative = m >> 15 ? m & 0x7FFFu : 0u;
                 const uint32_t most = u > (int)negative ? (uint32_t)u : negative;
-                largest = __uint_as_float((u >= 0 ? (uint32_t)u : l) << 16);
-                if (__any(most > 0x7F80u)) { /* NaNs */
-                    largest = value(0);
-#pragma unroll
-                    for (int e = 1; e < E; ++e) largest = fmaxf(largest, value(e));
+                largest = sure = __uint_as_float((u >= 0 ? (uint32_t)u : l) << 16);
+                if (most > 0x7F80u) { /* a NaN: nothing known */
+                    largest = __builtin_inff();
+                    sure = -__builtin_inff();
                 }
                 plain = __all(most < (uint32_t)kBeamTableHigh);
             } else {
@@ -415,12 +436,15 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                     largest = fmaxf(largest, value(e));
                     least = fminf(least, value(e));
                 }
+                sure = largest;
                 plain = __all(least >= -a.cap.limit && largest <= a.cap.limit);
             }
+            if constexpr (DT == 1) forget(r);
             const int count = a.vocab - first < TILE ? a.vocab - first : TILE;
             list_tile<BLOCK, E>(
-                best, largest, value, [&](int e) { return (uint32_t)(first + offset(e)); }, count,
+                best, largest, sure, value, [&](int e) { return (uint32_t)(first + offset(e)); }, count,
                 entry, a.n, sh);
+            if constexpr (DT == 1) forget(r);
 
             if constexpr (MODE != kCapExact) {
                 /* most waves; then those with masked logits or NaNs (which minimum
@@ -428,24 +452,33 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                  * it costs the others no registers, those with logits beyond the limit */
                 double part = 0.0;
                 if constexpr (TABLE) {
-                    const char* table = reinterpret_cast<const char*>(dyn);
+                    const uint32_t table = (uint32_t)(uintptr_t)(LdsFloat*)dyn;
                     if (plain) {
+                        u16x2 four = (u16x2)4;
+                        const u16x2 start = (u16x2)(uint16_t)(table - 4 * kBeamTableLow);
+                        __asm__("" : "+v"(four)); /* multiplied and added at once */
 #pragma unroll
                         for (int i = 0; i < 4 * NV; i += 2) {
                             float t[4];
 #pragma unroll
                             for (int q = 0; q < 2; ++q) {
+                                /* byte addresses modulo 2^16, where the parts may
+                                 * overflow: 4 (max(magnitude, low) - low) + table, and
+                                 * half the table further where negative */
                                 const uint32_t w = r[(i + q) / 4][(i + q) % 4];
                                 u16x2 m = __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu);
-                                const u16x2 neg =
-                                    __builtin_bit_cast(u16x2, (w >> 15) & 0x00010001u);
+                                u16x2 neg = __builtin_bit_cast(
+                                    u16x2, __builtin_bit_cast(i16x2, w) >> 15);
+                                __asm__("" : "+v"(neg)); /* a factor, no selection */
                                 m = __builtin_elementwise_max(m, (u16x2)kBeamTableLow);
-                                m = (m - (u16x2)kBeamTableLow + neg * (u16x2)kBeamTableHalf) << 2;
+                                m = m * four + start;
+                                m = neg * (u16x2)(uint16_t)(-4 * kBeamTableHalf) + m;
                                 const uint32_t at = __builtin_bit_cast(uint32_t, m);
-                                t[2 * q] = *reinterpret_cast<const float*>(table + (at & 0xFFFFu));
-                                t[2 * q + 1] = *reinterpret_cast<const float*>(table + (at >> 16));
+                                t[2 * q] = *(LdsFloat*)(uintptr_t)(at & 0xFFFFu);
+                                t[2 * q + 1] = *(LdsFloat*)(uintptr_t)(at >> 16);
                             }
                             part += sum_four(t);
+                            if (i % 4 == 2) __builtin_amdgcn_sched_barrier(0);
                         }
                     } else {
                         bool far = false;
@@ -461,10 +494,11 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                                 m = m < (uint32_t)kBeamTableLow ? kBeamTableLow : m;
                                 m = m >= (uint32_t)kBeamTableHigh ? kBeamTableHigh - 1 : m;
                                 m += (bits >> 15) * kBeamTableHalf - kBeamTableLow;
-                                const float u = *reinterpret_cast<const float*>(table + 4 * m);
+                                const float u = *(LdsFloat*)(uintptr_t)(table + 4 * m);
                                 t[q] = v > kMasked ? u : 0.0f;
                             }
                             part += sum_four(t);
+                            __builtin_amdgcn_sched_barrier(0);
                         }
                         if (__any(far)) {
                             part = 0.0;
@@ -609,7 +643,7 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
             largest = fmaxf(largest, x[e]);
         }
         list_tile<BLOCK, E>(
-            best, largest, [&](int e) { return x[e]; }, [&](int e) { return tok[e]; }, count,
+            best, largest, largest, [&](int e) { return x[e]; }, [&](int e) { return tok[e]; }, count,
             entry, a.n, sh);
     }
     __syncthreads();
