@@ -136,9 +136,8 @@ struct SelectShared {
     int misc[8];
     int scan[BLOCK / 64];
     double red[BLOCK / 64];
-    int count;
+    int count[3]; /* candidates that a tile listed, the tiles in turn */
     int flag;
-    int hit[2]; /* number of the last tile, odd and even, with a candidate above the floor */
     uint32_t far[BLOCK / 64][kBeamMaxTiles / 32]; /* tiles that a wave left for later */
     alignas(16) uint64_t list[kListCap]; /* candidates, in any order */
     alignas(16) uint64_t sorted[kNMax];
@@ -155,13 +154,11 @@ __device__ __forceinline__ int rank_in(const uint64_t* list, int cnt, uint64_t m
 }
 
 /* A lower bound of the n-th largest logit of the workgroup's tile, from the threads'
- * largest ones: below kMasked where fewer than n threads hold a candidate. */
+ * largest keys in sh.tmax: -inf where fewer than n threads hold a candidate. */
 template <int BLOCK>
-__device__ __forceinline__ float tile_bound(float largest, int n, SelectShared<BLOCK>& sh)
+__device__ __forceinline__ float tile_bound(int n, SelectShared<BLOCK>& sh)
 {
     const int lane = threadIdx.x & 63;
-    sh.tmax[threadIdx.x] = cand_key(largest);
-    __syncthreads();
     uint32_t v[BLOCK / 64];
     int nz = 0;
 #pragma unroll
@@ -179,36 +176,35 @@ __device__ __forceinline__ float tile_bound(float largest, int n, SelectShared<B
  * logits the earlier come first. */
 struct Best {
     float floor = kMasked;
+    float before = kMasked; /* the floor before the last tile */
     int listed = 0;
-    int tiles = 0;
+    int tile = 0;
 };
 
-/* A tile's candidates join the list.  x(e), e < E: this thread's logits, token(e)
- * their tokens; none is above `largest`, and one is `sure` or larger unless that is -inf;
- * entry(i), i < count: all of the tile's, in token order, read again.
+/* A tile's candidates join the list; a barrier a tile.  x(e), e < E: this thread's
+ * logits, token(e) their tokens; none is above `largest`, and one is `sure` or
+ * larger unless that is -inf.
  *
  * The first tile lists what reaches tile_bound, few elements beside the n
- * best for n well below the threads; later ones what is above the floor.  If
- * that is more than the list holds, the bound is used there too; if that
- * is still more (equal logits in masses), the tile's n-th largest key is
- * selected exactly and of its copies the first are taken.  A list that has
- * grown is cut down to its n best, whose last is the new floor. */
-template <int BLOCK, int E, typename ValueF, typename TokenF, typename EntryF>
+ * best for n well below the threads; later ones what is above the floor, and
+ * where more lanes than n hold such, what reaches their wave's n-th lane.  The
+ * count of a tile is looked at behind the next one's barrier (list_settle), so
+ * its word must stay until the one after. */
+template <int BLOCK, int E, typename ValueF, typename TokenF>
 __device__ __forceinline__ void list_tile(Best& best, float largest, float sure, ValueF x,
-                                          TokenF token,
-                                          int count, EntryF entry, int n,
-                                          SelectShared<BLOCK>& sh)
+                                          TokenF token, int n, SelectShared<BLOCK>& sh)
 {
-    const int tid = threadIdx.x;
-    /* one barrier a tile: a word is written again two tiles later, when all
-     * threads are past the barrier in between and so have read it */
-    int* hit = &sh.hit[++best.tiles & 1];
-    if (largest > best.floor) *hit = best.tiles;
-    __syncthreads();
-    if (*hit != best.tiles) return;
+    const int at = best.tile % 3;
+    if (threadIdx.x == 0) sh.count[(best.tile + 1) % 3] = 0;
+    best.before = best.floor;
     float bound = -__builtin_inff();
-    auto append = [&] {
-        if (!__any(largest > best.floor && largest >= bound)) return;
+    if (best.tile == 0) {
+        bound = tile_bound<BLOCK>(n, sh);
+    } else if (__popcll(__ballot(sure > best.floor)) > n) {
+        const uint32_t key[1] = {cand_key(sure)};
+        bound = key2f(wave_kth_bound<1>(key, n, 10));
+    }
+    if (__any(largest > best.floor && largest >= bound)) {
         /* few elements pass: by eights, most of which no lane takes further (and
          * one after another, or they would hold registers together) */
 #pragma unroll
@@ -221,58 +217,56 @@ __device__ __forceinline__ void list_tile(Best& best, float largest, float sure,
                 for (int e = e0; e < e0 + 8; ++e) {
                     const float v = x(e);
                     if (v > best.floor && v >= bound) {
-                        const int p = atomicAdd(&sh.count, 1);
+                        const int p = best.listed + atomicAdd(&sh.count[at], 1);
                         if (p < kListCap) sh.list[p] = entry_of(f2key(v), token(e));
                     }
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
         }
-    };
-    const bool first = best.listed == 0;
-    if (first) {
-        if (tid == 0) sh.count = 0;
-        bound = tile_bound<BLOCK>(sure, n, sh);
     }
-    append();
-    __syncthreads();
-    int cnt = sh.count;
-    if (cnt > kListCap && !first) {
-        __syncthreads();
-        if (tid == 0) sh.count = best.listed;
-        bound = tile_bound<BLOCK>(sure, n, sh);
-        append();
-        __syncthreads();
-        cnt = sh.count;
-    }
+    if (best.tile == 0 && bound > best.floor) best.floor = bound;
+    ++best.tile;
+}
+
+/* Behind a barrier, after a tile: entry(i), i < count, are all of its candidates, in token
+ * order, read again.  Where they were more than the list holds (equal logits
+ * in masses), the tile's n-th largest key is selected exactly and of its
+ * copies the first are taken.  A list that has grown is cut down to its n
+ * best, whose last is the new floor. */
+template <int BLOCK, typename EntryF>
+__device__ __forceinline__ void list_settle(Best& best, int count, EntryF entry, int n,
+                                            SelectShared<BLOCK>& sh)
+{
+    const int tid = threadIdx.x;
+    int* word = &sh.count[(best.tile - 1) % 3];
+    int cnt = best.listed + *word;
     if (cnt > kListCap) {
         __syncthreads();
-        if (tid == 0) sh.count = best.listed;
+        if (tid == 0) *word = 0;
         auto key = [&](int i) {
             const uint64_t c = entry(i);
-            return c && key2f(entry_key(c)) > best.floor ? entry_key(c) : 0u;
+            return c && key2f(entry_key(c)) > best.before ? entry_key(c) : 0u;
         };
         int gt, eq;
-        bound = key2f(block_radix_kth<BLOCK>(
-            count, n, key, [&](int i) { return key(i) != 0u; }, sh.hist, sh.misc, &gt, &eq));
-        const uint32_t kth = f2key(bound);
+        const uint32_t kth = block_radix_kth<BLOCK>(
+            count, n, key, [&](int i) { return key(i) != 0u; }, sh.hist, sh.misc, &gt, &eq);
         int taken = gt;
 #pragma unroll 1
         for (int i0 = 0; i0 < count; i0 += BLOCK) {
             const uint64_t c = i0 + tid < count ? entry(i0 + tid) : 0ull;
             const uint32_t k = entry_key(c);
-            if (k > kth) sh.list[atomicAdd(&sh.count, 1)] = c;
+            if (k > kth) sh.list[best.listed + atomicAdd(word, 1)] = c;
             const int same = c != 0ull && k == kth;
             int total;
             const int p = taken + block_exclusive_scan<BLOCK>(same, sh.scan, total);
             if (same && p < n) sh.list[best.listed + p] = c;
             taken += total;
         }
-        __syncthreads();
-        if (tid == 0) sh.count = best.listed + n;
+        best.floor = key2f(kth);
         cnt = best.listed + n;
+        __syncthreads();
     }
-    if (bound > best.floor) best.floor = bound;
     if (cnt >= 2 * n + 32 || cnt > kListCap - kNMax) {
         for (int i = tid; i < cnt; i += BLOCK) {
             const uint64_t e = sh.list[i];
@@ -283,15 +277,30 @@ __device__ __forceinline__ void list_tile(Best& best, float largest, float sure,
         cnt = n;
         for (int i = tid; i < n; i += BLOCK) sh.list[i] = sh.sorted[i];
         best.floor = key2f(entry_key(sh.sorted[n - 1]));
-        if (tid == 0) sh.count = n;
     }
     best.listed = cnt;
+}
+
+/* The list's n best into sh.sorted (behind a barrier); returns how many. */
+template <int BLOCK>
+__device__ __forceinline__ int list_sort(const Best& best, int n, SelectShared<BLOCK>& sh)
+{
+    for (int i = threadIdx.x; i < best.listed; i += BLOCK) {
+        const uint64_t e = sh.list[i];
+        const int rank = rank_in(sh.list, best.listed, e);
+        if (rank < n) sh.sorted[rank] = e;
+    }
+    __syncthreads();
+    return best.listed < n ? best.listed : n;
 }
 
 /* ------------------------------------------------------------------ chunks */
 
 template <int MODE, int BLOCK>
 __device__ void merge_row(const BeamSelectArgs& a, int row, SelectShared<BLOCK>& sh);
+template <int MODE, int BLOCK>
+__device__ void end_row(const BeamSelectArgs& a, int row, int cnt, double sum,
+                        SelectShared<BLOCK>& sh);
 template <int BLOCK>
 __device__ void merge_sequence(const BeamSelectArgs& a, int b, SelectShared<BLOCK>& sh,
                                double* sc);
@@ -357,7 +366,7 @@ __device__ __forceinline__ double sum_four(const float (&t)[4])
  * The workgroup that ends last in a row merges its chunks, the one that ends
  * last in a sequence its rows. */
 template <int DT, int MODE, bool TABLE, int BLOCK>
-__global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamSelectArgs a)
+__global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
 {
     constexpr int VW = Elem<DT>::VW;
     constexpr int TILE = TABLE ? kBeamTableTile : kBeamTile;
@@ -385,11 +394,20 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
             /* (complete behind the first tile's barrier) */
         }
         for (int i = tid & 63; i < kBeamMaxTiles / 32; i += 64) sh.far[tid / 64][i] = 0u;
-        if (tid < 2) sh.hit[tid] = 0;
-        __syncthreads();
+        if (tid < 3) sh.count[tid] = 0;
         Best best;
         double s = 0.0;
         bool redo = MODE == kCapExact;
+        /* the tile at `from` is all listed */
+        auto settle = [&](int from) {
+            list_settle<BLOCK>(
+                best, a.vocab - from < TILE ? a.vocab - from : TILE,
+                [&](int i) {
+                    const uint32_t key = cand_key(load_elem<DT>(base, (int64_t)from + i));
+                    return key ? entry_of(key, (uint32_t)(from + i)) : 0ull;
+                },
+                a.n, sh);
+        };
         for (int tile = 0; first < end; first += TILE, ++tile) {
             u32x4 next[NV];
             if (first + TILE < end) {
@@ -400,10 +418,6 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
             }
             auto value = [&](int e) { return raw_value<DT, NV>(r, e); };
             auto offset = [&](int e) { return ((e / VW) * BLOCK + tid) * VW + e % VW; };
-            auto entry = [&](int i) {
-                const uint32_t key = cand_key(load_elem<DT>(base, (int64_t)first + i));
-                return key ? entry_of(key, (uint32_t)(first + i)) : 0ull;
-            };
             float largest, sure, least;
             bool plain; /* every logit unmasked and within the way's limit */
             if constexpr (TABLE) {
@@ -440,10 +454,12 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
                 plain = __all(least >= -a.cap.limit && largest <= a.cap.limit);
             }
             if constexpr (DT == 1) forget(r);
-            const int count = a.vocab - first < TILE ? a.vocab - first : TILE;
+            if (tile == 0) sh.tmax[tid] = cand_key(sure);
+            __syncthreads();
+            if (tile > 0) settle(first - TILE);
             list_tile<BLOCK, E>(
-                best, largest, sure, value, [&](int e) { return (uint32_t)(first + offset(e)); }, count,
-                entry, a.n, sh);
+                best, largest, sure, value, [&](int e) { return (uint32_t)(first + offset(e)); },
+                a.n, sh);
             if constexpr (DT == 1) forget(r);
 
             if constexpr (MODE != kCapExact) {
@@ -563,18 +579,11 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
             }
         }
         __syncthreads();
-        const int64_t at = (int64_t)row * a.chunks + ch;
-        uint64_t* cand = a.ws.cand + at * a.n;
-        const int listed = best.listed;
-        for (int i = tid; i < listed; i += BLOCK) {
-            const uint64_t e = sh.list[i];
-            const int rank = rank_in(sh.list, listed, e);
-            if (rank < a.n) st_dev(&cand[rank], e);
-            if (rank == 0) sh.sorted[0] = e;
-        }
-        for (int i = listed + tid; i < a.n; i += BLOCK) st_dev(&cand[i], (uint64_t)0);
+        settle(first - TILE);
+        __syncthreads();
+        const int cnt = list_sort<BLOCK>(best, a.n, sh);
         double ref = 0.0;
-        if (MODE != kCapPoly && __syncthreads_or(redo && listed)) {
+        if (MODE != kCapPoly && __syncthreads_or(redo && cnt)) {
             /* relative to the chunk's largest logit, in a second pass */
             const float top = key2f(entry_key(sh.sorted[0]));
             ref = value64<MODE>(top, a.cap);
@@ -587,16 +596,22 @@ __global__ __launch_bounds__(BLOCK, TABLE ? 4 : 5) void beam_select_kernel(BeamS
             }
         }
         s = block_sum_f64<BLOCK>(s, sh.red);
-        if (tid == 0) {
-            st_dev(&a.ws.sums[2 * at], d2u(s));
-            st_dev(&a.ws.sums[2 * at + 1], d2u(ref));
-        }
-        if (a.chunks > 1 && !elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
         if (a.chunks == 1) {
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
+            if (cnt)
+                s *= term64(ref * kLn2,
+                            value64<MODE>(key2f(entry_key(sh.sorted[0])), a.cap) * kLn2);
+            end_row<MODE, BLOCK>(a, row, cnt, s, sh);
+        } else {
+            const int64_t at = (int64_t)row * a.chunks + ch;
+            for (int i = tid; i < a.n; i += BLOCK)
+                st_dev(&a.ws.cand[at * a.n + i], i < cnt ? sh.sorted[i] : (uint64_t)0);
+            if (tid == 0) {
+                st_dev(&a.ws.sums[2 * at], d2u(s));
+                st_dev(&a.ws.sums[2 * at + 1], d2u(ref));
+            }
+            if (!elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
+            merge_row<MODE, BLOCK>(a, row, sh);
         }
-        merge_row<MODE, BLOCK>(a, row, sh);
     } else {
         if (ch != 0) return;
         if (tid == 0 && a.lse) a.lse[row] = -__builtin_inff();
@@ -624,40 +639,41 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
     const int tid = threadIdx.x;
     const uint64_t* cand = a.ws.cand + (int64_t)row * a.chunks * a.n;
     const int total = a.chunks * a.n;
-    if (tid < 2) sh.hit[tid] = 0;
-    __syncthreads();
+    if (tid < 3) sh.count[tid] = 0;
     Best best;
+    int base = 0;
     /* the chunks' lists lie in token order, so copies of one key do too */
-    for (int base = 0; base < total; base += E * BLOCK) {
-        const int count = total - base < E * BLOCK ? total - base : E * BLOCK;
-        auto entry = [&](int i) { return ld_dev(&cand[base + i]); };
+    auto count = [&](int from) { return total - from < E * BLOCK ? total - from : E * BLOCK; };
+    auto settle = [&](int from) {
+        list_settle<BLOCK>(
+            best, count(from), [&](int i) { return ld_dev(&cand[from + i]); }, a.n, sh);
+    };
+    for (; base < total; base += E * BLOCK) {
         float x[E];
         uint32_t tok[E];
         float largest = -__builtin_inff();
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int i = e * BLOCK + tid;
-            const uint64_t c = e * BLOCK < count && i < count ? entry(i) : 0ull;
+            const uint64_t c =
+                e * BLOCK < count(base) && i < count(base) ? ld_dev(&cand[base + i]) : 0ull;
             x[e] = c ? key2f(entry_key(c)) : -__builtin_inff();
             tok[e] = entry_token(c);
             largest = fmaxf(largest, x[e]);
         }
+        if (base == 0) sh.tmax[tid] = cand_key(largest);
+        __syncthreads();
+        if (base) settle(base - E * BLOCK);
         list_tile<BLOCK, E>(
-            best, largest, largest, [&](int e) { return x[e]; }, [&](int e) { return tok[e]; }, count,
-            entry, a.n, sh);
+            best, largest, largest, [&](int e) { return x[e]; }, [&](int e) { return tok[e]; },
+            a.n, sh);
     }
     __syncthreads();
-    for (int i = tid; i < best.listed; i += BLOCK) {
-        const uint64_t e = sh.list[i];
-        const int rank = rank_in(sh.list, best.listed, e);
-        if (rank < a.n) sh.sorted[rank] = e;
-    }
-    const int cnt = best.listed < a.n ? best.listed : a.n;
+    settle(base - E * BLOCK);
     __syncthreads();
+    const int cnt = list_sort<BLOCK>(best, a.n, sh);
     /* the chunks' sums relative to the row's largest logit */
-    const float first = cnt ? key2f(entry_key(sh.sorted[0])) : 0.0f;
-    const double top = cnt ? softcap64<MODE>(first, a.cap) : -__builtin_inf();
-    const double vtop = value64<MODE>(first, a.cap);
+    const double vtop = cnt ? value64<MODE>(key2f(entry_key(sh.sorted[0])), a.cap) : 0.0;
     double s = 0.0;
     for (int c = tid; c < a.chunks; c += BLOCK) {
         const int64_t at = (int64_t)row * a.chunks + c;
@@ -665,15 +681,27 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
         const double ref = u2d(ld_dev(&a.ws.sums[2 * at + 1]));
         if (sum > 0.0) s += sum * term64(ref * kLn2, vtop * kLn2);
     }
+    end_row<MODE, BLOCK>(a, row, cnt, block_sum_f64<BLOCK>(s, sh.red), sh);
+}
+
+/* The row's cnt best candidates in sh.sorted; sum, in thread 0: its terms relative to the
+ * largest. */
+template <int MODE, int BLOCK>
+__device__ __forceinline__ void end_row(const BeamSelectArgs& a, int row, int cnt, double sum,
+                                        SelectShared<BLOCK>& sh)
+{
+    const int tid = threadIdx.x;
     for (int i = tid; i < cnt; i += BLOCK)
         sh.y[i] = softcap64<MODE>(key2f(entry_key(sh.sorted[i])), a.cap);
-    s = block_sum_f64<BLOCK>(s, sh.red); /* (a barrier: y is complete) */
+    __syncthreads();
+    const double top = cnt ? sh.y[0] : -__builtin_inf();
     for (int i = tid; i < a.n; i += BLOCK) {
         uint64_t e = i < cnt ? sh.sorted[i] : 0ull;
         double y = -__builtin_inf();
         if (e) {
             /* where tanh saturates its last bit may waver: the list may not rise */
             y = top;
+#pragma unroll 8
             for (int j = 1; j <= i; ++j) y = fmin(y, sh.y[j]);
             /* beside an infinite largest logit the rest have probability 0 */
             if (top == __builtin_inf() && y != top) e = 0ull;
@@ -682,7 +710,7 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
         st_dev(&a.ws.y[(int64_t)row * a.n + i], d2u(y));
     }
     if (tid == 0) {
-        const double ls = log64(s);
+        const double ls = log64(sum);
         st_dev(&a.ws.norm[2 * row], d2u(top));
         st_dev(&a.ws.norm[2 * row + 1], d2u(ls));
         if (a.lse) a.lse[row] = cnt ? (float)(top + ls) : -__builtin_inff();
