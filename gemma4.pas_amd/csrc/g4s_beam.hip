@@ -813,7 +813,8 @@ __global__ __launch_bounds__(kB) void beam_reorder_kernel(BeamReorderArgs a)
                 const bool ok = p >= 0 && p < W;
                 const int from = ok ? p : r;
                 if (!inplace || from != r)
-                    *reinterpret_cast<T*>(a.dst + at + (int64_t)r * a.row_stride) = v[r];
+                    __builtin_nontemporal_store(
+                        v[r], reinterpret_cast<T*>(a.dst + at + (int64_t)r * a.row_stride));
             }
     }
 }

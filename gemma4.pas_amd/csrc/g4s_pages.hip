@@ -279,7 +279,8 @@ __device__ __forceinline__ void copy_segment(const g4s_page_geometry& g, const c
     for (int q = 0; q < kCopyItems; ++q) {
         const uint32_t i = i0 + q * kB;
         if (i < total)
-            *reinterpret_cast<T*>(dst + page_offset(g, plane, job.dst, 0, 1, 0) + off[q]) = v[q];
+            __builtin_nontemporal_store(
+                v[q], reinterpret_cast<T*>(dst + page_offset(g, plane, job.dst, 0, 1, 0) + off[q]));
     }
 }
 
@@ -414,7 +415,7 @@ uint64_t copy_bits(const g4s_page_geometry& g, const void* src, const void* dst)
            (uint64_t)g.plane_stride | (uint64_t)g.page_stride;
 }
 
-constexpr int kMaxGrid = 2048; /* 8 workgroups per CU */
+constexpr int kMaxGrid = 1 << 20;
 
 template <typename T>
 unsigned copy_grid(const g4s_page_geometry& g, int64_t jobs, int64_t other)
