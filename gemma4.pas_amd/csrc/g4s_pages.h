@@ -18,7 +18,6 @@
 
 namespace g4s {
 
-constexpr int kPageBlock = 1024; /* pages per scan block */
 constexpr int64_t kMaxPageBytes = (int64_t)1 << 30;
 
 /* What one row does in a step. */
@@ -96,23 +95,20 @@ struct PageJob {
 
 /* What the kernels of one call tell each other. */
 struct PagePlan {
-    int32_t code;     /* G4S_OK or the first error (the lowest status) */
-    int32_t jobs;     /* pages to copy */
-    int32_t distinct; /* pages taken over by some row */
-    int32_t live;     /* compact: live pages */
-    int32_t below;    /* compact: live pages among the first `live` */
+    uint32_t ticket;   /* 0 between calls, as the next two */
+    int32_t bad;       /* the first error (the lowest status) */
+    uint32_t distinct; /* pages taken over by some row */
+    int32_t code;
+    int32_t jobs;  /* pages to copy */
+    int32_t live;  /* compact: live pages */
+    int32_t below; /* compact: live pages among the first `live` */
 };
 
 struct PageWorkspace {
-    uint32_t* count;   /* [n_pages] rows that hold the page; 0 between calls */
-    uint32_t* writers; /* [n_pages] rows that go on writing it; 0 between calls */
-    int32_t* first;    /* [n_pages] the first of them; INT32_MAX between calls */
-    uint16_t* list;    /* [blocks*1024] a block's live pages from its front, free
-                          pages from its back */
-    uint16_t* rank;    /* [n_pages] a page's place among its block's live / free pages */
-    int32_t* nfree;    /* [blocks] */
-    int32_t* before;   /* [blocks+1] free pages before the block */
-    PageJob* jobs;     /* [max_rows] */
+    uint32_t* count;  /* [n_pages] rows that hold the page; 0 between calls */
+    uint64_t* free;   /* [words] a bit for each free page, 64 pages a word */
+    uint32_t* before; /* [words + 1] compact: free pages before the word */
+    PageJob* jobs;    /* [max_rows] */
     PagePlan* plan;
 };
 
@@ -124,7 +120,7 @@ struct PagesArgs {
     const int32_t* grow;
     char* pool;
     int32_t* status;
-    int32_t blocks;
+    int32_t words;
     PageWorkspace ws;
 };
 

@@ -25,89 +25,32 @@ constexpr int kCopyItems = 4; /* vectors per thread in flight */
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-/* ------------------------------------------------------------------- scans */
+/* ------------------------------------------------------- tables and counts */
 
-/* Per block of 1024 pages: its free pages counted, its live and free pages listed. */
-__global__ __launch_bounds__(kB) void pages_scan_kernel(PagesArgs a)
+constexpr int kScanPages = 4 * kB; /* pages of a scanning workgroup */
+constexpr int kGatherRows = 4;     /* rows of a gathering one, 256 slots of each */
+
+__host__ __device__ inline int scan_groups(int n_pages)
 {
-    __shared__ int s_wave[kB / 64];
-    const int tid = threadIdx.x, blk = blockIdx.x;
-    if (blk == 0 && tid == 0) *a.ws.plan = PagePlan{};
-    int live[4], in[4], mine = 0;
+    return (n_pages + kScanPages - 1) / kScanPages;
+}
+__host__ __device__ inline int slot_groups(int slots) { return (slots + kB - 1) / kB; }
+
+/* The free pages of kScanPages pages, as bits. */
+__device__ __forceinline__ void scan_pages(const PagesArgs& a, int group)
+{
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int p = blk * kPageBlock + tid * 4 + q;
-        in[q] = p < a.geo.n_pages;
-        live[q] = in[q] && a.from.refs[p] > 0;
-        mine += live[q];
+    for (int q = 0; q < kScanPages / kB; ++q) {
+        const int p = group * kScanPages + q * kB + (int)threadIdx.x;
+        const bool in = p < a.geo.n_pages;
+        const uint64_t w = __ballot(in && a.from.refs[in ? p : 0] <= 0);
+        if ((threadIdx.x & 63) == 0 && in) st_dev(&a.ws.free[p / 64], w);
     }
-    int total;
-    int at = block_exclusive_scan<kB>(mine, s_wave, total);
-    int held = a.geo.n_pages - blk * kPageBlock;
-    held = held < kPageBlock ? held : kPageBlock;
-    uint16_t* list = a.ws.list + blk * kPageBlock;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        const int l = tid * 4 + q;
-        if (!in[q]) continue;
-        const int r = live[q] ? at : l - at;
-        list[live[q] ? r : kPageBlock - 1 - r] = (uint16_t)l;
-        a.ws.rank[blk * kPageBlock + l] = (uint16_t)r;
-        at += live[q];
-    }
-    if (tid == 0) a.ws.nfree[blk] = held - total;
-}
-
-/* Free pages before each block, in global memory; returns how many there are. */
-__device__ int scan_blocks(const PagesArgs& a, int* s_wave)
-{
-    int base = 0;
-    for (int b0 = 0; b0 < a.blocks; b0 += kB) {
-        const int b = b0 + (int)threadIdx.x;
-        const int f = b < a.blocks ? a.ws.nfree[b] : 0;
-        int total;
-        const int pre = block_exclusive_scan<kB>(f, s_wave, total);
-        if (b < a.blocks) a.ws.before[b] = base + pre;
-        base += total;
-    }
-    if (threadIdx.x == 0) a.ws.before[a.blocks] = base;
-    __syncthreads();
-    return base;
-}
-
-/* The i-th free page (0 <= i < free pages), and the i-th live one. */
-__device__ __forceinline__ int free_page(const PagesArgs& a, int i)
-{
-    int lo = 0, hi = a.blocks - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.ws.before[mid] <= i)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo * kPageBlock + a.ws.list[lo * kPageBlock + kPageBlock - 1 - (i - a.ws.before[lo])];
-}
-__device__ __forceinline__ int live_before(const PagesArgs& a, int blk)
-{
-    return blk * kPageBlock - a.ws.before[blk];
-}
-__device__ __forceinline__ int live_page(const PagesArgs& a, int i)
-{
-    int lo = 0, hi = a.blocks - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (live_before(a, mid) <= i)
-            lo = mid;
-        else
-            hi = mid - 1;
-    }
-    return lo * kPageBlock + a.ws.list[lo * kPageBlock + i - live_before(a, lo)];
 }
 
 __device__ __forceinline__ void report(const PagesArgs& a, int code)
 {
-    atomicMin(&a.ws.plan->code, code);
+    atomicMin(&a.ws.plan->bad, code);
 }
 
 /* A table entry is a page of the pool that the state holds. */
@@ -118,64 +61,172 @@ __device__ __forceinline__ bool page_ok(const PagesArgs& a, int p)
 
 __device__ __forceinline__ RowStep step_of(const PagesArgs& a, int r, int& parent)
 {
-    parent = a.parents[r];
+    parent = a.parents ? a.parents[r] : r;
     const int len = parent >= 0 && parent < a.from_rows ? a.from.lengths[parent] : 0;
     return row_step(parent, a.from_rows, len, a.grow ? a.grow[r] : 0, a.geo.page_tokens,
                     a.geo.max_slots);
 }
 
-/* ----------------------------------------------------------------- advance */
-
-/* Tables gathered from the parents' rows, their pages counted. */
-__global__ __launch_bounds__(kB) void pages_gather_kernel(PagesArgs a)
+/* kGatherRows rows of the new tables, 256 slots of each, gathered from
+ * their parents' rows, and their pages counted: neighbouring rows that share
+ * a page count it at once.  CHECK: nothing but whether the tables are valid. */
+template <bool CHECK>
+__device__ __forceinline__ void gather_rows(const PagesArgs& a, int group)
 {
-    const int r = blockIdx.y;
-    const int slot = blockIdx.x * kB + threadIdx.x;
-    int parent;
-    const RowStep s = step_of(a, r, parent);
-    bool fresh = false;
-    if (slot < s.kept) {
-        const int p = a.from.table[(int64_t)parent * a.geo.max_slots + slot];
-        if (page_ok(a, p)) {
-            a.to.table[(int64_t)r * a.geo.max_slots + slot] = p;
-            fresh = atomicAdd(&a.ws.count[p], 1u) == 0u;
-        } else {
-            report(a, G4S_ERR_FORMAT);
+    const int across = slot_groups(a.geo.max_slots);
+    const int r0 = group / across * kGatherRows;
+    const int slot = group % across * kB + (int)threadIdx.x;
+    int page[kGatherRows];
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q) {
+        page[q] = -1;
+        if (r0 + q >= a.rows) continue;
+        int parent;
+        const RowStep s = step_of(a, r0 + q, parent);
+        if (s.bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
+        if (slot < s.kept) {
+            page[q] = a.from.table[(int64_t)parent * a.geo.max_slots + slot];
+            if (!page_ok(a, page[q])) {
+                page[q] = -1;
+                report(a, G4S_ERR_FORMAT);
+            }
         }
     }
-    const int n = __popcll(__ballot(fresh));
-    if ((threadIdx.x & 63) == 0 && n) atomicAdd(&a.ws.plan->distinct, n);
-    if (s.bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
+    if (CHECK) return;
+    uint32_t fresh = 0, run = 0;
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q) {
+        if (page[q] >= 0) a.to.table[(int64_t)(r0 + q) * a.geo.max_slots + slot] = page[q];
+        ++run;
+        if (q + 1 == kGatherRows || page[q + 1] != page[q]) {
+            if (page[q] >= 0) fresh += atomicAdd(&a.ws.count[page[q]], run) == 0u;
+            run = 0;
+        }
+    }
+    const int n = wave_sum_i32((int)fresh);
+    if ((threadIdx.x & 63) == 0 && n) atomicAdd(&a.ws.plan->distinct, (uint32_t)n);
 }
 
-/* The page that row r goes on writing, or -1. */
-__device__ __forceinline__ int written_page(const PagesArgs& a, const RowStep& s, int parent)
+/* Free pages before this thread's share of the words, shares in thread order. */
+struct FreeShare {
+    int words, first; /* words of a share, and this thread's first */
+    int before, total;
+};
+__device__ __forceinline__ FreeShare share_free(const PagesArgs& a, int* s_wave)
 {
-    if (s.tail == 0) return -1;
-    const int p = a.from.table[(int64_t)parent * a.geo.max_slots + s.kept - 1];
-    return page_ok(a, p) ? p : -1;
+    FreeShare f;
+    f.words = (a.words + kB - 1) / kB;
+    f.first = f.words * (int)threadIdx.x;
+    int n = 0;
+    for (int w = 0; w < f.words; ++w)
+        if (f.first + w < a.words) n += __popcll(ld_dev(&a.ws.free[f.first + w]));
+    f.before = block_exclusive_scan<kB>(n, s_wave, f.total);
+    return f;
 }
 
-/* One workgroup: which rows copy the page they write, what each row takes, and who gets
+/* The i-th set bit of w (0 <= i < its bits). */
+__device__ __forceinline__ int nth_bit(uint64_t w, int i)
+{
+    int at = 0;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        const int n = __popcll(w & (((uint64_t)1 << d) - 1));
+        if (i >= n) {
+            i -= n;
+            w >>= d;
+            at += d;
+        }
+    }
+    return at;
+}
+
+/* ----------------------------------------------------------------- advance */
+
+/* Rows that go on writing one page, by page, in LDS: open addressing over twice the rows. */
+struct Writers {
+    int* page;  /* -1 = empty */
+    int* rows;
+    int* first;
+    uint32_t mask;
+};
+__device__ __forceinline__ uint32_t find_writer(const Writers& t, int page, bool add)
+{
+    uint32_t at = (uint32_t)page * 2654435761u >> 7 & t.mask;
+    for (;;) {
+        const int k = add ? atomicCAS(&t.page[at], -1, page) : t.page[at];
+        if (k == page || (add && k == -1)) return at;
+        at = (at + 1) & t.mask;
+    }
+}
+
+__host__ __device__ inline uint32_t writer_slots(int rows)
+{
+    uint32_t n = 64;
+    while (n < 2u * (uint32_t)rows) n <<= 1;
+    return n;
+}
+/* LDS words of the plan: four a row and one, three a slot of the writers. */
+__host__ __device__ inline size_t plan_lds(int rows)
+{
+    return sizeof(int) * (4 * (size_t)rows + 1 + 3 * (size_t)writer_slots(rows));
+}
+
+/* Scan and gather, all side by side; the workgroup that ends last then decides
+ * which rows copy the page they write, what each row takes, and who gets
  * which free page. */
-__global__ __launch_bounds__(kB) void pages_plan_kernel(PagesArgs a)
+__global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
 {
+    extern __shared__ int lds[];
     __shared__ int s_wave[kB / 64];
-    __shared__ int before[G4S_PAGES_MAX_ROWS + 1]; /* pages taken before row r */
-    __shared__ int kept[G4S_PAGES_MAX_ROWS];       /* its kept slots * 2 + whether it copies */
-    __shared__ int s_code;
+    __shared__ int s_share[kB + 1]; /* free pages before each thread's share */
+    __shared__ int s_flag, s_code;
     const int tid = threadIdx.x;
-    const int nfree = scan_blocks(a, s_wave);
+    const int scans = scan_groups(a.geo.n_pages);
+    if ((int)blockIdx.x < scans)
+        scan_pages(a, blockIdx.x);
+    else
+        gather_rows<false>(a, blockIdx.x - scans);
+    if (!elect_last(&a.ws.plan->ticket, gridDim.x, &s_flag)) return;
+
+    int* before = lds;            /* [rows + 1] pages taken before the row */
+    int* kept = before + a.rows + 1; /* [rows] its kept slots * 2 + whether it copies */
+    int* page = kept + a.rows;    /* [rows] the page it goes on writing, or -1 */
+    int* tail = page + a.rows;    /* [rows] tokens in it */
+    Writers w;
+    w.page = tail + a.rows;
+    const uint32_t slots = writer_slots(a.rows);
+    w.mask = slots - 1;
+    w.rows = w.page + slots;
+    w.first = w.rows + slots;
+    for (uint32_t i = tid; i < slots; i += kB) {
+        w.page[i] = -1;
+        w.rows[i] = 0;
+        w.first[i] = INT_MAX;
+    }
+    const FreeShare f = share_free(a, s_wave); /* (a barrier: the writers are empty) */
+    s_share[tid] = f.before;
+    if (tid == 0) s_share[kB] = f.total;
+    const int bad = (int)ld_dev((const uint32_t*)&a.ws.plan->bad);
+    const int distinct = (int)ld_dev(&a.ws.plan->distinct);
     for (int r = tid; r < a.rows; r += kB) {
         int parent;
         const RowStep s = step_of(a, r, parent);
-        const int w = written_page(a, s, parent);
-        if (w >= 0) {
-            atomicAdd(&a.ws.writers[w], 1u);
-            atomicMin(&a.ws.first[w], r);
+        int p = -1;
+        if (s.tail) {
+            p = a.from.table[(int64_t)parent * a.geo.max_slots + s.kept - 1];
+            if (!page_ok(a, p)) p = -1;
+        }
+        before[r] = s.fresh;
+        kept[r] = s.kept * 2;
+        page[r] = p;
+        tail[r] = s.tail;
+        a.to.lengths[r] = (int)s.length; /* (0 instead on an error, below) */
+        if (p >= 0) {
+            const uint32_t at = find_writer(w, p, true);
+            atomicAdd(&w.rows[at], 1);
+            atomicMin(&w.first[at], r);
         }
     }
-    __threadfence();
     __syncthreads();
     int64_t taken = 0;
     int copies = 0;
@@ -183,14 +234,12 @@ __global__ __launch_bounds__(kB) void pages_plan_kernel(PagesArgs a)
         const int r = r0 + tid;
         int need = 0, copy = 0, total;
         if (r < a.rows) {
-            int parent;
-            const RowStep s = step_of(a, r, parent);
-            const int w = written_page(a, s, parent);
-            if (w >= 0)
-                copy = !(ld_dev(&a.ws.count[w]) == ld_dev(&a.ws.writers[w]) &&
-                         (int)ld_dev((const uint32_t*)&a.ws.first[w]) == r);
-            need = s.fresh + copy;
-            kept[r] = s.kept * 2 + copy;
+            if (page[r] >= 0) {
+                const uint32_t at = find_writer(w, page[r], false);
+                copy = !((int)ld_dev(&a.ws.count[page[r]]) == w.rows[at] && w.first[at] == r);
+            }
+            need = before[r] + copy;
+            kept[r] += copy;
         }
         const int pre = block_exclusive_scan<kB>(need, s_wave, total);
         if (r < a.rows) before[r] = (int)(taken + pre < INT_MAX ? taken + pre : INT_MAX);
@@ -198,46 +247,38 @@ __global__ __launch_bounds__(kB) void pages_plan_kernel(PagesArgs a)
         block_exclusive_scan<kB>(copy, s_wave, total);
         copies += total;
     }
-    if (tid == 0) before[a.rows] = (int)(taken < INT_MAX ? taken : INT_MAX);
     if (tid == 0) {
-        int code = (int)ld_dev((const uint32_t*)&a.ws.plan->code);
-        if (code == G4S_OK && taken > nfree) code = G4S_ERR_OUT_OF_MEMORY;
+        const int code = bad != G4S_OK ? bad : taken > f.total ? G4S_ERR_OUT_OF_MEMORY : G4S_OK;
         s_code = code;
         a.status[0] = code;
-        a.status[1] = code ? a.geo.n_pages
-                           : a.geo.n_pages - (int)ld_dev((const uint32_t*)&a.ws.plan->distinct) -
-                                 (int)taken;
+        a.status[1] = code ? a.geo.n_pages : a.geo.n_pages - distinct - (int)taken;
         a.status[2] = code ? 0 : (int)taken;
         a.status[3] = code ? 0 : copies;
         a.ws.plan->code = code;
         a.ws.plan->jobs = code ? 0 : copies;
+        st_dev((uint32_t*)&a.ws.plan->bad, 0u);
+        st_dev(&a.ws.plan->distinct, 0u);
     }
     __syncthreads();
-    const int code = s_code;
+    if (s_code) {
+        for (int r = tid; r < a.rows; r += kB) a.to.lengths[r] = 0;
+        return;
+    }
     int job = 0;
     for (int r0 = 0; r0 < a.rows; r0 += kB) {
         const int r = r0 + tid;
-        int copy = 0, total, w = -1, tail = 0;
-        if (r < a.rows) {
-            int parent;
-            const RowStep s = step_of(a, r, parent);
-            w = written_page(a, s, parent);
-            tail = s.tail;
-            if (w >= 0) {
-                a.ws.writers[w] = 0u;
-                a.ws.first[w] = INT_MAX;
-            }
-            a.to.lengths[r] = code ? 0 : (int)s.length;
-            copy = code ? 0 : kept[r] & 1;
-        }
+        const int copy = r < a.rows ? kept[r] & 1 : 0;
+        int total;
         const int at = job + block_exclusive_scan<kB>(copy, s_wave, total);
         if (copy) {
-            atomicSub(&a.ws.count[w], 1u);
-            a.ws.jobs[at] = PageJob{w, free_page(a, before[r]), tail};
+            atomicSub(&a.ws.count[page[r]], 1u);
+            a.ws.jobs[at].src = page[r];
+            a.ws.jobs[at].tokens = tail[r];
+            tail[r] = at; /* its job, for whoever hands out its first page */
         }
         job += total;
     }
-    if (code) return;
+    __syncthreads();
     for (int k = tid; k < (int)taken; k += kB) {
         int lo = 0, hi = a.rows - 1; /* the row that takes free page k */
         while (lo < hi) {
@@ -247,9 +288,21 @@ __global__ __launch_bounds__(kB) void pages_plan_kernel(PagesArgs a)
             else
                 hi = mid - 1;
         }
-        const int p = free_page(a, k);
-        const int slot = (kept[lo] >> 1) - (kept[lo] & 1) + (k - before[lo]);
-        a.to.table[(int64_t)lo * a.geo.max_slots + slot] = p;
+        int from = 0, to = kB - 1; /* the share that it lies in */
+        while (from < to) {
+            const int mid = (from + to + 1) >> 1;
+            if (s_share[mid] <= k)
+                from = mid;
+            else
+                to = mid - 1;
+        }
+        int i = k - s_share[from], word = from * f.words;
+        uint64_t bits = ld_dev(&a.ws.free[word]);
+        for (int n; i >= (n = __popcll(bits)); i -= n) bits = ld_dev(&a.ws.free[++word]);
+        const int p = word * 64 + nth_bit(bits, i);
+        const int nth = k - before[lo];
+        a.to.table[(int64_t)lo * a.geo.max_slots + (kept[lo] >> 1) - (kept[lo] & 1) + nth] = p;
+        if (nth == 0 && (kept[lo] & 1)) a.ws.jobs[tail[lo]].dst = p;
         atomicAdd(&a.ws.count[p], 1u);
     }
 }
@@ -291,15 +344,19 @@ __host__ __device__ inline int copy_segments(const g4s_page_geometry& g)
     return (int)((n + kB * kCopyItems - 1) / (kB * kCopyItems));
 }
 
+/* Each job in a column of workgroups, its planes and segments in turn. */
 template <typename T, typename JobF>
-__device__ void copy_all(const g4s_page_geometry& g, const char* src, char* dst, int jobs, JobF job)
+__device__ __forceinline__ void copy_all(const g4s_page_geometry& g, const char* src, char* dst,
+                                         int jobs, JobF job)
 {
     const int segs = copy_segments<T>(g);
-    const int64_t units = (int64_t)jobs * g.planes * segs;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int64_t pj = u / segs;
-        const int plane = (int)(pj / jobs);
-        copy_segment<T>(g, src, dst, plane, (int)(u - pj * segs), job((int)(pj - (int64_t)plane * jobs)));
+    const uint32_t units = (uint32_t)g.planes * (uint32_t)segs;
+    for (int64_t j = blockIdx.x; j < jobs; j += gridDim.x) {
+        const PageJob it = job((int)j);
+        for (uint32_t u = blockIdx.y; u < units; u += gridDim.y) {
+            const uint32_t plane = u / (uint32_t)segs;
+            copy_segment<T>(g, src, dst, (int)plane, (int)(u - plane * (uint32_t)segs), it);
+        }
     }
 }
 
@@ -308,10 +365,11 @@ template <typename T>
 __global__ __launch_bounds__(kB) void pages_finish_kernel(PagesArgs a)
 {
     const bool ok = a.ws.plan->code == G4S_OK;
-    for (int p = blockIdx.x * kB + threadIdx.x; p < a.geo.n_pages; p += gridDim.x * kB) {
-        a.to.refs[p] = ok ? (int32_t)a.ws.count[p] : 0;
-        a.ws.count[p] = 0u;
-    }
+    if (blockIdx.y == 0)
+        for (int p = blockIdx.x * kB + threadIdx.x; p < a.geo.n_pages; p += gridDim.x * kB) {
+            a.to.refs[p] = ok ? (int32_t)a.ws.count[p] : 0;
+            a.ws.count[p] = 0u;
+        }
     copy_all<T>(a.geo, a.pool, a.pool, a.ws.plan->jobs, [&](int j) { return a.ws.jobs[j]; });
 }
 
@@ -332,39 +390,67 @@ __global__ __launch_bounds__(kB) void pages_copy_kernel(g4s_page_geometry g, con
 
 /* ----------------------------------------------------------------- compact */
 
-/* Tables and lengths are valid: nothing is written before that is known. */
-__global__ __launch_bounds__(kB) void pages_check_kernel(PagesArgs a)
-{
-    const int r = blockIdx.y;
-    const int slot = blockIdx.x * kB + threadIdx.x;
-    const RowStep s = row_step(r, a.rows, a.from.lengths[r], 0, a.geo.page_tokens, a.geo.max_slots);
-    if (s.bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
-    if (slot < s.kept && !page_ok(a, a.from.table[(int64_t)r * a.geo.max_slots + slot]))
-        report(a, G4S_ERR_FORMAT);
-}
-
-__global__ __launch_bounds__(kB) void pages_compact_plan_kernel(PagesArgs a)
+/* Scan and checks side by side: nothing is written before the tables are known to be valid.
+ * The workgroup that ends last numbers the free pages. */
+__global__ __launch_bounds__(kB) void pages_number_kernel(PagesArgs a)
 {
     __shared__ int s_wave[kB / 64];
+    __shared__ int s_flag;
     const int tid = threadIdx.x;
-    const int nfree = scan_blocks(a, s_wave);
-    const int live = a.geo.n_pages - nfree;
-    const int code = (int)ld_dev((const uint32_t*)&a.ws.plan->code);
-    /* live pages below `live`: whole blocks, then the one it falls into */
-    const int blk = live / kPageBlock;
+    const int scans = scan_groups(a.geo.n_pages);
+    if ((int)blockIdx.x < scans)
+        scan_pages(a, blockIdx.x);
+    else
+        gather_rows<true>(a, blockIdx.x - scans);
+    if (!elect_last(&a.ws.plan->ticket, gridDim.x, &s_flag)) return;
+    const FreeShare f = share_free(a, s_wave);
+    const int live = a.geo.n_pages - f.total;
+    /* free pages below `live`: as many live ones lie above and move down */
     int mine = 0;
-    for (int p = blk * kPageBlock + tid; p < live; p += kB) mine += a.from.refs[p] > 0;
-    mine = block_sum_i32<kB>(mine, s_wave);
-    if (tid == 0) {
-        const int below = (blk < a.blocks ? live_before(a, blk) : live) + mine;
-        a.ws.plan->live = live;
-        a.ws.plan->below = below;
-        a.ws.plan->jobs = code ? 0 : live - below;
-        a.status[0] = code;
-        a.status[1] = code ? a.geo.n_pages : nfree;
-        a.status[2] = 0;
-        a.status[3] = code ? 0 : live - below;
+    for (int w = 0, at = f.before; w < f.words; ++w) {
+        const int word = f.first + w;
+        if (word >= a.words) break;
+        const uint64_t bits = ld_dev(&a.ws.free[word]);
+        a.ws.before[word] = (uint32_t)at;
+        at += __popcll(bits);
+        const int in = live - word * 64;
+        if (in > 0) mine += __popcll(in >= 64 ? bits : bits & (((uint64_t)1 << in) - 1));
     }
+    const int holes = block_sum_i32<kB>(mine, s_wave);
+    if (tid == 0) {
+        const int code = (int)ld_dev((const uint32_t*)&a.ws.plan->bad);
+        st_dev((uint32_t*)&a.ws.plan->bad, 0u);
+        a.ws.plan->code = code;
+        a.ws.plan->live = live;
+        a.ws.plan->below = live - holes;
+        a.ws.plan->jobs = code ? 0 : holes;
+        a.status[0] = code;
+        a.status[1] = code ? a.geo.n_pages : f.total;
+        a.status[2] = 0;
+        a.status[3] = code ? 0 : holes;
+    }
+}
+
+/* Free pages before page p, and the i-th free and live page. */
+__device__ __forceinline__ int free_before(const PagesArgs& a, int p)
+{
+    return (int)a.ws.before[p / 64] +
+           __popcll(a.ws.free[p / 64] & (((uint64_t)1 << (p & 63)) - 1));
+}
+template <bool FREE>
+__device__ __forceinline__ int nth_page(const PagesArgs& a, int i)
+{
+    auto before = [&](int w) { return FREE ? (int)a.ws.before[w] : w * 64 - (int)a.ws.before[w]; };
+    int lo = 0, hi = a.words - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (before(mid) <= i)
+            lo = mid;
+        else
+            hi = mid - 1;
+    }
+    const uint64_t bits = a.ws.free[lo];
+    return lo * 64 + nth_bit(FREE ? bits : ~bits, i - before(lo));
 }
 
 template <typename T>
@@ -372,40 +458,37 @@ __global__ __launch_bounds__(kB) void pages_compact_kernel(PagesArgs a)
 {
     const PagePlan plan = *a.ws.plan;
     const bool ok = plan.code == G4S_OK;
-    const int at = blockIdx.x * kB + threadIdx.x, step = gridDim.x * kB;
-    for (int p = at; p < a.geo.n_pages; p += step) {
-        int refs = 0;
-        if (ok && p < plan.live) {
-            refs = a.from.refs[p];
-            if (refs <= 0)
-                refs = a.from.refs[live_page(
-                    a, plan.below + a.ws.before[p / kPageBlock] + a.ws.rank[p])];
+    if (blockIdx.y == 0) {
+        const int at = blockIdx.x * kB + threadIdx.x, step = gridDim.x * kB;
+        for (int p = at; p < a.geo.n_pages; p += step) {
+            int refs = 0;
+            if (ok && p < plan.live) {
+                refs = a.from.refs[p];
+                if (refs <= 0) refs = a.from.refs[nth_page<false>(a, plan.below + free_before(a, p))];
+            }
+            a.to.refs[p] = refs;
         }
-        a.to.refs[p] = refs;
-    }
-    for (int r = at; r < a.rows; r += step) a.to.lengths[r] = ok ? a.from.lengths[r] : 0;
-    const int64_t S = a.geo.max_slots, cells = ok ? a.rows * S : 0;
-    for (int64_t c = at; c < cells; c += step) {
-        const int r = (int)(c / S);
-        const int used = (a.from.lengths[r] + a.geo.page_tokens - 1) / a.geo.page_tokens;
-        if (c - r * S >= used) continue;
-        int p = a.from.table[c];
-        if (p >= plan.live)
-            p = free_page(a, live_before(a, p / kPageBlock) + a.ws.rank[p] - plan.below);
-        a.to.table[c] = p;
+        for (int r = at; r < a.rows; r += step) a.to.lengths[r] = ok ? a.from.lengths[r] : 0;
+        const int64_t S = a.geo.max_slots, cells = ok ? a.rows * S : 0;
+        for (int64_t c = at; c < cells; c += step) {
+            const int r = (int)(c / S);
+            const int used = (a.from.lengths[r] + a.geo.page_tokens - 1) / a.geo.page_tokens;
+            if (c - r * S >= used) continue;
+            int p = a.from.table[c];
+            if (p >= plan.live) p = nth_page<true>(a, p - free_before(a, p) - plan.below);
+            a.to.table[c] = p;
+        }
     }
     copy_all<T>(a.geo, a.pool, a.pool, plan.jobs, [&](int j) {
-        return PageJob{live_page(a, plan.below + j), free_page(a, j), a.geo.page_tokens};
+        return PageJob{nth_page<false>(a, plan.below + j), nth_page<true>(a, j),
+                       a.geo.page_tokens};
     });
 }
 
 __global__ __launch_bounds__(kB) void pages_init_kernel(PageWorkspace ws, int n)
 {
-    for (int p = blockIdx.x * kB + threadIdx.x; p < n; p += gridDim.x * kB) {
-        ws.count[p] = 0u;
-        ws.writers[p] = 0u;
-        ws.first[p] = INT_MAX;
-    }
+    for (int p = blockIdx.x * kB + threadIdx.x; p < n; p += gridDim.x * kB) ws.count[p] = 0u;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *ws.plan = PagePlan{};
 }
 
 /* Widest vectors that every address of a copy is a multiple of. */
@@ -415,14 +498,21 @@ uint64_t copy_bits(const g4s_page_geometry& g, const void* src, const void* dst)
            (uint64_t)g.plane_stride | (uint64_t)g.page_stride;
 }
 
-constexpr int kMaxGrid = 1 << 20;
+/* At most `jobs` jobs: a workgroup for each, and as many side by side as its planes and
+ * segments fill until there are kCopyGroups, some rounds of the device. */
+constexpr int kCopyGroups = 1 << 15;
 
 template <typename T>
-unsigned copy_grid(const g4s_page_geometry& g, int64_t jobs, int64_t other)
+dim3 copy_grid(const g4s_page_geometry& g, int64_t jobs, int64_t least)
 {
-    const int64_t units = jobs * g.planes * copy_segments<T>(g);
-    const int64_t want = units > other ? units : other;
-    return (unsigned)(want < 1 ? 1 : want > kMaxGrid ? kMaxGrid : want);
+    const int64_t units = (int64_t)g.planes * copy_segments<T>(g);
+    int64_t x = jobs > least ? jobs : least;
+    x = x < 1 ? 1 : x > kCopyGroups ? kCopyGroups : x;
+    int64_t y = kCopyGroups / (jobs < 1 ? 1 : jobs);
+    y = y > units ? units : y > 65535 ? 65535 : y;
+    y = y < 1 ? 1 : y;
+    const int64_t each = (units + y - 1) / y; /* as many for each */
+    return dim3((unsigned)x, (unsigned)(each < 1 ? 1 : (units + each - 1) / each));
 }
 
 }  // namespace
@@ -443,15 +533,18 @@ hipError_t pages_init_launch(const PageWorkspace& ws, int32_t n_pages, hipStream
             CALL(uint8_t);          \
     } while (0)
 
+static unsigned first_grid(const PagesArgs& a)
+{
+    return (unsigned)(scan_groups(a.geo.n_pages) +
+                      (a.rows + kGatherRows - 1) / kGatherRows * slot_groups(a.geo.max_slots));
+}
+
 hipError_t pages_advance_launch(const PagesArgs& a, hipStream_t stream)
 {
-    const dim3 cells((unsigned)((a.geo.max_slots + kB - 1) / kB), (unsigned)a.rows);
-    pages_scan_kernel<<<(unsigned)a.blocks, kB, 0, stream>>>(a);
-    pages_gather_kernel<<<cells, kB, 0, stream>>>(a);
-    pages_plan_kernel<<<1, kB, 0, stream>>>(a);
-    const int64_t other = (a.geo.n_pages + kB - 1) / kB;
+    pages_advance_kernel<<<first_grid(a), kB, plan_lds(a.rows), stream>>>(a);
+    const int64_t least = (a.geo.n_pages + kB - 1) / kB;
 #define G4S_CALL(T) \
-    pages_finish_kernel<T><<<copy_grid<T>(a.geo, a.rows, other), kB, 0, stream>>>(a)
+    pages_finish_kernel<T><<<copy_grid<T>(a.geo, a.rows, least), kB, 0, stream>>>(a)
     G4S_BY_WIDTH(copy_bits(a.geo, a.pool, a.pool), G4S_CALL);
 #undef G4S_CALL
     return hipGetLastError();
@@ -459,14 +552,11 @@ hipError_t pages_advance_launch(const PagesArgs& a, hipStream_t stream)
 
 hipError_t pages_compact_launch(const PagesArgs& a, hipStream_t stream)
 {
-    const dim3 cells((unsigned)((a.geo.max_slots + kB - 1) / kB), (unsigned)a.rows);
-    pages_scan_kernel<<<(unsigned)a.blocks, kB, 0, stream>>>(a);
-    pages_check_kernel<<<cells, kB, 0, stream>>>(a);
-    pages_compact_plan_kernel<<<1, kB, 0, stream>>>(a);
+    pages_number_kernel<<<first_grid(a), kB, 0, stream>>>(a);
     const int64_t cell = (int64_t)a.rows * a.geo.max_slots;
-    const int64_t other = ((cell > a.geo.n_pages ? cell : a.geo.n_pages) + kB - 1) / kB;
+    const int64_t least = ((cell > a.geo.n_pages ? cell : a.geo.n_pages) + kB - 1) / kB;
 #define G4S_CALL(T) \
-    pages_compact_kernel<T><<<copy_grid<T>(a.geo, a.geo.n_pages / 2, other), kB, 0, stream>>>(a)
+    pages_compact_kernel<T><<<copy_grid<T>(a.geo, a.geo.n_pages / 2, least), kB, 0, stream>>>(a)
     G4S_BY_WIDTH(copy_bits(a.geo, a.pool, a.pool), G4S_CALL);
 #undef G4S_CALL
     return hipGetLastError();

@@ -50,7 +50,7 @@ struct g4s_beam : Handle {
 
 struct g4s_pages : Handle {
     g4s_page_geometry geo{};
-    int32_t blocks = 0;
+    int32_t words = 0;
     void* memory = nullptr;
     g4s::PageWorkspace ws{};
 };
@@ -399,16 +399,12 @@ G4S_API int g4s_pages_create(g4s_pages** out, const g4s_page_geometry* geometry,
     h->device = device;
     h->stream = (hipStream_t)hip_stream;
     h->geo = g;
-    h->blocks = (g.n_pages + g4s::kPageBlock - 1) / g4s::kPageBlock;
+    h->words = (g.n_pages + 63) / 64;
     Carver c;
     auto lay = [&] {
         c.add(&h->ws.count, (size_t)g.n_pages);
-        c.add(&h->ws.writers, (size_t)g.n_pages);
-        c.add(&h->ws.first, (size_t)g.n_pages);
-        c.add(&h->ws.list, (size_t)h->blocks * g4s::kPageBlock);
-        c.add(&h->ws.rank, (size_t)h->blocks * g4s::kPageBlock);
-        c.add(&h->ws.nfree, (size_t)h->blocks);
-        c.add(&h->ws.before, (size_t)h->blocks + 1);
+        c.add(&h->ws.free, (size_t)h->words);
+        c.add(&h->ws.before, (size_t)h->words + 1);
         c.add(&h->ws.jobs, (size_t)g.max_rows);
         c.add(&h->ws.plan, 1);
     };
@@ -477,7 +473,7 @@ g4s::PagesArgs pages_args(g4s_pages* h, const g4s_page_state* from, const g4s_pa
     a.rows = rows;
     a.pool = (char*)d_pool;
     a.status = d_status;
-    a.blocks = h->blocks;
+    a.words = h->words;
     a.ws = h->ws;
     return a;
 }

@@ -14,7 +14,7 @@ from .native import DTYPE_F32, G4S_OK, SamplerError, _ptr
 
 MAX_BEAMS = 64
 MAX_ROWS = 65535
-PAGES_MAX_ROWS = 4096
+PAGES_MAX_ROWS = 2048
 PAGES_MAX_PAGES = 1048576
 
 # words of the status of PageCache.advance and compact

@@ -26,7 +26,7 @@ const
 
   G4S_BEAM_MAX_BEAMS = 64;
   G4S_BEAM_MAX_ROWS = 65535;
-  G4S_PAGES_MAX_ROWS = 4096;
+  G4S_PAGES_MAX_ROWS = 2048;
   G4S_PAGES_MAX_PAGES = 1048576;
 
 type

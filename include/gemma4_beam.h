@@ -32,7 +32,7 @@ extern "C" {
  * rows and pages of a page cache. */
 #define G4S_BEAM_MAX_BEAMS 64
 #define G4S_BEAM_MAX_ROWS 65535
-#define G4S_PAGES_MAX_ROWS 4096
+#define G4S_PAGES_MAX_ROWS 2048
 #define G4S_PAGES_MAX_PAGES 1048576
 
 /* ------------------------------------------------------------------ search */
