@@ -500,7 +500,7 @@ uint64_t copy_bits(const g4s_page_geometry& g, const void* src, const void* dst)
 
 /* At most `jobs` jobs: a workgroup for each, and as many side by side as its planes and
  * segments fill until there are kCopyGroups, some rounds of the device. */
-constexpr int kCopyGroups = 1 << 15;
+constexpr int kCopyGroups = 1 << 14;
 
 template <typename T>
 dim3 copy_grid(const g4s_page_geometry& g, int64_t jobs, int64_t least)

@@ -203,6 +203,57 @@ def test_infinite_score():
     check(x, np.array([-1, np.inf], F32), 2, 4)
 
 
+def special_rows(rng, V):
+    """Rows that the common way does not suit, 24 of them: (name, logits)."""
+    n = rng.standard_normal
+    wave = (np.arange(V) % 8192 < 64)
+    rows = [("ascending", np.linspace(-20, 20, V)), ("descending", np.linspace(20, -20, V)),
+            ("low start", np.where(np.arange(V) < 17000, -28 + n(V) * .01, n(V) * 3)),
+            ("low tiles", np.where(np.arange(V) % 16384 < 8000, -30, n(V))),
+            ("zero", np.zeros(V)), ("equal", np.full(V, -7.25)),
+            ("two values", rng.integers(0, 2, V) * 3.0), ("negative", -np.abs(n(V)) - 5),
+            ("tiny", n(V) * 1e-6), ("tinier", n(V) * 1e-9), ("both signs tiny", n(V) * 3e-8),
+            ("masked half", np.where(rng.random(V) < .5, NONE, n(V) * 3)),
+            ("masked lowest", np.where(rng.random(V) < .9, -3.38e38, n(V) * 3)),
+            ("masked tiles", np.where(np.arange(V) < 20000, NONE, n(V) * 3)),
+            ("all but one", np.where(np.arange(V) == V - 3, -12.0, NONE)),
+            ("nothing", np.full(V, NONE)), ("nan", np.where(wave, np.nan, n(V) * 3)),
+            ("mostly nan", np.where(rng.random(V) < .999, np.nan, n(V))),
+            ("negative nan", np.where(rng.random(V) < .1, -np.nan, -np.abs(n(V)))),
+            ("large", n(V) * 40), ("few large", np.where(wave, n(V) * 60, n(V) * 2)),
+            ("very negative", n(V) - 70), ("infinite", np.where(rng.random(V) < 1e-3, np.inf,
+                                                                 n(V))),
+            ("large and masked", np.where(rng.random(V) < .3, NONE, n(V) * 35))]
+    return rows
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap, V, batch, beams, n", [
+    (30.0, 40009, 57, 6, 12), (0.0, 40009, 57, 6, 6), (50.0, 33000, 6, 64, 128),
+    (100.0, 20000, 50, 6, 12), (30.0, 262144, 8, 12, 24)])
+def test_many_rows(dtype, cap, V, batch, beams, n):
+    """Batches whose workgroups take several tiles each (and bf16 looks its
+    terms up), with rows of every other kind among them."""
+    rng = np.random.default_rng(20 + batch)
+    x = (rng.standard_normal((batch * beams, V), dtype=F32) * F32(3))
+    at = rng.integers(0, V, (batch * beams, 8))
+    np.put_along_axis(x, at, rng.uniform(10, 18, at.shape).astype(F32), 1)
+    special = special_rows(rng, V)
+    for i, (_, row) in enumerate(special):
+        with np.errstate(over="ignore"):
+            x[1 + i * 3 % (batch * beams - 1)] = row.astype(F32)
+    if dtype == "bf16":
+        odd = ~np.isfinite(x)
+        b = bo.bf16(np.where(odd, 0, x))
+        b[odd] = (x[odd].view(np.uint32) >> 16) | (np.isnan(x[odd]) * 0x40).astype(np.uint32)
+        x = b
+    # one beam a sequence is far ahead, and scores of neighbours never near
+    s = (-np.arange(batch * beams) % beams * 40).astype(F32) + \
+        rng.uniform(-3, 0, batch * beams).astype(F32)
+    check(x, s, beams, n, cap=cap)
+    check(x, running(rng, batch * beams), beams, n, cap=cap)
+
+
 def test_stride_no_lse_and_scores_in_place():
     rng = np.random.default_rng(15)
     x = peaky(rng, 6, 10007, "bf16")
