@@ -25,6 +25,10 @@ typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
 constexpr int kB = 256;
 constexpr int kListCap = 512; /* candidates of a workgroup kept for ranking */
 constexpr int kNMax = 2 * G4S_BEAM_MAX_BEAMS;
+/* Bits of a bound below the keys' common prefix: with values of both signs
+ * four of the mantissa, with any others more.  Six let so many elements pass that lists overflow
+ * (38 us where these take 18); sixteen cost 0.4 us. */
+constexpr int kBoundBits = 13;
 constexpr float kMasked = -1e30f; /* a logit not above it is no candidate */
 
 __device__ __forceinline__ uint64_t entry_of(uint32_t key, uint32_t token)
@@ -166,7 +170,7 @@ __device__ __forceinline__ float tile_bound(int n, SelectShared<BLOCK>& sh)
         v[q] = sh.tmax[lane + 64 * q];
         nz += __popcll(__ballot(v[q] != 0u));
     }
-    const uint32_t t = nz >= n ? wave_kth_bound<BLOCK / 64>(v, n, 10) : 0u;
+    const uint32_t t = nz >= n ? wave_kth_bound<BLOCK / 64>(v, n, kBoundBits) : 0u;
     return t == 0u ? -__builtin_inff() : key2f(t);
 }
 
@@ -202,7 +206,7 @@ __device__ __forceinline__ void list_tile(Best& best, float largest, float sure,
         bound = tile_bound<BLOCK>(n, sh);
     } else if (__popcll(__ballot(sure > best.floor)) > n) {
         const uint32_t key[1] = {cand_key(sure)};
-        bound = key2f(wave_kth_bound<1>(key, n, 10));
+        bound = key2f(wave_kth_bound<1>(key, n, kBoundBits));
     }
     if (__any(largest > best.floor && largest >= bound)) {
         /* few elements pass: by eights, most of which no lane takes further (and
@@ -640,6 +644,13 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
     const uint64_t* cand = a.ws.cand + (int64_t)row * a.chunks * a.n;
     const int total = a.chunks * a.n;
     if (tid < 3) sh.count[tid] = 0;
+    /* one chunk's sum a thread, on its way while the candidates are merged */
+    const uint64_t* sums = a.ws.sums + (int64_t)row * a.chunks * 2;
+    double sum = 0.0, ref = 0.0;
+    if (tid < a.chunks) {
+        sum = u2d(ld_dev(&sums[2 * tid]));
+        ref = u2d(ld_dev(&sums[2 * tid + 1]));
+    }
     Best best;
     int base = 0;
     /* the chunks' lists lie in token order, so copies of one key do too */
@@ -675,11 +686,13 @@ __device__ __forceinline__ void merge_row(const BeamSelectArgs& a, int row,
     /* the chunks' sums relative to the row's largest logit */
     const double vtop = cnt ? value64<MODE>(key2f(entry_key(sh.sorted[0])), a.cap) : 0.0;
     double s = 0.0;
-    for (int c = tid; c < a.chunks; c += BLOCK) {
-        const int64_t at = (int64_t)row * a.chunks + c;
-        const double sum = u2d(ld_dev(&a.ws.sums[2 * at]));
-        const double ref = u2d(ld_dev(&a.ws.sums[2 * at + 1]));
+    for (int c = tid; c < a.chunks;) {
         if (sum > 0.0) s += sum * term64(ref * kLn2, vtop * kLn2);
+        c += BLOCK;
+        if (c < a.chunks) {
+            sum = u2d(ld_dev(&sums[2 * c]));
+            ref = u2d(ld_dev(&sums[2 * c + 1]));
+        }
     }
     end_row<MODE, BLOCK>(a, row, cnt, block_sum_f64<BLOCK>(s, sh.red), sh);
 }
