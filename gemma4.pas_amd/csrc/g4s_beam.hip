@@ -408,6 +408,10 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
         Best best;
         double s = 0.0;
         bool redo = MODE == kCapExact;
+        /* unmasked and beyond what the table or the polynomial serves */
+        auto is_far = [&](float v) {
+            return v > kMasked && (TABLE ? fabsf(v) >= 64.0f : fabsf(v) > a.cap.limit);
+        };
         /* the tile at `from` is all listed */
         auto settle = [&](int from) {
             list_settle<BLOCK>(
@@ -477,6 +481,7 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
                  * and maximum do not see); then, behind the loop, so that
                  * it costs the others no registers, those with logits beyond the limit */
                 double part = 0.0;
+                bool far = false;
                 if constexpr (TABLE) {
                     const uint32_t table = (uint32_t)(uintptr_t)(LdsFloat*)dyn;
                     if (plain) {
@@ -507,7 +512,6 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
                             if (i % 4 == 2) __builtin_amdgcn_sched_barrier(0);
                         }
                     } else {
-                        bool far = false;
 #pragma unroll
                         for (int e = 0; e < E; e += 4) {
                             float t[4];
@@ -516,20 +520,16 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
                                 const float v = value(e + q);
                                 const uint32_t bits = __float_as_uint(v) >> 16;
                                 uint32_t m = bits & 0x7FFFu;
-                                far |= v > kMasked && m >= (uint32_t)kBeamTableHigh;
+                                far |= is_far(v);
+                                const bool here = v > kMasked && !is_far(v);
                                 m = m < (uint32_t)kBeamTableLow ? kBeamTableLow : m;
                                 m = m >= (uint32_t)kBeamTableHigh ? kBeamTableHigh - 1 : m;
                                 m += (bits >> 15) * kBeamTableHalf - kBeamTableLow;
                                 const float u = *(LdsFloat*)(uintptr_t)(table + 4 * m);
-                                t[q] = v > kMasked ? u : 0.0f;
+                                t[q] = here ? u : 0.0f;
                             }
                             part += sum_four(t);
                             __builtin_amdgcn_sched_barrier(0);
-                        }
-                        if (__any(far)) {
-                            part = 0.0;
-                            redo = true;
-                            if ((tid & 63) == 0) sh.far[tid / 64][tile / 32] |= 1u << (tile & 31);
                         }
                     }
                 } else {
@@ -547,27 +547,24 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
                     }
                     if (!done) {
                         part = 0.0;
-                        least = 0.0f;
+                        forget(r);
 #pragma unroll
-                        for (int e = 0; e < E; ++e)
-                            least = fminf(least, value(e) > kMasked ? value(e) : 0.0f);
-                        if (__all(least >= -a.cap.limit && largest <= a.cap.limit)) {
+                        for (int e = 0; e < E; e += 4) {
+                            float t[4];
 #pragma unroll
-                            for (int e = 0; e < E; e += 4) {
-                                float t[4];
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    const float v = value(e + q);
-                                    t[q] = near_term<MODE>(v, a.cap);
-                                    t[q] = v > kMasked ? t[q] : 0.0f;
-                                }
-                                part += sum_four(t);
+                            for (int q = 0; q < 4; ++q) {
+                                const float v = value(e + q);
+                                far |= is_far(v);
+                                t[q] = near_term<MODE>(v, a.cap);
+                                t[q] = v > kMasked && !is_far(v) ? t[q] : 0.0f;
                             }
-                        } else {
-                            redo = true;
-                            if ((tid & 63) == 0) sh.far[tid / 64][tile / 32] |= 1u << (tile & 31);
+                            part += sum_four(t);
                         }
                     }
+                }
+                if (__any(far)) {
+                    redo = true;
+                    if ((tid & 63) == 0) sh.far[tid / 64][tile / 32] |= 1u << (tile & 31);
                 }
                 s += part;
             }
@@ -580,12 +577,20 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
             for (int t = 0; t < a.tiles; ++t) {
                 if (!(sh.far[tid / 64][t / 32] >> (t & 31) & 1u)) continue;
                 const int64_t from = ((int64_t)ch * a.tiles + t) * TILE;
-#pragma unroll 1
-                for (int e = 0; e < E; ++e) {
-                    const int64_t i = from + ((e / VW) * BLOCK + tid) * VW + e % VW;
-                    const float v = i < a.vocab ? load_elem<DT>(base, i) : -__builtin_inff();
-                    if (v > kMasked) s += (double)far_term<MODE>(v, 0.0, a.cap);
-                }
+                auto at = [&](int e) { return from + ((e / VW) * BLOCK + tid) * VW + e % VW; };
+#pragma unroll
+                for (int j = 0; j < NV; ++j)
+                    r[j] = load_raw<DT>(base, at(j * VW), a.vocab);
+                uint32_t which = 0;
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+                    which |= is_far(raw_value<DT, NV>(r, e)) ? 1u << e : 0u;
+                while (__any(which != 0u))
+                    if (which) {
+                        const int e = __builtin_ctz(which);
+                        which &= which - 1;
+                        s += (double)far_term<MODE>(load_elem<DT>(base, at(e)), 0.0, a.cap);
+                    }
             }
         }
         __syncthreads();
@@ -619,14 +624,17 @@ __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
                 st_dev(&a.ws.sums[2 * at], d2u(s));
                 st_dev(&a.ws.sums[2 * at + 1], d2u(ref));
             }
-            if (!elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
-            merge_row<MODE, BLOCK>(a, row, sh);
         }
-    } else {
-        if (ch != 0) return;
+    }
+    /* a dead row's workgroups arrive too: the last of a sequence may overwrite
+     * its scores, which all of them must have read */
+    if (a.chunks > 1 && !elect_last(&a.ws.tickets[row], (uint32_t)a.chunks, &sh.flag)) return;
+    if (!live) {
         if (tid == 0 && a.lse) a.lse[row] = -__builtin_inff();
         for (int i = tid; i < a.n; i += BLOCK)
             st_dev(&a.ws.best[(int64_t)row * a.n + i], (uint64_t)0);
+    } else if (a.chunks > 1) {
+        merge_row<MODE, BLOCK>(a, row, sh);
     }
     if (a.beams > 1 &&
         !elect_last(&a.ws.tickets[a.batch * a.beams + b], (uint32_t)a.beams, &sh.flag))
@@ -822,18 +830,16 @@ __global__ __launch_bounds__(kB) void beam_reorder_kernel(BeamReorderArgs a)
 #pragma unroll
         for (int r = 0; r < WMAX; ++r)
             if (r < W) {
-                const int p = a.parents[b * W + r] - b * W;
-                const bool ok = p >= 0 && p < W;
-                const int from = ok ? p : r;
+                const uint32_t p = (uint32_t)a.parents[b * W + r] - (uint32_t)(b * W);
+                const int from = p < (uint32_t)W ? (int)p : r;
                 if (!inplace || from != r)
                     v[r] = *reinterpret_cast<const T*>(a.src + at + (int64_t)from * a.row_stride);
             }
 #pragma unroll
         for (int r = 0; r < WMAX; ++r)
             if (r < W) {
-                const int p = a.parents[b * W + r] - b * W;
-                const bool ok = p >= 0 && p < W;
-                const int from = ok ? p : r;
+                const uint32_t p = (uint32_t)a.parents[b * W + r] - (uint32_t)(b * W);
+                const int from = p < (uint32_t)W ? (int)p : r;
                 if (!inplace || from != r)
                     __builtin_nontemporal_store(
                         v[r], reinterpret_cast<T*>(a.dst + at + (int64_t)r * a.row_stride));

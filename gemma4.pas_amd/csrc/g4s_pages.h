@@ -66,7 +66,8 @@ G4S_PAGE_HD bool geometry_ok(const g4s_page_geometry& g)
 {
     if (g.page_tokens < 1 || g.page_tokens > 65536 || g.n_pages < 1 ||
         g.n_pages > G4S_PAGES_MAX_PAGES || g.max_rows < 1 || g.max_rows > G4S_PAGES_MAX_ROWS ||
-        g.max_slots < 1 || (int64_t)g.max_slots * g.page_tokens > INT32_MAX || g.planes < 0 ||
+        g.max_slots < 1 || g.max_slots > G4S_PAGES_MAX_PAGES ||
+        (int64_t)g.max_slots * g.page_tokens > INT32_MAX || g.planes < 0 ||
         g.planes > 65536)
         return false;
     if (g.planes == 0) return true;

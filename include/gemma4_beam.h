@@ -106,7 +106,8 @@ typedef struct g4s_page_geometry {
     int32_t page_tokens; /* 1 .. 65536 */
     int32_t n_pages;     /* 1 .. G4S_PAGES_MAX_PAGES */
     int32_t max_rows;    /* 1 .. G4S_PAGES_MAX_ROWS */
-    int32_t max_slots;   /* pages of a row at most; row stride of the tables */
+    int32_t max_slots;   /* 1 .. G4S_PAGES_MAX_PAGES, pages of a row at most (at most 2^31 - 1
+                            tokens); row stride of the tables */
     int32_t planes;
     int32_t parts;
     int64_t token_bytes; /* of a token in one part of one plane */

@@ -39,7 +39,8 @@ GOOD = dict(page_tokens=16, n_pages=8, max_rows=4, max_slots=4, planes=2, parts=
     dict(page_tokens=0), dict(page_tokens=65537), dict(n_pages=0),
     dict(n_pages=beam.PAGES_MAX_PAGES + 1), dict(max_rows=0),
     dict(max_rows=beam.PAGES_MAX_ROWS + 1), dict(max_slots=0),
-    dict(page_tokens=65536, max_slots=32768), dict(planes=-1), dict(parts=0),
+    dict(page_tokens=65536, max_slots=32768),
+    dict(page_tokens=1, max_slots=beam.PAGES_MAX_PAGES + 1), dict(planes=-1), dict(parts=0),
     dict(token_bytes=0), dict(token_bytes=-32), dict(token_bytes=1 << 30),
     dict(page_stride=1023), dict(page_stride=-1024), dict(plane_stride=1024 * 8 - 1),
     dict(page_stride=2048, plane_stride=1023), dict(page_stride=1 << 60)])

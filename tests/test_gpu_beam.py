@@ -261,6 +261,32 @@ def test_stride_no_lse_and_scores_in_place():
     check(x, running(rng, 6), 3, 3, inplace=True)
 
 
+@pytest.mark.parametrize("batch", [1, 40])
+def test_scores_in_place_with_dead_beams(batch):
+    """The scores of dead rows are overwritten by live ones while other
+    workgroups of those rows may not have started; three calls in a row."""
+    rng = np.random.default_rng(30 + batch)
+    V, W = 100003, 4
+    search = beam.BeamSearch(V, batch, W, 30.0)
+    for _ in range(3):
+        x = peaky(rng, batch * W, V, "f32")
+        s = np.full(batch * W, NONE, F32)
+        s[::W] = rng.uniform(-3, 0, batch).astype(F32)
+        check(x, s, W, W, inplace=True, search=search)
+    search.close()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_top_logits_beyond_the_cap(dtype):
+    """Raw logits of 40 to 90 before the softcap, a few in each row."""
+    rng = np.random.default_rng(33)
+    x = (rng.standard_normal((12, 50021)) * 4).astype(F32)
+    at = rng.integers(0, 50021, (12, 40))
+    np.put_along_axis(x, at, rng.uniform(36, 90, at.shape).astype(F32), 1)
+    np.put_along_axis(x, at[:, ::2] // 2, rng.uniform(-90, -36, (12, 20)).astype(F32), 1)
+    check(x if dtype == "f32" else bo.bf16(x), running(rng, 12), 4, 8)
+
+
 def test_calls_in_a_row_and_smaller_shapes():
     """One handle, shapes that grow and shrink: nothing of a call is left over."""
     rng = np.random.default_rng(16)
