@@ -110,6 +110,7 @@ struct PageWorkspace {
     uint64_t* free;   /* [words] a bit for each free page, 64 pages a word */
     uint32_t* before; /* [words + 1] compact: free pages before the word */
     PageJob* jobs;    /* [max_rows] */
+    uint64_t* steps;  /* [max_rows][3]  kept and fresh slots; written page and its tokens; length */
     PagePlan* plan;
 };
 

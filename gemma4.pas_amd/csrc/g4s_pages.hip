@@ -77,15 +77,20 @@ __device__ __forceinline__ void gather_rows(const PagesArgs& a, int group)
     const int r0 = group / across * kGatherRows;
     const int slot = group % across * kB + (int)threadIdx.x;
     int page[kGatherRows];
+    bool ours[kGatherRows]; /* the slot of a page that the row goes on writing is
+                               the deciding workgroup's to write, alone: nothing orders plain
+                               stores of two XCDs to one word within a launch */
 #pragma unroll
     for (int q = 0; q < kGatherRows; ++q) {
         page[q] = -1;
+        ours[q] = false;
         if (r0 + q >= a.rows) continue;
         int parent;
         const RowStep s = step_of(a, r0 + q, parent);
         if (s.bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
         if (slot < s.kept) {
             page[q] = a.from.table[(int64_t)parent * a.geo.max_slots + slot];
+            ours[q] = s.tail == 0 || slot != s.kept - 1;
             if (!page_ok(a, page[q])) {
                 page[q] = -1;
                 report(a, G4S_ERR_FORMAT);
@@ -93,10 +98,28 @@ __device__ __forceinline__ void gather_rows(const PagesArgs& a, int group)
         }
     }
     if (CHECK) return;
+    /* the rows' steps for the workgroup that decides, by threads of the last
+     * wave, whose slots are the least often used: one read there instead of four that
+     * depend on each other */
+    const int mine = (int)threadIdx.x - (kB - 64);
+    if (group % across == 0 && mine >= 0 && mine < kGatherRows && r0 + mine < a.rows) {
+        const int r = r0 + mine;
+        int parent;
+        const RowStep s = step_of(a, r, parent);
+        int p = -1;
+        if (s.tail) {
+            p = a.from.table[(int64_t)parent * a.geo.max_slots + s.kept - 1];
+            if (!page_ok(a, p)) p = -1;
+        }
+        st_dev(&a.ws.steps[3 * r], (uint64_t)(uint32_t)s.fresh << 32 | (uint32_t)s.kept);
+        st_dev(&a.ws.steps[3 * r + 1], (uint64_t)(uint32_t)s.tail << 32 | (uint32_t)p);
+        st_dev(&a.ws.steps[3 * r + 2], (uint64_t)s.length);
+    }
     uint32_t fresh = 0, run = 0;
 #pragma unroll
     for (int q = 0; q < kGatherRows; ++q) {
-        if (page[q] >= 0) a.to.table[(int64_t)(r0 + q) * a.geo.max_slots + slot] = page[q];
+        if (page[q] >= 0 && ours[q])
+            a.to.table[(int64_t)(r0 + q) * a.geo.max_slots + slot] = page[q];
         ++run;
         if (q + 1 == kGatherRows || page[q + 1] != page[q]) {
             if (page[q] >= 0) fresh += atomicAdd(&a.ws.count[page[q]], run) == 0u;
@@ -211,18 +234,14 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
     const int bad = (int)ld_dev((const uint32_t*)&a.ws.plan->bad);
     const int distinct = (int)ld_dev(&a.ws.plan->distinct);
     for (int r = tid; r < a.rows; r += kB) {
-        int parent;
-        const RowStep s = step_of(a, r, parent);
-        int p = -1;
-        if (s.tail) {
-            p = a.from.table[(int64_t)parent * a.geo.max_slots + s.kept - 1];
-            if (!page_ok(a, p)) p = -1;
-        }
-        before[r] = s.fresh;
-        kept[r] = s.kept * 2;
+        const uint64_t slots_of = ld_dev(&a.ws.steps[3 * r]);
+        const uint64_t written = ld_dev(&a.ws.steps[3 * r + 1]);
+        a.to.lengths[r] = (int)ld_dev(&a.ws.steps[3 * r + 2]); /* (0 instead on an error) */
+        const int p = (int)(uint32_t)written;
+        before[r] = (int)(slots_of >> 32);
+        kept[r] = (int)(uint32_t)slots_of * 2;
         page[r] = p;
-        tail[r] = s.tail;
-        a.to.lengths[r] = (int)s.length; /* (0 instead on an error, below) */
+        tail[r] = (int)(written >> 32);
         if (p >= 0) {
             const uint32_t at = find_writer(w, p, true);
             atomicAdd(&w.rows[at], 1);
@@ -277,6 +296,8 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
             a.ws.jobs[at].src = page[r];
             a.ws.jobs[at].tokens = tail[r];
             tail[r] = at; /* its job, for whoever hands out its first page */
+        } else if (r < a.rows && page[r] >= 0) {
+            a.to.table[(int64_t)r * a.geo.max_slots + (kept[r] >> 1) - 1] = page[r];
         }
         job += total;
     }

@@ -406,6 +406,7 @@ G4S_API int g4s_pages_create(g4s_pages** out, const g4s_page_geometry* geometry,
         c.add(&h->ws.free, (size_t)h->words);
         c.add(&h->ws.before, (size_t)h->words + 1);
         c.add(&h->ws.jobs, (size_t)g.max_rows);
+        c.add(&h->ws.steps, (size_t)g.max_rows * 3);
         c.add(&h->ws.plan, 1);
     };
     lay();

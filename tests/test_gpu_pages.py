@@ -253,6 +253,49 @@ def test_many_rows():
     rig.compact()
 
 
+def test_captured_steps():
+    """Two steps, there and back between the states, in one captured graph that is
+    replayed with other parents, eager steps of the same cache between."""
+    from test_gpu_beam import _capture
+    st = hip.Stream(nonblocking=True)
+    rig = Rig(4, 300, 8, 30, stream=st)
+    rig.advance([-1] * 8, [9, 5, 4, 1, 7, 16, 2, 3])
+    rng = np.random.default_rng(5)
+    d_par = [hip.Buffer(32), hip.Buffer(32)]
+    d_grow = hip.Buffer.from_array(np.ones(8, I32))
+    at = rig.d_pool.offset(0)
+
+    def record():
+        rig.cache.advance(rig.dev[0][1], 8, rig.dev[1][1], 8, d_par[0], d_grow, at, rig.d_status)
+        rig.cache.advance(rig.dev[1][1], 8, rig.dev[0][1], 8, d_par[1], d_grow, at, rig.d_status)
+    destroy, launch = _capture(st, record)
+    for _ in range(5):
+        parents = [np.sort(rng.integers(0, 8, 8)).astype(I32), rng.permutation(8).astype(I32)]
+        st.synchronize()
+        for d, p in zip(d_par, parents):
+            d.upload(p)
+        want = [rig.cur, rig.read(rig.dev[1])]
+        for i in range(2):
+            status, copies = bo.advance(want[0], 8, want[1], 8, parents[i], np.ones(8, I32), 4)
+            v = rig.pages(rig.pool)
+            old = v.copy()
+            for a, b, n in copies:
+                v[:, b, :, :n] = old[:, a, :, :n]
+            want.reverse()
+        launch()
+        st.synchronize()
+        got = rig.read(rig.dev[0])
+        for k in ("table", "lengths", "refs"):
+            assert np.array_equal(getattr(got, k), getattr(want[0], k)), k
+        assert tuple(rig.d_status.download(I32)[:4]) == status
+        assert np.array_equal(rig.d_pool.download(np.uint8), rig.pool)
+        rig.cur = want[0]
+        rig.advance(rng.integers(0, 8, 8), np.zeros(8, I32))  # eager, and back again
+        rig.advance(np.arange(8), None)
+    destroy()
+    st.destroy()
+
+
 def test_copy():
     for shape in SHAPES[:6]:
         rig = Rig(**shape)
