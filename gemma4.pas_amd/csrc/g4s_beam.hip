@@ -758,15 +758,19 @@ __device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b,
     const uint64_t* best = a.ws.best + (int64_t)b * total;
     const uint64_t* ys = a.ws.y + (int64_t)b * total;
     int found = 0;
+    uint64_t mine = 0ull; /* this thread's first candidate */
     for (int i = tid; i < total; i += BLOCK) {
         const int w = i / n;
+        const uint64_t* norm = a.ws.norm + 2 * ((int64_t)b * W + w);
+        const uint64_t e = ld_dev(&best[i]);
+        const double y = u2d(ld_dev(&ys[i]));
+        const double top = u2d(ld_dev(&norm[0])), ls = u2d(ld_dev(&norm[1]));
         double s = -__builtin_inf();
-        if (ld_dev(&best[i])) {
-            const uint64_t* norm = a.ws.norm + 2 * ((int64_t)b * W + w);
-            const double top = u2d(ld_dev(&norm[0])), y = u2d(ld_dev(&ys[i]));
-            s = (double)a.scores[b * W + w] + ((y == top ? 0.0 : y - top) - u2d(ld_dev(&norm[1])));
+        if (e) { /* (of a dead row nothing else was written) */
+            s = (double)a.scores[b * W + w] + ((y == top ? 0.0 : y - top) - ls);
             ++found;
         }
+        if (i == tid) mine = e;
         sc[i] = s;
     }
     found = block_sum_i32<BLOCK>(found, sh.scan);
@@ -794,7 +798,7 @@ __device__ __forceinline__ void merge_sequence(const BeamSelectArgs& a, int b,
         }
         if (rank < n) {
             parents[rank] = b * W + w;
-            tokens[rank] = (int32_t)entry_token(ld_dev(&best[i]));
+            tokens[rank] = (int32_t)entry_token(i == tid ? mine : ld_dev(&best[i]));
             out[rank] = (float)s;
         }
     }

@@ -194,6 +194,21 @@ __host__ __device__ inline size_t plan_lds(int rows)
     return sizeof(int) * (4 * (size_t)rows + 1 + 3 * (size_t)writer_slots(rows));
 }
 
+/* A row's step as gather_rows left it, and how many rows hold the page it writes. */
+struct RowRecord {
+    int kept, fresh, page, tail, length, holders;
+};
+__device__ __forceinline__ RowRecord read_row(const PagesArgs& a, int r)
+{
+    const uint64_t slots = ld_dev(&a.ws.steps[3 * r]);
+    const uint64_t written = ld_dev(&a.ws.steps[3 * r + 1]);
+    const uint64_t length = ld_dev(&a.ws.steps[3 * r + 2]);
+    RowRecord s{(int)(uint32_t)slots, (int)(slots >> 32), (int)(uint32_t)written,
+                (int)(written >> 32), (int)length, 0};
+    if (s.page >= 0) s.holders = (int)ld_dev(&a.ws.count[s.page]);
+    return s;
+}
+
 /* Scan and gather, all side by side; the workgroup that ends last then decides
  * which rows copy the page they write, what each row takes, and who gets
  * which free page.  Bound by the chain of reads that each depend on the last (parent, length,
@@ -213,6 +228,12 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
         gather_rows<false>(a, blockIdx.x - scans);
     if (!elect_last(&a.ws.plan->ticket, gridDim.x, &s_flag)) return;
 
+    /* everything that comes from other workgroups at once, the first row of
+     * each thread ahead of what it is needed for */
+    const int bad = (int)ld_dev((const uint32_t*)&a.ws.plan->bad);
+    const int distinct = (int)ld_dev(&a.ws.plan->distinct);
+    RowRecord row{};
+    if (tid < a.rows) row = read_row(a, tid);
     int* before = lds;            /* [rows + 1] pages taken before the row */
     int* kept = before + a.rows + 1; /* [rows] its kept slots * 2 + whether it copies */
     int* page = kept + a.rows;    /* [rows] the page it goes on writing, or -1 */
@@ -223,6 +244,7 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
     w.mask = slots - 1;
     w.rows = w.page + slots;
     w.first = w.rows + slots;
+    int held = 0; /* holders of the first row's page */
     for (uint32_t i = tid; i < slots; i += kB) {
         w.page[i] = -1;
         w.rows[i] = 0;
@@ -231,22 +253,19 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
     const FreeShare f = share_free(a, s_wave); /* (a barrier: the writers are empty) */
     s_share[tid] = f.before;
     if (tid == 0) s_share[kB] = f.total;
-    const int bad = (int)ld_dev((const uint32_t*)&a.ws.plan->bad);
-    const int distinct = (int)ld_dev(&a.ws.plan->distinct);
     for (int r = tid; r < a.rows; r += kB) {
-        const uint64_t slots_of = ld_dev(&a.ws.steps[3 * r]);
-        const uint64_t written = ld_dev(&a.ws.steps[3 * r + 1]);
-        a.to.lengths[r] = (int)ld_dev(&a.ws.steps[3 * r + 2]); /* (0 instead on an error) */
-        const int p = (int)(uint32_t)written;
-        before[r] = (int)(slots_of >> 32);
-        kept[r] = (int)(uint32_t)slots_of * 2;
-        page[r] = p;
-        tail[r] = (int)(written >> 32);
-        if (p >= 0) {
-            const uint32_t at = find_writer(w, p, true);
+        if (r != tid) row = read_row(a, r);
+        a.to.lengths[r] = row.length; /* (0 instead on an error) */
+        before[r] = row.fresh;
+        kept[r] = row.kept * 2;
+        page[r] = row.page;
+        tail[r] = row.tail;
+        if (row.page >= 0) {
+            const uint32_t at = find_writer(w, row.page, true);
             atomicAdd(&w.rows[at], 1);
             atomicMin(&w.first[at], r);
         }
+        if (r == tid) held = row.holders;
     }
     __syncthreads();
     int64_t taken = 0;
@@ -257,7 +276,8 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
         if (r < a.rows) {
             if (page[r] >= 0) {
                 const uint32_t at = find_writer(w, page[r], false);
-                copy = !((int)ld_dev(&a.ws.count[page[r]]) == w.rows[at] && w.first[at] == r);
+                const int n = r0 == 0 ? held : (int)ld_dev(&a.ws.count[page[r]]);
+                copy = !(n == w.rows[at] && w.first[at] == r);
             }
             need = before[r] + copy;
             kept[r] += copy;
