@@ -53,20 +53,6 @@ __device__ __forceinline__ void report(const PagesArgs& a, int code)
     atomicMin(&a.ws.plan->bad, code);
 }
 
-/* A table entry is a page of the pool that the state holds. */
-__device__ __forceinline__ bool page_ok(const PagesArgs& a, int p)
-{
-    return p >= 0 && p < a.geo.n_pages && a.from.refs[p] > 0;
-}
-
-__device__ __forceinline__ RowStep step_of(const PagesArgs& a, int r, int& parent)
-{
-    parent = a.parents ? a.parents[r] : r;
-    const int len = parent >= 0 && parent < a.from_rows ? a.from.lengths[parent] : 0;
-    return row_step(parent, a.from_rows, len, a.grow ? a.grow[r] : 0, a.geo.page_tokens,
-                    a.geo.max_slots);
-}
-
 /* kGatherRows rows of the new tables, 256 slots of each, gathered from
  * their parents' rows, and their pages counted: neighbouring rows that share
  * a page count it at once.  CHECK: nothing but whether the tables are valid. */
@@ -76,45 +62,57 @@ __device__ __forceinline__ void gather_rows(const PagesArgs& a, int group)
     const int across = slot_groups(a.geo.max_slots);
     const int r0 = group / across * kGatherRows;
     const int slot = group % across * kB + (int)threadIdx.x;
-    int page[kGatherRows];
+    /* in stages, each loading for all the rows at once (from a valid place where a row has
+     * nothing to load): row by row the loads would wait for each other */
+    int parent[kGatherRows], grow[kGatherRows], length[kGatherRows], page[kGatherRows];
+    int held[kGatherRows];
+    RowStep step[kGatherRows];
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q) {
+        const int r = r0 + q < a.rows ? r0 + q : r0;
+        parent[q] = a.parents ? a.parents[r] : r;
+        grow[q] = a.grow ? a.grow[r] : 0;
+    }
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q)
+        length[q] =
+            a.from.lengths[parent[q] >= 0 && parent[q] < a.from_rows ? parent[q] : 0];
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q) {
+        step[q] = row_step(parent[q], a.from_rows, length[q], grow[q], a.geo.page_tokens,
+                           a.geo.max_slots);
+        const bool in = slot < step[q].kept;
+        page[q] = a.from.table[in ? (int64_t)parent[q] * a.geo.max_slots + slot : 0];
+    }
+#pragma unroll
+    for (int q = 0; q < kGatherRows; ++q)
+        held[q] = a.from.refs[page[q] >= 0 && page[q] < a.geo.n_pages ? page[q] : 0];
     bool ours[kGatherRows]; /* the slot of a page that the row goes on writing is
                                the deciding workgroup's to write, alone: nothing orders plain
                                stores of two XCDs to one word within a launch */
 #pragma unroll
     for (int q = 0; q < kGatherRows; ++q) {
-        page[q] = -1;
-        ours[q] = false;
-        if (r0 + q >= a.rows) continue;
-        int parent;
-        const RowStep s = step_of(a, r0 + q, parent);
-        if (s.bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
-        if (slot < s.kept) {
-            page[q] = a.from.table[(int64_t)parent * a.geo.max_slots + slot];
-            ours[q] = s.tail == 0 || slot != s.kept - 1;
-            if (!page_ok(a, page[q])) {
-                page[q] = -1;
-                report(a, G4S_ERR_FORMAT);
-            }
+        const bool in = r0 + q < a.rows && slot < step[q].kept;
+        /* a table entry is a page of the pool that the state holds */
+        const bool ok = page[q] >= 0 && page[q] < a.geo.n_pages && held[q] > 0;
+        if (in && !ok) report(a, G4S_ERR_FORMAT);
+        if (r0 + q < a.rows && step[q].bad && slot == 0) report(a, G4S_ERR_INVALID_ARGUMENT);
+        page[q] = in && ok ? page[q] : -1;
+        ours[q] = step[q].tail == 0 || slot != step[q].kept - 1;
+        if (CHECK) continue;
+        /* the row's step for the workgroup that decides, by the thread that holds
+         * its last kept slot: one read there instead of four that depend on each other */
+        if (r0 + q < a.rows && slot == (step[q].kept > 0 ? step[q].kept - 1 : 0)) {
+            const int64_t r = r0 + q;
+            st_dev(&a.ws.steps[3 * r],
+                   (uint64_t)(uint32_t)step[q].fresh << 32 | (uint32_t)step[q].kept);
+            st_dev(&a.ws.steps[3 * r + 1],
+                   (uint64_t)(uint32_t)step[q].tail << 32 |
+                       (uint32_t)(step[q].tail ? page[q] : -1));
+            st_dev(&a.ws.steps[3 * r + 2], (uint64_t)step[q].length);
         }
     }
     if (CHECK) return;
-    /* the rows' steps for the workgroup that decides, by threads of the last
-     * wave, whose slots are the least often used: one read there instead of four that
-     * depend on each other */
-    const int mine = (int)threadIdx.x - (kB - 64);
-    if (group % across == 0 && mine >= 0 && mine < kGatherRows && r0 + mine < a.rows) {
-        const int r = r0 + mine;
-        int parent;
-        const RowStep s = step_of(a, r, parent);
-        int p = -1;
-        if (s.tail) {
-            p = a.from.table[(int64_t)parent * a.geo.max_slots + s.kept - 1];
-            if (!page_ok(a, p)) p = -1;
-        }
-        st_dev(&a.ws.steps[3 * r], (uint64_t)(uint32_t)s.fresh << 32 | (uint32_t)s.kept);
-        st_dev(&a.ws.steps[3 * r + 1], (uint64_t)(uint32_t)s.tail << 32 | (uint32_t)p);
-        st_dev(&a.ws.steps[3 * r + 2], (uint64_t)s.length);
-    }
     uint32_t fresh = 0, run = 0;
 #pragma unroll
     for (int q = 0; q < kGatherRows; ++q) {
