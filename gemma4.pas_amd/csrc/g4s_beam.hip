@@ -370,11 +370,11 @@ __device__ __forceinline__ double sum_four(const float (&t)[4])
  * The workgroup that ends last in a row merges its chunks, the one that ends
  * last in a sequence its rows.
  *
- * 512 rows of 262,144 bf16 logits: 72 us, 3.7 TB/s, of which the lookups and
- * additions issue for about 45 us beside the loads and the listing adds 6; without the
- * table 181 us (issue), with the binary64 softmax throughout 841.  64 binary32 rows: 36 us, a
- * third of it issue, the rest the start and the two merges, which
- * nothing overlaps.  Four rows: 17 us, all of it latency. */
+ * 512 rows of 262,144 bf16 logits: 72 us, 3.7 TB/s; their tiles move 4.8, and the start and
+ * the end of the workgroups, 17 us, overlap nothing.  Without the table 181 us
+ * (issue), with the binary64 softmax throughout 841.  64 binary32 rows: 36 us,
+ * 11 of them the terms' issue, 20 the start and the merges.  Four rows:
+ * 17 us, all of it latency. */
 template <int DT, int MODE, bool TABLE, int BLOCK>
 __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
 {

@@ -210,8 +210,9 @@ __device__ __forceinline__ RowRecord read_row(const PagesArgs& a, int r)
 /* Scan and gather, all side by side; the workgroup that ends last then decides
  * which rows copy the page they write, what each row takes, and who gets
  * which free page.  Bound by the chain of reads that each depend on the last (parent, length,
- * page, count): 9 us for one sequence of four beams, 12.5 us for 192 rows of
- * some 125 pages; three launches for the same took 12 and 18. */
+ * page, count): 8 us for one sequence of four beams, half of them the
+ * gathering, 11 us for 192 rows of some 125 pages; three launches for the same took
+ * 12 and 18. */
 __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
 {
     extern __shared__ int lds[];
