@@ -13,7 +13,7 @@ import beam_oracle as bo
 from gemma4_sampler import beam, hip, native
 
 pytestmark = pytest.mark.gpu
-F32 = np.float32
+F32, I32 = np.float32, np.int32
 LSE = 2e-7
 NONE = -np.inf
 
@@ -304,6 +304,39 @@ def test_other_stream_and_another_handle():
     for st in streams:
         check(peaky(rng, 4, 9999, "f32"), running(rng, 4), 4, 8, stream=st)
     for st in streams:
+        st.destroy()
+
+
+def test_two_handles_side_by_side():
+    """Calls of two handles on two streams, none waited for before the last."""
+    rng = np.random.default_rng(40)
+    V, W, n = 60013, 4, 8
+    jobs = []
+    for k in range(2):
+        st = hip.Stream(nonblocking=True)
+        jobs.append((st, beam.BeamSearch(V, 6, W, 30.0, stream=st)))
+    calls = []
+    for k in range(6):
+        st, search = jobs[k % 2]
+        batch = 1 + k
+        x, s = peaky(rng, batch * W, V, "f32"), running(rng, batch * W)
+        stride = (V + 3) // 4 * 4
+        buf = np.zeros((batch * W, stride), F32)
+        buf[:, :V] = x
+        d = [hip.Buffer.from_array(a) for a in (buf, s)] + [hip.Buffer(4 * batch * n)
+                                                            for _ in range(3)]
+        calls.append((search, batch, stride, x, s, d))
+    hip.synchronize()
+    for search, batch, stride, _, _, d in calls:
+        search.select(d[0], batch, W, d[1], n, d[2], d[3], d[4], row_stride=stride)
+    hip.synchronize()
+    for _, batch, _, x, s, d in calls:
+        p, t, o, _ = bo.select(x, s, W, n, 30.0)
+        assert np.array_equal(d[2].download(I32).reshape(p.shape), p)
+        assert np.array_equal(d[3].download(I32).reshape(t.shape), t)
+        assert close(d[4].download(F32).reshape(o.shape).astype(np.float64), o)
+    for st, search in jobs:
+        search.close()
         st.destroy()
 
 
