@@ -944,13 +944,20 @@ void select_launch(const BeamSelectArgs& a, const BeamPlan& plan, hipStream_t st
 BeamPlan beam_plan(int32_t vocab, int32_t rows, int32_t dtype, int32_t mode, int32_t ncu)
 {
     BeamPlan p{};
-    const int64_t big = (vocab + kBeamTableTile - 1) / kBeamTableTile;
-    p.table = dtype == G4S_DTYPE_BF16 && mode != kCapExact && rows * big >= 4 * (int64_t)ncu;
+    /* Looking terms up takes loading the table (30 KiB a workgroup) and tiles of four times
+     * the size.  It pays from about half such a tile a CU on: 8 rows of 262,144 take 19 us
+     * with it and 21 without, 64 rows 25.5 and 34.3, 160 rows 41 and 61 (4 rows 18.6 and 17.3;
+     * 64 rows of 33,000 20 and 18).  Rows that do not fill two tiles are better without:
+     * 2,048 rows of 8,000 take 64 us with it and 37 without, of 16,000 59 and 56; 512 rows of
+     * 33,000 26 and 43. */
+    p.table = dtype == G4S_DTYPE_BF16 && mode != kCapExact && vocab >= 2 * kBeamTableTile &&
+              (int64_t)rows * vocab >= (int64_t)ncu * kBeamTableTile / 2;
     const int32_t tile = p.table ? kBeamTableTile : kBeamTile;
     const int32_t all = (vocab + tile - 1) / tile;
     /* a row's workgroups: the fewest tiles that some CU takes one after another, its workgroups
-     * side by side counted as if in turn from `full` on, where they fill it; the
-     * start and end of a workgroup cost about a tile */
+     * side by side counted as if in turn from `full` on, where they fill it; the start and end
+     * of a workgroup cost about a tile (two with a table: 160 rows of 50,000 in four
+     * workgroups a row take 37 us, in two 27) */
     const int64_t full = p.table ? 2 : 3;
     int64_t least = INT64_MAX;
     for (int32_t tiles = 1; tiles <= all; ++tiles) {
@@ -958,7 +965,7 @@ BeamPlan beam_plan(int32_t vocab, int32_t rows, int32_t dtype, int32_t mode, int
         if (chunks > 1 && (int64_t)rows * chunks > beam_max_chunks(vocab, rows, ncu)) continue;
         int64_t each = ((int64_t)rows * chunks + ncu - 1) / ncu;
         if (each < full) each = full;
-        const int64_t cost = each * (tiles + 1);
+        const int64_t cost = each * (tiles + (p.table ? 2 : 1));
         if (cost < least) {
             least = cost;
             p.chunks = chunks;

@@ -164,7 +164,8 @@ int g4s_pages_advance(g4s_pages* pages, const g4s_page_state* from, int32_t from
  * page at n or above moves into the i-th free page below n, in the pool and
  * in the tables of `to`, which holds pages 0 .. n-1 alone.  Arguments, status
  * (word 2 is 0, word 3 the pages moved) and errors as for g4s_pages_advance;
- * `from` stays valid. */
+ * `from` stays valid.  `rows` covers every row that holds pages: the tables of
+ * rows behind them are left as they are, but the pages move. */
 int g4s_pages_compact(g4s_pages* pages, const g4s_page_state* from, const g4s_page_state* to,
                       int32_t rows, void* d_pool, int32_t* d_status);
 

@@ -254,6 +254,24 @@ def test_many_rows(dtype, cap, V, batch, beams, n):
     check(x, running(rng, batch * beams), beams, n, cap=cap)
 
 
+@pytest.mark.parametrize("V, batch, beams, n", [
+    (32767, 8, 9, 18), (32768, 8, 8, 16), (32769, 13, 5, 10), (65536, 4, 8, 9), (65537, 3, 11, 22),
+    (262143, 2, 4, 8), (262144, 1, 8, 16), (100003, 7, 3, 6)])
+def test_bf16_rows_of_few_tiles(V, batch, beams, n):
+    """About the fewest rows, and the shortest, whose terms are looked up: a
+    workgroup has one tile or two, the last of them with a few tokens."""
+    rng = np.random.default_rng(V + batch)
+    x = peaky(rng, batch * beams, V, "bf16")
+    x[1, :16384] = 0xFF80               # a tile without candidates
+    x[2, -5:] = bo.bf16(np.array([21, 22, 23, 24, 25], F32))
+    x[3] = 0xFF80
+    x[4, V - 1], x[5, 7] = 0x7FC1, 0x7F80
+    check(x, running(rng, batch * beams), beams, n)
+    s = running(rng, batch * beams)
+    s[::3] = NONE
+    check(x, s, beams, beams, inplace=True)
+
+
 def test_stride_no_lse_and_scores_in_place():
     rng = np.random.default_rng(15)
     x = peaky(rng, 6, 10007, "bf16")
