@@ -363,7 +363,7 @@ __device__ __forceinline__ double sum_four(const float (&t)[4])
  * issue as binary32's other than multiply-add do on this machine (4.7 against 2.7
  * cycles measured), and its fraction alone goes through binary32's exponential:
  * binary32 throughout leaves errors of 1e-6 in the terms of equal logits, and rows of
- * bf16 have thousands of those.  bf16 logits of large batches need no
+ * bf16 have thousands of those.  bf16 logits in long rows of a batch need no
  * arithmetic: their terms are looked up (TABLE), 30 KiB in LDS that hold the
  * terms of all values from 2^-24 to 64.
  *
