@@ -31,6 +31,12 @@ struct RowStep {
                        without tokens is returned) */
 };
 
+/* Slots of a row of `tokens` tokens.  A row may hold 2^31 - 1: the sum passes 32 bits. */
+G4S_PAGE_HD int32_t used_slots(int64_t tokens, int32_t page_tokens)
+{
+    return (int32_t)((tokens + page_tokens - 1) / page_tokens);
+}
+
 G4S_PAGE_HD RowStep row_step(int32_t parent, int32_t from_rows, int32_t parent_length, int32_t grow,
                         int32_t page_tokens, int32_t max_slots)
 {
@@ -44,8 +50,8 @@ G4S_PAGE_HD RowStep row_step(int32_t parent, int32_t from_rows, int32_t parent_l
     if (now > room) return s;
     const int64_t keep = old < now ? old : now;
     s.length = now;
-    s.kept = (int32_t)((keep + page_tokens - 1) / page_tokens);
-    s.fresh = (int32_t)((now + page_tokens - 1) / page_tokens) - s.kept;
+    s.kept = used_slots(keep, page_tokens);
+    s.fresh = used_slots(now, page_tokens) - s.kept;
     s.tail = now > keep ? (int32_t)(keep % page_tokens) : 0;
     s.bad = 0;
     return s;

@@ -518,8 +518,7 @@ __global__ __launch_bounds__(kB) void pages_compact_kernel(PagesArgs a)
         const int64_t S = a.geo.max_slots, cells = ok ? a.rows * S : 0;
         for (int64_t c = at; c < cells; c += step) {
             const int r = (int)(c / S);
-            const int used = (a.from.lengths[r] + a.geo.page_tokens - 1) / a.geo.page_tokens;
-            if (c - r * S >= used) continue;
+            if (c - r * S >= used_slots(a.from.lengths[r], a.geo.page_tokens)) continue;
             int p = a.from.table[c];
             if (p >= plan.live) p = nth_page<true>(a, p - free_before(a, p) - plan.below);
             a.to.table[c] = p;

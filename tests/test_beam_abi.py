@@ -194,6 +194,14 @@ def test_row_step(host, args, want):
     assert host.step(*args) == want
 
 
+@pytest.mark.parametrize("tokens, page_tokens, want", [
+    (0, 1, 0), (1, 16, 1), (16, 16, 1), (17, 16, 2), (MAX, 1, MAX), (MAX, 65536, 32768),
+    (3000 * 715827, 3000, 715827), (3000 * 715827 - 2999, 3000, 715827)])
+def test_used_slots(host, tokens, page_tokens, want):
+    host.t_used_slots.argtypes = [ctypes.c_int64, ctypes.c_int32]
+    assert host.t_used_slots(tokens, page_tokens) == want
+
+
 def test_offsets_pass_32_bits(host):
     g = beam.PageGeometry(32, 1 << 20, 1, 1, 4, 2, 4096, (1 << 20) * 262144, 262144)
     assert host.t_geometry_ok(ctypes.byref(g)) == 1

@@ -243,6 +243,16 @@ def test_compact_edges():
     rig.compact()
 
 
+def test_compact_longest_rows():
+    """A row of nearly 2^31 tokens, all of max_slots pages, behind one that ends:
+    the tokens of its last page are counted past 32 bits."""
+    P, S = 3000, 715827
+    rig = Rig(P, 715900, 2, S, planes=0, parts=0, token=0)
+    assert rig.advance([-1, -1], [7 * P, S * P])[:3] == (0, 66, 715834)
+    rig.advance([-1, 1], None)
+    assert rig.compact() == (0, 73, 0, 7)
+
+
 def test_many_rows():
     """More rows than a workgroup has threads, all writing one page."""
     R = 1100
