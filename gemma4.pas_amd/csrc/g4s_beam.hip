@@ -859,22 +859,34 @@ __global__ __launch_bounds__(kB) void beam_reorder_kernel(BeamReorderArgs a)
 }
 
 template <typename T>
-hipError_t reorder_with(const BeamReorderArgs& a, hipStream_t stream)
+hipError_t reorder_with(const BeamReorderArgs& all, hipStream_t stream)
 {
-    const int64_t cols = a.row_bytes / (int64_t)sizeof(T);
-    const int64_t groups = (int64_t)a.batch * a.planes;
-    const dim3 grid((unsigned)((cols + kB - 1) / kB), (unsigned)(groups < 65535 ? groups : 65535));
-    if (a.beams <= 4)
-        beam_reorder_kernel<T, 4><<<grid, kB, 0, stream>>>(a);
-    else if (a.beams <= 8)
-        beam_reorder_kernel<T, 8><<<grid, kB, 0, stream>>>(a);
-    else if (a.beams <= 16)
-        beam_reorder_kernel<T, 16><<<grid, kB, 0, stream>>>(a);
-    else if (a.beams <= 32)
-        beam_reorder_kernel<T, 32><<<grid, kB, 0, stream>>>(a);
-    else
-        beam_reorder_kernel<T, 64><<<grid, kB, 0, stream>>>(a);
-    return hipGetLastError();
+    /* a launch has fewer than 2^32 threads across, and more would be cut off
+     * without an error: longer rows (odd ones of 4 GiB) go column range by column range */
+    constexpr int64_t kMost = (int64_t)1 << 31;
+    const int64_t cols = all.row_bytes / (int64_t)sizeof(T);
+    const int64_t groups = (int64_t)all.batch * all.planes;
+    for (int64_t first = 0; first < cols; first += kMost) {
+        BeamReorderArgs a = all;
+        const int64_t n = cols - first < kMost ? cols - first : kMost;
+        a.src += first * (int64_t)sizeof(T);
+        a.dst += first * (int64_t)sizeof(T);
+        a.row_bytes = n * (int64_t)sizeof(T);
+        const dim3 grid((unsigned)((n + kB - 1) / kB), (unsigned)(groups < 65535 ? groups : 65535));
+        if (a.beams <= 4)
+            beam_reorder_kernel<T, 4><<<grid, kB, 0, stream>>>(a);
+        else if (a.beams <= 8)
+            beam_reorder_kernel<T, 8><<<grid, kB, 0, stream>>>(a);
+        else if (a.beams <= 16)
+            beam_reorder_kernel<T, 16><<<grid, kB, 0, stream>>>(a);
+        else if (a.beams <= 32)
+            beam_reorder_kernel<T, 32><<<grid, kB, 0, stream>>>(a);
+        else
+            beam_reorder_kernel<T, 64><<<grid, kB, 0, stream>>>(a);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace

@@ -455,6 +455,24 @@ def test_reorder_refusals():
     s.close()
 
 
+def test_reorder_rows_past_32_bits():
+    """Rows of more than 2^32 bytes at an odd address, a thread a byte."""
+    row = (1 << 32) + 1027
+    rng = np.random.default_rng(19)
+    s = beam.BeamSearch(100, 1, 2, 30.0)
+    d = hip.Buffer(1 + 2 * row).zero()
+    at = [0, 1 << 31, (1 << 32) - 300, row - 600]
+    data = {(r, a): rng.integers(1, 256, 600, dtype=np.uint8) for r in range(2) for a in at}
+    for (r, a), piece in data.items():
+        d.upload(piece, 1 + r * row + a)
+    s.reorder(d.offset(1), d.offset(1), 1, 0, 1, 2, row, row,
+              hip.Buffer.from_array(np.array([1, 0], I32)))
+    hip.synchronize()
+    for (r, a), piece in data.items():
+        assert np.array_equal(d.download(np.uint8, 600, 1 + (1 - r) * row + a), piece), (r, a)
+    s.close()
+
+
 def test_captured_step():
     """Selection and reordering in one captured graph, replayed on new logits
     with eager calls between."""
