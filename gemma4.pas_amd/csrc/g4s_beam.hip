@@ -12,6 +12,7 @@
  */
 #include "g4s_beam.h"
 
+#include "g4s_launch.h"
 #include "g4s_select.h"
 
 namespace g4s {
@@ -873,17 +874,17 @@ hipError_t reorder_with(const BeamReorderArgs& all, hipStream_t stream)
         a.dst += first * (int64_t)sizeof(T);
         a.row_bytes = n * (int64_t)sizeof(T);
         const dim3 grid((unsigned)((n + kB - 1) / kB), (unsigned)(groups < 65535 ? groups : 65535));
+        hipError_t e;
         if (a.beams <= 4)
-            beam_reorder_kernel<T, 4><<<grid, kB, 0, stream>>>(a);
+            e = launch(beam_reorder_kernel<T, 4>, grid, kB, 0, stream, a);
         else if (a.beams <= 8)
-            beam_reorder_kernel<T, 8><<<grid, kB, 0, stream>>>(a);
+            e = launch(beam_reorder_kernel<T, 8>, grid, kB, 0, stream, a);
         else if (a.beams <= 16)
-            beam_reorder_kernel<T, 16><<<grid, kB, 0, stream>>>(a);
+            e = launch(beam_reorder_kernel<T, 16>, grid, kB, 0, stream, a);
         else if (a.beams <= 32)
-            beam_reorder_kernel<T, 32><<<grid, kB, 0, stream>>>(a);
+            e = launch(beam_reorder_kernel<T, 32>, grid, kB, 0, stream, a);
         else
-            beam_reorder_kernel<T, 64><<<grid, kB, 0, stream>>>(a);
-        const hipError_t e = hipGetLastError();
+            e = launch(beam_reorder_kernel<T, 64>, grid, kB, 0, stream, a);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
@@ -936,19 +937,18 @@ __global__ __launch_bounds__(kB) void beam_init_kernel(BeamWorkspace ws, BeamSof
 }
 
 template <int DT, int MODE>
-void select_launch(const BeamSelectArgs& a, const BeamPlan& plan, hipStream_t stream)
+hipError_t select_launch(const BeamSelectArgs& a, const BeamPlan& plan, hipStream_t stream)
 {
     const dim3 grid((unsigned)a.chunks, (unsigned)(a.batch * a.beams));
     const size_t scores = sizeof(double) * a.beams * a.n;
     if constexpr (DT == 1 && MODE != kCapExact) {
         if (plan.table) {
             const size_t table = sizeof(float) * 2 * kBeamTableHalf;
-            beam_select_kernel<DT, MODE, true, 512>
-                <<<grid, 512, table > scores ? table : scores, stream>>>(a);
-            return;
+            return launch(beam_select_kernel<DT, MODE, true, 512>, grid, 512,
+                          table > scores ? table : scores, stream, a);
         }
     }
-    beam_select_kernel<DT, MODE, false, kB><<<grid, kB, scores, stream>>>(a);
+    return launch(beam_select_kernel<DT, MODE, false, kB>, grid, kB, scores, stream, a);
 }
 
 }  // namespace
@@ -998,10 +998,8 @@ hipError_t beam_init_launch(const BeamWorkspace& ws, const BeamSoftcap& cap, int
                             hipStream_t stream)
 {
     if (cap.mode == kCapNone)
-        beam_init_kernel<kCapNone><<<64, kB, 0, stream>>>(ws, cap, tickets);
-    else
-        beam_init_kernel<kCapPoly><<<64, kB, 0, stream>>>(ws, cap, tickets);
-    return hipGetLastError();
+        return launch(beam_init_kernel<kCapNone>, 64, kB, 0, stream, ws, cap, tickets);
+    return launch(beam_init_kernel<kCapPoly>, 64, kB, 0, stream, ws, cap, tickets);
 }
 
 hipError_t beam_select_launch(const BeamSelectArgs& a, const BeamPlan& plan, int32_t dtype,
@@ -1009,12 +1007,13 @@ hipError_t beam_select_launch(const BeamSelectArgs& a, const BeamPlan& plan, int
 {
     const bool f32 = dtype == G4S_DTYPE_F32;
     if (a.cap.mode == kCapNone)
-        f32 ? select_launch<0, kCapNone>(a, plan, stream) : select_launch<1, kCapNone>(a, plan, stream);
-    else if (a.cap.mode == kCapPoly)
-        f32 ? select_launch<0, kCapPoly>(a, plan, stream) : select_launch<1, kCapPoly>(a, plan, stream);
-    else
-        f32 ? select_launch<0, kCapExact>(a, plan, stream) : select_launch<1, kCapExact>(a, plan, stream);
-    return hipGetLastError();
+        return f32 ? select_launch<0, kCapNone>(a, plan, stream)
+                   : select_launch<1, kCapNone>(a, plan, stream);
+    if (a.cap.mode == kCapPoly)
+        return f32 ? select_launch<0, kCapPoly>(a, plan, stream)
+                   : select_launch<1, kCapPoly>(a, plan, stream);
+    return f32 ? select_launch<0, kCapExact>(a, plan, stream)
+               : select_launch<1, kCapExact>(a, plan, stream);
 }
 
 hipError_t beam_reorder_launch(const BeamReorderArgs& a, hipStream_t stream)

@@ -15,6 +15,7 @@
 #include <limits.h>
 
 #include "g4s_device.h"
+#include "g4s_launch.h"
 
 namespace g4s {
 
@@ -566,8 +567,7 @@ dim3 copy_grid(const g4s_page_geometry& g, int64_t jobs, int64_t least)
 
 hipError_t pages_init_launch(const PageWorkspace& ws, int32_t n_pages, hipStream_t stream)
 {
-    pages_init_kernel<<<256, kB, 0, stream>>>(ws, n_pages);
-    return hipGetLastError();
+    return launch(pages_init_kernel, 256, kB, 0, stream, ws, n_pages);
 }
 
 #define G4S_BY_WIDTH(bits, CALL)    \
@@ -588,37 +588,41 @@ static unsigned first_grid(const PagesArgs& a)
 
 hipError_t pages_advance_launch(const PagesArgs& a, hipStream_t stream)
 {
-    pages_advance_kernel<<<first_grid(a), kB, plan_lds(a.rows), stream>>>(a);
+    hipError_t e = launch(pages_advance_kernel, first_grid(a), kB, plan_lds(a.rows), stream, a);
+    if (e != hipSuccess) return e;
     const int64_t least = (a.geo.n_pages + kB - 1) / kB;
 #define G4S_CALL(T) \
-    pages_finish_kernel<T><<<copy_grid<T>(a.geo, a.rows, least), kB, 0, stream>>>(a)
+    e = launch(pages_finish_kernel<T>, copy_grid<T>(a.geo, a.rows, least), kB, 0, stream, a)
     G4S_BY_WIDTH(copy_bits(a.geo, a.pool, a.pool), G4S_CALL);
 #undef G4S_CALL
-    return hipGetLastError();
+    return e;
 }
 
 hipError_t pages_compact_launch(const PagesArgs& a, hipStream_t stream)
 {
-    pages_number_kernel<<<first_grid(a), kB, 0, stream>>>(a);
+    hipError_t e = launch(pages_number_kernel, first_grid(a), kB, 0, stream, a);
+    if (e != hipSuccess) return e;
     const int64_t cell = (int64_t)a.rows * a.geo.max_slots;
     const int64_t least = ((cell > a.geo.n_pages ? cell : a.geo.n_pages) + kB - 1) / kB;
-#define G4S_CALL(T) \
-    pages_compact_kernel<T><<<copy_grid<T>(a.geo, a.geo.n_pages / 2, least), kB, 0, stream>>>(a)
+#define G4S_CALL(T)                                                                         \
+    e = launch(pages_compact_kernel<T>, copy_grid<T>(a.geo, a.geo.n_pages / 2, least), kB, 0, \
+               stream, a)
     G4S_BY_WIDTH(copy_bits(a.geo, a.pool, a.pool), G4S_CALL);
 #undef G4S_CALL
-    return hipGetLastError();
+    return e;
 }
 
 hipError_t pages_copy_launch(const g4s_page_geometry& geo, const char* src, char* dst, int32_t n,
                              const int32_t* d_src, const int32_t* d_dst, const int32_t* d_tokens,
                              hipStream_t stream)
 {
-#define G4S_CALL(T)                                                                     \
-    pages_copy_kernel<T><<<copy_grid<T>(geo, n, 1), kB, 0, stream>>>(geo, src, dst, n, d_src, \
-                                                                     d_dst, d_tokens)
+    hipError_t e;
+#define G4S_CALL(T)                                                                       \
+    e = launch(pages_copy_kernel<T>, copy_grid<T>(geo, n, 1), kB, 0, stream, geo, src, dst, n, \
+               d_src, d_dst, d_tokens)
     G4S_BY_WIDTH(copy_bits(geo, src, dst), G4S_CALL);
 #undef G4S_CALL
-    return hipGetLastError();
+    return e;
 }
 
 }  // namespace g4s

@@ -473,6 +473,46 @@ def test_reorder_rows_past_32_bits():
     s.close()
 
 
+def test_an_earlier_failure_is_not_the_calls():
+    """A failed HIP call of the caller leaves its error with the thread; the
+    calls report their own launches."""
+    import ctypes
+
+    def earlier():
+        assert hip.lib().hipSetDevice(ctypes.c_int(1 << 20)) != 0
+    rng = np.random.default_rng(21)
+    earlier()
+    s = beam.BeamSearch(1001, 1, 3, 30.0)
+    x = peaky(rng, 3, 1001, "f32")
+    orig = s.select
+    s.select = lambda *a, **k: (earlier(), orig(*a, **k))
+    check(x, running(rng, 3), 3, 6, search=s)
+    d, par = hip.Buffer(3 * 64).zero(), hip.Buffer.from_array(np.array([1, 0, 2], I32))
+    data = rng.integers(0, 256, (3, 64), dtype=np.uint8)
+    d.upload(data)
+    earlier()
+    s.reorder(d, d, 1, 0, 1, 3, 64, 64, par)
+    hip.synchronize()
+    assert np.array_equal(d.download(np.uint8).reshape(3, 64), data[[1, 0, 2]])
+    earlier()
+    c = beam.PageCache(4, 8, 2, 4, planes=1, parts=1, token_bytes=16)
+    states = []
+    for _ in range(2):
+        bufs = [hip.Buffer(4 * n).zero() for n in (8, 2, 8)]
+        states.append((bufs, beam.PageState(*bufs)))
+    (_, a), (_, b) = states
+    pool, status, one = hip.Buffer(8 * 64).zero(), hip.Buffer(16), hip.Buffer(64).zero()
+    for call in (lambda: c.advance(a, 2, b, 2, one, None, pool, status),
+                 lambda: c.compact(a, b, 2, pool, status),
+                 lambda: c.copy(pool, pool, 1, one,
+                                hip.Buffer.from_array(np.array([1], I32)))):
+        earlier()
+        call()
+        hip.synchronize()
+    s.close()
+    c.close()
+
+
 def test_captured_step():
     """Selection and reordering in one captured graph, replayed on new logits
     with eager calls between."""
