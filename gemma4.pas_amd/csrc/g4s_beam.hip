@@ -47,12 +47,15 @@ constexpr double kLn2 = 0x1.62e42fefa39efp-1;
 __device__ __forceinline__ uint64_t d2u(double x) { return __builtin_bit_cast(uint64_t, x); }
 __device__ __forceinline__ double u2d(uint64_t u) { return __builtin_bit_cast(double, u); }
 
-/* cap * tanh(x / cap), off by some 2^-52 of the cap. */
+/* cap * tanh(x / cap).  kCapPoly (caps of up to 80): off by some 2^-52 of the cap,
+ * below 1e-13.  kCapExact, whatever the cap: by less than 2^-49 of the value itself, since 1 - e
+ * would leave nothing of a logit far below its cap. */
 template <int MODE>
 __device__ __forceinline__ double softcap64(float x, const BeamSoftcap& c)
 {
     if constexpr (MODE == kCapNone) return (double)x;
     const double cap = (double)c.cap;
+    if constexpr (MODE == kCapExact) return cap * cr::tanh_fast_d((double)x / cap);
     const double e = exp_fast_d(fmax(-2.0 * fabs((double)x) / cap, -80.0));
     return copysign(cap * ((1.0 - e) / (1.0 + e)), (double)x);
 }

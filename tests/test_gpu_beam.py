@@ -98,6 +98,17 @@ def test_softcaps(cap):
     check(bo.bf16(x), running(rng, 8), 4, 8, cap=cap)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e9, 1e15, 1e30])
+def test_softcaps_far_above_the_logits(cap, dtype):
+    """A cap that is practically none leaves the logits as they are: the error of
+    the softcap is relative to its value, not to the cap."""
+    rng = np.random.default_rng(50)
+    x = peaky(rng, 8, 20011, "f32") * F32(2)
+    x[:, 100] = 1e-3
+    check(x if dtype == "f32" else bo.bf16(x), running(rng, 8), 4, 8, cap=cap)
+
+
 def test_most_beams():
     rng = np.random.default_rng(6)
     check(peaky(rng, 128, 3001, "f32"), running(rng, 128), 64, 128)
