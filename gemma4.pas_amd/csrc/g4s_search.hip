@@ -127,6 +127,17 @@ bool overlap(const void* a, int64_t na, const void* b, int64_t nb)
     return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
 }
 
+/* An array of a call; NULL ones overlap nothing. */
+struct Span {
+    const char* name;
+    const void* at;
+    int64_t bytes;
+};
+bool overlap(const Span& a, const Span& b)
+{
+    return a.at && b.at && overlap(a.at, a.bytes, b.at, b.bytes);
+}
+
 /* Parts of one allocation, each on a 256-byte boundary. */
 class Carver {
 public:
@@ -345,10 +356,28 @@ G4S_API int g4s_beam_select(g4s_beam* h, const void* d_logits, int32_t dtype, in
     if (n_select < 1 || n_select > 2 * h->max_beams)
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "n_select %d outside [1, %d]", n_select,
                     2 * h->max_beams);
-    if ((d_out != d_scores || n_select != beams) &&
-        overlap(d_out, (int64_t)batch * n_select * 4, d_scores, (int64_t)batch * beams * 4))
-        return fail(h, G4S_ERR_INVALID_ARGUMENT,
-                    "d_out overlaps d_scores (allowed as the same array where n_select == beams)");
+    /* a sequence's results are written while others' logits and scores, or its own lse, are
+     * still to be read or written */
+    const int64_t rows = (int64_t)batch * beams, found = (int64_t)batch * n_select * 4;
+    const int64_t esize = dtype == G4S_DTYPE_F32 ? 4 : 2;
+    const Span out[4] = {{"d_parents", d_parents, found},
+                         {"d_tokens", d_tokens, found},
+                         {"d_out", d_out, found},
+                         {"d_lse", d_lse, rows * 4}};
+    const Span in[2] = {{"d_scores", d_scores, rows * 4},
+                        {"d_logits", d_logits, ((rows - 1) * row_stride + h->vocab) * esize}};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j]))
+                return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s overlaps %s", out[i].name,
+                            out[j].name);
+        for (const Span& x : in)
+            if (overlap(out[i], x) &&
+                !(i == 2 && &x == &in[0] && d_out == d_scores && n_select == beams))
+                return fail(h, G4S_ERR_INVALID_ARGUMENT,
+                            "%s overlaps %s (d_out may be d_scores where n_select == beams)",
+                            out[i].name, x.name);
+    }
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, G4S_ERR_HIP, "device %d cannot be made current", h->device);
     return select(h, d_logits, dtype, row_stride, batch, beams, d_scores, n_select, d_parents,

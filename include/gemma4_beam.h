@@ -67,10 +67,12 @@ const char* g4s_beam_last_error(const g4s_beam* beam);
  *   d_parents  device [batch*n_select]  row that is continued
  *   d_tokens   device [batch*n_select]  its next token
  *   d_out      device [batch*n_select]  score, rounded once to binary32;
- *              may be d_scores only where n_select == beams
+ *              may be d_scores where n_select == beams
  *   d_lse      device [batch*beams] lse of each row, or NULL; -inf for a dead
  *              row and for one without candidates
  * Where a sequence has fewer candidates the rest is -1, -1, -inf.
+ * An output that overlaps another array of the call, or the span of the
+ * logits, is refused but for d_out == d_scores.
  * Stream-ordered.  lse is within 2e-7 of the exact value, absolutely: scores
  * of different beams that lie closer than that may come in either order. */
 int g4s_beam_select(g4s_beam* beam, const void* d_logits, int32_t dtype, int64_t row_stride,

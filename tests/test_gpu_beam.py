@@ -386,6 +386,32 @@ def test_select_refusals():
     s.close()
 
 
+def test_select_refuses_overlapping_arrays():
+    """Results of one sequence are written while scores and logits of others,
+    or its own, are still read."""
+    s = beam.BeamSearch(1000, 2, 4, 30.0)
+    d = hip.Buffer(8 * 1000 * 4)
+    o = hip.Buffer(8192).zero()
+    good = dict(d_logits=d.zero(), batch=2, beams=4, d_scores=o, n_select=4,
+                d_parents=o.offset(512), d_tokens=o.offset(1024), d_out=o.offset(1536),
+                d_lse=o.offset(2048))
+    out = ["d_parents", "d_tokens", "d_out", "d_lse"]
+    clashes = [{k: o.offset(28)} for k in out] + [{k: o} for k in out if k != "d_out"] + \
+        [{k: d.offset(8 * 4000 - 4)} for k in out] + [{k: d.offset(2000)} for k in out] + \
+        [{a: good[b]} for a in out for b in out if a != b] + \
+        [{"d_tokens": o.offset(512 + 28)}, {"d_out": o, "d_lse": o.offset(4)},
+         {"d_out": o, "d_parents": o}, {"d_out": o, "n_select": 3}, {"d_out": o, "n_select": 8}]
+    for change in clashes:
+        with pytest.raises(native.SamplerError) as e:
+            s.select(**dict(good, **change))
+        assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT and "overlaps" in str(e.value)
+    for change in [{}, {"d_out": o}, {"d_lse": None}, {"d_lse": o.offset(32)},
+                   {"d_parents": o.offset(1536 + 32)}]:
+        s.select(**dict(good, **change))
+    hip.synchronize()
+    s.close()
+
+
 # ----------------------------------------------------------------- reorder
 
 
