@@ -324,6 +324,8 @@ int reorder(g4s_beam* h, const void* d_src, void* d_dst, int64_t planes, int64_t
     const int64_t extent = (planes - 1) * plane_stride + (rows - 1) * row_stride + row_bytes;
     if (d_src != d_dst && overlap(d_src, extent, d_dst, extent))
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "d_src and d_dst overlap");
+    if (overlap(d_parents, rows * 4, d_dst, extent))
+        return fail(h, G4S_ERR_INVALID_ARGUMENT, "d_parents overlaps d_dst");
     if (row_bytes == 0) return G4S_OK;
     g4s::BeamReorderArgs a{};
     a.src = (const char*)d_src;

@@ -492,6 +492,20 @@ def test_reorder_refusals():
     s.close()
 
 
+def test_reorder_refuses_parents_in_the_destination():
+    s = beam.BeamSearch(100, 2, 4, 30.0)
+    d, e = hip.Buffer(1 << 16).zero(), hip.Buffer(1 << 16).zero()
+    size = 8192 + 7 * 1000 + 900
+    for src, par in [(d, d), (d, d.offset(size - 4)), (d, d.offset(7992)), (e, d.offset(996))]:
+        with pytest.raises(native.SamplerError) as err:
+            s.reorder(src, d, 2, 8192, 2, 4, 1000, 900, par)
+        assert err.value.code == native.G4S_ERR_INVALID_ARGUMENT
+    s.reorder(d, d, 2, 8192, 2, 4, 1000, 900, d.offset(size))
+    s.reorder(e, d, 2, 8192, 2, 4, 1000, 900, e)
+    hip.synchronize()
+    s.close()
+
+
 def test_reorder_rows_past_32_bits():
     """Rows of more than 2^32 bytes at an odd address, a thread a byte."""
     row = (1 << 32) + 1027
