@@ -472,8 +472,17 @@ G4S_API int g4s_pages_destroy(g4s_pages* h)
 
 namespace {
 
+/* Bytes from a pool's start to the end of its last page. */
+int64_t pool_extent(const g4s_page_geometry& g)
+{
+    if (g.planes == 0) return 0;
+    return (g.planes - 1) * g.plane_stride + (g.n_pages - 1) * g.page_stride +
+           (int64_t)g.parts * g.page_tokens * g.token_bytes;
+}
+
 int check_states(g4s_pages* h, const g4s_page_state* from, const g4s_page_state* to, int32_t rows,
-                 const void* d_pool, const int32_t* d_status)
+                 const int32_t* d_parents, const int32_t* d_grow, const void* d_pool,
+                 const int32_t* d_status)
 {
     if (!from || !to || !from->table || !from->lengths || !from->refs || !to->table ||
         !to->lengths || !to->refs || !d_status || (!d_pool && h->geo.planes > 0))
@@ -491,6 +500,26 @@ int check_states(g4s_pages* h, const g4s_page_state* from, const g4s_page_state*
         for (int j = 0; j < 3; ++j)
             if (overlap(f[i], n[i], t[j], n[j]))
                 return fail(h, G4S_ERR_INVALID_ARGUMENT, "the two states share memory");
+    /* what the call writes lies apart from all that it reads or writes besides */
+    const Span out[5] = {{"to->table", to->table, cells},
+                         {"to->lengths", to->lengths, lens},
+                         {"to->refs", to->refs, refs},
+                         {"d_status", d_status, 16},
+                         {"d_pool", d_pool, pool_extent(h->geo)}};
+    const Span in[5] = {{"from->table", from->table, cells},
+                        {"from->lengths", from->lengths, lens},
+                        {"from->refs", from->refs, refs},
+                        {"d_parents", d_parents, (int64_t)rows * 4},
+                        {"d_grow", d_grow, (int64_t)rows * 4}};
+    for (int i = 0; i < 5; ++i) {
+        for (int j = 0; j < i; ++j)
+            if (overlap(out[i], out[j]))
+                return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s overlaps %s", out[i].name,
+                            out[j].name);
+        for (const Span& x : in)
+            if (overlap(out[i], x))
+                return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s overlaps %s", out[i].name, x.name);
+    }
     return G4S_OK;
 }
 
@@ -518,7 +547,7 @@ G4S_API int g4s_pages_advance(g4s_pages* h, const g4s_page_state* from, int32_t 
 {
     if (!h) return fail(h, G4S_ERR_INVALID_ARGUMENT, "pages is NULL");
     h->err[0] = 0;
-    const int rc = check_states(h, from, to, rows, d_pool, d_status);
+    const int rc = check_states(h, from, to, rows, d_parents, d_grow, d_pool, d_status);
     if (rc) return rc;
     if (!d_parents) return fail(h, G4S_ERR_INVALID_ARGUMENT, "d_parents is NULL");
     if (from_rows < 1 || from_rows > h->geo.max_rows)
@@ -539,7 +568,7 @@ G4S_API int g4s_pages_compact(g4s_pages* h, const g4s_page_state* from, const g4
 {
     if (!h) return fail(h, G4S_ERR_INVALID_ARGUMENT, "pages is NULL");
     h->err[0] = 0;
-    const int rc = check_states(h, from, to, rows, d_pool, d_status);
+    const int rc = check_states(h, from, to, rows, nullptr, nullptr, d_pool, d_status);
     if (rc) return rc;
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, G4S_ERR_HIP, "device %d cannot be made current", h->device);
@@ -559,10 +588,12 @@ G4S_API int g4s_pages_copy(g4s_pages* h, const void* d_src_pool, void* d_dst_poo
     if (!d_src_pool || !d_dst_pool || !d_src_pages || !d_dst_pages)
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "pools and page lists must be non-NULL");
     const g4s_page_geometry& g = h->geo;
-    const int64_t extent = (g.planes - 1) * g.plane_stride + (g.n_pages - 1) * g.page_stride +
-                           (int64_t)g.parts * g.page_tokens * g.token_bytes;
+    const int64_t extent = pool_extent(g);
     if (d_src_pool != d_dst_pool && overlap(d_src_pool, extent, d_dst_pool, extent))
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "the two pools overlap");
+    for (const int32_t* list : {d_src_pages, d_dst_pages, d_tokens})
+        if (list && overlap(list, (int64_t)n * 4, d_dst_pool, extent))
+            return fail(h, G4S_ERR_INVALID_ARGUMENT, "a page list overlaps d_dst_pool");
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, G4S_ERR_HIP, "device %d cannot be made current", h->device);
     const hipError_t e =

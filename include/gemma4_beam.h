@@ -157,8 +157,9 @@ const char* g4s_pages_last_error(const g4s_pages* pages);
  * (G4S_ERR_FORMAT) `to` is left with empty rows and no page held, status
  * words 2 and 3 are 0, and the pool is not written.  `from` stays valid in any case
  * (its live pages are not written, so the call can be repeated from it); the
- * two states share no memory.  Rows of `to` from `rows` on are left alone.
- * Stream-ordered. */
+ * two states share no memory, and the arrays of `to`, the pool and d_status none
+ * with each other or with any other array of the call.  Rows of `to` from `rows`
+ * on are left alone.  Stream-ordered. */
 int g4s_pages_advance(g4s_pages* pages, const g4s_page_state* from, int32_t from_rows,
                       const g4s_page_state* to, int32_t rows, const int32_t* d_parents,
                       const int32_t* d_grow, void* d_pool, int32_t* d_status);
@@ -176,7 +177,8 @@ int g4s_pages_compact(g4s_pages* pages, const g4s_page_state* from, const g4s_pa
  * (pools of this geometry, or the same pool), the first d_tokens[i] tokens of
  * each part (d_tokens NULL = whole pages; clamped to 0 .. page_tokens).  A
  * pair with a page outside [0, n_pages) is left out.  The destination pages differ
- * from each other, and within one pool from the source pages.  Stream-ordered. */
+ * from each other, and within one pool from the source pages; the lists lie
+ * outside the destination pool.  Stream-ordered. */
 int g4s_pages_copy(g4s_pages* pages, const void* d_src_pool, void* d_dst_pool, int32_t n,
                    const int32_t* d_src_pages, const int32_t* d_dst_pages,
                    const int32_t* d_tokens);

@@ -393,3 +393,57 @@ def test_refusals():
         with pytest.raises(native.SamplerError) as e:
             rig.cache.copy(**dict(good, **change))
         assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT, change
+
+
+def test_overlapping_arrays_are_refused():
+    """One workgroup writes while others read: the status over a table, parents
+    inside the new state, lists inside the pool that is written."""
+    N, R, S = 8, 2, 4
+    c = beam.PageCache(4, N, R, S, planes=2, parts=1, token_bytes=16)
+    pool_bytes = 2 * N * 64
+    mem = hip.Buffer(8192).zero()
+    at = {"from": (0, 64, 128), "to": (256, 320, 384)}
+    pool, status, one, grow = (mem.offset(o) for o in (4096, 512, 576, 640))
+
+    def state(key, **other):
+        o = dict(zip(("table", "lengths", "refs"), at[key]))
+        o.update(other)
+        return beam.PageState(*(mem.offset(o[k]) for k in ("table", "lengths", "refs")))
+    good = dict(src=state("from"), src_rows=R, dst=state("to"), rows=R, d_parents=one, d_grow=grow,
+                d_pool=pool, d_status=status)
+    bad = [dict(d_status=mem.offset(o)) for o in (0, 28, 64, 156, 256, 320, 384, 576, 636, 4096,
+                                                  4096 + pool_bytes - 4)]
+    bad += [{k: mem.offset(o)} for k in ("d_parents", "d_grow")
+            for o in (256, 284, 320, 412, 512, 4096 + pool_bytes - 4)]
+    bad += [dict(dst=state("to", **k)) for k in (dict(lengths=284), dict(refs=260),
+                                                 dict(refs=320), dict(table=4096))]
+    bad += [dict(d_pool=mem.offset(o)) for o in (0, 160, 384, 512, 644)]
+    for change in bad:
+        for only in (None, "compact"):
+            args = dict(good, **change)
+            if only:
+                if "d_parents" in change or "d_grow" in change or \
+                        change.get("d_status", one).value in (one.value, one.value + 60):
+                    continue
+                args = {k: args[k] for k in ("src", "dst", "rows", "d_pool", "d_status")}
+                if change.get("d_pool", pool).value == mem.offset(644).value:
+                    continue
+            with pytest.raises(native.SamplerError) as e:
+                (c.compact if only else c.advance)(**args)
+            assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT, change
+    c.advance(**good)
+    c.advance(**dict(good, d_grow=one))                   # both are only read
+    c.advance(**dict(good, d_pool=mem.offset(656), d_status=mem.offset(4096)))
+    hip.synchronize()
+    mem.upload(np.array([0, 1, 2, 3], I32), 4096 - 16)
+    lists = [mem.offset(4096 - 8), mem.offset(4096 - 16)]
+    good = dict(d_src_pool=mem.offset(1024), d_dst_pool=pool, n=2, d_src_pages=lists[0],
+                d_dst_pages=lists[1], d_tokens=None)
+    for k in ("d_src_pages", "d_dst_pages", "d_tokens"):
+        for o in (4096 - 4, 4096 + pool_bytes - 4):
+            with pytest.raises(native.SamplerError) as e:
+                c.copy(**dict(good, **{k: mem.offset(o)}))
+            assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT, (k, o)
+    c.copy(**dict(good, d_tokens=mem.offset(1024)))       # inside the source: only read
+    hip.synchronize()
+    c.close()
