@@ -792,7 +792,11 @@ int generate(g4s_beam* h, int32_t batch, const g4s_beam_config& cfg, const void*
         }
         const g4s_beam_step step{p.step_tokens, p.step_parents, d.step_tokens,
                                  d.step_parents, rows,          current};
-        if (forward(user, &step) != 0)
+        const int refused = forward(user, &step);
+        /* it may have left another device current, whose null stream is not ours */
+        e = hipSetDevice(h->device);
+        if (e != hipSuccess) return hip_fail(h, e, "the search's device behind the forward call");
+        if (refused != 0)
             return fail(h, G4S_ERR_ABORTED, "the forward callback failed");
     }
     for (int32_t b = 0; b < batch; ++b)

@@ -228,8 +228,8 @@ typedef struct g4s_beam_step {
 
 /* The caller's model step: on return the raw logits of each row with a token
  * are in that row of the loop's logits buffer, written by work on the search's
- * stream or already complete.  0 to go on; anything else ends the loop with
- * G4S_ERR_ABORTED. */
+ * stream or already complete.  It may leave another device current.  0 to go
+ * on; anything else ends the loop with G4S_ERR_ABORTED. */
 typedef int (*g4s_beam_forward_fn)(void* user, const g4s_beam_step* step);
 
 /* Beam search for `batch` sequences at once.  Row sequence * beams of d_logits

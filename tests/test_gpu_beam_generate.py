@@ -192,6 +192,29 @@ def test_generate_without_states():
     s.close()
 
 
+@pytest.mark.skipif(hip.device_count() < 2, reason="needs a second device")
+def test_generate_whose_forward_leaves_another_device_current():
+    """On the null stream: the loop's launches and copies go to the search's device."""
+    found = []
+    for other in (0, 1):
+        eng = Engine(PROMPTS[:2], 3, 2.0)
+        s = beam.BeamSearch(V, 2, 3, 30.0)
+
+        def forward(step):
+            hip.check(hip.lib().hipSetDevice(ctypes.c_int(0)))
+            ok = eng.forward(step)
+            hip.check(hip.lib().hipSetDevice(ctypes.c_int(other)))
+            return ok
+        found.append(s.Generate(eng.logits, 2, 3, 6, forward, states=eng.beam_states,
+                                cache=eng.beam_cache))
+        now = ctypes.c_int(-1)
+        hip.check(hip.lib().hipGetDevice(ctypes.byref(now)))
+        assert now.value == 0
+        s.close()
+    for a, b in zip(*found):
+        assert [(tuple(t), x) for t, x in a] == [(tuple(t), x) for t, x in b]
+
+
 def test_generate_refusals_and_failures():
     eng = Engine(PROMPTS[:2], 3, 0.0, pages=6)
     s = beam.BeamSearch(V, 2, 3, 30.0)
