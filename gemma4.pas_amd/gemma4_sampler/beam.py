@@ -170,7 +170,9 @@ class BeamSearch:
         def fwd(_, step):
             try:
                 return 0 if forward(step.contents) else 1
-            except Exception as e:  # noqa: BLE001 -- reported after the loop
+            # an exception that left the callback would be printed and dropped, and the
+            # search would go on over stale logits: an interrupt ends it too
+            except BaseException as e:  # noqa: BLE001 -- raised again after the loop
                 errors.append(e)
                 return 1
 

@@ -77,6 +77,39 @@ def test_null_handles():
                                None) == INVALID
 
 
+# ------------------------------------------------------------- Python binding
+
+
+class FakeLibrary:
+    """Calls forward once, as g4s_beam_generate would, and keeps its arguments."""
+
+    def g4s_beam_generate(self, *args):
+        self.args = args
+        self.status = args[8](None, ctypes.pointer(beam.BeamStep()))
+        return native.G4S_OK if self.status == 0 else -9
+
+    def g4s_beam_last_error(self, h):
+        return b"the forward callback failed"
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    library = FakeLibrary()
+    monkeypatch.setattr(beam, "load", lambda: library)
+    library.search = beam.BeamSearch.__new__(beam.BeamSearch)
+    library.search.h, library.search.vocab = ctypes.c_void_p(), 100
+    return library
+
+
+@pytest.mark.parametrize("error", [ValueError, KeyboardInterrupt, SystemExit])
+def test_an_exception_of_the_forward_ends_the_search(fake, error):
+    def forward(step):
+        raise error("stop")
+    with pytest.raises(error):
+        fake.search.Generate(1 << 20, 1, 1, 1, forward)
+    assert fake.status != 0
+
+
 # ------------------------------------------------------------- Pascal unit
 
 
