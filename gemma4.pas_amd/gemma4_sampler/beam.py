@@ -31,12 +31,14 @@ class PageGeometry(ctypes.Structure):
 
 
 class PageState(ctypes.Structure):
-    """g4s_page_state: device arrays of a state (table, lengths, refs)."""
+    """g4s_page_state: device arrays of a state (table, lengths, refs), which live as
+    long as the record."""
     _fields_ = [("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p),
                 ("refs", ctypes.c_void_p)]
 
     def __init__(self, table=None, lengths=None, refs=None):
         super().__init__(_ptr(table), _ptr(lengths), _ptr(refs))
+        self._owners = (table, lengths, refs)
 
 
 class BeamConfig(ctypes.Structure):
@@ -55,15 +57,20 @@ class BeamStates(ctypes.Structure):
     def __init__(self, d_state, planes, plane_stride, row_stride, row_bytes):
         super().__init__(_ptr(d_state), int(planes), int(plane_stride), int(row_stride),
                          int(row_bytes))
+        self._owners = (d_state,)
 
 
 class BeamCache(ctypes.Structure):
-    """g4s_beam_cache"""
+    """g4s_beam_cache; the PageCache, its states and the pool live as long as
+    the record."""
     _fields_ = [("pages", ctypes.c_void_p), ("states", PageState * 2),
                 ("d_pool", ctypes.c_void_p)]
 
     def __init__(self, cache, states, d_pool):
+        states = tuple(states)
         super().__init__(cache.h, (PageState * 2)(*states), _ptr(d_pool))
+        self.cache = cache
+        self._owners = (states, d_pool)
 
 
 class BeamStep(ctypes.Structure):
@@ -176,6 +183,8 @@ class BeamSearch:
                 errors.append(e)
                 return 1
 
+        if cache is not None:
+            cache.pages = cache.cache.h  # NULL, and so refused, once it is closed
         stride = self.vocab if row_stride is None else int(row_stride)
         rc = load().g4s_beam_generate(
             self.h, int(batch), ctypes.byref(cfg), _ptr(d_logits), int(dtype), stride,

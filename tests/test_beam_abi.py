@@ -2,9 +2,11 @@
 what the entry points refuse without a GPU, the Pascal unit against the
 header, and the rules that the page kernels run, on the CPU."""
 import ctypes
+import gc
 import os
 import re
 import subprocess
+import weakref
 
 import numpy as np
 import pytest
@@ -85,6 +87,7 @@ class FakeLibrary:
 
     def g4s_beam_generate(self, *args):
         self.args = args
+        self.pages = args[7]._obj.pages if args[7] is not None else None
         self.status = args[8](None, ctypes.pointer(beam.BeamStep()))
         return native.G4S_OK if self.status == 0 else -9
 
@@ -98,6 +101,8 @@ def fake(monkeypatch):
     monkeypatch.setattr(beam, "load", lambda: library)
     library.search = beam.BeamSearch.__new__(beam.BeamSearch)
     library.search.h, library.search.vocab = ctypes.c_void_p(), 100
+    library.destroyed = []
+    library.g4s_pages_destroy = lambda h: library.destroyed.append(h.value)
     return library
 
 
@@ -108,6 +113,39 @@ def test_an_exception_of_the_forward_ends_the_search(fake, error):
     with pytest.raises(error):
         fake.search.Generate(1 << 20, 1, 1, 1, forward)
     assert fake.status != 0
+
+
+def test_records_keep_what_they_name(fake):
+    """A page cache, a state's arrays and a pool that only a record names live as
+    long as it; a cache that was closed is not passed on."""
+    class Array(hip.Buffer):
+        def __init__(self, addr):
+            self.nbytes, self.ptr = 8, ctypes.c_void_p(addr)
+
+        def free(self):
+            pass
+
+    def cache():
+        c = beam.PageCache.__new__(beam.PageCache)
+        c.h = ctypes.c_void_p(77)
+        return c
+    arrays = [Array(i + 1) for i in range(8)]
+    alive = [weakref.ref(a) for a in arrays]
+    record = beam.BeamCache(cache(), [beam.PageState(*arrays[:3]), beam.PageState(*arrays[3:6])],
+                            arrays[6])
+    states = beam.BeamStates(arrays[7], 1, 0, 8, 8)
+    del arrays
+    gc.collect()
+    assert fake.destroyed == [] and all(r() is not None for r in alive)
+    fake.search.Generate(1 << 20, 1, 1, 1, lambda step: True, states=states, cache=record)
+    assert fake.pages == 77 and [record.states[i].refs for i in range(2)] == [3, 6]
+    record.cache.close()
+    assert fake.destroyed == [77]
+    fake.search.Generate(1 << 20, 1, 1, 1, lambda step: True, cache=record)
+    assert fake.pages is None
+    del record, states, fake.args
+    gc.collect()
+    assert all(r() is None for r in alive) and fake.destroyed == [77]
 
 
 # ------------------------------------------------------------- Pascal unit
