@@ -152,12 +152,13 @@ type
     procedure Close();
 
     // the search around the engine's forward pass; AConfig^.NBest results
-    // per sequence
+    // per sequence.  ARowStride: elements from row to row of ADevLogits, 0 = the
+    // vocabulary; rows start on multiples of 16 bytes
     function Generate(const ABatch: Integer; const AConfig: PG4SBeamConfig;
       const ADevLogits: Pointer; const ADType: Integer; const AStates: PG4SBeamStates;
       const ACache: PG4SBeamCache; const AForward: TG4SBeamForwardFn;
       const AUser: Pointer; const ATokens: PInteger; const ALengths: PInteger;
-      const AScores: PSingle): Boolean;
+      const AScores: PSingle; const ARowStride: Int64 = 0): Boolean;
 
     function LastError(): string;
 

@@ -223,6 +223,24 @@ def test_pascal_and_python_constants_match_the_header():
                           "G4S_PAGES_MAX_PAGES"))
 
 
+def test_pascal_search_names_the_row_stride():
+    """Rows of a vocabulary that does not fill whole 16-byte vectors are padded, and
+    a search of more than one row is refused without their stride."""
+    s = _pascal()
+    intf, impl = s[:s.index("implementation")], s[s.index("implementation"):]
+    at = intf.index("TGpuBeamSearch = class")
+    method = re.search(r"function Generate\((.*?)\): Boolean", intf[at:], re.S).group(1)
+    assert re.search(r"const ARowStride: Int64 = 0$", method.strip())
+    body = impl[impl.index("function TGpuBeamSearch.Generate"):]
+    call = re.search(r"g4s_beam_generate\((.*?)\)", body, re.S).group(1)
+    external = re.search(r"function g4s_beam_generate\((.*?)\)", intf, re.S).group(1)
+    names = [n.strip() for g in external.split(";") for n in g.split(":")[0].split(",")]
+    stride = [a.strip() for a in call.split(",")][names.index("ARowStride")]
+    before = body[:body.index("g4s_beam_generate")]
+    assert re.search(r"\b%s := ARowStride;" % stride, before)
+    assert re.search(r"if %s = 0 then\s+%s := FVocab;" % (stride, stride), before)
+
+
 # ---------------------------------------------------------- the pages' rules
 
 
