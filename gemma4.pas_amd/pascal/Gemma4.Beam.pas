@@ -228,12 +228,17 @@ end;
 function TGpuBeamSearch.Generate(const ABatch: Integer; const AConfig: PG4SBeamConfig;
   const ADevLogits: Pointer; const ADType: Integer; const AStates: PG4SBeamStates;
   const ACache: PG4SBeamCache; const AForward: TG4SBeamForwardFn; const AUser: Pointer;
-  const ATokens: PInteger; const ALengths: PInteger; const AScores: PSingle): Boolean;
+  const ATokens: PInteger; const ALengths: PInteger; const AScores: PSingle;
+  const ARowStride: Int64): Boolean;
 var
   LStatus: Integer;
+  LRowStride: Int64;
 begin
-  LStatus := g4s_beam_generate(FHandle, ABatch, AConfig, ADevLogits, ADType, FVocab, AStates,
-    ACache, AForward, AUser, ATokens, ALengths, AScores);
+  LRowStride := ARowStride;
+  if LRowStride = 0 then
+    LRowStride := FVocab;
+  LStatus := g4s_beam_generate(FHandle, ABatch, AConfig, ADevLogits, ADType, LRowStride,
+    AStates, ACache, AForward, AUser, ATokens, ALengths, AScores);
   if LStatus <> G4S_OK then
     Exit(Fail(LStatus));
   Result := True;
