@@ -351,7 +351,9 @@ __device__ __forceinline__ void forget(u32x4 (&r)[NV])
 }
 
 /* Sum of four terms: in binary32, which rounds twice; such sums are added in
- * binary64. */
+ * binary64.  A row's sum, and so lse, is off by less than 2.6e-7 of itself: these two
+ * roundings 2^-23, a term's exponential 8.4e-8 (v_exp_f32 over [-1/2, 1/2], every value
+ * measured) and its argument's rounding 1.1e-8, the polynomial 5.4e-10 of the cap, at most 4.4e-8. */
 __device__ __forceinline__ double sum_four(const float (&t)[4])
 {
     return (double)((t[0] + t[1]) + (t[2] + t[3]));

@@ -55,12 +55,12 @@ const char* g4s_beam_last_error(const g4s_beam* beam);
  *   y = softcap * tanh(x / softcap)   (x where softcap <= 0)
  *   lse(r) = log(sum over the row's tokens of exp(y))
  *   score(r, token) = s(r) + (y - lse(r))
- * they are taken by score, evaluated in 64 bits, the largest first; equal
- * scores go to the lower beam, then to the larger logit, then to the lower
- * token.  A logit that is not above -1e30 (-inf, NaN, the type's lowest value:
- * the samplers' rule) is no candidate and counts nothing in the sum; a row
- * whose score is not above -1e30 is dead: it has no candidates and is not
- * read.
+ * they are taken by score, the largest first: y and the score in 64 bits, the
+ * terms of lse in 32, summed in 64.  Equal scores go to the lower beam, then to
+ * the larger logit, then to the lower token.  A logit that is not above -1e30
+ * (-inf, NaN, the type's lowest value: the samplers' rule) is no candidate and
+ * counts nothing in the sum; a row whose score is not above -1e30 is dead: it
+ * has no candidates and is not read.
  *   d_logits, dtype, row_stride  as for g4s_sample, batch * beams rows
  *   d_scores   device [batch*beams]
  *   n_select   1 .. 2 * max_beams
@@ -73,8 +73,9 @@ const char* g4s_beam_last_error(const g4s_beam* beam);
  * Where a sequence has fewer candidates the rest is -1, -1, -inf.
  * An output that overlaps another array of the call, or the span of the
  * logits, is refused but for d_out == d_scores.
- * Stream-ordered.  lse is within 2e-7 of the exact value, absolutely: scores
- * of different beams that lie closer than that may come in either order. */
+ * Stream-ordered.  The lse that scores are made from is off by less than
+ * 2.6e-7 + 2^-49 |lse|, and d_lse is that value rounded once to binary32: scores of
+ * different beams that lie closer than 5.2e-7 may come in either order. */
 int g4s_beam_select(g4s_beam* beam, const void* d_logits, int32_t dtype, int64_t row_stride,
                     int32_t batch, int32_t beams, const float* d_scores, int32_t n_select,
                     int32_t* d_parents, int32_t* d_tokens, float* d_out, float* d_lse);
