@@ -263,6 +263,19 @@ def test_many_rows():
     rig.compact()
 
 
+def test_most_rows_and_pages():
+    """The limits of the handle: 2,048 rows that write one page, in a pool of 2^20."""
+    R, N = beam.PAGES_MAX_ROWS, beam.PAGES_MAX_PAGES
+    rig = Rig(4, N, R, 600, planes=1, parts=1, token=4)
+    # 512 rows of 599 pages, then the row that all others follow
+    grow = np.zeros(R, I32)
+    grow[:512], grow[512] = 4 * 599, 6
+    assert rig.advance([-1] * R, grow) == (0, N - 512 * 599 - 2, 512 * 599 + 2, 0)
+    assert rig.advance([512] * R, [1] * R)[2:] == (R - 1, R - 1)
+    rig.advance(np.arange(R)[::-1], [2] * R)
+    assert rig.compact()[3] > 0
+
+
 def test_captured_steps():
     """Two steps, there and back between the states, in one captured graph that is
     replayed with other parents, eager steps of the same cache between."""
