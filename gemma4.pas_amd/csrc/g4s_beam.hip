@@ -962,13 +962,18 @@ BeamPlan beam_plan(int32_t vocab, int32_t rows, int32_t dtype, int32_t mode, int
 {
     BeamPlan p{};
     /* Looking terms up takes loading the table (30 KiB a workgroup) and tiles of four times
-     * the size.  It pays from about half such a tile a CU on: 8 rows of 262,144 take 19 us
-     * with it and 21 without, 64 rows 25.5 and 34.3, 160 rows 41 and 61 (4 rows 18.6 and 17.3;
-     * 64 rows of 33,000 20 and 18).  Rows that do not fill two tiles are better without:
-     * 2,048 rows of 8,000 take 64 us with it and 37 without, of 16,000 59 and 56; 512 rows of
-     * 33,000 26 and 43. */
+     * the size.  It pays from about half such a tile a CU on: 8 rows of 262,144 take 18.5 us
+     * with it and 20.5 without, 64 rows 25 and 34, 256 rows 46 and 83 (4 rows 18.6 and 17.3);
+     * 48 rows of 50,000 18.8 and 18.5, 64 rows 19.2 and 20.0.  Rows of less than three tiles,
+     * whose last is up to half of the work and may be all but empty, need three times as much:
+     * 64 rows of 33,000 take 19.6 us with it and 17.8 without, 192 rows 24.7 and 24.0, 512
+     * rows 24.9 and 41.5; 128 rows of 45,000 22.4 and 21.6, 160 rows 22.3 and 24.7.  Rows that do
+     * not fill two tiles are better without: 2,048 rows of 8,000 take 64 us with it and
+     * 37 without, of 16,000 59 and 56.  What the rule leaves is 6 per cent at most, where either
+     * way fills a round of the device by a little (192 rows of 100,003: 42.8 and 40.4). */
+    const int64_t half = (int64_t)ncu * kBeamTableTile / 2;
     p.table = dtype == G4S_DTYPE_BF16 && mode != kCapExact && vocab >= 2 * kBeamTableTile &&
-              (int64_t)rows * vocab >= (int64_t)ncu * kBeamTableTile / 2;
+              (int64_t)rows * vocab >= (vocab >= 3 * kBeamTableTile ? half : 3 * half);
     const int32_t tile = p.table ? kBeamTableTile : kBeamTile;
     const int32_t all = (vocab + tile - 1) / tile;
     /* a row's workgroups: the fewest tiles that some CU takes one after another, its workgroups

@@ -283,6 +283,22 @@ def test_bf16_rows_of_few_tiles(V, batch, beams, n):
     check(x, s, beams, beams, inplace=True)
 
 
+@pytest.mark.parametrize("V, batch, beams, n", [
+    (32768, 24, 8, 16), (32769, 48, 4, 8), (40000, 20, 8, 16), (49151, 33, 4, 4),
+    (49152, 11, 4, 8), (49153, 6, 7, 14)])
+def test_bf16_rows_of_two_and_three_tiles(V, batch, beams, n):
+    """Batches about the fewest whose terms are looked up, in rows of two tiles
+    and of a few logits more than two and three."""
+    rng = np.random.default_rng(V)
+    x = peaky(rng, batch * beams, V, "bf16")
+    x[1, :16384] = 0xFF80
+    x[2, -1:] = bo.bf16(np.array([25], F32))
+    x[3] = 0xFF80
+    x[4, V - 1], x[5, 7] = 0x7FC1, 0x7F80
+    s = running(rng, beams)
+    check(x, np.concatenate([s + F32(b * 2.0 ** -6) for b in range(batch)]), beams, n)
+
+
 def test_stride_no_lse_and_scores_in_place():
     rng = np.random.default_rng(15)
     x = peaky(rng, 6, 10007, "bf16")
