@@ -115,6 +115,29 @@ def test_most_beams():
     check(peaky(rng, 64, 70001, "bf16"), running(rng, 64), 64, 128)
 
 
+@pytest.mark.parametrize("batch, beams, n", [(65535, 1, 2), (1023, 64, 128), (21845, 3, 3)])
+def test_most_rows(batch, beams, n):
+    """As many rows as a call takes, of a handful of logits."""
+    rng = np.random.default_rng(51)
+    x = rng.permuted(np.tile(np.arange(5, dtype=F32) * F32(1.25), (batch * beams, 1)), axis=1)
+    x += rng.integers(-2, 3, (batch * beams, 1)).astype(F32)
+    x[7], x[8, 1:] = NONE, np.nan
+    # scores a third apart, logits multiples of a quarter: no two candidates are near
+    s = np.tile(-np.arange(beams) * F32(0.3125) - F32(1), batch).astype(F32)
+    x += (np.arange(batch * beams) % beams % 7)[:, None].astype(F32) * F32(0.03)
+    check(x, s, beams, n)
+
+
+@pytest.mark.parametrize("dtype, batch, beams, n", [("f32", 1, 1, 128), ("f32", 1, 3, 6),
+                                                    ("bf16", 1, 1, 2), ("bf16", 2, 4, 8)])
+def test_longest_rows(dtype, batch, beams, n):
+    rng = np.random.default_rng(52)
+    V = 1 << 22
+    x = peaky(rng, batch * beams, V, dtype)
+    x[0, V - 1] = 25 if dtype == "f32" else bo.bf16(np.array([25], F32))[0]
+    check(x, running(rng, batch * beams), beams, n)
+
+
 def test_flat_rows_and_offsets():
     """Rows whose mass lies in many tokens, far from 0 and from the cap."""
     rng = np.random.default_rng(7)

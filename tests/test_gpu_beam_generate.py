@@ -192,6 +192,35 @@ def test_generate_without_states():
     s.close()
 
 
+def test_generate_without_candidates():
+    """A sequence whose prompt leaves no token, one whose second step leaves none, and
+    one that goes on beside them."""
+    W, prompts = 3, PROMPTS[:3]
+    eng = Engine(prompts, W, 2.0)
+    s = beam.BeamSearch(V, 3, W, 30.0)
+    rows = eng.logits.download(F32).reshape(9, V)
+    rows[0] = -np.inf
+    eng.logits.upload(rows)
+
+    def forward(step):
+        assert (step.Tokens()[:W] == -1).all()
+        ok = eng.forward(step)
+        rows = eng.logits.download(F32).reshape(9, V)
+        rows[W:2 * W] = np.nan
+        eng.logits.upload(rows)
+        return ok
+    got = s.Generate(eng.logits, 3, W, 6, forward, n_best=W, states=eng.beam_states,
+                     cache=eng.beam_cache)
+    first = bo.select(model(prompts[1], 2.0)[None], [0.0], 1, 2 * W, 30.0)[1][0]
+    ends = [int(t) for t in first[:W] if t in ENDS]
+    assert got[0] == [] and [[int(x) for x in t] for t, _ in got[1]] == [[e] for e in ends]
+    gaps = []
+    want = plain_search(prompts[2], W, 6, W, False, 1.0, 2.0, gaps)
+    assert min(gaps) > 4e-7 + max(abs(float(d[1])) for d in want) * 2.0 ** -23
+    assert [tuple(int(x) for x in t) for t, _ in got[2]] == [t for t, _ in want]
+    s.close()
+
+
 @pytest.mark.skipif(hip.device_count() < 2, reason="needs a second device")
 def test_generate_whose_forward_leaves_another_device_current():
     """On the null stream: the loop's launches and copies go to the search's device."""
