@@ -647,15 +647,16 @@ struct LoopArrays {
     }
 };
 
-/* One generated token and the one before it. */
+/* One generated token and the one before it.  Indices in 64 bits: 65,535 rows
+ * make 2^31 nodes in 32,768 steps. */
 struct Node {
     int32_t token;
-    int32_t before; /* -1 = the prompt */
+    int64_t before; /* -1 = the prompt */
 };
 
 struct Result {
     float score; /* with the length penalty */
-    int32_t last;
+    int64_t last;
     int32_t length;
 };
 
@@ -689,7 +690,7 @@ int generate(g4s_beam* h, int32_t batch, const g4s_beam_config& cfg, const void*
     const size_t step_bytes = bytes - ((char*)p.step_parents - (char*)p.parents);
 
     std::vector<Node> nodes;
-    std::vector<int32_t> at((size_t)rows, -1), next((size_t)rows, -1); /* rows' last nodes */
+    std::vector<int64_t> at((size_t)rows, -1), next((size_t)rows, -1); /* rows' last nodes */
     std::vector<std::vector<Result>> results((size_t)batch);
     std::vector<uint8_t> done((size_t)batch, 0);
     for (int32_t r = 0; r < rows; ++r) {
@@ -701,7 +702,7 @@ int generate(g4s_beam* h, int32_t batch, const g4s_beam_config& cfg, const void*
                                   hipMemcpyHostToDevice, h->stream);
     if (e != hipSuccess) return hip_fail(h, e, "upload of the first scores");
     int32_t current = 0;
-    auto add = [&](int32_t b, float score, int32_t last, int32_t length) {
+    auto add = [&](int32_t b, float score, int64_t last, int32_t length) {
         auto& rs = results[(size_t)b];
         const Result r{penalised(score, length, cfg.length_penalty), last, length};
         auto it = std::find_if(rs.begin(), rs.end(),
@@ -734,12 +735,12 @@ int generate(g4s_beam* h, int32_t batch, const g4s_beam_config& cfg, const void*
                 if (is_end(token)) {
                     if (i >= W) continue;
                     nodes.push_back({token, at[(size_t)parent]});
-                    add(b, score, (int32_t)nodes.size() - 1, length);
+                    add(b, score, (int64_t)nodes.size() - 1, length);
                     continue;
                 }
                 const int32_t r = b * W + go++;
                 nodes.push_back({token, at[(size_t)parent]});
-                next[(size_t)r] = (int32_t)nodes.size() - 1;
+                next[(size_t)r] = (int64_t)nodes.size() - 1;
                 p.step_parents[r] = parent;
                 p.step_tokens[r] = token;
                 p.grow[r] = 1;
@@ -806,7 +807,7 @@ int generate(g4s_beam* h, int32_t batch, const g4s_beam_config& cfg, const void*
             lengths[o] = have ? results[(size_t)b][(size_t)k].length : 0;
             scores[o] = have ? results[(size_t)b][(size_t)k].score : none;
             int32_t i = lengths[o];
-            for (int32_t node = have ? results[(size_t)b][(size_t)k].last : -1; node >= 0;
+            for (int64_t node = have ? results[(size_t)b][(size_t)k].last : -1; node >= 0;
                  node = nodes[(size_t)node].before)
                 tokens[o * (size_t)cfg.max_tokens + (size_t)--i] = nodes[(size_t)node].token;
         }
