@@ -376,11 +376,16 @@ __device__ __forceinline__ double sum_four(const float (&t)[4])
  * The workgroup that ends last in a row merges its chunks, the one that ends
  * last in a sequence its rows.
  *
- * 512 rows of 262,144 bf16 logits: 72 us, 3.7 TB/s; their tiles move 4.8, and the start and
- * the end of the workgroups, 17 us, overlap nothing.  Without the table 181 us
- * (issue), with the binary64 softmax throughout 841.  64 binary32 rows: 36 us,
+ * 512 rows of 262,144 bf16 logits: 72 us, 3.7 TB/s, bound by neither side alone: the
+ * vector units issue for 38 us of it (11 instructions a logit), memory would take 43, and the
+ * start and the end of the workgroups, 17 us, overlap nothing.  Without the table
+ * 181 us (issue), with the binary64 softmax throughout 841.  64 binary32 rows: 36 us,
  * 11 of them the terms' issue, 20 the start and the merges.  Four rows:
- * 17 us, all of it latency. */
+ * 17 us, all of it latency.
+ *
+ * The longer ways: with half of the logits at -1e4 or -1e9, which are not masked, four binary32
+ * rows take 23 us, 64 85 and 512 bf16 rows 423; without a cap 20, 59 and 306; with a cap
+ * above 80, evaluated in a second pass, 23, 76 to 86 and 450 to 525. */
 template <int DT, int MODE, bool TABLE, int BLOCK>
 __global__ __launch_bounds__(BLOCK, 4) void beam_select_kernel(BeamSelectArgs a)
 {
@@ -1031,7 +1036,9 @@ hipError_t beam_reorder_launch(const BeamReorderArgs& a, hipStream_t stream)
     const uint64_t bits = (uint64_t)(uintptr_t)a.src | (uint64_t)(uintptr_t)a.dst |
                           (uint64_t)a.plane_stride | (uint64_t)a.row_stride |
                           (uint64_t)a.row_bytes;
-    /* 64 beams of 16 bytes would not stay in registers: 4 bytes from 17 beams on */
+    /* 64 beams of 16 bytes would not stay in registers: 4 bytes from 17 beams on, which
+     * move 2.1 to 2.6 TB/s (352,944-byte rows of 16 x 17 beams in eight planes 552 us; of
+     * 16 x 16 beams by 16 bytes 244).  Rows of odd sizes: 0.6 to 0.8 TB/s */
     if ((bits & 15) == 0 && a.beams <= 16) return reorder_with<u32x4>(a, stream);
     if ((bits & 3) == 0) return reorder_with<uint32_t>(a, stream);
     return reorder_with<uint8_t>(a, stream);

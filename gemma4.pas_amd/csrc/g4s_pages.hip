@@ -352,9 +352,10 @@ __global__ __launch_bounds__(kB) void pages_advance_kernel(PagesArgs a)
 
 /* ------------------------------------------------------------------ copies */
 
-/* Copies are bound by memory: 1,501 pages of 16 x 16 KiB take 134 us, 5.3 TB/s, with
- * streaming stores and a workgroup for each 16 KiB (170 us from a grid that
- * stays resident, 145 without the streaming; two and eight vectors a thread 136 and 268). */
+/* Copies are bound by memory: 1,501 pages of 16 x 16 KiB take 134 to 144 us by the card, 5.3 to
+ * 5.0 TB/s, with streaming stores and a workgroup for each 16 KiB (where they took 134:
+ * 170 us from a grid that stays resident, 145 without the streaming; two and eight
+ * vectors a thread 136 and 268). */
 
 /* Segment `seg` (256 x kCopyItems vectors) of the first `tokens` tokens of a
  * page in one plane. */

@@ -87,8 +87,8 @@ int g4s_beam_select(g4s_beam* beam, const void* d_logits, int32_t dtype, int64_t
  * parent of another sequence, or -1, leaves row r of d_dst as it is in place
  * and copies row r of d_src otherwise.  Bytes between rows are left alone.
  * d_src and d_dst are the same pointer or do not overlap, and d_parents lies
- * outside d_dst.  Any alignment; multiples of 16 bytes throughout are fastest.
- * Stream-ordered. */
+ * outside d_dst.  Any alignment; multiples of 16 bytes throughout and at most 16
+ * beams are fastest.  Stream-ordered. */
 int g4s_beam_reorder(g4s_beam* beam, const void* d_src, void* d_dst, int64_t planes,
                      int64_t plane_stride, int32_t batch, int32_t beams, int64_t row_stride,
                      int64_t row_bytes, const int32_t* d_parents);

@@ -563,13 +563,20 @@ def test_reorder_rows_past_32_bits():
     s.close()
 
 
-def test_an_earlier_failure_is_not_the_calls():
-    """A failed HIP call of the caller leaves its error with the thread; the
-    calls report their own launches."""
+@pytest.fixture
+def earlier():
+    """A failing HIP call of the caller's own, whose error stays with the thread
+    until it is asked for."""
     import ctypes
 
-    def earlier():
+    def fail():
         assert hip.lib().hipSetDevice(ctypes.c_int(1 << 20)) != 0
+    yield fail
+    hip.lib().hipGetLastError()
+
+
+def test_an_earlier_failure_is_not_the_calls(earlier):
+    """The calls report their own launches."""
     rng = np.random.default_rng(21)
     earlier()
     s = beam.BeamSearch(1001, 1, 3, 30.0)
