@@ -56,11 +56,12 @@ const char* g4s_beam_last_error(const g4s_beam* beam);
  *   lse(r) = log(sum over the row's tokens of exp(y))
  *   score(r, token) = s(r) + (y - lse(r))
  * they are taken by score, the largest first: y and the score in 64 bits, the
- * terms of lse in 32, summed in 64.  Equal scores go to the lower beam, then to
- * the larger logit, then to the lower token.  A logit that is not above -1e30
- * (-inf, NaN, the type's lowest value: the samplers' rule) is no candidate and
- * counts nothing in the sum; a row whose score is not above -1e30 is dead: it
- * has no candidates and is not read.
+ * terms of lse in 32, added by fours in 32 and from there on in 64.  Equal
+ * scores go to the lower beam, then to the larger logit, then to the lower
+ * token.  A logit that is not above -1e30 (-inf, NaN, the type's lowest value:
+ * the samplers' rule) is no candidate and counts nothing in the sum; a row
+ * whose score is not above -1e30 is dead: it has no candidates and is not
+ * read.
  *   d_logits, dtype, row_stride  as for g4s_sample, batch * beams rows
  *   d_scores   device [batch*beams]
  *   n_select   1 .. 2 * max_beams
