@@ -1,0 +1,145 @@
+/*
+ * g4s_cache.h -- launch interface of the kernels of the 8-bit cache
+ * (g4s_append.hip, g4s_attend.hip), and the rules of places, addresses and scales,
+ * which the host can run too.
+ */
+#ifndef G4S_CACHE_H
+#define G4S_CACHE_H
+
+#include <stdint.h>
+
+#include "g4s_pages.h"
+#include "gemma4_cache.h"
+
+namespace g4s {
+
+/* n / d for 0 <= n < 2^31 and 1 <= d <= 2^31: with s = ceil(log2 d) and
+ * m = floor(2^(31+s) / d) + 1, m * d - 2^(31+s) is at most 2^s, so the error of
+ * n * m / 2^(31+s) stays below 1 / d. */
+struct Divisor {
+    uint32_t m;
+    int32_t s, d;
+};
+inline Divisor divisor(int32_t d)
+{
+    int s = 0;
+    while (((int64_t)1 << s) < d) ++s;
+    return Divisor{(uint32_t)((((uint64_t)1 << (31 + s)) / (uint32_t)d) + 1), 31 + s, d};
+}
+G4S_PAGE_HD int32_t divide(int32_t n, const Divisor& d)
+{
+    return (int32_t)(((uint64_t)(uint32_t)n * d.m) >> d.s);
+}
+
+/* The pool as the kernels see it. */
+struct CachePool {
+    int64_t plane_stride, page_stride;
+    int32_t part_bytes, token_bytes; /* of a head in a page, of a token */
+    int32_t n_pages, max_slots;
+    Divisor page_tokens;
+    Divisor scale_tokens;
+    int32_t head_dim;
+};
+
+/* Most tokens of a row. */
+G4S_PAGE_HD int64_t cache_room(const CachePool& p) { return (int64_t)p.max_slots * p.page_tokens.d; }
+
+/* Bytes from a plane's start to token `place` of head `head`, its page known. */
+G4S_PAGE_HD int64_t cache_offset(const CachePool& p, int32_t page, int32_t in_page, int32_t head)
+{
+    return (int64_t)page * p.page_stride + (int64_t)head * p.part_bytes +
+           (int64_t)in_page * p.token_bytes;
+}
+
+/* Tokens of a row in a call, the first of the views, and the row's length; a
+ * length outside the table gives bad = 1 and d_starts that do not fit the call no
+ * tokens. */
+struct RowTokens {
+    int32_t start, count, length, bad;
+};
+G4S_PAGE_HD RowTokens row_tokens(const int32_t* starts, const int32_t* lengths, int32_t row,
+                                 int32_t tokens, int64_t room)
+{
+    RowTokens r{row, 1, lengths[row], 0};
+    if (starts) {
+        r.start = starts[row];
+        const int32_t end = starts[row + 1];
+        r.count = r.start >= 0 && end > r.start && end <= tokens ? end - r.start : 0;
+    }
+    if (r.length < 0 || r.length > room) {
+        r.length = 0;
+        r.bad = 1;
+    }
+    return r;
+}
+
+/* Least e from kScaleLow to kScaleHigh with top <= 448 * 2^e.  448 = 0.875 * 2^9: with
+ * top = m * 2^x and m in [0.5, 1), that is x - 9 for m <= 0.875 and one more above. */
+constexpr int kScaleLow = -100, kScaleHigh = 119;
+G4S_PAGE_HD int32_t scale_exponent(double top)
+{
+    if (!(top > 0.0)) return kScaleLow;
+    union {
+        double d;
+        uint64_t u;
+    } b{top};
+    const int32_t field = (int32_t)(b.u >> 52) & 0x7FF; /* (subnormals end at kScaleLow too) */
+    const uint64_t fraction = b.u & (((uint64_t)1 << 52) - 1);
+    int32_t e = field - 1022 - 9 + (fraction > ((uint64_t)3 << 50) ? 1 : 0);
+    e = e < kScaleLow ? kScaleLow : e;
+    return e > kScaleHigh ? kScaleHigh : e;
+}
+
+/* The row whose share of `x` holds slot x, where row r's share begins at
+ * starts[r] / unit + extra * r: the last one that begins at or before x.  A row
+ * of n tokens has floor(n / unit) + extra slots at least. */
+G4S_PAGE_HD int64_t share_begin(const int32_t* starts, int32_t row, int32_t unit, int32_t extra)
+{
+    return (int64_t)(starts ? starts[row] : row) / unit + (int64_t)extra * row;
+}
+
+#if defined(__HIPCC__)
+
+struct CacheView {
+    char* data;
+    int64_t token_stride, head_stride; /* elements */
+};
+
+struct AppendArgs {
+    CachePool pool;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int32_t rows, tokens;
+    CacheView q, k, v, q_out; /* data NULL: none */
+    const int32_t* positions;
+    const float* freqs;
+    char* k_plane;
+    char* v_plane;
+    int32_t heads, kv_heads, rotary_dims, rotary_pairs;
+};
+
+struct AttendArgs {
+    CachePool pool;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* starts;
+    int32_t rows, tokens;
+    CacheView q, out;
+    const char* k_plane;
+    const char* v_plane;
+    float* lse;
+    float scale;
+    int32_t window;
+    int32_t heads, kv_heads;
+    Divisor group;
+};
+
+hipError_t append_launch(const AppendArgs& a, int32_t dtype, hipStream_t stream);
+hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
+
+#endif
+
+}  // namespace g4s
+
+#endif

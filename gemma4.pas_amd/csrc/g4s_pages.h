@@ -94,6 +94,14 @@ G4S_PAGE_HD bool geometry_ok(const g4s_page_geometry& g)
     return inner_pages || inner_planes;
 }
 
+/* Bytes from a pool's start to the end of its last page. */
+G4S_PAGE_HD int64_t pool_extent(const g4s_page_geometry& g)
+{
+    if (g.planes == 0) return 0;
+    return (g.planes - 1) * g.plane_stride + (g.n_pages - 1) * g.page_stride +
+           (int64_t)g.parts * g.page_tokens * g.token_bytes;
+}
+
 #if defined(__HIPCC__)
 
 struct PageJob {

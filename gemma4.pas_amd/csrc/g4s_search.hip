@@ -9,33 +9,27 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdarg>
-#include <cstdio>
-#include <cstring>
 #include <limits>
 #include <new>
 #include <vector>
 
 #include "g4s_beam.h"
+#include "g4s_host.h"
 #include "g4s_pages.h"
 
-#define G4S_API extern "C" __attribute__((visibility("default")))
+using g4s::Carver;
+using g4s::DeviceGuard;
+using g4s::fail_in;
+using g4s::Handle;
+using g4s::overlap;
+using g4s::pick_device;
+using g4s::pool_extent;
+using g4s::Span;
 
 namespace {
 
-struct Handle {
-    int device = 0;
-    hipStream_t stream = nullptr;
-    char err[512] = "";
-};
-
 thread_local char t_beam_error[512] = "";
 thread_local char t_pages_error[512] = "";
-
-int fail_in(char (&buf)[512], int code, const char* fmt, va_list ap)
-{
-    vsnprintf(buf, sizeof(buf), fmt, ap);
-    return code;
-}
 
 }  // namespace
 
@@ -81,84 +75,6 @@ int hip_fail(H* h, hipError_t e, const char* what)
     return fail(h, G4S_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
-/* The handle's device is current while a call works with it. */
-class DeviceGuard {
-public:
-    explicit DeviceGuard(int device)
-    {
-        if (hipGetDevice(&old_) != hipSuccess) old_ = device;
-        if (old_ != device)
-            ok_ = hipSetDevice(device) == hipSuccess;
-        else
-            old_ = -1;
-    }
-    ~DeviceGuard()
-    {
-        if (old_ >= 0) (void)hipSetDevice(old_);
-    }
-    bool ok() const { return ok_; }
-
-private:
-    int old_ = -1;
-    bool ok_ = true;
-};
-
-/* The current device, if the library runs on it. */
-template <typename H>
-int pick_device(H* none, int* device, int* ncu = nullptr)
-{
-    int n = 0;
-    if (hipGetDeviceCount(&n) != hipSuccess || n < 1)
-        return fail(none, G4S_ERR_NO_DEVICE, "no HIP device visible");
-    hipDeviceProp_t prop;
-    if (hipGetDevice(device) != hipSuccess ||
-        hipGetDeviceProperties(&prop, *device) != hipSuccess)
-        return fail(none, G4S_ERR_NO_DEVICE, "the current HIP device is not usable");
-    if (std::strncmp(prop.gcnArchName, "gfx950", 6) != 0)
-        return fail(none, G4S_ERR_NO_DEVICE, "device %d is %s; this library targets gfx950",
-                    *device, prop.gcnArchName);
-    if (ncu) *ncu = prop.multiProcessorCount;
-    return G4S_OK;
-}
-
-bool overlap(const void* a, int64_t na, const void* b, int64_t nb)
-{
-    const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-    return na > 0 && nb > 0 && x < y + (uintptr_t)nb && y < x + (uintptr_t)na;
-}
-
-/* An array of a call; NULL ones overlap nothing. */
-struct Span {
-    const char* name;
-    const void* at;
-    int64_t bytes;
-};
-bool overlap(const Span& a, const Span& b)
-{
-    return a.at && b.at && overlap(a.at, a.bytes, b.at, b.bytes);
-}
-
-/* Parts of one allocation, each on a 256-byte boundary. */
-class Carver {
-public:
-    template <typename T>
-    void add(T** p, size_t count)
-    {
-        if (base_) *p = reinterpret_cast<T*>(base_ + used_);
-        used_ += (count * sizeof(T) + 255) & ~(size_t)255;
-    }
-    size_t used() const { return used_; }
-    void start(void* base)
-    {
-        base_ = static_cast<char*>(base);
-        used_ = 0;
-    }
-
-private:
-    char* base_ = nullptr;
-    size_t used_ = 0;
-};
-
 constexpr int64_t kMaxExtent = (int64_t)1 << 56;
 
 /* `outer` blocks of `inner` pieces of `bytes`, neither overlapping the other. */
@@ -195,7 +111,8 @@ G4S_API int g4s_beam_create(g4s_beam** out, int32_t vocab, int32_t max_batch, in
     if (!std::isfinite(softcap))
         return fail(none, G4S_ERR_INVALID_ARGUMENT, "softcap %g is not finite", softcap);
     int device = 0, ncu = 0;
-    const int rc = pick_device(none, &device, &ncu);
+    auto refuse = [&](int code, auto... a) { return fail(none, code, a...); };
+    const int rc = pick_device(refuse, &device, &ncu);
     if (rc) return rc;
     g4s_beam* h = new (std::nothrow) g4s_beam();
     if (!h) return fail(none, G4S_ERR_OUT_OF_MEMORY, "host memory");
@@ -423,7 +340,8 @@ G4S_API int g4s_pages_create(g4s_pages** out, const g4s_page_geometry* geometry,
                     g.page_tokens, g.n_pages, g.max_rows, g.max_slots, g.planes, g.parts,
                     (long long)g.token_bytes, (long long)g.plane_stride, (long long)g.page_stride);
     int device = 0;
-    const int rc = pick_device(none, &device);
+    auto refuse = [&](int code, auto... a) { return fail(none, code, a...); };
+    const int rc = pick_device(refuse, &device);
     if (rc) return rc;
     g4s_pages* h = new (std::nothrow) g4s_pages();
     if (!h) return fail(none, G4S_ERR_OUT_OF_MEMORY, "host memory");
@@ -471,14 +389,6 @@ G4S_API int g4s_pages_destroy(g4s_pages* h)
 }
 
 namespace {
-
-/* Bytes from a pool's start to the end of its last page. */
-int64_t pool_extent(const g4s_page_geometry& g)
-{
-    if (g.planes == 0) return 0;
-    return (g.planes - 1) * g.plane_stride + (g.n_pages - 1) * g.page_stride +
-           (int64_t)g.parts * g.page_tokens * g.token_bytes;
-}
 
 int check_states(g4s_pages* h, const g4s_page_state* from, const g4s_page_state* to, int32_t rows,
                  const int32_t* d_parents, const int32_t* d_grow, const void* d_pool,
