@@ -64,7 +64,10 @@ EXPORTS = ("g4s_version", "g4s_params_set_defaults", "g4s_max_top_k", "g4s_creat
            # gemma4_beam.h, bound in beam.py
            "g4s_beam_create", "g4s_beam_destroy", "g4s_beam_last_error", "g4s_beam_select",
            "g4s_beam_reorder", "g4s_pages_create", "g4s_pages_destroy", "g4s_pages_last_error",
-           "g4s_pages_advance", "g4s_pages_compact", "g4s_pages_copy", "g4s_beam_generate")
+           "g4s_pages_advance", "g4s_pages_compact", "g4s_pages_copy", "g4s_beam_generate",
+           # gemma4_cache.h, bound in cache.py
+           "g4s_cache_create", "g4s_cache_destroy", "g4s_cache_last_error", "g4s_cache_append",
+           "g4s_cache_attend")
 
 FORWARD_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int32),
                               ctypes.c_int32)

@@ -1,0 +1,55 @@
+/*
+ * Host build of the rules of g4s_cache.h that the kernels of the 8-bit cache run:
+ * division, a row's tokens, places in a plane and scales.
+ */
+#include "../../gemma4.pas_amd/csrc/g4s_cache.h"
+
+using namespace g4s;
+
+extern "C" {
+int32_t t_divide(int32_t n, int32_t d) { return divide(n, divisor(d)); }
+/* Divisors `from` to `to` - 1, at the numerators next to their multiples. */
+int t_divide_all(int32_t from, int32_t to)
+{
+    for (int32_t d = from; d < to; ++d) {
+        const Divisor v = divisor(d);
+        const int64_t most = INT32_MAX / d;
+        const int64_t step = most / 97 + 1;
+        for (int64_t k = 0;; k = k + step < most ? k + step : most) {
+            for (int64_t n = k * d - 1; n <= k * d + 1; ++n)
+                if (n >= 0 && n <= INT32_MAX && divide((int32_t)n, v) != n / d) return d;
+            if (k == most) break;
+        }
+        if (divide(INT32_MAX, v) != INT32_MAX / d) return d;
+    }
+    return 0;
+}
+void t_row_tokens(const int32_t* starts, const int32_t* lengths, int32_t row, int32_t tokens,
+                  int64_t room, int32_t* out)
+{
+    const RowTokens r = row_tokens(starts, lengths, row, tokens, room);
+    out[0] = r.start;
+    out[1] = r.count;
+    out[2] = r.length;
+    out[3] = r.bad;
+}
+int64_t t_cache_offset(int64_t page_stride, int32_t part_bytes, int32_t token_bytes, int32_t page,
+                       int32_t in_page, int32_t head)
+{
+    CachePool p{};
+    p.page_stride = page_stride;
+    p.part_bytes = part_bytes;
+    p.token_bytes = token_bytes;
+    return cache_offset(p, page, in_page, head);
+}
+int32_t t_scale_exponent(double top) { return scale_exponent(top); }
+/* Slots of a grid that no tile of a row of `count` tokens from place `from` on
+ * finds room in (rows one behind the other from token `start` on): 0. */
+int32_t t_missing_slots(int32_t start, int32_t count, int32_t from, int32_t tile)
+{
+    const int32_t starts[2] = {start, start + count};
+    const int64_t slots = share_begin(starts, 1, tile, 2) - share_begin(starts, 0, tile, 2);
+    const int64_t tiles = count ? (from + count - 1) / tile - from / tile + 1 : 0;
+    return (int32_t)(tiles > slots ? tiles - slots : 0);
+}
+}
