@@ -1,0 +1,162 @@
+/*
+ * g4s_attend.h -- what the attention kernels share: tiles of 32 tokens in matrix
+ * registers, the softmax between them, and the joining of partial results.
+ *
+ * Products are taken as S^T = K Q^T and O^T = V^T P^T in 16x16x32 bf16 matrix
+ * instructions.  A lane l (m = l % 16, g = l / 16) then has, for query column m of
+ * a tile of 32 tokens, the scores of tokens 4 g + i and 16 + 4 g + i (i = 0 .. 3), and
+ * these eight are what the second product wants from it, if its eight tokens
+ * are taken in that order on both sides: weights go from one product to the
+ * next without leaving their lane.  A lane's dims of O^T are (D / 16) (4 g + r) + i:
+ * consecutive ones.
+ */
+#ifndef G4S_ATTEND_H
+#define G4S_ATTEND_H
+
+#include "g4s_cache.h"
+#include "g4s_device.h"
+
+namespace g4s {
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
+
+/* Eight bf16 of a matrix operand. */
+union Frag {
+    uint32_t w[4];
+    bf16x8 v;
+};
+
+__device__ __forceinline__ float inf32() { return __builtin_inff(); }
+__device__ __forceinline__ float nan32() { return __builtin_nanf(""); }
+
+/* Two codes of a word and their scale (a power of two) as bf16, which holds every product. */
+template <bool HI>
+__device__ __forceinline__ uint32_t widen2(uint32_t w, float scale)
+{
+    const bf16x2 r = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI);
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+/* Low and high halves of two words. */
+__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b)
+{
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b)
+{
+    return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b)
+{
+    bf16x2 r;
+    r[0] = (__bf16)a;
+    r[1] = (__bf16)b;
+    return __builtin_bit_cast(uint32_t, r);
+}
+
+/* 1 in each byte of a word that is a NaN code. */
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w)
+{
+    return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
+}
+__device__ __forceinline__ bool has_nan(uint32_t w) { return nan_codes(w) != 0u; }
+/* The word with +0 in the place of NaN codes. */
+__device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~(nan_codes(w) * 0xFFu); }
+
+/* Words of four dims of eight tokens, as operands of eight tokens for each of the dims. */
+__device__ __forceinline__ void value_frags(const uint32_t (&w)[8], const float (&scale)[8],
+                                            Frag (&f)[4])
+{
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const uint32_t a0 = widen2<false>(w[j], scale[j]);
+        const uint32_t b0 = widen2<true>(w[j], scale[j]);
+        const uint32_t a1 = widen2<false>(w[j + 1], scale[j + 1]);
+        const uint32_t b1 = widen2<true>(w[j + 1], scale[j + 1]);
+        f[0].w[j >> 1] = lows(a0, a1);
+        f[1].w[j >> 1] = highs(a0, a1);
+        f[2].w[j >> 1] = lows(b0, b1);
+        f[3].w[j >> 1] = highs(b0, b1);
+    }
+}
+
+/* Sixteen consecutive elements of a query as matrix operands: bf16 as they are, binary32 cut
+ * into three bf16 pieces of eight bits, which together are the value (their
+ * products with bf16 are exact).  What is not finite becomes NaN. */
+template <int DT>
+__device__ __forceinline__ void load_query(const char* p, bool in, Frag (&lo)[DT == G4S_DTYPE_F32 ? 3 : 1],
+                                           Frag (&hi)[DT == G4S_DTYPE_F32 ? 3 : 1])
+{
+    if constexpr (DT == G4S_DTYPE_F32) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Frag* f = h ? hi : lo;
+#pragma unroll
+            for (int v = 0; v < 2; ++v) {
+                const f32x4 x = in ? reinterpret_cast<const f32x4*>(p)[h * 2 + v] : f32x4{0, 0, 0, 0};
+                uint32_t part[3][4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const bool finite = __builtin_fabsf(x[i]) < inf32();
+                    const float a = __uint_as_float(__float_as_uint(x[i]) & 0xFFFF0000u);
+                    const float r = x[i] - a;
+                    const float b = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+                    part[0][i] = finite ? __float_as_uint(a) : 0x7FC00000u;
+                    part[1][i] = finite ? __float_as_uint(b) : 0u;
+                    part[2][i] = finite ? __float_as_uint(r - b) : 0u;
+                }
+#pragma unroll
+                for (int s = 0; s < 3; ++s) {
+                    f[s].w[v * 2] = highs(part[s][0], part[s][1]);
+                    f[s].w[v * 2 + 1] = highs(part[s][2], part[s][3]);
+                }
+            }
+        }
+    } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Frag* f = h ? hi : lo;
+            const u32x4 x = in ? reinterpret_cast<const u32x4*>(p)[h] : u32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t w = x[i];
+                if ((w & 0x7F80u) == 0x7F80u) w = (w & 0xFFFF0000u) | 0x7FC0u;
+                if ((w & 0x7F800000u) == 0x7F800000u) w = (w & 0xFFFFu) | 0x7FC00000u;
+                f[0].w[i] = w;
+            }
+        }
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ void store4(char* p, f32x4 x)
+{
+    if constexpr (DT == G4S_DTYPE_F32) {
+        *reinterpret_cast<f32x4*>(p) = x;
+    } else {
+        uint2 w;
+        w.x = pack_bf16(x[0], x[1]);
+        w.y = pack_bf16(x[2], x[3]);
+        *reinterpret_cast<uint2*>(p) = w;
+    }
+}
+
+/* Writes to LDS of this wave are read by its other lanes from here on. */
+__device__ __forceinline__ void wave_fence()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+}  // namespace g4s
+
+#endif

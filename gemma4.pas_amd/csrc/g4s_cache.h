@@ -90,6 +90,18 @@ G4S_PAGE_HD int32_t scale_exponent(double top)
     return e > kScaleHigh ? kScaleHigh : e;
 }
 
+/* Units of work shared out among `groups` workgroups, total >= groups: group w takes
+ * units total * w / groups up to total * (w + 1) / groups, and unit x is the group's
+ * that unit_group gives (the last w with total * w / groups < x + 1). */
+G4S_PAGE_HD int64_t first_unit(int64_t total, int32_t w, int32_t groups)
+{
+    return total * w / groups;
+}
+G4S_PAGE_HD int32_t unit_group(int64_t x, int64_t total, int32_t groups)
+{
+    return (int32_t)(((x + 1) * groups - 1) / total);
+}
+
 /* The row whose share of `x` holds slot x, where row r's share begins at
  * starts[r] / unit + extra * r: the last one that begins at or before x.  A row
  * of n tokens has floor(n / unit) + extra slots at least. */
@@ -119,6 +131,14 @@ struct AppendArgs {
     int32_t heads, kv_heads, rotary_dims, rotary_pairs;
 };
 
+/* Workspace of the attention: what several workgroups found for one item. */
+struct AttendSpace {
+    float* stats;      /* [slots][cols][2] maximum (base two) and sum */
+    float* sums;       /* [slots][cols][head_dim rounded up] */
+    uint32_t* tickets; /* 0 between calls */
+    int32_t groups;    /* workgroups of a launch at most; two slots and a ticket each */
+};
+
 struct AttendArgs {
     CachePool pool;
     const int32_t* table;
@@ -133,10 +153,17 @@ struct AttendArgs {
     int32_t window;
     int32_t heads, kv_heads;
     Divisor group;
+    AttendSpace ws;
 };
 
 hipError_t append_launch(const AppendArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
+
+/* Columns of a slot and floats of a column's sums for a head_dim; tickets to be cleared. */
+constexpr int kAttendCols = 16;
+int32_t attend_groups(int32_t ncu, int32_t head_dim);
+int32_t attend_width(int32_t head_dim);
+hipError_t attend_init_launch(const AttendSpace& ws, hipStream_t stream);
 
 #endif
 

@@ -27,6 +27,8 @@ struct g4s_cache : g4s::Handle {
     g4s_page_geometry geo{};
     g4s_cache_config config{};
     g4s::CachePool pool{};
+    void* memory = nullptr;
+    g4s::AttendSpace ws{};
 };
 
 namespace {
@@ -200,7 +202,8 @@ G4S_API int g4s_cache_create(g4s_cache** out, const g4s_page_geometry* geometry,
                     (long long)g.plane_stride, (long long)g.page_stride);
     int device = 0;
     auto refuse = [&](int code, auto... a) { return fail(none, code, a...); };
-    const int rc = g4s::pick_device(refuse, &device);
+    int ncu = 0;
+    const int rc = g4s::pick_device(refuse, &device, &ncu);
     if (rc) return rc;
     g4s_cache* h = new (std::nothrow) g4s_cache();
     if (!h) return fail(none, G4S_ERR_OUT_OF_MEMORY, "host memory");
@@ -217,6 +220,30 @@ G4S_API int g4s_cache_create(g4s_cache** out, const g4s_page_geometry* geometry,
     h->pool.page_tokens = g4s::divisor(g.page_tokens);
     h->pool.scale_tokens = g4s::divisor(c.scale_tokens);
     h->pool.head_dim = c.head_dim;
+    h->ws.groups = g4s::attend_groups(ncu, c.head_dim);
+    const size_t slots = 2 * (size_t)h->ws.groups;
+    g4s::Carver w;
+    auto lay = [&] {
+        w.add(&h->ws.stats, slots * g4s::kAttendCols * 2);
+        w.add(&h->ws.sums, slots * g4s::kAttendCols * g4s::attend_width(c.head_dim));
+        w.add(&h->ws.tickets, (size_t)h->ws.groups);
+    };
+    lay();
+    const size_t bytes = w.used();
+    if (hipMalloc(&h->memory, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        delete h;
+        return fail(none, G4S_ERR_OUT_OF_MEMORY, "workspace of %zu bytes", bytes);
+    }
+    w.start(h->memory);
+    lay();
+    hipError_t e = g4s::attend_init_launch(h->ws, h->stream);
+    if (e == hipSuccess) e = hipStreamSynchronize(h->stream);
+    if (e != hipSuccess) {
+        (void)hipFree(h->memory);
+        delete h;
+        return fail(none, G4S_ERR_HIP, "workspace initialisation: %s", hipGetErrorString(e));
+    }
     *out = h;
     return G4S_OK;
 }
@@ -226,6 +253,7 @@ G4S_API int g4s_cache_destroy(g4s_cache* h)
     if (!h) return G4S_OK;
     DeviceGuard guard(h->device);
     (void)hipStreamSynchronize(h->stream);
+    (void)hipFree(h->memory);
     delete h;
     return G4S_OK;
 }
@@ -353,6 +381,7 @@ G4S_API int g4s_cache_attend(g4s_cache* h, const g4s_page_state* state, int32_t 
     a.heads = c.heads;
     a.kv_heads = c.kv_heads;
     a.group = g4s::divisor(c.heads / c.kv_heads);
+    a.ws = h->ws;
     const hipError_t e = g4s::attend_launch(a, dtype, h->stream);
     if (e != hipSuccess) return fail(h, G4S_ERR_HIP, "attention launch: %s", hipGetErrorString(e));
     return G4S_OK;
