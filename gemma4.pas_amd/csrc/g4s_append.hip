@@ -215,22 +215,10 @@ __device__ __forceinline__ bool find_tile(const AppendArgs& a, int64_t x, int ti
 {
     int row = (int)x;
     if (a.starts) {
-        /* every lane looks at one row in 64, then at one in this stretch, ... */
-        int lo = 0, n = a.rows;
-        const int lane = threadIdx.x & 63;
-        while (n > 1) {
-            const int each = (n + 63) / 64;
-            const int r = lo + lane * each;
-            const bool at = lane * each < n && share_begin(a.starts, r, tile, 2) <= x;
-            const uint64_t m = __ballot(at);
-            const int last = m ? 63 - __clzll(m) : 0;
-            lo += last * each;
-            n = n - last * each < each ? n - last * each : each;
-        }
-        row = lo;
+        row = find_share(a.starts, a.rows, x, 1, tile, 2);
     }
     const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    int64_t nth = a.starts ? x - share_begin(a.starts, row, tile, 2) : 0;
+    int64_t nth = a.starts ? x - share_begin(a.starts, row, 1, tile, 2) : 0;
     if (r.count == 0 || r.length == 0 || nth < 0) return false;
     const int from = r.length > r.count ? r.length - r.count : 0; /* the first place */
     const int64_t begin = (from / tile + nth) * tile;

@@ -88,50 +88,42 @@ __device__ __forceinline__ void value_frags(const uint32_t (&w)[8], const float 
     }
 }
 
-/* Sixteen consecutive elements of a query as matrix operands: bf16 as they are, binary32 cut
+/* Eight consecutive elements of a query as matrix operands: bf16 as they are, binary32 cut
  * into three bf16 pieces of eight bits, which together are the value (their
  * products with bf16 are exact).  What is not finite becomes NaN. */
 template <int DT>
-__device__ __forceinline__ void load_query(const char* p, bool in, Frag (&lo)[DT == G4S_DTYPE_F32 ? 3 : 1],
-                                           Frag (&hi)[DT == G4S_DTYPE_F32 ? 3 : 1])
+__device__ __forceinline__ void load_query(const char* p, bool in,
+                                           Frag (&f)[DT == G4S_DTYPE_F32 ? 3 : 1])
 {
     if constexpr (DT == G4S_DTYPE_F32) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            Frag* f = h ? hi : lo;
+        for (int v = 0; v < 2; ++v) {
+            const f32x4 x = in ? reinterpret_cast<const f32x4*>(p)[v] : f32x4{0, 0, 0, 0};
+            uint32_t part[3][4];
 #pragma unroll
-            for (int v = 0; v < 2; ++v) {
-                const f32x4 x = in ? reinterpret_cast<const f32x4*>(p)[h * 2 + v] : f32x4{0, 0, 0, 0};
-                uint32_t part[3][4];
+            for (int i = 0; i < 4; ++i) {
+                const bool finite = __builtin_fabsf(x[i]) < inf32();
+                const float a = __uint_as_float(__float_as_uint(x[i]) & 0xFFFF0000u);
+                const float r = x[i] - a;
+                const float b = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
+                part[0][i] = finite ? __float_as_uint(a) : 0x7FC00000u;
+                part[1][i] = finite ? __float_as_uint(b) : 0u;
+                part[2][i] = finite ? __float_as_uint(r - b) : 0u;
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const bool finite = __builtin_fabsf(x[i]) < inf32();
-                    const float a = __uint_as_float(__float_as_uint(x[i]) & 0xFFFF0000u);
-                    const float r = x[i] - a;
-                    const float b = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
-                    part[0][i] = finite ? __float_as_uint(a) : 0x7FC00000u;
-                    part[1][i] = finite ? __float_as_uint(b) : 0u;
-                    part[2][i] = finite ? __float_as_uint(r - b) : 0u;
-                }
-#pragma unroll
-                for (int s = 0; s < 3; ++s) {
-                    f[s].w[v * 2] = highs(part[s][0], part[s][1]);
-                    f[s].w[v * 2 + 1] = highs(part[s][2], part[s][3]);
-                }
+            for (int s = 0; s < 3; ++s) {
+                f[s].w[v * 2] = highs(part[s][0], part[s][1]);
+                f[s].w[v * 2 + 1] = highs(part[s][2], part[s][3]);
             }
         }
     } else {
+        const u32x4 x = in ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            Frag* f = h ? hi : lo;
-            const u32x4 x = in ? reinterpret_cast<const u32x4*>(p)[h] : u32x4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t w = x[i];
-                if ((w & 0x7F80u) == 0x7F80u) w = (w & 0xFFFF0000u) | 0x7FC0u;
-                if ((w & 0x7F800000u) == 0x7F800000u) w = (w & 0xFFFFu) | 0x7FC00000u;
-                f[0].w[i] = w;
-            }
+        for (int i = 0; i < 4; ++i) {
+            uint32_t w = x[i];
+            if ((w & 0x7F80u) == 0x7F80u) w = (w & 0xFFFF0000u) | 0x7FC0u;
+            if ((w & 0x7F800000u) == 0x7F800000u) w = (w & 0xFFFFu) | 0x7FC00000u;
+            f[0].w[i] = w;
         }
     }
 }

@@ -17,7 +17,8 @@ namespace g4s {
 namespace {
 
 constexpr int kTile = 32; /* tokens of a wave's step */
-constexpr int kCols = kAttendCols;
+constexpr int kB = 256;
+constexpr int kCols = 16; /* query columns of a workgroup's part */
 constexpr int kPass = 128; /* dims that the waves join at once */
 
 /* What a row asks for. */
@@ -33,7 +34,7 @@ __device__ __forceinline__ Work row_work(const AttendArgs& a, int row)
     const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
     Work w{r.start, r.count, r.length, r.bad, 0, 0, 0, 0, 0};
     w.cols = r.count * a.group.d;
-    if (r.count > 1 && w.cols > kCols) return w; /* the other kernel's */
+    if (is_prompt(r.count, a.group.d)) return w;
     w.blocks = (w.cols + kCols - 1) / kCols;
     const int64_t from = a.window > 0 ? (int64_t)r.length - r.count + 1 - a.window : 0;
     w.from = from > 0 ? (int)from : 0;
@@ -121,7 +122,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
     constexpr int KC = D / 64;                      /* 16-dim chunks of a lane of K and Q */
     constexpr int VW = D / 64;                      /* words of a lane of V */
     constexpr int DB = D / 16;                      /* blocks of 16 dims, and dims of a lane */
-    constexpr int WIDTH = D;
+    static_assert(2 * kCols * D <= kAttendSums && 4 * kCols <= kAttendStats, "two slots a workgroup");
     extern __shared__ char lds[];
     auto& s = *reinterpret_cast<Shared<DT, D, NW>*>(lds);
     int64_t* before = reinterpret_cast<int64_t*>(lds + ((sizeof(s) + 15) & ~(size_t)15));
@@ -174,8 +175,9 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
             for (int k = wave; k < KC; k += NW) {
                 const int d0 = k * 64 + g * 16;
                 Frag f[2][QP];
-                load_query<DT>(at + (int64_t)d0 * Elem<DT>::SIZE, has_col && d0 < a.pool.head_dim,
-                               f[0], f[1]);
+                const bool in = has_col && d0 < a.pool.head_dim;
+                load_query<DT>(at + (int64_t)d0 * Elem<DT>::SIZE, in, f[0]);
+                load_query<DT>(at + (int64_t)(d0 + 8) * Elem<DT>::SIZE, in, f[1]);
 #pragma unroll
                 for (int b = 0; b < QP; ++b) {
                     s.q[k][0][b][lane] = f[0][b];
@@ -409,7 +411,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
                 for (int w = 0; w < NW; ++w)
                     v += *reinterpret_cast<const f32x4*>(&s.o[w][k][d0]) * s.l[w][k];
                 if (!whole) {
-                    uint64_t* to = reinterpret_cast<uint64_t*>(a.ws.sums + (slot * kCols + k) * WIDTH + dim);
+                    uint64_t* to = reinterpret_cast<uint64_t*>(a.ws.sums + (slot * kCols + k) * D + dim);
                     st_dev(to, (uint64_t)__float_as_uint(v[0]) | (uint64_t)__float_as_uint(v[1]) << 32);
                     st_dev(to + 1, (uint64_t)__float_as_uint(v[2]) | (uint64_t)__float_as_uint(v[3]) << 32);
                 } else if (dim < a.pool.head_dim) {
@@ -453,7 +455,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
                 const uint64_t st = ld_dev(
                     reinterpret_cast<const uint64_t*>(a.ws.stats + (part_slot(w) * kCols + k) * 2));
                 const uint64_t* at = reinterpret_cast<const uint64_t*>(
-                    a.ws.sums + (part_slot(w) * kCols + k) * WIDTH + dim);
+                    a.ws.sums + (part_slot(w) * kCols + k) * D + dim);
                 const uint64_t v0 = ld_dev(at), v1 = ld_dev(at + 1);
                 const float tw = __uint_as_float((uint32_t)st), lw = __uint_as_float((uint32_t)(st >> 32));
                 const float f = tw == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(tw - best);
@@ -472,128 +474,6 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
         }
         __syncthreads();
     }
-}
-
-/* ------------------------------------------------------------ many queries */
-
-constexpr int kB = 256;
-constexpr int kDims = G4S_CACHE_MAX_HEAD_DIM / 64;
-
-template <int DT>
-__device__ __forceinline__ float load_one(const char* p, int64_t i)
-{
-    if constexpr (DT == G4S_DTYPE_F32)
-        return reinterpret_cast<const float*>(p)[i];
-    else
-        return __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16);
-}
-template <int DT>
-__device__ __forceinline__ void store_one(char* p, int64_t i, float x)
-{
-    if constexpr (DT == G4S_DTYPE_F32)
-        reinterpret_cast<float*>(p)[i] = x;
-    else
-        reinterpret_cast<__bf16*>(p)[i] = (__bf16)x;
-}
-
-__device__ __forceinline__ float code(const char* p)
-{
-    return __builtin_amdgcn_cvt_f32_fp8(*reinterpret_cast<const uint8_t*>(p), 0);
-}
-
-/* A workgroup per query and head: each wave takes every fourth token. */
-template <int DT>
-__global__ __launch_bounds__(kB) void attend_kernel(AttendArgs a)
-{
-    __shared__ float s_m[4], s_l[4], s_o[4][G4S_CACHE_MAX_HEAD_DIM];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int head = blockIdx.y, d = a.pool.head_dim;
-    int row = blockIdx.x;
-    if (a.starts) {
-        int lo = 0, hi = a.rows - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi + 1) >> 1;
-            if (a.starts[mid] <= (int)blockIdx.x)
-                lo = mid;
-            else
-                hi = mid - 1;
-        }
-        row = lo;
-    }
-    const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    const int64_t token = blockIdx.x, nth = token - r.start;
-    if (nth < 0 || nth >= r.count || r.count == 1 || r.count * a.group.d <= kCols) return;
-    const int64_t place = (int64_t)r.length - r.count + nth;
-    int64_t from = a.window > 0 ? place - a.window + 1 : 0;
-    if (from < 0) from = 0;
-    const int kv = divide(head, a.group);
-    float q[kDims], o[kDims];
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < kDims; ++i) {
-        const int x = i * 64 + lane;
-        q[i] = x < d ? load_one<DT>(a.q.data, token * a.q.token_stride + head * a.q.head_stride + x)
-                     : 0.0f;
-        finite = finite && __builtin_fabsf(q[i]) < inf32();
-        o[i] = 0.0f;
-    }
-    finite = __all(finite);
-    float m = -inf32(), l = 0.0f;
-    for (int64_t t = from + wave; t <= place; t += 4) {
-        const int slot = divide((int)t, a.pool.page_tokens);
-        const int in = (int)t - slot * a.pool.page_tokens.d;
-        const int first = divide(in, a.pool.scale_tokens) * a.pool.scale_tokens.d;
-        int page = a.table[(int64_t)row * a.pool.max_slots + slot];
-        const bool ok = page >= 0 && page < a.pool.n_pages;
-        if (!ok) page = 0;
-        const int64_t at = cache_offset(a.pool, page, in, kv);
-        const int64_t sc = cache_offset(a.pool, page, first, kv) + d;
-        const float ks = *reinterpret_cast<const float*>(a.k_plane + sc);
-        const float vs = *reinterpret_cast<const float*>(a.v_plane + sc);
-        float s = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kDims; ++i) {
-            const int x = i * 64 + lane;
-            if (x < d) s += q[i] * (code(a.k_plane + at + x) * ks);
-        }
-        for (int w = 32; w; w >>= 1) s += __shfl_xor(s, w);
-        s = ok && finite ? s * a.scale * kLog2e : nan32();
-        const float now = s > m ? s : m;
-        const float keep = __builtin_exp2f(m - now), p = __builtin_exp2f(s - now);
-        m = now;
-        l = m == -inf32() ? nan32() : l * keep + p;
-#pragma unroll
-        for (int i = 0; i < kDims; ++i) {
-            const int x = i * 64 + lane;
-            if (x < d) o[i] = o[i] * keep + p * (code(a.v_plane + at + x) * vs);
-        }
-    }
-    if (lane == 0) {
-        s_m[wave] = m;
-        s_l[wave] = l;
-    }
-#pragma unroll
-    for (int i = 0; i < kDims; ++i)
-        if (i * 64 + lane < d) s_o[wave][i * 64 + lane] = o[i];
-    __syncthreads();
-    const float top = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float sum = 0.0f, f[4];
-    for (int w = 0; w < 4; ++w) {
-        f[w] = s_m[w] == -inf32() ? 0.0f : __builtin_exp2f(s_m[w] - top);
-        sum += s_l[w] != s_l[w] ? s_l[w] : s_l[w] * f[w];
-    }
-    const bool empty = !r.bad && place < 0;
-    const float inv = empty ? 0.0f : r.bad ? nan32() : 1.0f / sum;
-    for (int x = threadIdx.x; x < d; x += kB) {
-        float v = 0.0f;
-        for (int w = 0; w < 4; ++w) v += s_o[w][x] * f[w];
-        store_one<DT>(a.out.data, token * a.out.token_stride + head * a.out.head_stride + x,
-                      empty ? 0.0f : v * inv);
-    }
-    if (a.lse && threadIdx.x == 0)
-        a.lse[token * a.heads + head] = empty ? -inf32()
-                                        : r.bad ? nan32()
-                                                : (top + __builtin_log2f(sum)) * kLn2;
 }
 
 template <int DT, int D, int NW>
@@ -631,21 +511,17 @@ int32_t attend_width(int32_t head_dim)
     return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512;
 }
 
-int32_t attend_groups(int32_t ncu, int32_t) { return ncu; }
+int32_t attend_groups(int32_t ncu) { return ncu; }
 
 hipError_t attend_init_launch(const AttendSpace& ws, hipStream_t stream)
 {
     return launch(attend_init_kernel, 4, kB, 0, stream, ws.tickets, ws.groups);
 }
 
-hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream)
+hipError_t attend_rows_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream)
 {
-    hipError_t e = dtype == G4S_DTYPE_F32 ? by_width<G4S_DTYPE_F32>(a, stream)
-                                          : by_width<G4S_DTYPE_BF16>(a, stream);
-    if (e != hipSuccess || !a.starts) return e;
-    const dim3 grid((unsigned)a.tokens, (unsigned)a.heads);
-    return dtype == G4S_DTYPE_F32 ? launch(attend_kernel<G4S_DTYPE_F32>, grid, kB, 0, stream, a)
-                                  : launch(attend_kernel<G4S_DTYPE_BF16>, grid, kB, 0, stream, a);
+    return dtype == G4S_DTYPE_F32 ? by_width<G4S_DTYPE_F32>(a, stream)
+                                  : by_width<G4S_DTYPE_BF16>(a, stream);
 }
 
 }  // namespace g4s

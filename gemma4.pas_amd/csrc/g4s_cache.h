@@ -102,15 +102,34 @@ G4S_PAGE_HD int32_t unit_group(int64_t x, int64_t total, int32_t groups)
     return (int32_t)(((x + 1) * groups - 1) / total);
 }
 
-/* The row whose share of `x` holds slot x, where row r's share begins at
- * starts[r] / unit + extra * r: the last one that begins at or before x.  A row
- * of n tokens has floor(n / unit) + extra slots at least. */
-G4S_PAGE_HD int64_t share_begin(const int32_t* starts, int32_t row, int32_t unit, int32_t extra)
+/* Where a row's slots of a grid begin: `times` columns a token, `unit` columns a slot.  A row of
+ * n tokens has floor(n * times / unit) + extra slots at least. */
+G4S_PAGE_HD int64_t share_begin(const int32_t* starts, int32_t row, int32_t times, int32_t unit,
+                                int32_t extra)
 {
-    return (int64_t)(starts ? starts[row] : row) / unit + (int64_t)extra * row;
+    return (int64_t)(starts ? starts[row] : row) * times / unit + (int64_t)extra * row;
 }
 
 #if defined(__HIPCC__)
+
+/* The row whose share holds slot x: the last one that begins at or before it.  Every lane
+ * looks at one row of 64 stretches, then within a stretch, ... */
+__device__ __forceinline__ int find_share(const int32_t* starts, int rows, int64_t x, int times,
+                                          int unit, int extra)
+{
+    int lo = 0, n = rows;
+    const int lane = threadIdx.x & 63;
+    while (n > 1) {
+        const int each = (n + 63) / 64;
+        const bool at = lane * each < n &&
+                        share_begin(starts, lo + lane * each, times, unit, extra) <= x;
+        const uint64_t m = __ballot(at);
+        const int last = m ? 63 - __clzll(m) : 0;
+        lo += last * each;
+        n = n - last * each < each ? n - last * each : each;
+    }
+    return lo;
+}
 
 struct CacheView {
     char* data;
@@ -131,13 +150,14 @@ struct AppendArgs {
     int32_t heads, kv_heads, rotary_dims, rotary_pairs;
 };
 
-/* Workspace of the attention: what several workgroups found for one item. */
+/* Workspace of the attention: what several workgroups found for the same columns. */
 struct AttendSpace {
-    float* stats;      /* [slots][cols][2] maximum (base two) and sum */
-    float* sums;       /* [slots][cols][head_dim rounded up] */
-    uint32_t* tickets; /* 0 between calls */
-    int32_t groups;    /* workgroups of a launch at most; two slots and a ticket each */
+    float* sums;       /* kAttendSums for each workgroup */
+    float* stats;      /* kAttendStats */
+    uint32_t* tickets; /* one; 0 between calls */
+    int32_t groups;    /* workgroups with parts of columns in a launch at most */
 };
+constexpr int kAttendSums = 32768, kAttendStats = 512;
 
 struct AttendArgs {
     CachePool pool;
@@ -159,9 +179,19 @@ struct AttendArgs {
 hipError_t append_launch(const AppendArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 
-/* Columns of a slot and floats of a column's sums for a head_dim; tickets to be cleared. */
-constexpr int kAttendCols = 16;
-int32_t attend_groups(int32_t ncu, int32_t head_dim);
+hipError_t attend_rows_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
+hipError_t attend_prompts_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
+
+/* Rows with more than one token and more than kFewCols columns (tokens x heads of a key head)
+ * are the prompts' kernel's, the others the rows' kernel's. */
+constexpr int kFewCols = 16;
+G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group)
+{
+    return count > 1 && (int64_t)count * group > kFewCols;
+}
+
+int32_t attend_groups(int32_t ncu);
+/* Dims that the kernels are made for, at least head_dim. */
 int32_t attend_width(int32_t head_dim);
 hipError_t attend_init_launch(const AttendSpace& ws, hipStream_t stream);
 

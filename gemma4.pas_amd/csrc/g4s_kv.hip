@@ -220,13 +220,13 @@ G4S_API int g4s_cache_create(g4s_cache** out, const g4s_page_geometry* geometry,
     h->pool.page_tokens = g4s::divisor(g.page_tokens);
     h->pool.scale_tokens = g4s::divisor(c.scale_tokens);
     h->pool.head_dim = c.head_dim;
-    h->ws.groups = g4s::attend_groups(ncu, c.head_dim);
-    const size_t slots = 2 * (size_t)h->ws.groups;
+    h->ws.groups = g4s::attend_groups(ncu);
+    const size_t groups = (size_t)h->ws.groups;
     g4s::Carver w;
     auto lay = [&] {
-        w.add(&h->ws.stats, slots * g4s::kAttendCols * 2);
-        w.add(&h->ws.sums, slots * g4s::kAttendCols * g4s::attend_width(c.head_dim));
-        w.add(&h->ws.tickets, (size_t)h->ws.groups);
+        w.add(&h->ws.sums, groups * g4s::kAttendSums);
+        w.add(&h->ws.stats, groups * g4s::kAttendStats);
+        w.add(&h->ws.tickets, groups);
     };
     lay();
     const size_t bytes = w.used();
@@ -382,7 +382,9 @@ G4S_API int g4s_cache_attend(g4s_cache* h, const g4s_page_state* state, int32_t 
     a.kv_heads = c.kv_heads;
     a.group = g4s::divisor(c.heads / c.kv_heads);
     a.ws = h->ws;
-    const hipError_t e = g4s::attend_launch(a, dtype, h->stream);
+    /* rows of one token each have no prompts among them */
+    hipError_t e = g4s::attend_rows_launch(a, dtype, h->stream);
+    if (e == hipSuccess && d_starts) e = g4s::attend_prompts_launch(a, dtype, h->stream);
     if (e != hipSuccess) return fail(h, G4S_ERR_HIP, "attention launch: %s", hipGetErrorString(e));
     return G4S_OK;
 }

@@ -43,13 +43,33 @@ int64_t t_cache_offset(int64_t page_stride, int32_t part_bytes, int32_t token_by
     return cache_offset(p, page, in_page, head);
 }
 int32_t t_scale_exponent(double top) { return scale_exponent(top); }
-/* Slots of a grid that no tile of a row of `count` tokens from place `from` on
- * finds room in (rows one behind the other from token `start` on): 0. */
+/* Tiles of a row of `count` tokens from place `from` on that find no slot in the grid
+ * of the append (rows one behind the other from token `start` on): 0. */
 int32_t t_missing_slots(int32_t start, int32_t count, int32_t from, int32_t tile)
 {
     const int32_t starts[2] = {start, start + count};
-    const int64_t slots = share_begin(starts, 1, tile, 2) - share_begin(starts, 0, tile, 2);
+    const int64_t slots = share_begin(starts, 1, 1, tile, 2) - share_begin(starts, 0, 1, tile, 2);
     const int64_t tiles = count ? (from + count - 1) / tile - from / tile + 1 : 0;
     return (int32_t)(tiles > slots ? tiles - slots : 0);
+}
+/* The same of blocks of `unit` columns in the grid of the attention. */
+int32_t t_missing_blocks(int32_t start, int32_t count, int32_t group, int32_t unit)
+{
+    const int32_t starts[2] = {start, start + count};
+    const int64_t slots =
+        share_begin(starts, 1, group, unit, 1) - share_begin(starts, 0, group, unit, 1);
+    const int64_t blocks = ((int64_t)count * group + unit - 1) / unit;
+    return (int32_t)(blocks > slots ? blocks - slots : 0);
+}
+/* Whether units are shared out without gaps and unit_group names their workgroup. */
+int t_units_shared(int64_t total, int32_t groups)
+{
+    if (first_unit(total, 0, groups) != 0 || first_unit(total, groups, groups) != total) return 0;
+    for (int32_t w = 0; w < groups; ++w) {
+        const int64_t a = first_unit(total, w, groups), b = first_unit(total, w + 1, groups);
+        if (b <= a || unit_group(a, total, groups) != w || unit_group(b - 1, total, groups) != w)
+            return 0;
+    }
+    return 1;
 }
 }

@@ -186,3 +186,18 @@ def test_every_tile_of_a_row_has_a_slot(host):
             for count in list(range(0, 2 * tile + 3)) + [1000, 65537]:
                 for first in (0, 1, tile - 1, tile, 12345):
                     assert host.t_missing_slots(start, count, first, tile) == 0
+
+
+def test_every_block_of_columns_has_a_slot(host):
+    for unit in (64, 128, 256):
+        for group in (1, 3, 8, 17, 64):
+            for start in (0, 1, 63, 64, 1000, 1048000):
+                for count in list(range(0, 70)) + [255, 256, 257, 576]:
+                    assert host.t_missing_blocks(start, count, group, unit) == 0
+
+
+def test_units_are_shared_out_whole(host):
+    host.t_units_shared.argtypes = [ctypes.c_int64, ctypes.c_int32]
+    for groups in (1, 2, 3, 255, 256, 512):
+        for total in (groups, groups + 1, 2 * groups - 1, 1000 * groups + 7, (1 << 43) + 5):
+            assert host.t_units_shared(total, groups) == 1
