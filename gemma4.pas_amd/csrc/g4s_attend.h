@@ -88,42 +88,42 @@ __device__ __forceinline__ void value_frags(const uint32_t (&w)[8], const float 
     }
 }
 
-/* Eight consecutive elements of a query as matrix operands: bf16 as they are, binary32 cut
+/* Eight consecutive elements of a query as a matrix operand: bf16 as they are, binary32 cut
  * into three bf16 pieces of eight bits, which together are the value (their
- * products with bf16 are exact).  What is not finite becomes NaN. */
+ * products with bf16 are exact).  An infinity becomes NaN (in binary32 the second piece does by
+ * itself).  `in` false gives zeros, p is read all the same: a branch for each load costs more. */
 template <int DT>
-__device__ __forceinline__ void load_query(const char* p, bool in,
+__device__ __forceinline__ void load_query(const char* p, bool in, bool negate,
                                            Frag (&f)[DT == G4S_DTYPE_F32 ? 3 : 1])
 {
+    const uint32_t keep = in ? ~0u : 0u, sign = negate ? 0x80008000u : 0u;
     if constexpr (DT == G4S_DTYPE_F32) {
 #pragma unroll
         for (int v = 0; v < 2; ++v) {
-            const f32x4 x = in ? reinterpret_cast<const f32x4*>(p)[v] : f32x4{0, 0, 0, 0};
+            const u32x4 x = reinterpret_cast<const u32x4*>(p)[v];
             uint32_t part[3][4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool finite = __builtin_fabsf(x[i]) < inf32();
-                const float a = __uint_as_float(__float_as_uint(x[i]) & 0xFFFF0000u);
-                const float r = x[i] - a;
-                const float b = __uint_as_float(__float_as_uint(r) & 0xFFFF0000u);
-                part[0][i] = finite ? __float_as_uint(a) : 0x7FC00000u;
-                part[1][i] = finite ? __float_as_uint(b) : 0u;
-                part[2][i] = finite ? __float_as_uint(r - b) : 0u;
+                const uint32_t u = x[i] & keep;
+                const float r = __uint_as_float(u) - __uint_as_float(u & 0xFFFF0000u);
+                const uint32_t w = __float_as_uint(r);
+                part[0][i] = u;
+                part[1][i] = w;
+                part[2][i] = __float_as_uint(r - __uint_as_float(w & 0xFFFF0000u));
             }
 #pragma unroll
             for (int s = 0; s < 3; ++s) {
-                f[s].w[v * 2] = highs(part[s][0], part[s][1]);
-                f[s].w[v * 2 + 1] = highs(part[s][2], part[s][3]);
+                f[s].w[v * 2] = highs(part[s][0], part[s][1]) ^ sign;
+                f[s].w[v * 2 + 1] = highs(part[s][2], part[s][3]) ^ sign;
             }
         }
     } else {
-        const u32x4 x = in ? *reinterpret_cast<const u32x4*>(p) : u32x4{0, 0, 0, 0};
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            uint32_t w = x[i];
-            if ((w & 0x7F80u) == 0x7F80u) w = (w & 0xFFFF0000u) | 0x7FC0u;
-            if ((w & 0x7F800000u) == 0x7F800000u) w = (w & 0xFFFFu) | 0x7FC00000u;
-            f[0].w[i] = w;
+            const uint32_t w = x[i] & keep;
+            /* (an exponent of ones carries into the sign's bit, which then sets the first of the fraction) */
+            f[0].w[i] = (w | (((w & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 9) ^ sign;
         }
     }
 }

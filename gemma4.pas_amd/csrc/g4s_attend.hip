@@ -134,7 +134,8 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
     if ((int)blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
     const int64_t x_end = first_unit(total, blockIdx.x + 1, groups);
-    const float c = a.scale * kLog2e;
+    /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
+    const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
 
     while (x < x_end) {
         Part p;
@@ -175,9 +176,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
             for (int k = wave; k < KC; k += NW) {
                 const int d0 = k * 64 + g * 16;
                 Frag f[2][QP];
-                const bool in = has_col && d0 < a.pool.head_dim;
-                load_query<DT>(at + (int64_t)d0 * Elem<DT>::SIZE, in, f[0]);
-                load_query<DT>(at + (int64_t)(d0 + 8) * Elem<DT>::SIZE, in, f[1]);
+                const bool in = d0 < a.pool.head_dim;
+                const char* q0 = at + (int64_t)(in ? d0 : 0) * Elem<DT>::SIZE;
+                load_query<DT>(q0, has_col && in, a.scale < 0.0f, f[0]);
+                load_query<DT>(q0 + 8 * Elem<DT>::SIZE, has_col && in, a.scale < 0.0f, f[1]);
 #pragma unroll
                 for (int b = 0; b < QP; ++b) {
                     s.q[k][0][b][lane] = f[0][b];
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
             }
             float y[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = sc[j >> 2][j & 3] * c;
+            for (int j = 0; j < 8; ++j) y[j] = sc[j >> 2][j & 3];
             const bool partly = bad != 0 || t0 < full_from || t0 + kTile - 1 > full_to;
             bool nan_v = false;
             if (partly) {
@@ -297,18 +299,18 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
             now = fmaxf(now, __shfl_xor(now, 32));
             now = fmaxf(now, top);
             if (__any(now > top)) {
-                const float keep = now > top ? __builtin_amdgcn_exp2f(top - now) : 1.0f;
+                const float keep = now > top ? __builtin_amdgcn_exp2f((top - now) * c) : 1.0f;
                 sum *= keep;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[i] *= keep;
                 top = now;
             }
-            const float base = top == -inf32() ? 0.0f : top;
+            const float base = top == -inf32() ? 0.0f : top * c;
             Frag pw[PP];
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(y[j] - base);
-                const float e1 = __builtin_amdgcn_exp2f(y[j + 1] - base);
+                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], c, -base));
+                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j + 1], c, -base));
                 sum += e0 + e1;
                 pw[0].w[j >> 1] = pack_bf16(e0, e1);
                 if constexpr (PP == 2) {
@@ -370,7 +372,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
         sum += __shfl_xor(sum, 16);
         sum += __shfl_xor(sum, 32);
         if (g == 0) {
-            s.m[wave][m] = top;
+            s.m[wave][m] = top == -inf32() ? top : top * c;
             s.l[wave][m] = sum;
         }
         __syncthreads();

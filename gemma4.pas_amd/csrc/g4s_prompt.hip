@@ -6,8 +6,8 @@
  * tokens that they see in tiles of KT: all its threads widen the next tile's codes into LDS, keys as
  * [token][dim] and values as [dim][token], while its waves multiply the present one, each
  * for NT x 16 columns of its own with the softmax in registers.  Where there are fewer columns than
- * workgroups the tokens are split too, and the last workgroup of a block of columns joins what
- * the others found, in their order.
+ * workgroups the tokens are split too, and a second launch joins what the parts of a block
+ * found, in their order.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -25,6 +25,77 @@ __device__ __forceinline__ int value_piece(int dim, int piece)
     return piece ^ ((dim ^ (dim >> 3)) & (KT / 8 - 1));
 }
 
+/* A block of a row's query columns for each key head, and the tiles of the tokens
+ * that its queries see; no columns where a slot of the grid has none. */
+struct Block {
+    RowTokens r;
+    int row, col0, cols;
+    int from, end;    /* places that any of its queries sees */
+    int first, tiles; /* tiles of them */
+    int parts;        /* workgroups that share the tiles */
+};
+__device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
+{
+    const int64_t f = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
+    return f > 0 ? (int)f : 0;
+}
+__device__ __forceinline__ Block find_block(const AttendArgs& a, int64_t x, int unit, int tile,
+                                            int splits)
+{
+    Block b{};
+    b.row = find_share(a.starts, a.rows, x, a.group.d, unit, 1);
+    b.r = row_tokens(a.starts, a.lengths, b.row, a.tokens, cache_room(a.pool));
+    const int64_t block = x - share_begin(a.starts, b.row, a.group.d, unit, 1);
+    const int64_t all = (int64_t)b.r.count * a.group.d;
+    if (!is_prompt(b.r.count, a.group.d) || block < 0 || block * unit >= all) return b;
+    b.col0 = (int)(block * unit);
+    b.cols = all - b.col0 < unit ? (int)(all - b.col0) : unit;
+    const int before = b.r.length - b.r.count;
+    b.from = sees_from(a, before + divide(b.col0, a.group));
+    b.end = before + divide(b.col0 + b.cols - 1, a.group) + 1;
+    b.first = b.from / tile;
+    b.tiles = b.end > b.from ? (b.end + tile - 1) / tile - b.first : 0;
+    b.parts = b.tiles < 2 ? 1 : b.tiles < splits ? b.tiles : splits;
+    return b;
+}
+
+/* A query column: the token it is of, its head and place. */
+struct Column {
+    int nth, head, place;
+};
+__device__ __forceinline__ Column column(const AttendArgs& a, const RowTokens& r, int kv_head, int col)
+{
+    const int nth = divide(col, a.group);
+    return Column{nth, kv_head * a.group.d + col - nth * a.group.d, r.length - r.count + nth};
+}
+template <int DT>
+__device__ __forceinline__ void put(const AttendArgs& a, const RowTokens& r, const Column& c, int dim,
+                                    f32x4 v)
+{
+    if (dim >= a.pool.head_dim) return;
+    if (r.bad) v = f32x4{nan32(), nan32(), nan32(), nan32()};
+    else if (c.place < 0) v = f32x4{0, 0, 0, 0};
+    store4<DT>(a.out.data + ((int64_t)(r.start + c.nth) * a.out.token_stride +
+                             (int64_t)c.head * a.out.head_stride + dim) * Elem<DT>::SIZE, v);
+}
+__device__ __forceinline__ void put_lse(const AttendArgs& a, const RowTokens& r, const Column& c,
+                                        float top, float sum)
+{
+    if (a.lse)
+        a.lse[(int64_t)(r.start + c.nth) * a.heads + c.head] =
+            r.bad ? nan32() : c.place < 0 ? -inf32() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+/* x, computed anew where it is used: what follows from it is not kept in registers over a
+ * loop. */
+__device__ __forceinline__ int again(int x)
+{
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+constexpr int kJoin = 256; /* threads of a joining workgroup */
+
 template <int D, int KT>
 struct Shared {
     alignas(16) uint16_t k[2][KT][D + 8];
@@ -33,8 +104,23 @@ struct Shared {
     float scale[3][2][KT];
     uint64_t bad[3];
     int nan[2];
-    int flag;
 };
+
+/* `steps` reads of a matrix operand from LDS and `each` products with it, as the compiler is to lay
+ * them out: kAhead reads ahead of their products.  Left to itself it reads everything first
+ * and spills registers. */
+constexpr int kAhead = 4;
+template <int STEPS, int EACH>
+__device__ __forceinline__ void lay_out()
+{
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int i = 0; i < STEPS - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH * kAhead, 0);
+}
 
 template <int DT, int D, int NW, int NT, int KT>
 __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a, int splits)
@@ -55,47 +141,32 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     /* heads side by side; the last columns of a row, which see most, first */
     const int head = blockIdx.x, part = blockIdx.z;
     const int64_t x = (int64_t)gridDim.y - 1 - blockIdx.y;
-    const int row = find_share(a.starts, a.rows, x, a.group.d, CB, 1);
-    const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    const int64_t block = x - share_begin(a.starts, row, a.group.d, CB, 1);
-    const int64_t all_cols = (int64_t)r.count * a.group.d;
-    if (!is_prompt(r.count, a.group.d) || block < 0 || block * CB >= all_cols) return;
-    const int col0 = (int)(block * CB);
-    const int cols = all_cols - col0 < CB ? (int)(all_cols - col0) : CB;
-
-    /* places that the block's queries see */
-    const int first_place = r.length - r.count + divide(col0, a.group);
-    const int last_place = r.length - r.count + divide(col0 + cols - 1, a.group);
-    auto sees_from = [&](int place) {
-        const int64_t f = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
-        return f > 0 ? (int)f : 0;
-    };
-    const int from0 = sees_from(first_place), end0 = last_place + 1;
-    const int t_first = from0 / KT;
-    const int tiles = end0 > from0 ? (end0 + KT - 1) / KT - t_first : 0;
-    const int parts = splits == 1 || tiles < 2 ? 1 : tiles < splits ? tiles : splits;
-    if (part >= parts) return;
-    const int n0 = (int)((int64_t)tiles * part / parts), n1 = (int)((int64_t)tiles * (part + 1) / parts);
+    const Block b = find_block(a, x, CB, KT, splits);
+    if (b.cols == 0 || part >= b.parts) return;
+    const RowTokens r = b.r;
+    const int row = b.row, col0 = b.col0, cols = b.cols, parts = b.parts;
+    const int from0 = b.from, end0 = b.end, t_first = b.first;
+    const int n0 = (int)((int64_t)b.tiles * part / parts);
+    const int n1 = (int)((int64_t)b.tiles * (part + 1) / parts);
 
     /* this lane's columns */
-    int place[NT], from[NT], nth[NT], qhead[NT];
-    bool has[NT];
+    int place[NT], from[NT];
     Frag q[NT][KS][QP];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int c = (wave * NT + t) * 16 + m;
-        has[t] = c < cols;
-        const int col = col0 + (has[t] ? c : 0);
-        nth[t] = divide(col, a.group);
-        qhead[t] = head * a.group.d + col - nth[t] * a.group.d;
-        place[t] = r.length - r.count + nth[t];
-        from[t] = sees_from(place[t]);
-        const char* at = a.q.data + ((int64_t)(r.start + nth[t]) * a.q.token_stride +
-                                     (int64_t)qhead[t] * a.q.head_stride) * Elem<DT>::SIZE;
+        const bool has = c < cols;
+        const Column at = column(a, r, head, col0 + (has ? c : 0));
+        place[t] = at.place;
+        from[t] = sees_from(a, at.place);
+        const char* q0 = a.q.data + ((int64_t)(r.start + at.nth) * a.q.token_stride +
+                                     (int64_t)at.head * a.q.head_stride) * Elem<DT>::SIZE;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             const int d0 = k * 32 + g * 8;
-            load_query<DT>(at + (int64_t)d0 * Elem<DT>::SIZE, has[t] && d0 < a.pool.head_dim, q[t][k]);
+            const bool in = d0 < a.pool.head_dim;
+            load_query<DT>(q0 + (int64_t)(in ? d0 : 0) * Elem<DT>::SIZE, has && in, a.scale < 0.0f,
+                           q[t][k]);
         }
     }
     /* places that any and that all of the wave's queries see */
@@ -104,9 +175,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     const bool busy = wcol0 < cols;
     const int w_first = r.length - r.count + divide(col0 + (busy ? wcol0 : 0), a.group);
     const int w_last = r.length - r.count + divide(col0 + (busy ? wcol1 - 1 : 0), a.group);
-    const int any_from = sees_from(w_first), all_from = sees_from(w_last);
+    const int any_from = sees_from(a, w_first), all_from = sees_from(a, w_last);
 
-    const float c = a.scale * kLog2e;
+    /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
+    const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
     f32x4 o[NT][DB];
     float top[NT], sum[NT];
 #pragma unroll
@@ -142,6 +214,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     uint32_t kw[KL][4], vw[VL][4];
     auto load = [&](int n) {
         const int b = n % 3;
+        const int tid = again(threadIdx.x);
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = tid + i * THREADS, t = u / (D / 16), d0 = u % (D / 16) * 16;
@@ -165,6 +238,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     };
     auto store = [&](int n) {
         const int b = n % 3, to = n & 1;
+        const int tid = again(threadIdx.x);
         bool any = false;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
@@ -240,6 +314,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                             sc[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, q[t][k][p].v, sc[t][b], 0, 0, 0);
                 }
             }
+            lay_out<TB * KS, NT * QP>();
             const uint64_t bad = s.bad[n % 3];
             const bool partly = bad != 0 || t0 < all_from || t0 + KT - 1 > w_first;
             const bool nan_v = partly && s.nan[buf] != 0;
@@ -247,10 +322,6 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 float now = -inf32();
-#pragma unroll
-                for (int b = 0; b < TB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[t][b][i] *= c;
                 if (partly) {
 #pragma unroll
                     for (int b = 0; b < TB; ++b)
@@ -269,19 +340,19 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                 now = fmaxf(now, __shfl_xor(now, 32));
                 now = fmaxf(now, top[t]);
                 if (__any(now > top[t])) {
-                    const float keep = now > top[t] ? __builtin_amdgcn_exp2f(top[t] - now) : 1.0f;
+                    const float keep = now > top[t] ? __builtin_amdgcn_exp2f((top[t] - now) * c) : 1.0f;
                     sum[t] *= keep;
 #pragma unroll
                     for (int i = 0; i < DB; ++i) o[t][i] *= keep;
                     top[t] = now;
                 }
-                const float base = top[t] == -inf32() ? 0.0f : top[t];
+                const float base = top[t] == -inf32() ? 0.0f : top[t] * c;
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
 #pragma unroll
                     for (int i = 0; i < 4; i += 2) {
-                        const float e0 = __builtin_amdgcn_exp2f(sc[t][b][i] - base);
-                        const float e1 = __builtin_amdgcn_exp2f(sc[t][b][i + 1] - base);
+                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i], c, -base));
+                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i + 1], c, -base));
                         sum[t] += e0 + e1;
                         Frag* f = pw[t][b >> 1];
                         const int w = (b & 1) * 2 + (i >> 1);
@@ -291,10 +362,14 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                                                   e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
                     }
             }
+            /* value_piece(i * 16 + m, h * 4 + g) is that of m and g, exchanged by 2 i and 4 h: few
+             * addresses for all */
+            const char* const v0 = reinterpret_cast<const char*>(&s.v[buf][m][0]);
+            const int piece = value_piece<KT>(m, g);
             auto value = [&](int i, int h) {
-                const int dim = i * 16 + m;
+                const int p = piece ^ ((h * 4) ^ (i * 2)) & (KT / 8 - 1);
                 Frag f;
-                f.v = *reinterpret_cast<const bf16x8*>(&s.v[buf][dim][value_piece<KT>(dim, h * 4 + g) * 8]);
+                f.v = *reinterpret_cast<const bf16x8*>(v0 + p * 16 + i * 16 * KT * 2);
                 return f;
             };
             if (!nan_v) {
@@ -309,6 +384,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                             for (int p = PP - 1; p >= 0; --p)
                                 o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
                     }
+                lay_out<DB * TB / 2, NT * PP>();
             } else {
                 /* a NaN that some queries see and others do not (0 times NaN is NaN): the
                  * products go without it, and whoever sees one, counted by a product too,
@@ -355,76 +431,71 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     for (int t = 0; t < NT; ++t) {
         sum[t] += __shfl_xor(sum[t], 16);
         sum[t] += __shfl_xor(sum[t], 32);
-    }
-    auto finish = [&](int nt, int qh, int dim, f32x4 v) {
-        store4<DT>(a.out.data + ((int64_t)(r.start + nt) * a.out.token_stride +
-                                 (int64_t)qh * a.out.head_stride + dim) * Elem<DT>::SIZE, v);
-    };
-    auto log_sum = [&](int nt, int qh, float best, float all, bool empty) {
-        if (a.lse)
-            a.lse[(int64_t)(r.start + nt) * a.heads + qh] =
-                r.bad ? nan32() : empty ? -inf32() : (best + __builtin_amdgcn_logf(all)) * kLn2;
-    };
-    const int64_t item = x * gridDim.x + head;
-    if (parts == 1) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            if (!has[t]) continue;
-            const bool empty = !r.bad && place[t] < 0;
-            const float inv = r.bad ? nan32() : 1.0f / sum[t];
-#pragma unroll
-            for (int i = 0; i < DB; ++i) {
-                const int dim = i * 16 + g * 4;
-                if (dim < a.pool.head_dim)
-                    finish(nth[t], qhead[t], dim, empty ? f32x4{0, 0, 0, 0} : o[t][i] * inv);
-            }
-            if (g == 0) log_sum(nth[t], qhead[t], top[t], sum[t], empty);
-        }
-        return;
-    }
-    const int64_t slot0 = item * splits;
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        if (!has[t]) continue;
         const int k = (wave * NT + t) * 16 + m;
-        float* to = a.ws.sums + (slot0 + part) * kAttendSums + (int64_t)k * D;
+        if (k >= cols) continue;
+        const float base = top[t] == -inf32() ? top[t] : top[t] * c;
+        if (parts == 1) {
+            const Column at = column(a, r, head, col0 + k);
+            const float inv = 1.0f / sum[t];
 #pragma unroll
-        for (int i = 0; i < DB; ++i) {
-            uint64_t* w = reinterpret_cast<uint64_t*>(to + i * 16 + g * 4);
-            st_dev(w, (uint64_t)__float_as_uint(o[t][i][0]) | (uint64_t)__float_as_uint(o[t][i][1]) << 32);
-            st_dev(w + 1, (uint64_t)__float_as_uint(o[t][i][2]) | (uint64_t)__float_as_uint(o[t][i][3]) << 32);
+            for (int i = 0; i < DB; ++i) put<DT>(a, r, at, i * 16 + g * 4, o[t][i] * inv);
+            if (g == 0) put_lse(a, r, at, base, sum[t]);
+            continue;
         }
+        const int64_t slot = (x * gridDim.x + head) * splits + part;
+        float* to = a.ws.sums + slot * kAttendSums + (int64_t)k * D;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[t][i];
         if (g == 0)
-            st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot0 + part) * kAttendStats + k * 2),
-                   (uint64_t)__float_as_uint(top[t]) | (uint64_t)__float_as_uint(sum[t]) << 32);
+            *reinterpret_cast<float2*>(a.ws.stats + slot * kAttendStats + k * 2) =
+                make_float2(base, sum[t]);
     }
-    if (!elect_last(&a.ws.tickets[item], (uint32_t)parts, &s.flag)) return;
-    for (int i = tid; i < cols * (D / 4); i += THREADS) {
-        const int k = i / (D / 4), dim = i % (D / 4) * 4;
-        if (dim >= a.pool.head_dim) continue;
-        const int col = col0 + k, nt = divide(col, a.group);
-        const int qh = head * a.group.d + col - nt * a.group.d;
-        float best = -inf32(), all = 0.0f;
-        f32x4 v = f32x4{0, 0, 0, 0};
-        for (int w = 0; w < parts; ++w) {
-            const uint64_t st = ld_dev(reinterpret_cast<const uint64_t*>(
-                a.ws.stats + (slot0 + w) * kAttendStats + k * 2));
-            const uint64_t* at = reinterpret_cast<const uint64_t*>(
-                a.ws.sums + (slot0 + w) * kAttendSums + (int64_t)k * D + dim);
-            const uint64_t v0 = ld_dev(at), v1 = ld_dev(at + 1);
-            const float tw = __uint_as_float((uint32_t)st), lw = __uint_as_float((uint32_t)(st >> 32));
-            const float now = fmaxf(best, tw);
-            const float keep = best == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(best - now);
-            const float f = tw == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(tw - now);
-            best = now;
-            all = all * keep + lw * f;
-            v = v * keep + f32x4{__uint_as_float((uint32_t)v0), __uint_as_float((uint32_t)(v0 >> 32)),
-                                 __uint_as_float((uint32_t)v1), __uint_as_float((uint32_t)(v1 >> 32))} * f;
+}
+
+/* What the parts of each block of columns found, joined: four dims of a column a thread.  A launch of
+ * its own, as a block's parts are up to 128 KiB each: one workgroup took 200 us to join 14 of them. */
+template <int DT, int D, int CB, int KT>
+__global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int splits)
+{
+    const int head = blockIdx.x;
+    const int64_t x = blockIdx.y;
+    const Block b = find_block(a, x, CB, KT, splits);
+    if (b.cols == 0 || b.parts == 1) return;
+    const int i = blockIdx.z * kJoin + threadIdx.x, k = i / (D / 4), dim = i % (D / 4) * 4;
+    if (k >= b.cols || dim >= a.pool.head_dim) return;
+    const int64_t slot = (x * gridDim.x + head) * splits;
+    const float* stats = a.ws.stats + slot * kAttendStats + k * 2;
+    const float* sums = a.ws.sums + slot * kAttendSums + (int64_t)k * D + dim;
+    float best = -inf32(), all = 0.0f;
+    f32x4 v = f32x4{0, 0, 0, 0};
+    constexpr int N = 8; /* parts in flight */
+    for (int w0 = 0; w0 < b.parts; w0 += N) {
+        float2 st[N];
+        f32x4 p[N];
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            const int64_t n = w0 + w < b.parts ? w0 + w : b.parts - 1;
+            st[w] = *reinterpret_cast<const float2*>(stats + n * kAttendStats);
+            p[w] = *reinterpret_cast<const f32x4*>(sums + n * kAttendSums);
         }
-        const bool empty = r.length - r.count + nt < 0;
-        finish(nt, qh, dim, empty ? f32x4{0, 0, 0, 0} : v * (1.0f / all));
-        if (dim == 0) log_sum(nt, qh, best, all, empty);
+        float now = best;
+#pragma unroll
+        for (int w = 0; w < N; ++w) now = fmaxf(now, st[w].x);
+        const float keep = best == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(best - now);
+        all *= keep;
+        v *= keep;
+        best = now;
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            if (w0 + w >= b.parts) break;
+            const float f = st[w].x == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(st[w].x - now);
+            all += st[w].y * f;
+            v += p[w] * f;
+        }
     }
+    const Column at = column(a, b.r, head, b.col0 + k);
+    put<DT>(a, b.r, at, dim, v * (1.0f / all));
+    if (dim == 0) put_lse(a, b.r, at, best, all);
 }
 
 template <int DT, int D, int NW, int NT, int KT>
@@ -436,17 +507,21 @@ hipError_t prompts_launch(const AttendArgs& a, hipStream_t stream)
     int64_t splits = a.ws.groups / items;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)slots, (unsigned)splits);
-    return launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64, sizeof(Shared<D, KT>),
-                  stream, a, (int)splits);
+    const hipError_t e = launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64,
+                                sizeof(Shared<D, KT>), stream, a, (int)splits);
+    if (e != hipSuccess || splits == 1) return e;
+    const dim3 join((unsigned)a.kv_heads, (unsigned)slots, (unsigned)(CB * D / 4 / kJoin));
+    return launch(join_prompts_kernel<DT, D, CB, KT>, join, kJoin, 0, stream, a, (int)splits);
 }
 
 template <int DT>
 hipError_t by_width(const AttendArgs& a, hipStream_t stream)
 {
+    constexpr bool F32 = DT == G4S_DTYPE_F32;
     switch (attend_width(a.pool.head_dim)) {
-    case 64: return prompts_launch<DT, 64, 8, 2, 64>(a, stream);
-    case 128: return prompts_launch<DT, 128, 8, 2, 64>(a, stream);
-    case 256: return prompts_launch<DT, 256, 4, 2, 64>(a, stream);
+    case 64: return prompts_launch<DT, 64, 8, F32 ? 1 : 2, 64>(a, stream);
+    case 128: return prompts_launch<DT, 128, 8, F32 ? 1 : 2, 64>(a, stream);
+    case 256: return prompts_launch<DT, 256, F32 ? 8 : 4, F32 ? 1 : 2, 64>(a, stream);
     default: return prompts_launch<DT, 512, 4, 1, 32>(a, stream);
     }
 }
