@@ -3,13 +3,14 @@
  * rotated by their positions on the way, and the queries rotated beside
  * them, on gfx950.
  *
- * A workgroup takes up to TILE places of one row, whole blocks of tokens that share a
- * scale, so that a scale and the codes under it have one writer.  It goes
- * over their keys and values twice: for the largest magnitude of each block and
- * head, and to store them (the second time they come from the caches).
- * Rotations are computed in binary64 and rounded once: next to a border between two codes
- * a rounding in between would choose the other one.  Cosines and sines are computed once per
- * token and pair, in LDS for all heads.
+ * A workgroup takes up to `tile` places of one row, whole blocks of tokens that share a
+ * scale, so that a scale and the codes under it have one writer, and some of the heads: of
+ * queries, or of keys and values.  Those it goes over twice, for the largest
+ * magnitude of each block and head, and to store them (the second time they come
+ * from registers where a thread has one vector, from the caches otherwise).
+ * Keys are rotated in binary64 and rounded once: next to a border between two codes a
+ * rounding in between would choose the other one.  Cosines and sines are computed once per
+ * token and pair, in LDS for all heads of the workgroup.
  */
 #include "g4s_cache.h"
 #include "g4s_device.h"
@@ -20,11 +21,14 @@ namespace g4s {
 namespace {
 
 constexpr int kB = 256;
-constexpr int kTile = 16;    /* places of a workgroup, or one block where that is longer */
-constexpr int kChunk = 8;    /* dims of a thread */
-constexpr int kStep = 8;     /* tokens whose angles are in LDS at once */
+constexpr int kTile = 16;  /* places of a workgroup, or one block where that is longer */
+constexpr int kChunk = 8;  /* dims of a thread */
+constexpr int kStep = 16;  /* tokens whose angles are in LDS at once */
+constexpr int kPairs = 2048; /* .. as long as they have no more pairs than this */
+constexpr int kQueryHeads = 8, kKeyHeads = 2; /* of a workgroup, where there are several tokens */
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 /* sin and cos of x (|x| < 2^40) to some 2^-52: x - n pi/2 with pi/2 in three
  * parts, then the Taylor series of both up to x^17 and x^18, whose next terms are below 2^-62 at
@@ -109,42 +113,32 @@ __device__ __forceinline__ float to_odd(double x)
     return __uint_as_float(__builtin_fabs(x) > __builtin_fabs(d) ? u + 1 : u - 1);
 }
 
-__device__ __forceinline__ uint16_t bf16_of(double x)
-{
-    const uint32_t u = __float_as_uint(to_odd(x));
-    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return (uint16_t)(u >> 16 | 0x40u);
-    return (uint16_t)((u + 0x7FFFu + (u >> 16 & 1u)) >> 16);
-}
-
+/* bf16 by way of binary32: off by 2^-16 of a bf16 step more than in one rounding. */
 template <int DT>
 __device__ __forceinline__ void store_chunk(char* p, const double (&y)[kChunk])
 {
-    if constexpr (DT == G4S_DTYPE_F32) {
-        float4 a, b;
-        a.x = (float)y[0], a.y = (float)y[1], a.z = (float)y[2], a.w = (float)y[3];
-        b.x = (float)y[4], b.y = (float)y[5], b.z = (float)y[6], b.w = (float)y[7];
-        reinterpret_cast<float4*>(p)[0] = a;
-        reinterpret_cast<float4*>(p)[1] = b;
-    } else {
-        uint32_t w[4];
+    float x[kChunk];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = (uint32_t)bf16_of(y[2 * i]) | (uint32_t)bf16_of(y[2 * i + 1]) << 16;
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < kChunk; ++i) x[i] = (float)y[i];
+    if constexpr (DT == G4S_DTYPE_F32) {
+        reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+        reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    } else {
+        bf16x8 w;
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) w[i] = (__bf16)x[i];
+        *reinterpret_cast<bf16x8*>(p) = w;
     }
 }
 
-/* x / scale as an e4m3 code: within the type's range first, as the conversion gives NaN
- * for what lies outside. */
-__device__ __forceinline__ uint32_t codes4(const double* y, double inv)
+/* Codes of four quotients (binary32, not between two codes where the exact ones are not): within
+ * the type's range first, as the conversion gives NaN for what lies outside. */
+__device__ __forceinline__ uint32_t codes4(const float* x)
 {
     float f[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const double v = y[i] * inv;
-        f[i] = to_odd(v > 448.0 ? 448.0 : v < -448.0 ? -448.0 : v);
-    }
-    int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+    for (int i = 0; i < 4; ++i) f[i] = x[i] > 448.0f ? 448.0f : x[i] < -448.0f ? -448.0f : x[i];
+    const int w = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
     return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], w, true);
 }
 
@@ -154,85 +148,143 @@ struct Tile {
     int before;          /* earlier tokens in the first block */
 };
 
-/* Chunk `c` of a head of one token, rotated where ROTATE. */
-template <int DT, bool ROTATE>
-__device__ __forceinline__ void rotated(const AppendArgs& a, const CacheView& view, int64_t token,
-                                        int head, int c, const double2* turn, double (&y)[kChunk])
+/* How dims are paired: halves or neighbours where no chunk of dims lies across a border, or
+ * whatever else, dim by dim. */
+enum Mode { kHalves, kNeighbours, kAny };
+
+/* Chunk `c` of a head of one token: what is in it, and what is paired with it. */
+struct Chunk {
+    float x[kChunk], o[kChunk];
+};
+template <int DT, int MODE>
+__device__ __forceinline__ void read_chunk(const AppendArgs& a, const CacheView& view, int64_t token,
+                                           int head, int c, bool rotate, Chunk& w)
 {
-    const int d0 = c * kChunk;
-    float x[kChunk];
-    load_chunk<DT>(element<DT>(view, token, head, d0), x);
+    const int d0 = c * kChunk, half = a.rotary_dims >> 1;
+    load_chunk<DT>(element<DT>(view, token, head, d0), w.x);
+    if (!rotate || d0 >= a.rotary_dims) return;
+    if (MODE == kHalves)
+        load_chunk<DT>(element<DT>(view, token, head, d0 < half ? d0 + half : d0 - half), w.o);
+    if (MODE == kAny) {
+        for (int i = 0; i < kChunk; ++i) {
+            const int d = d0 + i;
+            const int pair = a.rotary_pairs == G4S_ROTARY_NEIGHBOURS ? d ^ 1 : d < half ? d + half : d - half;
+            const float v = d < a.rotary_dims ? load_one<DT>(element<DT>(view, token, head, pair)) : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) y[i] = (double)x[i];
-    if (!ROTATE || d0 >= a.rotary_dims) return;
-    if (a.rotary_pairs == G4S_ROTARY_NEIGHBOURS) {
+            for (int k = 0; k < kChunk; ++k) w.o[k] = k == i ? v : w.o[k];
+        }
+    }
+}
+/* Cosines and sines for the dims of a chunk (1 and 0 behind the last dim that is rotated). */
+struct Turn {
+    double2 t[kChunk];
+};
+template <int MODE>
+__device__ __forceinline__ void read_turn(const AppendArgs& a, int c, const double2* turn, Turn& r)
+{
+    const int d0 = c * kChunk, half = a.rotary_dims >> 1;
+    if (d0 >= a.rotary_dims) return;
+    if (MODE == kHalves) {
+        const double2* at = turn + (d0 < half ? d0 : d0 - half);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) r.t[i] = at[i];
+    } else if (MODE == kNeighbours) {
+#pragma unroll
+        for (int i = 0; i < kChunk; i += 2) r.t[i] = turn[(d0 + i) >> 1];
+    } else {
+        for (int i = 0; i < kChunk; ++i) {
+            const int d = d0 + i;
+            const int f = a.rotary_pairs == G4S_ROTARY_NEIGHBOURS ? d >> 1 : d < half ? d : d - half;
+            const double2 t = d < a.rotary_dims ? turn[f] : make_double2(1.0, 0.0);
+#pragma unroll
+            for (int k = 0; k < kChunk; ++k) {
+                r.t[k].x = k == i ? t.x : r.t[k].x;
+                r.t[k].y = k == i ? t.y : r.t[k].y;
+            }
+        }
+    }
+}
+template <int MODE>
+__device__ __forceinline__ void rotate(const AppendArgs& a, const Chunk& w, int c, const Turn& r,
+                                       double (&y)[kChunk])
+{
+    const int d0 = c * kChunk, half = a.rotary_dims >> 1;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) y[i] = (double)w.x[i];
+    if (d0 >= a.rotary_dims) return;
+    if (MODE == kNeighbours) {
 #pragma unroll
         for (int i = 0; i < kChunk; i += 2) {
-            if (d0 + i >= a.rotary_dims) break;
-            const double2 t = turn[(d0 + i) >> 1];
-            const double u = y[i], w = y[i + 1];
-            y[i] = __builtin_fma(u, t.x, -(w * t.y));
-            y[i + 1] = __builtin_fma(w, t.x, u * t.y);
+            const double u = y[i], v = y[i + 1];
+            y[i] = __builtin_fma(u, r.t[i].x, -(v * r.t[i].y));
+            y[i + 1] = __builtin_fma(v, r.t[i].x, u * r.t[i].y);
         }
-        return;
-    }
-    const int half = a.rotary_dims >> 1;
-    float o[kChunk];
-    if ((half & (kChunk - 1)) == 0) {
-        load_chunk<DT>(element<DT>(view, token, head, d0 < half ? d0 + half : d0 - half), o);
     } else {
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
-            const int d = d0 + i;
-            o[i] = d < a.rotary_dims
-                       ? load_one<DT>(element<DT>(view, token, head, d < half ? d + half : d - half))
-                       : 0.0f;
+            const bool low = MODE == kHalves ? d0 < half
+                             : a.rotary_pairs == G4S_ROTARY_NEIGHBOURS ? (i & 1) == 0
+                                                                      : d0 + i < half;
+            const double v = (double)w.o[i] * r.t[i].y;
+            y[i] = __builtin_fma(y[i], r.t[i].x, low ? -v : v);
         }
-    }
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-        const int d = d0 + i;
-        if (d >= a.rotary_dims) break;
-        const bool low = d < half;
-        const double2 t = turn[low ? d : d - half];
-        /* (the order of the two products is the same for both dims of a pair) */
-        y[i] = low ? __builtin_fma(y[i], t.x, -((double)o[i] * t.y))
-                   : __builtin_fma(y[i], t.x, (double)o[i] * t.y);
     }
 }
 
+/* Where a row's places are.  The page of the first one is read ahead of its use. */
+struct Places {
+    const int32_t* pages; /* of the row */
+    int slot, page;
+};
+__device__ __forceinline__ Places places_of(const AppendArgs& a, int row, int first)
+{
+    Places p;
+    p.pages = a.table + (int64_t)row * a.pool.max_slots;
+    p.slot = divide(first, a.pool.page_tokens);
+    p.page = p.pages[p.slot];
+    return p;
+}
 /* Offset of a place in a plane, or -1 where its page is outside the pool. */
-__device__ __forceinline__ int64_t place_offset(const AppendArgs& a, int row, int place, int head)
+__device__ __forceinline__ int64_t place_offset(const AppendArgs& a, const Places& p, int place,
+                                                int head)
 {
     const int slot = divide(place, a.pool.page_tokens);
-    const int page = a.table[(int64_t)row * a.pool.max_slots + slot];
+    const int page = slot == p.slot ? p.page : p.pages[slot];
     if (page < 0 || page >= a.pool.n_pages) return -1;
     return cache_offset(a.pool, page, place - slot * a.pool.page_tokens.d, head);
 }
 
+/* A block's scale for new values of magnitude `top`, and in `grown` what codes that it
+ * holds under `old` are multiplied by (1: nothing). */
+__device__ __forceinline__ float block_scale(uint32_t top, bool earlier, float old, float& grown)
+{
+    const float scale = __builtin_ldexpf(1.0f, scale_exponent((double)__uint_as_float(top)));
+    grown = 1.0f;
+    if (!earlier) return scale;
+    if (old >= scale && old < __builtin_inff()) return old;
+    if (old > 0.0f) grown = old / scale;
+    return scale;
+}
 /* The row and places of slot x of the grid; false where it has none. */
 __device__ __forceinline__ bool find_tile(const AppendArgs& a, int64_t x, int tile, Tile& t)
 {
-    int row = (int)x;
-    if (a.starts) {
-        row = find_share(a.starts, a.rows, x, 1, tile, 2);
-    }
-    const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    int64_t nth = a.starts ? x - share_begin(a.starts, row, 1, tile, 2) : 0;
+    t.row = find_share(a.starts, a.rows, x, 1, tile, 2);
+    const RowTokens r = row_tokens(a.starts, a.lengths, t.row, a.tokens, cache_room(a.pool));
+    const int64_t nth = x - share_begin(a.starts, t.row, 1, tile, 2);
     if (r.count == 0 || r.length == 0 || nth < 0) return false;
     const int from = r.length > r.count ? r.length - r.count : 0; /* the first place */
     const int64_t begin = (from / tile + nth) * tile;
     if (begin >= r.length) return false;
-    t.row = row;
     t.first = (int)(begin > from ? begin : from);
     t.end = (int)(begin + tile < r.length ? begin + tile : r.length);
     t.token = (int64_t)r.start + (t.first - (r.length - r.count));
-    t.before = begin < t.first ? (t.first - (int)begin) % a.pool.scale_tokens.d : 0;
+    t.before = t.first - divide(t.first, a.pool.scale_tokens) * a.pool.scale_tokens.d;
     return true;
 }
 
-/* The largest finite magnitude of a chunk, as the bits of a binary64 (which are in order). */
-__device__ __forceinline__ uint64_t top_of(const double (&y)[kChunk])
+/* The largest finite magnitude of a chunk, as the bits of a binary32, which are in order.
+ * (to_odd keeps a value on its side of 448 * 2^e, whose last bit is even.) */
+__device__ __forceinline__ uint32_t top_of(const double (&y)[kChunk])
 {
     double m = 0.0;
 #pragma unroll
@@ -240,139 +292,338 @@ __device__ __forceinline__ uint64_t top_of(const double (&y)[kChunk])
         const double v = __builtin_fabs(y[i]);
         m = v > m && v < __builtin_inf() ? v : m;
     }
-    return (uint64_t)__double_as_longlong(m);
+    return __float_as_uint(to_odd(m));
+}
+__device__ __forceinline__ uint32_t top_of(const float (&x)[kChunk])
+{
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) {
+        const float v = __builtin_fabsf(x[i]);
+        m = v > m && v < __builtin_inff() ? v : m;
+    }
+    return __float_as_uint(m);
 }
 
-template <int DT>
-__global__ __launch_bounds__(kB) void append_kernel(AppendArgs a, int tile)
+/* Four codes under a scale that grew. */
+__device__ __forceinline__ uint32_t regrown(uint32_t w, float ratio)
+{
+    const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false);
+    const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+    const float x[4] = {lo[0] * ratio, lo[1] * ratio, hi[0] * ratio, hi[1] * ratio};
+    return codes4(x);
+}
+
+/* The largest of a vector's lanes (a power of two of them). */
+__device__ __forceinline__ uint32_t lanes_max(uint32_t m, int chunks)
+{
+    for (int d = 1; d < chunks; d <<= 1) {
+        const uint32_t o = (uint32_t)__shfl_xor((int)m, d);
+        m = o > m ? o : m;
+    }
+    return m;
+}
+
+/* Values are exact in binary32, and so are their products with a scale's inverse. */
+__device__ __forceinline__ void store_codes(char* at, bool value, const Chunk& w,
+                                            const double (&y)[kChunk], float scale)
+{
+    const float inv = 1.0f / scale;
+    float x[kChunk];
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) x[i] = value ? w.x[i] * inv : to_odd(y[i] * (double)inv);
+    uint32_t* to = reinterpret_cast<uint32_t*>(at);
+    to[0] = codes4(x);
+    to[1] = codes4(x + 4);
+}
+
+/* ------------------------------------------------------- a token for each row */
+
+/* A workgroup has the row's vectors (queries, keys, values) from first_vector on, one for each
+ * kChunk-dim lane group; a block's new values are those of one vector. */
+template <int DT, int MODE>
+__global__ __launch_bounds__(kB) void append_step_kernel(AppendArgs a, int queries, int vectors)
+{
+    __shared__ double2 turn[G4S_CACHE_MAX_HEAD_DIM / 2];
+    __shared__ uint32_t s_top[kB];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int row = blockIdx.x, half = a.rotary_dims >> 1;
+    const int chunks = a.pool.head_dim / kChunk, each = 64 / chunks;
+    const int g = lane / chunks, c = lane - g * chunks;
+    const int nth = wave * each + g, vector = (int)blockIdx.y * (kB / 64 * each) + nth;
+    const bool in = g < each && vector < vectors;
+    /* queries, keys, values */
+    const bool query = vector < queries;
+    const int item = vector - queries;
+    const bool value = !query && item >= a.kv_heads;
+    const int head = query ? vector : value ? item - a.kv_heads : item;
+    Chunk w;
+    if (in) read_chunk<DT, MODE>(a, query ? a.q : value ? a.v : a.k, row, head, c, !value, w);
+    const float freq = tid < half ? a.freqs[tid] : 0.0f;
+    const int position = a.positions ? a.positions[row] : 0;
+    const int length = a.lengths[row];
+    s_top[tid] = 0;
+    if (length <= 0 || length > cache_room(a.pool)) return;
+    const int place = length - 1;
+    const int before = place - divide(place, a.pool.scale_tokens) * a.pool.scale_tokens.d;
+    int64_t off = -1;
+    float old = 0.0f;
+    if (in && !query) {
+        const Places p = places_of(a, row, place);
+        off = place_offset(a, p, place - before, head);
+    }
+    char* const block = (value ? a.v_plane : a.k_plane) + off; /* its first token */
+    float* const scale_at = reinterpret_cast<float*>(block + a.pool.head_dim);
+    if (off >= 0 && before > 0) old = *scale_at;
+    for (int i = tid; i < half; i += kB) {
+        double s, t;
+        sincos64((double)(a.positions ? position : place) * (double)freq, s, t);
+        turn[i] = make_double2(t, s);
+    }
+    __syncthreads();
+    double y[kChunk];
+    if (in && !value) {
+        Turn t;
+        read_turn<MODE>(a, c, turn, t);
+        rotate<MODE>(a, w, c, t, y);
+    }
+    if (in && query)
+        store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, row, head, c * kChunk)), y);
+    uint32_t top = 0;
+    if (in && !query) top = value ? top_of(w.x) : top_of(y);
+    if ((chunks & (chunks - 1)) == 0) {
+        top = lanes_max(top, chunks);
+    } else {
+        if (in) atomicMax(&s_top[nth], top);
+        __syncthreads();
+        if (in) top = s_top[nth];
+    }
+    if (off < 0) return;
+    float grown;
+    const float scale = block_scale(top, before > 0, old, grown);
+    store_codes(block + (int64_t)before * a.pool.token_bytes + c * kChunk, value, w, y, scale);
+    if (c == 0) *scale_at = scale;
+    if (grown == 1.0f) return;
+    for (int j = 0; j < before; ++j) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(block + (int64_t)j * a.pool.token_bytes + c * kChunk);
+        const uint32_t w0 = at[0], w1 = at[1];
+        at[0] = regrown(w0, grown);
+        at[1] = regrown(w1, grown);
+    }
+}
+
+/* ------------------------------------------------------------- ragged tokens */
+
+/* How a workgroup's threads lie over tokens and chunks: `tokens` vectors at once. */
+struct Lanes {
+    int chunks, tokens;
+    int c, token; /* this thread's; token = tokens: none */
+};
+__device__ __forceinline__ Lanes lanes_of(int chunks)
+{
+    Lanes l;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, each = 64 / chunks;
+    const int g = lane / chunks;
+    l.chunks = chunks;
+    l.tokens = kB / 64 * each;
+    l.c = lane - g * chunks;
+    l.token = g < each ? wave * each + g : l.tokens;
+    return l;
+}
+
+/* Cosines and sines of n tokens from place s0 on. */
+__device__ __forceinline__ void fill_turns(const AppendArgs& a, const Tile& t, int s0, int n,
+                                           double2* turn)
+{
+    const int half = a.rotary_dims >> 1;
+    for (int i = threadIdx.x; i < n * half; i += kB) {
+        const int j = i / half, f = i - j * half;
+        const float freq = a.freqs[f];
+        const int p = a.positions ? a.positions[t.token + (s0 - t.first) + j] : s0 + j;
+        double s, c;
+        sincos64((double)p * (double)freq, s, c);
+        turn[i] = make_double2(c, s);
+    }
+}
+
+/* Queries: each vector in one wave, which has read it before it writes it, so that q_out may
+ * be q. */
+template <int DT, int MODE>
+__device__ __forceinline__ void append_queries(const AppendArgs& a, const Tile& t, int head0,
+                                               int heads, int step, double2* turn)
+{
+    const int half = a.rotary_dims >> 1;
+    const Lanes l = lanes_of(a.pool.head_dim / kChunk);
+    const int end = head0 + heads < a.heads ? head0 + heads : a.heads;
+    for (int s0 = t.first; s0 < t.end; s0 += step) {
+        const int n = t.end - s0 < step ? t.end - s0 : step;
+        const int64_t token0 = t.token + (s0 - t.first);
+        __syncthreads();
+        fill_turns(a, t, s0, n, turn);
+        __syncthreads();
+        if (l.token == l.tokens) continue;
+        for (int j = l.token; j < n; j += l.tokens) {
+            Turn r;
+            read_turn<MODE>(a, l.c, turn + j * half, r);
+#pragma unroll 2
+            for (int h = head0; h < end; ++h) {
+                Chunk w;
+                read_chunk<DT, MODE>(a, a.q, token0 + j, h, l.c, true, w);
+                double y[kChunk];
+                rotate<MODE>(a, w, l.c, r, y);
+                store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, token0 + j, h, l.c * kChunk)), y);
+            }
+        }
+    }
+}
+
+/* Keys, or values, of `heads` heads. */
+template <int DT, int MODE, bool VALUE>
+__device__ __forceinline__ void append_heads(const AppendArgs& a, const Tile& t, int head0, int heads,
+                                             int step, double2* turn, uint32_t* top, float* ratio)
+{
+    const int half = a.rotary_dims >> 1, B = a.pool.scale_tokens.d, tid = threadIdx.x;
+    const CacheView& view = VALUE ? a.v : a.k;
+    char* const plane = VALUE ? a.v_plane : a.k_plane;
+    const Places places = places_of(a, t.row, t.first);
+    const int first_block = t.first / B;
+    const int blocks = (t.end - 1) / B - first_block + 1;
+    const int end = head0 + heads < a.kv_heads ? head0 + heads : a.kv_heads;
+    heads = end - head0;
+    const Lanes l = lanes_of(a.pool.head_dim / kChunk);
+    const bool pow2 = (l.chunks & (l.chunks - 1)) == 0;
+    for (int i = tid; i < blocks * heads; i += kB) top[i] = 0;
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int s0 = t.first; s0 < t.end; s0 += step) {
+            const int n = t.end - s0 < step ? t.end - s0 : step;
+            const int64_t token0 = t.token + (s0 - t.first);
+            if (pass == 0 || t.end - t.first > step) {
+                __syncthreads();
+                if (!VALUE) fill_turns(a, t, s0, n, turn);
+                __syncthreads();
+            }
+            for (int j0 = 0; j0 < n; j0 += l.tokens) {
+                const int j = j0 + l.token;
+                const bool in = l.token < l.tokens && j < n;
+                const int place = s0 + j;
+                Turn r;
+                if (!VALUE && in) read_turn<MODE>(a, l.c, turn + j * half, r);
+                const int64_t off = pass == 1 && in ? place_offset(a, places, place, head0) : -1;
+                const int at = in ? (place / B - first_block) * heads : 0;
+#pragma unroll 2
+                for (int k = 0; k < heads; ++k) {
+                    Chunk w;
+                    double y[kChunk];
+                    if (in) {
+                        read_chunk<DT, MODE>(a, view, token0 + j, head0 + k, l.c, !VALUE, w);
+                        if (!VALUE) rotate<MODE>(a, w, l.c, r, y);
+                    }
+                    if (pass == 0) {
+                        uint32_t m = 0;
+                        if (in) m = VALUE ? top_of(w.x) : top_of(y);
+                        if (pow2) m = lanes_max(m, l.chunks);
+                        if (in && (!pow2 || l.c == 0)) atomicMax(&top[at + k], m);
+                    } else if (off >= 0) {
+                        store_codes(plane + off + (int64_t)k * a.pool.part_bytes + l.c * kChunk, VALUE,
+                                    w, y, __uint_as_float(top[at + k]));
+                    }
+                }
+            }
+        }
+        if (pass == 1) break;
+        __syncthreads();
+        /* scales in the place of the magnitudes */
+        for (int i = tid; i < blocks * heads; i += kB) {
+            const int b = i / heads, k = i - b * heads;
+            const int64_t off = place_offset(a, places, (first_block + b) * B, head0 + k);
+            const bool earlier = b == 0 && t.before > 0 && off >= 0;
+            float* at = reinterpret_cast<float*>(plane + off + a.pool.head_dim);
+            float grown;
+            const float scale = block_scale(top[i], earlier, earlier ? *at : 0.0f, grown);
+            if (off >= 0) *at = scale;
+            top[i] = __float_as_uint(scale);
+            if (b == 0) ratio[k] = grown;
+        }
+        __syncthreads();
+        if (t.before == 0) continue;
+        const int words = a.pool.head_dim / 4;
+        for (int i = tid; i < heads * t.before * words; i += kB) {
+            const int v = i / words, k = v / t.before, j = v - k * t.before;
+            if (ratio[k] == 1.0f) continue;
+            const int64_t off = place_offset(a, places, first_block * B + j, head0 + k);
+            if (off < 0) continue;
+            uint32_t* at = reinterpret_cast<uint32_t*>(plane + off) + (i - v * words);
+            *at = regrown(*at, ratio[k]);
+        }
+    }
+}
+
+/* Workgroups of queries, of keys and of values, one behind the other in y. */
+template <int DT, int MODE>
+__global__ __launch_bounds__(kB, 4) void append_tiles_kernel(AppendArgs a, int tile, int step,
+                                                             int q_heads, int q_slices, int kv_heads,
+                                                             int kv_slices)
 {
     extern __shared__ char lds[];
     Tile t;
     if (!find_tile(a, blockIdx.x, tile, t)) return;
-    const int tid = threadIdx.x;
-    const int half = a.rotary_dims >> 1;
-    const int chunks = a.pool.head_dim / kChunk;
-    const int B = a.pool.scale_tokens.d;
-    const int first_block = t.first / B;
-    const int blocks = (t.end - 1) / B - first_block + 1;
-    /* the heads of this slice: of queries, and of keys followed by values */
-    const int slice = blockIdx.y, slices = gridDim.y;
-    const int nq = a.q.data ? (a.heads - slice + slices - 1) / slices : 0;
-    const int items = a.k.data ? 2 * a.kv_heads : 0;
-    const int nkv = items > slice ? (items - slice + slices - 1) / slices : 0;
-    double2* turn = reinterpret_cast<double2*>(lds);                    /* [kStep][half] */
-    uint64_t* top = reinterpret_cast<uint64_t*>(turn + kStep * half);   /* [blocks][nkv] */
-    for (int i = tid; i < blocks * nkv; i += kB) top[i] = 0;
+    double2* turn = reinterpret_cast<double2*>(lds); /* [step][rotary_dims / 2] */
+    const int blocks = (tile + a.pool.scale_tokens.d - 1) / a.pool.scale_tokens.d;
+    uint32_t* top = reinterpret_cast<uint32_t*>(turn + step * (a.rotary_dims >> 1)); /* [blocks][heads] */
+    float* ratio = reinterpret_cast<float*>(top + blocks * kv_heads);                /* [heads] */
+    const int y = blockIdx.y;
+    if (y < q_slices)
+        append_queries<DT, MODE>(a, t, y * q_heads, q_heads, step, turn);
+    else if (y < q_slices + kv_slices)
+        append_heads<DT, MODE, false>(a, t, (y - q_slices) * kv_heads, kv_heads, step, turn, top, ratio);
+    else
+        append_heads<DT, MODE, true>(a, t, (y - q_slices - kv_slices) * kv_heads, kv_heads, step, turn,
+                                     top, ratio);
+}
 
-    for (int pass = 0; pass < (nkv > 0 ? 2 : 1); ++pass) {
-        for (int s0 = t.first; s0 < t.end; s0 += kStep) {
-            const int n = t.end - s0 < kStep ? t.end - s0 : kStep;
-            __syncthreads();
-            for (int i = tid; i < n * half; i += kB) {
-                const int j = i / half, f = i - j * half;
-                const int64_t token = t.token + (s0 - t.first) + j;
-                const int p = a.positions ? a.positions[token] : s0 + j;
-                double s, c;
-                sincos64((double)p * (double)a.freqs[f], s, c);
-                turn[i] = make_double2(c, s);
-            }
-            __syncthreads();
-            if (pass == 0 && nq > 0) {
-                /* the threads of a head's chunks lie in one wave: it has read the head
-                 * before it writes it, so that q_out may be q */
-                const int per_wave = 64 / chunks;
-                const int lane = tid & 63, c = lane % chunks, g = lane / chunks;
-                const int heads = nq * n;
-                for (int i0 = (tid >> 6) * per_wave; i0 < heads; i0 += kB / 64 * per_wave) {
-                    const int i = i0 + g;
-                    if (g >= per_wave || i >= heads) continue;
-                    const int j = i / nq, head = slice + (i - j * nq) * slices;
-                    const int64_t token = t.token + (s0 - t.first) + j;
-                    double y[kChunk];
-                    rotated<DT, true>(a, a.q, token, head, c, turn + j * half, y);
-                    store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, token, head, c * kChunk)),
-                                    y);
-                }
-            }
-            for (int i = tid; i < n * nkv * chunks; i += kB) {
-                const int c = i % chunks, u = i / chunks;
-                const int j = u / nkv, nth = u - j * nkv;
-                const int item = slice + nth * slices;
-                const bool value = item >= a.kv_heads;
-                const int head = value ? item - a.kv_heads : item;
-                const int place = s0 + j;
-                const int64_t token = t.token + (place - t.first);
-                double y[kChunk];
-                if (value)
-                    rotated<DT, false>(a, a.v, token, head, c, nullptr, y);
-                else
-                    rotated<DT, true>(a, a.k, token, head, c, turn + j * half, y);
-                uint64_t* at = &top[(place / B - first_block) * nkv + nth];
-                if (pass == 0) {
-                    atomicMax((unsigned long long*)at, (unsigned long long)top_of(y));
-                    continue;
-                }
-                const int64_t off = place_offset(a, t.row, place, head);
-                if (off < 0) continue;
-                const double inv = 1.0 / __longlong_as_double((long long)*at);
-                char* p = (value ? a.v_plane : a.k_plane) + off;
-                uint32_t* w = reinterpret_cast<uint32_t*>(p + c * kChunk);
-                w[0] = codes4(y, inv);
-                w[1] = codes4(y + 4, inv);
-            }
-        }
-        if (pass == 1 || nkv == 0) break;
-        __syncthreads();
-        /* scales, in the place of the magnitudes; what a block holds already brought to its new one */
-        for (int i = tid; i < blocks * nkv; i += kB) {
-            const int b = i / nkv, item = slice + (i - b * nkv) * slices;
-            const bool value = item >= a.kv_heads;
-            const int head = value ? item - a.kv_heads : item;
-            const int place = (first_block + b) * B;
-            const int64_t off = place_offset(a, t.row, place, head);
-            float scale = __builtin_ldexpf(1.0f, scale_exponent(__longlong_as_double((long long)top[i])));
-            if (off >= 0) {
-                char* p = (value ? a.v_plane : a.k_plane) + off;
-                float* at = reinterpret_cast<float*>(p + a.pool.head_dim);
-                if (b == 0 && t.before > 0) {
-                    const float old = *at;
-                    if (old >= scale && old < __builtin_inff()) {
-                        scale = old;
-                    } else if (old > 0.0f) {
-                        const float ratio = old / scale;
-                        for (int j = 0; j < t.before; ++j) {
-                            uint32_t* w = reinterpret_cast<uint32_t*>(p + (int64_t)j * a.pool.token_bytes);
-                            for (int c = 0; c < a.pool.head_dim / 4; ++c) {
-                                const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[c], false);
-                                const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[c], true);
-                                int v = __builtin_amdgcn_cvt_pk_fp8_f32(lo[0] * ratio, lo[1] * ratio, 0, false);
-                                w[c] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(hi[0] * ratio, hi[1] * ratio, v, true);
-                            }
-                        }
-                    }
-                }
-                *at = scale;
-            }
-            top[i] = (uint64_t)__double_as_longlong((double)scale);
-        }
+template <int DT, int MODE>
+hipError_t launch_mode(const AppendArgs& a, hipStream_t stream)
+{
+    if (!a.starts) {
+        const int at_once = kB / 64 * (64 / (a.pool.head_dim / kChunk));
+        const int queries = a.q.data ? a.heads : 0;
+        const int vectors = queries + (a.k.data ? 2 * a.kv_heads : 0);
+        const dim3 grid((unsigned)a.rows, (unsigned)((vectors + at_once - 1) / at_once));
+        return launch(append_step_kernel<DT, MODE>, grid, kB, 0, stream, a, queries, vectors);
     }
+    const int B = a.pool.scale_tokens.d, half = a.rotary_dims / 2;
+    const int tile = B > kTile ? B : kTile / B * B;
+    int step = half > 0 ? kPairs / half : kStep;
+    step = step > kStep ? kStep : step;
+    step = step > tile ? tile : step;
+    const int q_heads = a.heads < kQueryHeads ? a.heads : kQueryHeads;
+    const int kv_heads = a.kv_heads < kKeyHeads ? a.kv_heads : kKeyHeads;
+    const int q_slices = a.q.data ? (a.heads + q_heads - 1) / q_heads : 0;
+    const int kv_slices = a.k.data ? (a.kv_heads + kv_heads - 1) / kv_heads : 0;
+    const int64_t tiles = (int64_t)a.tokens / tile + 2 * (int64_t)a.rows;
+    const size_t lds = (size_t)step * half * sizeof(double2) +
+                       ((size_t)(tile + B - 1) / B + 1) * kv_heads * sizeof(uint32_t);
+    const dim3 grid((unsigned)tiles, (unsigned)(q_slices + 2 * kv_slices));
+    return launch(append_tiles_kernel<DT, MODE>, grid, kB, lds, stream, a, tile, step, q_heads,
+                  q_slices, kv_heads, kv_slices);
+}
+
+template <int DT>
+hipError_t by_mode(const AppendArgs& a, hipStream_t stream)
+{
+    if (a.rotary_pairs == G4S_ROTARY_HALVES && a.rotary_dims / 2 % kChunk == 0)
+        return launch_mode<DT, kHalves>(a, stream);
+    if (a.rotary_pairs == G4S_ROTARY_NEIGHBOURS && a.rotary_dims % kChunk == 0)
+        return launch_mode<DT, kNeighbours>(a, stream);
+    return launch_mode<DT, kAny>(a, stream);
 }
 
 }  // namespace
 
 hipError_t append_launch(const AppendArgs& a, int32_t dtype, hipStream_t stream)
 {
-    const int B = a.pool.scale_tokens.d;
-    const int tile = B > kTile ? B : kTile / B * B;
-    const int64_t tiles = a.starts ? (int64_t)a.tokens / tile + 2 * (int64_t)a.rows : a.rows;
-    const int slices = 1;
-    const int items = a.k.data ? 2 * a.kv_heads : 0;
-    const size_t lds = (size_t)kStep * (a.rotary_dims / 2) * sizeof(double2) +
-                       (size_t)((tile + B - 1) / B + 1) * ((items + slices - 1) / slices) *
-                           sizeof(uint64_t);
-    const dim3 grid((unsigned)tiles, (unsigned)slices);
-    return dtype == G4S_DTYPE_F32 ? launch(append_kernel<G4S_DTYPE_F32>, grid, kB, lds, stream, a, tile)
-                                  : launch(append_kernel<G4S_DTYPE_BF16>, grid, kB, lds, stream, a, tile);
+    return dtype == G4S_DTYPE_F32 ? by_mode<G4S_DTYPE_F32>(a, stream)
+                                  : by_mode<G4S_DTYPE_BF16>(a, stream);
 }
 
 }  // namespace g4s

@@ -99,7 +99,7 @@ const char* g4s_cache_last_error(const g4s_cache* cache);
  * so is every token of a row whose length is outside the table.
  *   angle(j) = position * d_freqs[j]
  *   (a, b) -> (a cos - b sin, b cos + a sin)     for each pair (a, b) of q and k
- * in 64 bits, rounded once to q_out's type.  Keys and values: with top the
+ * in 64 bits, rounded to q_out's type (to bf16 by way of binary32).  Keys and values: with top the
  * largest finite magnitude that is new in a block of scale_tokens tokens of one head, the
  * scale is the least power of two with top <= 448 * scale, from 2^-100 to
  * 2^119, or the one that the block has if it holds earlier tokens and theirs is
