@@ -67,7 +67,13 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w)
 {
     return (((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) >> 7;
 }
-__device__ __forceinline__ bool has_nan(uint32_t w) { return nan_codes(w) != 0u; }
+/* x, or NaN where the count n (0, 1, ..) is not 0.  (Arithmetic: comparisons for every register
+ * of a tile would each hold a mask.) */
+__device__ __forceinline__ float nan_where(float x, float n)
+{
+    const int32_t some = -(int32_t)__float_as_uint(n) >> 31;
+    return __uint_as_float(__float_as_uint(x) | ((uint32_t)some & 0x7FC00000u));
+}
 /* The word with +0 in the place of NaN codes. */
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~(nan_codes(w) * 0xFFu); }
 
@@ -138,6 +144,47 @@ __device__ __forceinline__ void store4(char* p, f32x4 x)
         w.x = pack_bf16(x[0], x[1]);
         w.y = pack_bf16(x[2], x[3]);
         *reinterpret_cast<uint2*>(p) = w;
+    }
+}
+
+/* 16 bytes at byte `at` of the workspace that another workgroup of this launch reads or wrote:
+ * past the caches that are not common to all (st_dev and ld_dev, four times as wide). */
+constexpr int kDeviceScope = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t shared_space(float* p, uint32_t bytes)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, (int)bytes, 0x00027000);
+}
+__device__ __forceinline__ void st_dev4(__amdgpu_buffer_rsrc_t space, uint32_t at, f32x4 v)
+{
+    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), space, (int)at, 0, kDeviceScope);
+}
+__device__ __forceinline__ f32x4 ld_dev4(__amdgpu_buffer_rsrc_t space, uint32_t at)
+{
+    return __builtin_bit_cast(
+        f32x4, __builtin_amdgcn_raw_buffer_load_b128(space, (int)at, 0, kDeviceScope));
+}
+
+/* The joining of parts of a column, `n` of them at once: their maximum so far, sum and sums. */
+struct Joined {
+    float top = -inf32(), sum = 0.0f;
+    f32x4 v = f32x4{0, 0, 0, 0};
+};
+template <int N>
+__device__ __forceinline__ void join(Joined& j, int n, const float2 (&stats)[N], const f32x4 (&part)[N])
+{
+    float now = j.top;
+#pragma unroll
+    for (int w = 0; w < N; ++w) now = fmaxf(now, w < n ? stats[w].x : now);
+    const float keep = j.top == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(j.top - now);
+    j.sum *= keep;
+    j.v *= keep;
+    j.top = now;
+#pragma unroll
+    for (int w = 0; w < N; ++w) {
+        if (w >= n) break;
+        const float f = stats[w].x == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(stats[w].x - now);
+        j.sum += stats[w].y * f;
+        j.v += part[w] * f;
     }
 }
 

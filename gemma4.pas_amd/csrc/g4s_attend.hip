@@ -2,12 +2,15 @@
  * g4s_attend.hip -- attention over the pages of an 8-bit cache for rows with few queries
  * (the tokens of a decode step), on gfx950.
  *
- * The work of a launch, counted in units of NW x 32 tokens of one row and key
- * head, is shared out evenly over the workgroups, whatever the rows' lengths;
- * every workgroup finds its share from the lengths by itself.  A wave takes 32 tokens of
- * each unit with a softmax of its own; the waves join in LDS, and where
- * several workgroups have parts of one row and head, the one that ends last joins
- * those, in their order, so that results do not depend on who that is.
+ * Neighbouring rows of one token each that begin with the same page (the beams of a search, requests
+ * with one prompt) are taken together, as far as 16 query columns hold them: as long as
+ * their pages are the same a tile of keys and values is read once for all, from the first
+ * page on that differs each row's tiles by themselves.  The work of a launch, counted in units of
+ * NW x 32 tokens of one such group and key head, is shared out evenly over the
+ * workgroups, whatever the lengths; every workgroup finds its share from them by itself.  A wave
+ * takes 32 tokens of each unit with a softmax of its own; the waves join in LDS, and where several
+ * workgroups have parts of one group and head, the one that ends last joins those, in their
+ * order, so that results do not depend on who that is.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -16,52 +19,108 @@ namespace g4s {
 
 namespace {
 
-constexpr int kTile = 32; /* tokens of a wave's step */
 constexpr int kB = 256;
-constexpr int kCols = 16; /* query columns of a workgroup's part */
+constexpr int kTile = 32;  /* tokens of a wave's step go by 32 */
+constexpr int kCols = 16;  /* query columns of a workgroup's part */
 constexpr int kPass = 128; /* dims that the waves join at once */
+constexpr int kUnits = 2;  /* units of a workgroup at least, where there are few */
+/* Bytes of parts that their last workgroup joins by itself: more are left to a launch of
+ * their own. */
+constexpr int kJoinBytes = 96 << 10;
 
-/* What a row asks for. */
-struct Work {
-    int start, count, length, bad; /* RowTokens */
-    int cols, blocks;              /* query columns (tokens x heads of a key head), 16 of them a block */
-    int from, first;               /* first place that any query sees, and its unit */
-    int units;                     /* of each key head and block: one at least, for the output */
+/* What the scan keeps of a row: its length (bad: -1), and the first page of one that may be taken
+ * together with others (-1: none). */
+struct RowInfo {
+    int length, key;
 };
-template <int UNIT>
-__device__ __forceinline__ Work row_work(const AttendArgs& a, int row)
+
+/* The rows of one part, and what they ask for of each key head. */
+struct Group {
+    int row, rows;    /* rows > 1: of one token each */
+    int start, count; /* of a single row */
+    int cols, blocks; /* query columns (tokens x heads of a key head), 16 of them a block */
+    int from, end;    /* places that any query sees */
+    int first, units; /* units of them: one at least, for the output */
+};
+
+__device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
 {
-    const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    Work w{r.start, r.count, r.length, r.bad, 0, 0, 0, 0, 0};
-    w.cols = r.count * a.group.d;
-    if (is_prompt(r.count, a.group.d)) return w;
-    w.blocks = (w.cols + kCols - 1) / kCols;
-    const int64_t from = a.window > 0 ? (int64_t)r.length - r.count + 1 - a.window : 0;
-    w.from = from > 0 ? (int)from : 0;
-    w.first = w.from / UNIT;
-    w.units = r.length > w.from ? (int)(((int64_t)r.length + UNIT - 1) / UNIT) - w.first : 1;
-    return w;
+    const int64_t f = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
+    return f > 0 ? (int)f : 0;
 }
 
-/* Work of the rows before each row, in units, into before[0 .. rows]. */
-template <int NW>
-__device__ __forceinline__ void scan_work(const AttendArgs& a, int64_t* before, int64_t* s_wave)
+/* Rows that are taken together at most: a power of two, of rows that begin at a multiple of it. */
+__device__ __forceinline__ int group_rows(const AttendArgs& a)
+{
+    const int n = kCols / a.group.d;
+    return n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+}
+
+template <int UNIT>
+__device__ __forceinline__ Group find_group(const AttendArgs& a, const RowInfo* info, int row)
+{
+    Group p{row, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    const int key = info[row].key, most = group_rows(a), in = row & (most - 1);
+    /* taken by a row before it */
+    if (key >= 0 && in > 0 && info[row - 1].key == key) return p;
+    p.rows = 1;
+    int from = 0, end = 0;
+    if (key >= 0) {
+        end = info[row].length;
+        from = sees_from(a, end - 1);
+        for (int i = 1; in + i < most && row + i < a.rows && info[row + i].key == key; ++i) {
+            const int n = info[row + i].length, f = sees_from(a, n - 1);
+            end = n > end ? n : end;
+            from = f < from ? f : from;
+            ++p.rows;
+        }
+    }
+    const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
+    p.start = r.start;
+    p.count = r.count;
+    if (key < 0) {
+        end = r.length;
+        from = sees_from(a, r.length - r.count);
+    }
+    p.cols = p.rows > 1 ? p.rows * a.group.d : is_prompt(r.count, a.group.d) ? 0 : r.count * a.group.d;
+    p.blocks = (p.cols + kCols - 1) / kCols;
+    p.from = from;
+    p.end = end;
+    p.first = from / UNIT;
+    p.units = end > from ? (int)(((int64_t)end + UNIT - 1) / UNIT) - p.first : 1;
+    return p;
+}
+
+/* info[0 .. rows - 1], and the work of the groups before each row, in units, in before[0 .. rows]. */
+template <int NW, int UNIT>
+__device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, int64_t* before,
+                                          int64_t* s_wave)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int each = (a.rows + NW * 64 - 1) / (NW * 64);
+    const int64_t room = cache_room(a.pool);
+    for (int r = tid; r < a.rows; r += NW * 64) {
+        const int page = a.table[(int64_t)r * a.pool.max_slots];
+        const RowTokens t = row_tokens(a.starts, a.lengths, r, a.tokens, room);
+        RowInfo i{t.bad ? -1 : t.length, -1};
+        if (t.count == 1 && t.length > 0 && page >= 0 && page < a.pool.n_pages) i.key = page;
+        info[r] = i;
+    }
+    __syncthreads();
     int64_t sum = 0;
     for (int i = 0; i < each; ++i) {
         const int r = tid * each + i;
         if (r >= a.rows) break;
-        const Work w = row_work<NW * kTile>(a, r);
-        before[r + 1] = (int64_t)w.units * w.blocks * a.kv_heads;
+        const Group p = find_group<UNIT>(a, info, r);
+        before[r + 1] = (int64_t)p.units * p.blocks * a.kv_heads;
         sum += before[r + 1];
     }
     int64_t x = sum;
-    for (int d = 1; d < 64; d <<= 1) {
-        const int64_t y = __shfl_up((long long)x, d);
-        if (lane >= d) x += y;
-    }
+    if (a.rows > 1)
+        for (int d = 1; d < 64 && d < a.rows; d <<= 1) {
+            const int64_t y = __shfl_up((long long)x, d);
+            if (lane >= d) x += y;
+        }
     if (lane == 63) s_wave[wave] = x;
     __syncthreads();
     x -= sum;
@@ -76,21 +135,16 @@ __device__ __forceinline__ void scan_work(const AttendArgs& a, int64_t* before, 
     __syncthreads();
 }
 
-/* A part of one row's tokens for one key head and 16 query columns. */
-struct Part {
-    int row, head, col0;
-    Work w;
-};
-
-template <int DT, int D, int NW>
+template <int DT, int D, int NW, int TT>
 struct Shared {
     Frag q[D / 64][2][DT == G4S_DTYPE_F32 ? 3 : 1][64]; /* the queries, as lanes take them */
-    int64_t offset[NW][kTile];
-    float scale[NW][2][kTile];
+    int64_t offset[NW][2][TT];
+    float scale[NW][2][2][TT];
     float m[NW][kCols], l[NW][kCols];
     float top[kCols], sum[kCols];
     float o[NW][kCols][kPass + 4];
     int64_t wave[NW];
+    int differs; /* the first slot whose page is not the same for all rows */
     int flag;
 };
 
@@ -104,80 +158,122 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[VW])
         const u32x2_4 x = *reinterpret_cast<const u32x2_4*>(p);
         w[0] = x[0], w[1] = x[1];
     } else {
+        const u32x4_4 x = *reinterpret_cast<const u32x4_4*>(p);
 #pragma unroll
-        for (int i = 0; i < VW; i += 4) {
-            const u32x4_4 x = *reinterpret_cast<const u32x4_4*>(p + 4 * i);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[i + k] = x[k];
-        }
+        for (int k = 0; k < 4; ++k) w[k] = x[k];
     }
 }
 
-template <int DT, int D, int NW>
-__global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
+/* Column k of a part: its token, head and place. */
+struct Column {
+    int token, head, place;
+};
+__device__ __forceinline__ Column column(const AttendArgs& a, const RowInfo* info, const Group& p,
+                                         int head, int k)
 {
-    constexpr int UNIT = NW * kTile;
+    const int nth = divide(k, a.group);
+    Column c;
+    c.head = head * a.group.d + k - nth * a.group.d;
+    if (p.rows > 1) {
+        c.token = a.starts ? a.starts[p.row + nth] : p.row + nth;
+        c.place = info[p.row + nth].length - 1;
+    } else {
+        c.token = p.start + nth;
+        c.place = (info[p.row].length < 0 ? 0 : info[p.row].length) - p.count + nth;
+    }
+    return c;
+}
+
+/* (a column that sees nothing has no maximum and no sum) */
+template <int DT>
+__device__ __forceinline__ void put(const AttendArgs& a, int token, int head, int dim, f32x4 v, float top,
+                                    float sum)
+{
+    const bool none = top == -inf32() && sum == 0.0f;
+    v = none ? f32x4{0, 0, 0, 0} : v * (1.0f / sum);
+    if (dim < a.pool.head_dim)
+        store4<DT>(a.out.data + ((int64_t)token * a.out.token_stride +
+                                 (int64_t)head * a.out.head_stride + dim) * Elem<DT>::SIZE, v);
+    if (dim == 0 && a.lse)
+        a.lse[(int64_t)token * a.heads + head] =
+            none ? -inf32() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+}
+
+/* How a kernel is made for a width of heads: tokens of a wave's step, a multiple of kTile as
+ * registers allow, and waves. */
+template <int DT, int D>
+struct Shape {
+    static constexpr int TT = D <= 128 ? 2 * kTile : kTile;
+    static constexpr int NW = D == 512 || (D == 256 && DT == G4S_DTYPE_F32) ? 4 : 8;
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel(AttendArgs a, int joins)
+{
+    constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT;
+    constexpr int UNIT = NW * TT;
+    constexpr int NB = TT / 16, NH = TT / kTile;    /* of 16 and of 32 tokens */
     constexpr int QP = DT == G4S_DTYPE_F32 ? 3 : 1; /* pieces of a query */
     constexpr int PP = DT == G4S_DTYPE_F32 ? 2 : 1; /* and of a weight */
     constexpr int KC = D / 64;                      /* 16-dim chunks of a lane of K and Q */
     constexpr int VW = D / 64;                      /* words of a lane of V */
+    constexpr int VL = VW < 4 ? VW : 4;             /* of one load */
     constexpr int DB = D / 16;                      /* blocks of 16 dims, and dims of a lane */
     static_assert(2 * kCols * D <= kAttendSums && 4 * kCols <= kAttendStats, "two slots a workgroup");
     extern __shared__ char lds[];
-    auto& s = *reinterpret_cast<Shared<DT, D, NW>*>(lds);
-    int64_t* before = reinterpret_cast<int64_t*>(lds + ((sizeof(s) + 15) & ~(size_t)15));
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    using S = Shared<DT, D, NW, TT>;
+    S& s = *reinterpret_cast<S*>(lds);
+    int64_t* before = reinterpret_cast<int64_t*>(lds + ((sizeof(S) + 15) & ~(size_t)15));
+    RowInfo* info = reinterpret_cast<RowInfo*>(before + a.rows + 1);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
-    scan_work<NW>(a, before, s.wave);
+    if (joins && tid == 0) a.ws.records[blockIdx.x].parts = 0;
+    scan_rows<NW, UNIT>(a, info, before, s.wave);
     const int64_t total = before[a.rows];
-    const int groups = total < gridDim.x ? (int)total : (int)gridDim.x;
+    const int64_t least = (total + kUnits - 1) / kUnits;
+    const int groups = least < gridDim.x ? (int)least : (int)gridDim.x;
     if ((int)blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
     const int64_t x_end = first_unit(total, blockIdx.x + 1, groups);
     /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
     const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
+    const __amdgpu_buffer_rsrc_t space = shared_space(a.ws.sums, (uint32_t)a.ws.groups * kAttendSums * 4);
 
     while (x < x_end) {
-        Part p;
-        {
-            int lo = 0, hi = a.rows - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (before[mid] <= x)
-                    lo = mid;
-                else
-                    hi = mid - 1;
-            }
-            p.row = lo;
+        /* the last row whose units begin at or before x: each lane looks at one of 64 stretches */
+        int lo = 0;
+        for (int n = a.rows; n > 1;) {
+            const int each = (n + 63) / 64;
+            const uint64_t at = __ballot(lane * each < n && before[lane * each < n ? lo + lane * each : 0] <= x);
+            const int last = 63 - __clzll(at | 1);
+            lo += last * each;
+            n = n - last * each < each ? n - last * each : each;
         }
-        p.w = row_work<UNIT>(a, p.row);
-        const int64_t in_row = x - before[p.row];
-        const int item = (int)(in_row / p.w.units);
-        const int u0 = (int)(in_row - (int64_t)item * p.w.units);
-        const int64_t left = x_end - x;
-        const int u1 = p.w.units - u0 < left ? p.w.units : u0 + (int)left;
-        p.head = item / p.w.blocks;
-        p.col0 = (item - p.head * p.w.blocks) * kCols;
+        lo = __builtin_amdgcn_readfirstlane(lo);
+        const Group p = find_group<UNIT>(a, info, lo);
+        const int64_t in_group = x - before[lo];
+        const int item = (int)quotient(in_group, p.units);
+        const int u0 = (int)(in_group - (int64_t)item * p.units);
+        const int u1 = p.units - u0 < x_end - x ? p.units : u0 + (int)(x_end - x);
+        const int head = p.blocks == 1 ? item : item / p.blocks;
+        const int col0 = (item - head * p.blocks) * kCols;
         const int64_t item_first = x - u0; /* its first unit among all */
         x += u1 - u0;
 
         /* this lane's query column */
-        const int col = p.col0 + m;
-        const int cols = p.w.cols - p.col0 < kCols ? p.w.cols - p.col0 : kCols;
+        const int cols = p.cols - col0 < kCols ? p.cols - col0 : kCols;
         const bool has_col = m < cols;
-        const int nth = has_col ? divide(col, a.group) : 0;
-        const int qhead = p.head * a.group.d + (has_col ? col - nth * a.group.d : 0);
-        const int place = p.w.length - p.w.count + nth; /* sees from .. place */
-        const int64_t from64 = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
-        const int from = from64 > 0 ? (int)from64 : 0;
+        const Column at = column(a, info, p, head, col0 + (has_col ? m : 0));
+        const int place = at.place, from = sees_from(a, place);
+        const int member = p.rows > 1 ? divide(has_col ? m : 0, a.group) : 0;
         {
-            const char* at = a.q.data + ((p.w.start + nth) * a.q.token_stride +
-                                         qhead * a.q.head_stride) * Elem<DT>::SIZE;
+            const char* q = a.q.data + ((int64_t)at.token * a.q.token_stride +
+                                        (int64_t)at.head * a.q.head_stride) * Elem<DT>::SIZE;
             for (int k = wave; k < KC; k += NW) {
                 const int d0 = k * 64 + g * 16;
                 Frag f[2][QP];
                 const bool in = d0 < a.pool.head_dim;
-                const char* q0 = at + (int64_t)(in ? d0 : 0) * Elem<DT>::SIZE;
+                const char* q0 = q + (int64_t)(in ? d0 : 0) * Elem<DT>::SIZE;
                 load_query<DT>(q0, has_col && in, a.scale < 0.0f, f[0]);
                 load_query<DT>(q0 + 8 * Elem<DT>::SIZE, has_col && in, a.scale < 0.0f, f[1]);
 #pragma unroll
@@ -186,74 +282,192 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
                     s.q[k][1][b][lane] = f[1][b];
                 }
             }
-            __syncthreads();
         }
+        /* places that all queries see */
+        int all_from = from, all_to = place;
+        if (p.rows > 1 || p.count > 1)
+            for (int d = 1; d < kCols; d <<= 1) {
+                const int f = __shfl_xor(all_from, d), t = __shfl_xor(all_to, d);
+                all_from = f > all_from ? f : all_from;
+                all_to = t < all_to ? t : all_to;
+            }
+        all_from = __builtin_amdgcn_readfirstlane(all_from);
+        all_to = __builtin_amdgcn_readfirstlane(all_to);
+        const bool multi = p.rows > 1 || p.count > 1;
+        /* the part's tiles: the first `shared` of them with the same pages for all rows */
+        const int t0 = (p.first + u0) * UNIT > p.from ? (p.first + u0) * UNIT : p.from;
+        const int t1 = (int64_t)(p.first + u1) * UNIT < p.end ? (p.first + u1) * UNIT : p.end;
+        const int a0 = t0 / TT, a1 = t1 > t0 ? (t1 + TT - 1) / TT : a0;
+        int a_shared = a1;
+        int ref = p.row; /* the longest row, whose table has every place */
+        if (p.rows > 1) {
+            for (int i = 1; i < p.rows; ++i)
+                if (info[p.row + i].length > info[ref].length) ref = p.row + i;
+            ref = __builtin_amdgcn_readfirstlane(ref);
+            if (tid == 0) s.differs = p.end;
+            __syncthreads();
+            const int s0 = divide(t0, a.pool.page_tokens), s1 = divide(t1 - 1, a.pool.page_tokens);
+            for (int i = tid; i < (s1 - s0 + 1) * p.rows; i += NW * 64) {
+                const int slot = s0 + i / p.rows, row = p.row + i % p.rows;
+                const int last = info[row].length - 1;
+                if (slot < divide(sees_from(a, last), a.pool.page_tokens) ||
+                    slot > divide(last, a.pool.page_tokens))
+                    continue;
+                if (a.table[(int64_t)row * a.pool.max_slots + slot] !=
+                    a.table[(int64_t)ref * a.pool.max_slots + slot])
+                    atomicMin(&s.differs, slot);
+            }
+        }
+        __syncthreads();
+        if (p.rows > 1) {
+            const int64_t t = (int64_t)s.differs * a.pool.page_tokens.d;
+            const int n = t < p.end ? (int)t / TT : a1;
+            a_shared = __builtin_amdgcn_readfirstlane(n < a0 ? a0 : n < a1 ? n : a1);
+        }
+
         f32x4 o[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
         float top = -inf32(), sum = 0.0f;
 
-        const int last_place = p.w.length - 1;
-        const int full_from = p.w.count > 1 && a.window > 0
-                                  ? (p.w.length - a.window > 0 ? p.w.length - a.window : 0)
-                                  : p.w.from;                  /* all queries see from here .. */
-        const int full_to = p.w.length - p.w.count;            /* .. to here */
-        const int32_t* pages = a.table + (int64_t)p.row * a.pool.max_slots;
-        const int end = p.w.length > p.w.from ? p.w.length : 0;
-        for (int u = u0; u < u1; ++u) {
-            const int t0 = (p.w.first + u) * UNIT + wave * kTile;
-            if (t0 >= end || t0 + kTile <= p.w.from) continue;
-            /* a token a lane, keys' and values' scales by halves; beyond the ends the one at
-             * the end stands in, which some query sees */
-            int t = t0 + (lane & 31);
-            t = t < p.w.from ? p.w.from : t > last_place ? last_place : t;
-            const int slot = divide(t, a.pool.page_tokens);
-            const int in = t - slot * a.pool.page_tokens.d;
-            int page = pages[slot];
+        /* steps, every NW-th of them the wave's: a tile for all rows (row -1), behind those a tile
+         * for each row that sees it */
+        struct Step {
+            int tile, row, first, last; /* first and last place that is read */
+        };
+        auto settle = [&](Step& t) {
+            if (t.row < 0) {
+                if (t.tile < a_shared) {
+                    t.first = p.from;
+                    t.last = p.end - 1;
+                    return;
+                }
+                t.row = t.tile - a_shared;
+                t.tile = a_shared;
+            }
+            for (;; t.row += NW) {
+                while (t.row >= p.rows && t.tile < a1) {
+                    t.row -= p.rows;
+                    ++t.tile;
+                }
+                if (t.tile >= a1) return;
+                t.last = __builtin_amdgcn_readfirstlane(info[p.row + t.row].length - 1);
+                t.first = sees_from(a, t.last);
+                if (t.tile * TT <= t.last && t.tile * TT + TT > t.first) return;
+            }
+        };
+        auto advance = [&](Step t) {
+            if (t.row < 0)
+                t.tile += NW;
+            else
+                t.row += NW;
+            settle(t);
+            return t;
+        };
+        /* the lane's token of a step: beyond the ends the one at the end stands in, which some
+         * query sees */
+        auto token = [&](const Step& t) {
+            const int i = t.tile * TT + (lane & (TT - 1));
+            return i < t.first ? t.first : i > t.last ? t.last : i;
+        };
+        auto find_page = [&](const Step& t) {
+            const int row = t.row >= 0 ? p.row + t.row : ref;
+            return a.table[(int64_t)row * a.pool.max_slots + divide(token(t), a.pool.page_tokens)];
+        };
+        const char* const keys = a.k_plane + (int64_t)head * a.pool.part_bytes;
+        const char* const values = a.v_plane + (int64_t)head * a.pool.part_bytes;
+        /* where its tokens are, a token a lane, and the keys' and values' scales (by halves of the
+         * lanes where there are 32) */
+        struct Scales {
+            float k, v;
+        };
+        auto locate = [&](const Step& t, int page, int b, Scales& scale) {
+            const int i = token(t);
+            const int in = i - divide(i, a.pool.page_tokens) * a.pool.page_tokens.d;
             const bool ok = page >= 0 && page < a.pool.n_pages;
-            if (!ok) page = 0;
-            const uint32_t bad = (uint32_t)__ballot(!ok);
-            const int64_t off = cache_offset(a.pool, page, in, p.head);
+            const int64_t off = (int64_t)(ok ? page : 0) * a.pool.page_stride + in * a.pool.token_bytes;
             const int in_block = in - divide(in, a.pool.scale_tokens) * a.pool.scale_tokens.d;
-            const float scale = *reinterpret_cast<const float*>(
-                (lane < 32 ? a.k_plane : a.v_plane) + off - (int64_t)in_block * a.pool.token_bytes +
-                a.pool.head_dim);
-            if (lane < 32) s.offset[wave][lane] = off;
-            s.scale[wave][lane >> 5][lane & 31] = scale;
-            wave_fence();
-
-            uint32_t kw[2][KC][4];
+            const int64_t at = off - in_block * a.pool.token_bytes + a.pool.head_dim;
+            if (TT == 64 || lane < 32) s.offset[wave][b][lane & (TT - 1)] = off;
+            if constexpr (TT == 64) {
+                scale.k = *reinterpret_cast<const float*>(keys + at);
+                scale.v = *reinterpret_cast<const float*>(values + at);
+            } else {
+                scale.k = *reinterpret_cast<const float*>((lane < 32 ? keys : values) + at);
+            }
+            return (uint64_t)__ballot(!ok);
+        };
+        auto keep_scales = [&](int b, const Scales& scale) {
+            if constexpr (TT == 64) {
+                s.scale[wave][b][0][lane] = scale.k;
+                s.scale[wave][b][1][lane] = scale.v;
+            } else {
+                s.scale[wave][b][lane >> 5][lane & 31] = scale.k;
+            }
+        };
+        /* (dims behind head_dim, whose queries are 0 and whose sums are not kept, are read in
+         * the last ones' place) */
+        const int last_key = a.pool.head_dim - 16, last_value = a.pool.head_dim - 4 * VL;
+        uint32_t kw[NB][KC][4], vw[NH][8][VW];
+        auto load_keys = [&](int b) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const char* at = a.k_plane + s.offset[wave][h * 16 + m];
+            for (int h = 0; h < NB; ++h) {
+                const char* from = keys + s.offset[wave][b][h * 16 + m];
 #pragma unroll
                 for (int k = 0; k < KC; ++k) {
                     const int d0 = k * 64 + g * 16;
-                    load_words<4>(at + (d0 < a.pool.head_dim ? d0 : 0), kw[h][k]);
+                    load_words<4>(from + (d0 < last_key ? d0 : last_key), kw[h][k]);
                 }
             }
-            uint32_t vw[8][VW];
-            const int vd = m * DB;
+        };
+        auto load_values = [&](int b) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const char* at = a.v_plane + s.offset[wave][(j & 4) * 4 + g * 4 + (j & 3)];
-                if constexpr (VW <= 4) {
-                    load_words<VW>(at + (vd < a.pool.head_dim ? vd : 0), vw[j]);
-                } else {
-                    uint32_t w4[4];
+            for (int h = 0; h < NH; ++h)
 #pragma unroll
-                    for (int i = 0; i < VW; i += 4) {
-                        load_words<4>(at + (vd + 4 * i < a.pool.head_dim ? vd + 4 * i : 0), w4);
+                for (int j = 0; j < 8; ++j) {
+                    const char* from = values + s.offset[wave][b][h * 32 + (j & 4) * 4 + g * 4 + (j & 3)];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) vw[j][i + k] = w4[k];
+                    for (int i = 0; i < VW; i += VL) {
+                        const int d0 = m * DB + 4 * i;
+                        uint32_t w[VL];
+                        load_words<VL>(from + (d0 < last_value ? d0 : last_value), w);
+#pragma unroll
+                        for (int k = 0; k < VL; ++k) vw[h][j][i + k] = w[k];
                     }
                 }
+        };
+
+        Step now{a0 + wave, -1, 0, 0};
+        settle(now);
+        Step next = now;
+        int buf = 0, page = 0;
+        uint64_t bad = 0;
+        if (now.tile < a1) {
+            Scales scale;
+            bad = locate(now, find_page(now), 0, scale);
+            keep_scales(0, scale);
+            wave_fence();
+            load_keys(0);
+            load_values(0);
+            next = advance(now);
+            if (next.tile < a1) page = find_page(next);
+        }
+        while (now.tile < a1) {
+            const bool more = next.tile < a1;
+            const uint64_t bad_now = bad;
+            Scales scale{0.0f, 0.0f};
+            Step after = next;
+            if (more) {
+                bad = locate(next, page, buf ^ 1, scale);
+                wave_fence();
+                after = advance(next);
+                if (after.tile < a1) page = find_page(after);
             }
 
-            f32x4 sc[2];
+            f32x4 sc[NB];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const float ks = s.scale[wave][0][h * 16 + m];
+            for (int h = 0; h < NB; ++h) {
+                const float ks = s.scale[wave][buf][0][h * 16 + m];
                 sc[h] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < KC; ++k) {
@@ -270,102 +484,125 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
                     }
                 }
             }
-            float y[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) y[j] = sc[j >> 2][j & 3];
-            const bool partly = bad != 0 || t0 < full_from || t0 + kTile - 1 > full_to;
+            if (more) load_keys(buf ^ 1);
+            /* y[j] of half h: token h * 32 + (j & 4) * 4 + g * 4 + (j & 3) */
+            const int tile0 = now.tile * TT;
+            const bool alone = now.row >= 0;
+            const bool partly = bad_now != 0 || tile0 < all_from || tile0 + TT - 1 > all_to || alone;
             bool nan_v = false;
             if (partly) {
+                const bool mine = !alone || member == now.row;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int i = (j & 4) * 4 + g * 4 + (j & 3);
-                    const int at = t0 + i;
-                    if (bad >> i & 1) y[j] = nan32();
-                    if (at < from || at > place) y[j] = -inf32();
-                }
-                if (p.w.count > 1) {
-                    bool any = false;
+                for (int h = 0; h < NB; ++h)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = h * 16 + g * 4 + j, t = tile0 + i;
+                        if (bad_now >> i & 1) sc[h][j] = nan32();
+                        if (t < from || t > place || !mine) sc[h][j] = -inf32();
+                    }
+                if (multi) {
+                    uint32_t any = 0;
 #pragma unroll
-                        for (int w = 0; w < VW; ++w) any = any || has_nan(vw[j][w]);
-                    nan_v = __any(any);
+                    for (int h = 0; h < NH; ++h)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int w = 0; w < VW; ++w) any |= nan_codes(vw[h][j][w]);
+                    nan_v = __any(any != 0);
                 }
             }
-            float now = y[0];
+            float best = sc[0][0];
 #pragma unroll
-            for (int j = 1; j < 8; ++j) now = fmaxf(now, y[j]);
-            now = fmaxf(now, __shfl_xor(now, 16));
-            now = fmaxf(now, __shfl_xor(now, 32));
-            now = fmaxf(now, top);
-            if (__any(now > top)) {
-                const float keep = now > top ? __builtin_amdgcn_exp2f((top - now) * c) : 1.0f;
+            for (int h = 0; h < NB; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) best = fmaxf(best, sc[h][j]);
+            best = fmaxf(best, __shfl_xor(best, 16));
+            best = fmaxf(best, __shfl_xor(best, 32));
+            best = fmaxf(best, top);
+            if (__any(best > top)) {
+                const float keep = best > top ? __builtin_amdgcn_exp2f((top - best) * c) : 1.0f;
                 sum *= keep;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[i] *= keep;
-                top = now;
+                top = best;
             }
             const float base = top == -inf32() ? 0.0f : top * c;
-            Frag pw[PP];
+            Frag pw[NH][PP];
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j], c, -base));
-                const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(y[j + 1], c, -base));
-                sum += e0 + e1;
-                pw[0].w[j >> 1] = pack_bf16(e0, e1);
-                if constexpr (PP == 2) {
-                    const float r0 = e0 - __uint_as_float(pw[0].w[j >> 1] << 16);
-                    const float r1 = e1 - __uint_as_float(pw[0].w[j >> 1] & 0xFFFF0000u);
-                    pw[1].w[j >> 1] = pack_bf16(r0, r1);
+            for (int h = 0; h < NB; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; j += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j], c, -base));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j + 1], c, -base));
+                    sum += e0 + e1;
+                    Frag* f = pw[h >> 1];
+                    const int w = (h & 1) * 2 + (j >> 1);
+                    f[0].w[w] = pack_bf16(e0, e1);
+                    if constexpr (PP == 2)
+                        f[1].w[w] = pack_bf16(e0 - __uint_as_float(f[0].w[w] << 16),
+                                              e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
                 }
-            }
-            float vs[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) vs[j] = s.scale[wave][1][(j & 4) * 4 + g * 4 + (j & 3)];
-            if (nan_v) {
-                /* a NaN that some queries see and others do not (0 times NaN is NaN): the products
-                 * go without it, and whoever sees one, counted by a product too, gets NaN */
-                Frag see;
+            for (int h = 0; h < NH; ++h) {
+                float vs[8];
 #pragma unroll
-                for (int j = 0; j < 8; j += 2)
-                    see.w[j >> 1] = (y[j] == -inf32() ? 0u : 0x3F80u) |
-                                    (y[j + 1] == -inf32() ? 0u : 0x3F800000u);
-                const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+                for (int j = 0; j < 8; ++j)
+                    vs[j] = s.scale[wave][buf][1][h * 32 + (j & 4) * 4 + g * 4 + (j & 3)];
+                if (nan_v) {
+                    /* a NaN that some queries see and others do not (0 times NaN is NaN): the
+                     * products go without it, and whoever sees one, counted by a product too,
+                     * gets NaN */
+                    Frag see;
+#pragma unroll
+                    for (int j = 0; j < 8; j += 2) {
+                        const f32x4 y = sc[h * 2 + (j >> 2)];
+                        see.w[j >> 1] = (y[j & 3] == -inf32() ? 0u : 0x3F80u) |
+                                        (y[(j & 3) + 1] == -inf32() ? 0u : 0x3F800000u);
+                    }
+                    const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) {
+                        uint32_t is[8];
+                        Frag f[4];
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            is[j] = nan_codes(vw[h][j][w]) * 0x38u; /* the code of 1 */
+                            vw[h][j][w] = without_nan(vw[h][j][w]);
+                        }
+                        value_frags(is, one, f);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                f[i].v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r)
+                                o[w * 4 + i][r] = nan_where(o[w * 4 + i][r], n[r]);
+                        }
+                    }
+                }
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
-                    uint32_t at[8];
+                    uint32_t word[8];
                     Frag f[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        at[j] = nan_codes(vw[j][w]) * 0x38u; /* the code of 1 */
-                        vw[j][w] = without_nan(vw[j][w]);
-                    }
-                    value_frags(at, one, f);
+                    for (int j = 0; j < 8; ++j) word[j] = vw[h][j][w];
+                    value_frags(word, vs, f);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            f[i].v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
+                    for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (n[r] > 0.0f) o[w * 4 + i][r] = nan32();
-                    }
+                        for (int b = PP - 1; b >= 0; --b)
+                            o[w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                                f[i].v, pw[h][b].v, o[w * 4 + i], 0, 0, 0);
                 }
             }
-#pragma unroll
-            for (int w = 0; w < VW; ++w) {
-                uint32_t at[8];
-                Frag f[4];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) at[j] = vw[j][w];
-                value_frags(at, vs, f);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int b = PP - 1; b >= 0; --b)
-                        o[w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                            f[i].v, pw[b].v, o[w * 4 + i], 0, 0, 0);
+            if (more) {
+                load_values(buf ^ 1);
+                keep_scales(buf ^ 1, scale);
             }
-            wave_fence(); /* the next tile's offsets and scales take the place of these */
+            wave_fence(); /* before what comes after the next tile takes the place of this one */
+            buf ^= 1;
+            now = next;
+            next = after;
         }
 
         /* the waves join */
@@ -385,13 +622,12 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
                 all += s.l[w][tid] * f;
                 s.l[w][tid] = f;
             }
-            s.top[tid] = best;
-            s.sum[tid] = all;
+            const bool bad_row = p.rows == 1 && info[p.row].length < 0;
+            s.top[tid] = bad_row ? nan32() : best;
+            s.sum[tid] = bad_row ? nan32() : all;
         }
-        const bool whole = u0 == 0 && u1 == p.w.units;
-        const int w_first = whole ? 0 : unit_group(item_first, total, groups);
-        const int w_last = whole ? 0 : unit_group(item_first + p.w.units - 1, total, groups);
-        const int64_t slot = 2 * (int64_t)blockIdx.x + (u0 == 0);
+        const bool whole = u0 == 0 && u1 == p.units;
+        const int slot = 2 * (int)blockIdx.x + (u0 == 0);
         for (int pass = 0; pass < (D + kPass - 1) / kPass; ++pass) {
             /* lanes with dims of this pass */
 #pragma unroll
@@ -412,92 +648,110 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_rows_kernel(AttendArgs a)
 #pragma unroll
                 for (int w = 0; w < NW; ++w)
                     v += *reinterpret_cast<const f32x4*>(&s.o[w][k][d0]) * s.l[w][k];
-                if (!whole) {
-                    uint64_t* to = reinterpret_cast<uint64_t*>(a.ws.sums + (slot * kCols + k) * D + dim);
-                    st_dev(to, (uint64_t)__float_as_uint(v[0]) | (uint64_t)__float_as_uint(v[1]) << 32);
-                    st_dev(to + 1, (uint64_t)__float_as_uint(v[2]) | (uint64_t)__float_as_uint(v[3]) << 32);
-                } else if (dim < a.pool.head_dim) {
-                    const int cc = p.col0 + k, n = divide(cc, a.group), qh = p.head * a.group.d + cc - n * a.group.d;
-                    const bool empty = p.w.length - p.w.count + n < 0 && !p.w.bad;
-                    const float inv = p.w.bad ? nan32() : empty ? 0.0f : 1.0f / s.sum[k];
-                    v = empty ? f32x4{0, 0, 0, 0} : v * inv;
-                    store4<DT>(a.out.data + ((p.w.start + n) * a.out.token_stride +
-                                             qh * a.out.head_stride + dim) * Elem<DT>::SIZE, v);
+                if (whole) {
+                    const Column to = column(a, info, p, head, col0 + k);
+                    put<DT>(a, to.token, to.head, dim, v, s.top[k], s.sum[k]);
+                } else {
+                    st_dev4(space, (uint32_t)((slot * kCols + k) * D + dim) * 4, v);
                 }
             }
-            if (pass == 0 && tid < cols) {
-                if (!whole) {
-                    st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot * kCols + tid) * 2),
-                           (uint64_t)__float_as_uint(s.top[tid]) | (uint64_t)__float_as_uint(s.sum[tid]) << 32);
-                } else if (a.lse) {
-                    const int cc = p.col0 + tid, n = divide(cc, a.group), qh = p.head * a.group.d + cc - n * a.group.d;
-                    const bool empty = p.w.length - p.w.count + n < 0 && !p.w.bad;
-                    a.lse[(int64_t)(p.w.start + n) * a.heads + qh] =
-                        p.w.bad ? nan32() : empty ? -inf32()
-                                : (s.top[tid] + __builtin_amdgcn_logf(s.sum[tid])) * kLn2;
-                }
-            }
+            if (pass == 0 && tid < cols && !whole)
+                st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot * kCols + tid) * 2),
+                       (uint64_t)__float_as_uint(s.top[tid]) | (uint64_t)__float_as_uint(s.sum[tid]) << 32);
             __syncthreads();
         }
         if (whole) continue;
+        const int w_first = unit_group(item_first, total, groups);
+        const int parts = unit_group(item_first + p.units - 1, total, groups) - w_first + 1;
+        if (joins && parts * cols * D * 4 > kJoinBytes) {
+            if (tid == 0 && u0 == 0)
+                a.ws.records[blockIdx.x] = AttendRecord{parts, cols, col0, head * a.group.d, p.row,
+                                                        p.rows > 1 ? -1 : p.start};
+            continue;
+        }
         /* the last of the workgroups that have a part of this item joins them */
-        const int parts = w_last - w_first + 1;
         if (!elect_last(&a.ws.tickets[w_first], (uint32_t)parts, &s.flag)) continue;
-        auto part_slot = [&](int i) { return 2 * (int64_t)(w_first + i) + (i == 0); };
         for (int i = tid; i < cols * (D / 4); i += NW * 64) {
             const int k = i / (D / 4), dim = i % (D / 4) * 4;
             if (dim >= a.pool.head_dim) continue;
-            float best = -inf32();
-            for (int w = 0; w < parts; ++w)
-                best = fmaxf(best, __uint_as_float((uint32_t)ld_dev(
-                    reinterpret_cast<const uint64_t*>(a.ws.stats + (part_slot(w) * kCols + k) * 2))));
-            float all = 0.0f;
-            f32x4 v = f32x4{0, 0, 0, 0};
-            for (int w = 0; w < parts; ++w) {
-                const uint64_t st = ld_dev(
-                    reinterpret_cast<const uint64_t*>(a.ws.stats + (part_slot(w) * kCols + k) * 2));
-                const uint64_t* at = reinterpret_cast<const uint64_t*>(
-                    a.ws.sums + (part_slot(w) * kCols + k) * D + dim);
-                const uint64_t v0 = ld_dev(at), v1 = ld_dev(at + 1);
-                const float tw = __uint_as_float((uint32_t)st), lw = __uint_as_float((uint32_t)(st >> 32));
-                const float f = tw == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(tw - best);
-                all += lw * f;
-                v += f32x4{__uint_as_float((uint32_t)v0), __uint_as_float((uint32_t)(v0 >> 32)),
-                           __uint_as_float((uint32_t)v1), __uint_as_float((uint32_t)(v1 >> 32))} * f;
+            Joined j;
+            constexpr int N = 8; /* parts in flight */
+            for (int w0 = 0; w0 < parts; w0 += N) {
+                float2 st[N];
+                f32x4 part[N];
+#pragma unroll
+                for (int w = 0; w < N; ++w) {
+                    const int n = w0 + w < parts ? w0 + w : parts - 1;
+                    const int slot = 2 * (w_first + n) + (n == 0);
+                    const uint64_t u = ld_dev(reinterpret_cast<const uint64_t*>(a.ws.stats + (slot * kCols + k) * 2));
+                    st[w] = make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
+                    part[w] = ld_dev4(space, (uint32_t)((slot * kCols + k) * D + dim) * 4);
+                }
+                join(j, parts - w0, st, part);
             }
-            const int cc = p.col0 + k, n = divide(cc, a.group), qh = p.head * a.group.d + cc - n * a.group.d;
-            const bool empty = p.w.length - p.w.count + n < 0;
-            v = empty ? f32x4{0, 0, 0, 0} : v * (1.0f / all);
-            store4<DT>(a.out.data + ((p.w.start + n) * a.out.token_stride + qh * a.out.head_stride +
-                                     dim) * Elem<DT>::SIZE, v);
-            if (dim == 0 && a.lse)
-                a.lse[(int64_t)(p.w.start + n) * a.heads + qh] =
-                    empty ? -inf32() : (best + __builtin_amdgcn_logf(all)) * kLn2;
+            const Column to = column(a, info, p, head, col0 + k);
+            put<DT>(a, to.token, to.head, dim, j.v, j.top, j.sum);
         }
         __syncthreads();
     }
 }
 
-template <int DT, int D, int NW>
+/* The parts that are left to it, joined: four dims of a column a thread. */
+template <int DT, int D>
+__global__ __launch_bounds__(kB) void join_rows_kernel(AttendArgs a)
+{
+    const AttendRecord r = a.ws.records[blockIdx.x];
+    const int i = blockIdx.y * kB + threadIdx.x, k = i / (D / 4), dim = i % (D / 4) * 4;
+    if (r.parts == 0 || k >= r.cols || dim >= a.pool.head_dim) return;
+    Joined j;
+    constexpr int N = 8; /* parts in flight */
+    for (int w0 = 0; w0 < r.parts; w0 += N) {
+        float2 st[N];
+        f32x4 part[N];
+#pragma unroll
+        for (int w = 0; w < N; ++w) {
+            const int n = w0 + w < r.parts ? w0 + w : r.parts - 1;
+            const int slot = 2 * ((int)blockIdx.x + n) + (n == 0);
+            st[w] = *reinterpret_cast<const float2*>(a.ws.stats + (slot * kCols + k) * 2);
+            part[w] = *reinterpret_cast<const f32x4*>(a.ws.sums + (int64_t)(slot * kCols + k) * D + dim);
+        }
+        join(j, r.parts - w0, st, part);
+    }
+    const int col = r.col0 + k, nth = divide(col, a.group);
+    const int token = r.start >= 0 ? r.start + nth : a.starts ? a.starts[r.row + nth] : r.row + nth;
+    put<DT>(a, token, r.head0 + col - nth * a.group.d, dim, j.v, j.top, j.sum);
+}
+
+template <int DT, int D>
 hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
 {
-    const size_t lds = ((sizeof(Shared<DT, D, NW>) + 15) & ~(size_t)15) + ((size_t)a.rows + 1) * 8;
-    /* no more workgroups than the rows can have units */
+    constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT, UNIT = NW * TT;
+    const size_t lds = ((sizeof(Shared<DT, D, NW, TT>) + 15) & ~(size_t)15) + ((size_t)a.rows + 1) * 8 +
+                       (size_t)a.rows * sizeof(RowInfo);
+    /* no more workgroups than the rows can have use for */
     const int64_t blocks = (a.group.d + kCols - 1) / kCols;
-    const int64_t units = (cache_room(a.pool) + NW * kTile - 1) / (NW * kTile) + 1;
-    const int64_t most = (int64_t)a.rows * a.kv_heads * blocks * units;
+    const int64_t units = (cache_room(a.pool) + UNIT - 1) / UNIT + 1;
+    const int64_t most = ((int64_t)a.rows * a.kv_heads * blocks * units + kUnits - 1) / kUnits;
     const int groups = most < a.ws.groups ? (int)most : a.ws.groups;
-    return launch(attend_rows_kernel<DT, D, NW>, groups, NW * 64, lds, stream, a);
+    /* the most that can be left to be joined of one item: a launch of its own is enqueued only
+     * where it may have something to do */
+    const int64_t cols = (int64_t)a.rows * a.group.d < kCols ? (int64_t)a.rows * a.group.d : kCols;
+    const int64_t share = groups / a.kv_heads + 2, parts = units < share ? units : share;
+    const int joins = parts * cols * D * 4 > kJoinBytes;
+    hipError_t e = launch(attend_rows_kernel<DT, D>, groups, NW * 64, lds, stream, a, joins);
+    if (e != hipSuccess || !joins) return e;
+    return launch(join_rows_kernel<DT, D>, dim3((unsigned)groups, (unsigned)(kCols * D / 4 / kB)), kB, 0,
+                  stream, a);
 }
 
 template <int DT>
 hipError_t by_width(const AttendArgs& a, hipStream_t stream)
 {
     switch (attend_width(a.pool.head_dim)) {
-    case 64: return rows_launch<DT, 64, 8>(a, stream);
-    case 128: return rows_launch<DT, 128, 8>(a, stream);
-    case 256: return rows_launch<DT, 256, DT == G4S_DTYPE_F32 ? 4 : 8>(a, stream);
-    default: return rows_launch<DT, 512, 4>(a, stream);
+    case 64: return rows_launch<DT, 64>(a, stream);
+    case 128: return rows_launch<DT, 128>(a, stream);
+    case 256: return rows_launch<DT, 256>(a, stream);
+    default: return rows_launch<DT, 512>(a, stream);
     }
 }
 

@@ -90,16 +90,23 @@ G4S_PAGE_HD int32_t scale_exponent(double top)
     return e > kScaleHigh ? kScaleHigh : e;
 }
 
+/* n / d (n >= 0, d > 0), in 32 bits where they hold both. */
+G4S_PAGE_HD int64_t quotient(int64_t n, int64_t d)
+{
+    if (((uint64_t)n | (uint64_t)d) >> 32) return n / d;
+    return (int64_t)((uint32_t)n / (uint32_t)d);
+}
+
 /* Units of work shared out among `groups` workgroups, total >= groups: group w takes
  * units total * w / groups up to total * (w + 1) / groups, and unit x is the group's
  * that unit_group gives (the last w with total * w / groups < x + 1). */
 G4S_PAGE_HD int64_t first_unit(int64_t total, int32_t w, int32_t groups)
 {
-    return total * w / groups;
+    return quotient(total * w, groups);
 }
 G4S_PAGE_HD int32_t unit_group(int64_t x, int64_t total, int32_t groups)
 {
-    return (int32_t)(((x + 1) * groups - 1) / total);
+    return (int32_t)quotient((x + 1) * groups - 1, total);
 }
 
 /* Where a row's slots of a grid begin: `times` columns a token, `unit` columns a slot.  A row of
@@ -150,11 +157,20 @@ struct AppendArgs {
     int32_t heads, kv_heads, rotary_dims, rotary_pairs;
 };
 
+/* Columns whose parts a launch of its own joins. */
+struct AttendRecord {
+    int32_t parts; /* 0: none */
+    int32_t cols;
+    int32_t col0, head0; /* first column, and first head of its key head */
+    int32_t row, start;  /* several rows' (start -1), or a single one's first token */
+};
+
 /* Workspace of the attention: what several workgroups found for the same columns. */
 struct AttendSpace {
     float* sums;       /* kAttendSums for each workgroup */
     float* stats;      /* kAttendStats */
     uint32_t* tickets; /* one; 0 between calls */
+    AttendRecord* records; /* one: what the rows' kernel leaves to be joined */
     int32_t groups;    /* workgroups with parts of columns in a launch at most */
 };
 constexpr int kAttendSums = 32768, kAttendStats = 512;

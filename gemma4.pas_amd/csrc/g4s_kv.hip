@@ -227,6 +227,7 @@ G4S_API int g4s_cache_create(g4s_cache** out, const g4s_page_geometry* geometry,
         w.add(&h->ws.sums, groups * g4s::kAttendSums);
         w.add(&h->ws.stats, groups * g4s::kAttendStats);
         w.add(&h->ws.tickets, groups);
+        w.add(&h->ws.records, groups);
     };
     lay();
     const size_t bytes = w.used();

@@ -239,7 +239,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     auto store = [&](int n) {
         const int b = n % 3, to = n & 1;
         const int tid = again(threadIdx.x);
-        bool any = false;
+        uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = tid + i * THREADS, t = u / (D / 16), d0 = u % (D / 16) * 16;
@@ -265,7 +265,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                     const float vs = s.scale[b][1][t + j];
                     lo[j] = widen2<false>(vw[i][j], vs);
                     hi[j] = widen2<true>(vw[i][j], vs);
-                    any = any || has_nan(vw[i][j]);
+                    any |= nan_codes(vw[i][j]);
                 }
                 /* tokens 4 k .. 4 k + 3 of 32 (k = 0 .. 7) at quads 2 (k % 4) + k / 4: in the order that a
                  * lane of the second product takes them */
@@ -281,7 +281,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                 }
             }
         }
-        if (__any(any) && lane == 0) s.nan[to] = 1;
+        if (__any(any != 0) && lane == 0) s.nan[to] = 1;
     };
 
     if (tid < 2) s.nan[tid] = 0;
@@ -396,10 +396,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                         Frag f = value(i, h), is;
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            const uint32_t lo = (f.w[w] & 0x7FFFu) > 0x7F80u ? 0xFFFFu : 0u;
-                            const uint32_t hi = (f.w[w] & 0x7FFF0000u) > 0x7F800000u ? 0xFFFF0000u : 0u;
-                            f.w[w] &= ~(lo | hi);
-                            is.w[w] = (lo | hi) & 0x3F803F80u;
+                            /* (an exponent of ones carries into the sign's bit) */
+                            const uint32_t nan = ((((f.w[w] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu;
+                            f.w[w] &= ~nan;
+                            is.w[w] = nan & 0x3F803F80u;
                         }
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                                 is.v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
 #pragma unroll
                             for (int j = 0; j < 4; ++j)
-                                if (e[j] > 0.0f) o[t][i][j] = nan32();
+                                o[t][i][j] = nan_where(o[t][i][j], e[j]);
 #pragma unroll
                             for (int p = PP - 1; p >= 0; --p)
                                 o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
@@ -466,8 +466,7 @@ __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int s
     const int64_t slot = (x * gridDim.x + head) * splits;
     const float* stats = a.ws.stats + slot * kAttendStats + k * 2;
     const float* sums = a.ws.sums + slot * kAttendSums + (int64_t)k * D + dim;
-    float best = -inf32(), all = 0.0f;
-    f32x4 v = f32x4{0, 0, 0, 0};
+    Joined j;
     constexpr int N = 8; /* parts in flight */
     for (int w0 = 0; w0 < b.parts; w0 += N) {
         float2 st[N];
@@ -478,24 +477,11 @@ __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int s
             st[w] = *reinterpret_cast<const float2*>(stats + n * kAttendStats);
             p[w] = *reinterpret_cast<const f32x4*>(sums + n * kAttendSums);
         }
-        float now = best;
-#pragma unroll
-        for (int w = 0; w < N; ++w) now = fmaxf(now, st[w].x);
-        const float keep = best == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(best - now);
-        all *= keep;
-        v *= keep;
-        best = now;
-#pragma unroll
-        for (int w = 0; w < N; ++w) {
-            if (w0 + w >= b.parts) break;
-            const float f = st[w].x == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(st[w].x - now);
-            all += st[w].y * f;
-            v += p[w] * f;
-        }
+        join(j, b.parts - w0, st, p);
     }
     const Column at = column(a, b.r, head, b.col0 + k);
-    put<DT>(a, b.r, at, dim, v * (1.0f / all));
-    if (dim == 0) put_lse(a, b.r, at, best, all);
+    put<DT>(a, b.r, at, dim, j.v * (1.0f / j.sum));
+    if (dim == 0) put_lse(a, b.r, at, j.top, j.sum);
 }
 
 template <int DT, int D, int NW, int NT, int KT>

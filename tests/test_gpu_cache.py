@@ -70,7 +70,7 @@ class Rig:
 
     def __init__(self, lengths, news=None, P=16, B=4, kv=2, group=4, d=64, rotary=None,
                  pairs="halves", dtype="bf16", planes=3, order=(2, 0), seed=0, slots=None,
-                 outer=False, spare=3, stream=None):
+                 outer=False, spare=3, stream=None, share=None):
         self.rng = rng = np.random.default_rng(seed)
         self.P, self.B, self.kv, self.heads, self.d, self.dtype = P, B, kv, kv * group, d, dtype
         self.lengths = np.asarray(lengths, I32)
@@ -83,6 +83,10 @@ class Rig:
         for r in range(self.rows):
             for s in range(used[r]):
                 self.table[r, s] = free.pop()
+        if share:  # rows in groups of share[0] have their first share[1] pages in common
+            for r in range(self.rows):
+                n = min(share[1], used[r], used[r - r % share[0]])
+                self.table[r, :n] = self.table[r - r % share[0], :n]
         page = kv * P * (d + 4)
         strides = dict(plane_stride=page, page_stride=page * planes) if outer else {}
         self.geo = cache.geometry(P, n_pages, self.rows, self.slots, kv, d, planes, **strides)
@@ -405,6 +409,56 @@ def test_attend_odd_queries(dtype, news):
         x[-1, 4] *= 300.0
     with np.errstate(all="ignore"):
         rig.attend(edit=edit)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("share", [(2, 3), (3, 100), (4, 9), (5, 2), (16, 6), (40, 4)])
+@pytest.mark.parametrize("kv, group, d, dtype", [(2, 4, 64, "bf16"), (1, 1, 128, "f32"),
+                                                 (1, 5, 256, "bf16"), (2, 8, 80, "f32"),
+                                                 (1, 2, 512, "bf16"), (1, 16, 64, "bf16")])
+def test_attend_shared_pages(kv, group, d, dtype, share, window):
+    """Rows that have their first pages in common, equally long or not."""
+    lengths = [150 + (r // share[0]) * 37 + (r % 3 if share[0] != 4 else 0) for r in range(21)]
+    lengths[9], lengths[14] = 0, 20
+    Rig(lengths, P=16, B=8, kv=kv, group=group, d=d, dtype=dtype, share=share).attend(window)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attend_shared_pages_of_all_kinds(dtype):
+    """A page that is none and NaN values in shared and in own pages, rows of several tokens
+    beside them."""
+    rig = Rig([90, 90, 91, 92, 70, 70, 70, 70, 33], news=[1, 1, 1, 1, 1, 2, 1, 1, 3], dtype=dtype,
+              share=(4, 3))
+    cells = rig.pool.reshape(3, rig.geo.n_pages, rig.kv, rig.P, rig.d + 4)
+    v = cells[rig.planes[1]]
+    v[rig.table[0, 1], 0, 3, 7] = 0x7F       # seen by the first four
+    v[rig.table[2, 4], 1, 5, 9] = 0xFF       # by the third alone
+    rig.d_pool.upload(rig.pool)
+    rig.table[6, 2], rig.table[3, 5] = -1, rig.geo.n_pages
+    rig.upload()
+    rig.attend()
+    rig.attend(window=40)
+
+
+@pytest.mark.parametrize("shape", [
+    dict(lengths=[2500, 2500, 2499], d=512, group=4, P=32, B=32, dtype="f32", share=(3, 70)),
+    dict(lengths=[7000], d=256, group=16, kv=1, P=64, B=4),
+    dict(lengths=[3000, 10, 2000], news=[4, 1, 2], d=512, group=4, kv=1, P=64, slots=400)])
+def test_attend_parts_joined_by_their_own_launch(shape):
+    """Parts of more than a workgroup joins by itself."""
+    rig = Rig(**shape)
+    rig.attend()
+    rig.attend(window=1700)
+    rig.attend()
+
+
+def test_attend_many_rows():
+    """More rows than a workgroup has threads, in groups or alone, some ended."""
+    rng = np.random.default_rng(5)
+    lengths = rng.integers(0, 40, 1300)
+    lengths[rng.random(1300) < 0.2] = 0
+    Rig(lengths, P=8, B=8, kv=1, group=4, d=16, share=(4, 2)).attend()
+    Rig(lengths[:700], news=rng.integers(0, 3, 700), P=8, B=8, kv=1, group=4, d=16).attend()
 
 
 def test_attend_same_bits():
