@@ -22,6 +22,7 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
@@ -31,6 +32,7 @@ typedef uint32_t u32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
 union Frag {
     uint32_t w[4];
     bf16x8 v;
+    i16x4 half; /* its first four */
 };
 
 __device__ __forceinline__ float inf32() { return __builtin_inff(); }
@@ -77,12 +79,13 @@ __device__ __forceinline__ float nan_where(float x, float n)
 /* The word with +0 in the place of NaN codes. */
 __device__ __forceinline__ uint32_t without_nan(uint32_t w) { return w & ~(nan_codes(w) * 0xFFu); }
 
-/* Words of four dims of eight tokens, as operands of eight tokens for each of the dims. */
-__device__ __forceinline__ void value_frags(const uint32_t (&w)[8], const float (&scale)[8],
+/* Words of four dims of eight (or four) tokens, as operands of these tokens for each of the dims. */
+template <int NJ>
+__device__ __forceinline__ void value_frags(const uint32_t (&w)[NJ], const float (&scale)[NJ],
                                             Frag (&f)[4])
 {
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
+    for (int j = 0; j < NJ; j += 2) {
         const uint32_t a0 = widen2<false>(w[j], scale[j]);
         const uint32_t b0 = widen2<true>(w[j], scale[j]);
         const uint32_t a1 = widen2<false>(w[j + 1], scale[j + 1]);
@@ -92,6 +95,15 @@ __device__ __forceinline__ void value_frags(const uint32_t (&w)[8], const float 
         f[2].w[j >> 1] = lows(b0, b1);
         f[3].w[j >> 1] = highs(b0, b1);
     }
+}
+/* The product over these tokens. */
+template <int NJ>
+__device__ __forceinline__ f32x4 multiply(const Frag& a, const Frag& b, f32x4 c)
+{
+    if constexpr (NJ == 8)
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a.half, b.half, c, 0, 0, 0);
 }
 
 /* Eight consecutive elements of a query as a matrix operand: bf16 as they are, binary32 cut
@@ -188,12 +200,21 @@ __device__ __forceinline__ void join(Joined& j, int n, const float2 (&stats)[N],
     }
 }
 
+/* A barrier for what is in LDS: loads and stores of memory stay in flight (the full one waits for a
+ * workgroup's partial sums to reach the memory, 2 to 3 us). */
+__device__ __forceinline__ void lds_barrier()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 /* Writes to LDS of this wave are read by its other lanes from here on. */
 __device__ __forceinline__ void wave_fence()
 {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
 
 }  // namespace g4s

@@ -20,10 +20,8 @@ namespace g4s {
 namespace {
 
 constexpr int kB = 256;
-constexpr int kTile = 32;  /* tokens of a wave's step go by 32 */
 constexpr int kCols = 16;  /* query columns of a workgroup's part */
 constexpr int kPass = 128; /* dims that the waves join at once */
-constexpr int kUnits = 2;  /* units of a workgroup at least, where there are few */
 /* Bytes of parts that their last workgroup joins by itself: more are left to a launch of
  * their own. */
 constexpr int kJoinBytes = 96 << 10;
@@ -34,19 +32,19 @@ struct RowInfo {
     int length, key;
 };
 
-/* The rows of one part, and what they ask for of each key head. */
+/* The rows that begin with a row and are taken together, and the places that any of their
+ * queries sees. */
 struct Group {
-    int row, rows;    /* rows > 1: of one token each */
-    int start, count; /* of a single row */
-    int cols, blocks; /* query columns (tokens x heads of a key head), 16 of them a block */
-    int from, end;    /* places that any query sees */
-    int first, units; /* units of them: one at least, for the output */
+    int rows;  /* of one token each; or -n: one row of n tokens; 0: none (taken by a row before it,
+                  without tokens, or the prompts' kernel's) */
+    int start; /* a single row's first token */
+    int from, end;
 };
 
 __device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
 {
-    const int64_t f = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
-    return f > 0 ? (int)f : 0;
+    const int from = a.window > 0 ? (int)((uint32_t)place - (uint32_t)a.window + 1u) : 0;
+    return from > 0 && a.window <= place ? from : 0;
 }
 
 /* Rows that are taken together at most: a power of two, of rows that begin at a multiple of it. */
@@ -56,45 +54,48 @@ __device__ __forceinline__ int group_rows(const AttendArgs& a)
     return n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
 }
 
-template <int UNIT>
 __device__ __forceinline__ Group find_group(const AttendArgs& a, const RowInfo* info, int row)
 {
-    Group p{row, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    Group p{0, 0, 0, 0};
     const int key = info[row].key, most = group_rows(a), in = row & (most - 1);
-    /* taken by a row before it */
-    if (key >= 0 && in > 0 && info[row - 1].key == key) return p;
-    p.rows = 1;
-    int from = 0, end = 0;
     if (key >= 0) {
-        end = info[row].length;
-        from = sees_from(a, end - 1);
+        if (in > 0 && info[row - 1].key == key) return p;
+        p.rows = 1;
+        p.end = info[row].length;
+        p.from = sees_from(a, p.end - 1);
         for (int i = 1; in + i < most && row + i < a.rows && info[row + i].key == key; ++i) {
             const int n = info[row + i].length, f = sees_from(a, n - 1);
-            end = n > end ? n : end;
-            from = f < from ? f : from;
+            p.end = n > p.end ? n : p.end;
+            p.from = f < p.from ? f : p.from;
             ++p.rows;
         }
+        if (p.rows > 1) return p;
     }
     const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
+    p.rows = is_prompt(r.count, a.group.d) ? 0 : -r.count;
     p.start = r.start;
-    p.count = r.count;
-    if (key < 0) {
-        end = r.length;
-        from = sees_from(a, r.length - r.count);
-    }
-    p.cols = p.rows > 1 ? p.rows * a.group.d : is_prompt(r.count, a.group.d) ? 0 : r.count * a.group.d;
-    p.blocks = (p.cols + kCols - 1) / kCols;
-    p.from = from;
-    p.end = end;
-    p.first = from / UNIT;
-    p.units = end > from ? (int)(((int64_t)end + UNIT - 1) / UNIT) - p.first : 1;
+    p.end = r.length;
+    p.from = sees_from(a, r.length - r.count);
     return p;
 }
 
-/* info[0 .. rows - 1], and the work of the groups before each row, in units, in before[0 .. rows]. */
+/* Query columns (tokens x heads of a key head) of a group, and units of UNIT tokens of each of
+ * its blocks of them: one at least, for the output. */
+__device__ __forceinline__ int group_cols(const AttendArgs& a, const Group& p)
+{
+    return (p.rows < 0 ? -p.rows : p.rows) * a.group.d;
+}
+template <int UNIT>
+__device__ __forceinline__ int group_units(const Group& p)
+{
+    return p.end > p.from ? (int)(((uint32_t)p.end + UNIT - 1) / UNIT) - p.from / UNIT : 1;
+}
+
+/* info and groups [0 .. rows - 1], and the work of the groups before each row, in units,
+ * in before[0 .. rows]. */
 template <int NW, int UNIT>
-__device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, int64_t* before,
-                                          int64_t* s_wave)
+__device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, Group* groups,
+                                          int64_t* before, int64_t* s_wave)
 {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int each = (a.rows + NW * 64 - 1) / (NW * 64);
@@ -106,25 +107,26 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, in
         if (t.count == 1 && t.length > 0 && page >= 0 && page < a.pool.n_pages) i.key = page;
         info[r] = i;
     }
-    __syncthreads();
+    lds_barrier();
     int64_t sum = 0;
     for (int i = 0; i < each; ++i) {
         const int r = tid * each + i;
         if (r >= a.rows) break;
-        const Group p = find_group<UNIT>(a, info, r);
-        before[r + 1] = (int64_t)p.units * p.blocks * a.kv_heads;
+        const Group p = find_group(a, info, r);
+        const int blocks = (group_cols(a, p) + kCols - 1) / kCols;
+        groups[r] = p;
+        before[r + 1] = (int64_t)(blocks * a.kv_heads) * group_units<UNIT>(p);
         sum += before[r + 1];
     }
-    int64_t x = sum;
-    if (a.rows > 1)
-        for (int d = 1; d < 64 && d < a.rows; d <<= 1) {
-            const int64_t y = __shfl_up((long long)x, d);
-            if (lane >= d) x += y;
-        }
-    if (lane == 63) s_wave[wave] = x;
-    __syncthreads();
+    /* (a row's units are below 2^39) */
+    int64_t x = (int64_t)wave_inclusive_scan((int)(sum >> 16)) * 65536 +
+                wave_inclusive_scan((int)(sum & 0xFFFF));
+    if (a.rows > 64 * each) {
+        if (lane == 63) s_wave[wave] = x;
+        lds_barrier();
+        for (int w = 0; w < wave; ++w) x += s_wave[w];
+    }
     x -= sum;
-    for (int w = 0; w < wave; ++w) x += s_wave[w];
     for (int i = 0; i < each; ++i) {
         const int r = tid * each + i;
         if (r >= a.rows) break;
@@ -132,17 +134,21 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, in
         before[r + 1] = x;
     }
     if (tid == 0) before[0] = 0;
-    __syncthreads();
+    lds_barrier();
 }
 
 template <int DT, int D, int NW, int TT>
 struct Shared {
-    Frag q[D / 64][2][DT == G4S_DTYPE_F32 ? 3 : 1][64]; /* the queries, as lanes take them */
+    union {
+        Frag q[D / 64][2][DT == G4S_DTYPE_F32 ? 3 : 1][64]; /* the queries, as lanes take them */
+        float o[NW][kCols][kPass + 4];                      /* the waves' sums */
+    };
     int64_t offset[NW][2][TT];
     float scale[NW][2][2][TT];
     float m[NW][kCols], l[NW][kCols];
     float top[kCols], sum[kCols];
-    float o[NW][kCols][kPass + 4];
+    int64_t out[kCols]; /* of each column: its first element of out, and its lse */
+    int lse[kCols];
     int64_t wave[NW];
     int differs; /* the first slot whose page is not the same for all rows */
     int flag;
@@ -164,55 +170,36 @@ __device__ __forceinline__ void load_words(const char* p, uint32_t (&w)[VW])
     }
 }
 
-/* Column k of a part: its token, head and place. */
-struct Column {
-    int token, head, place;
-};
-__device__ __forceinline__ Column column(const AttendArgs& a, const RowInfo* info, const Group& p,
-                                         int head, int k)
-{
-    const int nth = divide(k, a.group);
-    Column c;
-    c.head = head * a.group.d + k - nth * a.group.d;
-    if (p.rows > 1) {
-        c.token = a.starts ? a.starts[p.row + nth] : p.row + nth;
-        c.place = info[p.row + nth].length - 1;
-    } else {
-        c.token = p.start + nth;
-        c.place = (info[p.row].length < 0 ? 0 : info[p.row].length) - p.count + nth;
-    }
-    return c;
-}
-
-/* (a column that sees nothing has no maximum and no sum) */
+/* Output of a column whose sums over all parts are known.  (One that sees nothing has no
+ * maximum and no sum.) */
 template <int DT>
-__device__ __forceinline__ void put(const AttendArgs& a, int token, int head, int dim, f32x4 v, float top,
-                                    float sum)
+__device__ __forceinline__ void put(const AttendArgs& a, int64_t out, int64_t lse, int dim, f32x4 v,
+                                    float top, float sum)
 {
     const bool none = top == -inf32() && sum == 0.0f;
     v = none ? f32x4{0, 0, 0, 0} : v * (1.0f / sum);
-    if (dim < a.pool.head_dim)
-        store4<DT>(a.out.data + ((int64_t)token * a.out.token_stride +
-                                 (int64_t)head * a.out.head_stride + dim) * Elem<DT>::SIZE, v);
-    if (dim == 0 && a.lse)
-        a.lse[(int64_t)token * a.heads + head] =
-            none ? -inf32() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
+    if (dim < a.pool.head_dim) store4<DT>(a.out.data + (out + dim) * Elem<DT>::SIZE, v);
+    if (dim == 0 && a.lse) a.lse[lse] = none ? -inf32() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-/* How a kernel is made for a width of heads: tokens of a wave's step, a multiple of kTile as
- * registers allow, and waves. */
+/* How a kernel is made for a width of heads: tokens of a wave's step, as many as its registers
+ * hold beside the sums (16, 32 or 64). */
+constexpr int kWaves = 4;
 template <int DT, int D>
 struct Shape {
-    static constexpr int TT = D <= 128 ? 2 * kTile : kTile;
-    static constexpr int NW = D == 512 || (D == 256 && DT == G4S_DTYPE_F32) ? 4 : 8;
+    static constexpr int NW = kWaves;
+    static constexpr int TT = D <= 128 ? 64 : D <= 256 ? 32 : 16;
+    static constexpr int UNITS = D <= 128 ? 2 : 4; /* of a workgroup at least, where there are few */
 };
 
 template <int DT, int D>
-__global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel(AttendArgs a, int joins)
+__global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel(AttendArgs a, int joins)
 {
     constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT;
     constexpr int UNIT = NW * TT;
-    constexpr int NB = TT / 16, NH = TT / kTile;    /* of 16 and of 32 tokens */
+    constexpr int NB = TT / 16;                     /* blocks of 16 tokens of a step */
+    constexpr int NJ = TT < 32 ? 4 : 8;             /* tokens of a lane in a product with V .. */
+    constexpr int NH = TT / (4 * NJ);               /* .. of which a step has so many */
     constexpr int QP = DT == G4S_DTYPE_F32 ? 3 : 1; /* pieces of a query */
     constexpr int PP = DT == G4S_DTYPE_F32 ? 2 : 1; /* and of a weight */
     constexpr int KC = D / 64;                      /* 16-dim chunks of a lane of K and Q */
@@ -223,14 +210,16 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
     extern __shared__ char lds[];
     using S = Shared<DT, D, NW, TT>;
     S& s = *reinterpret_cast<S*>(lds);
-    int64_t* before = reinterpret_cast<int64_t*>(lds + ((sizeof(S) + 15) & ~(size_t)15));
+    Group* group = reinterpret_cast<Group*>(lds + ((sizeof(S) + 15) & ~(size_t)15));
+    int64_t* before = reinterpret_cast<int64_t*>(group + a.rows);
     RowInfo* info = reinterpret_cast<RowInfo*>(before + a.rows + 1);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int m = lane & 15, g = lane >> 4;
     if (joins && tid == 0) a.ws.records[blockIdx.x].parts = 0;
-    scan_rows<NW, UNIT>(a, info, before, s.wave);
+    scan_rows<NW, UNIT>(a, info, group, before, s.wave);
     const int64_t total = before[a.rows];
-    const int64_t least = (total + kUnits - 1) / kUnits;
+    constexpr int UNITS = Shape<DT, D>::UNITS;
+    const int64_t least = (total + UNITS - 1) / UNITS;
     const int groups = least < gridDim.x ? (int)least : (int)gridDim.x;
     if ((int)blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
@@ -250,25 +239,38 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             n = n - last * each < each ? n - last * each : each;
         }
         lo = __builtin_amdgcn_readfirstlane(lo);
-        const Group p = find_group<UNIT>(a, info, lo);
+        Group p = group[lo];
+        p.rows = __builtin_amdgcn_readfirstlane(p.rows);
+        p.start = __builtin_amdgcn_readfirstlane(p.start);
+        p.from = __builtin_amdgcn_readfirstlane(p.from);
+        p.end = __builtin_amdgcn_readfirstlane(p.end);
+        const bool several = p.rows > 1; /* rows */
+        const int all_cols = group_cols(a, p), blocks = (all_cols + kCols - 1) / kCols;
+        const int units = group_units<UNIT>(p), first = p.from / UNIT;
         const int64_t in_group = x - before[lo];
-        const int item = (int)quotient(in_group, p.units);
-        const int u0 = (int)(in_group - (int64_t)item * p.units);
-        const int u1 = p.units - u0 < x_end - x ? p.units : u0 + (int)(x_end - x);
-        const int head = p.blocks == 1 ? item : item / p.blocks;
-        const int col0 = (item - head * p.blocks) * kCols;
+        const int item = __builtin_amdgcn_readfirstlane((int)quotient(in_group, units));
+        const int u0 = __builtin_amdgcn_readfirstlane((int)(in_group - (int64_t)item * units));
+        const int u1 = units - u0 < x_end - x ? units : u0 + (int)(x_end - x);
+        const int head = blocks == 1 ? item : item / blocks;
+        const int col0 = (item - head * blocks) * kCols;
         const int64_t item_first = x - u0; /* its first unit among all */
         x += u1 - u0;
 
-        /* this lane's query column */
-        const int cols = p.cols - col0 < kCols ? p.cols - col0 : kCols;
+        /* this lane's query column: token x head, or row x head */
+        const int cols = all_cols - col0 < kCols ? all_cols - col0 : kCols;
         const bool has_col = m < cols;
-        const Column at = column(a, info, p, head, col0 + (has_col ? m : 0));
-        const int place = at.place, from = sees_from(a, place);
-        const int member = p.rows > 1 ? divide(has_col ? m : 0, a.group) : 0;
+        const int col = col0 + (has_col ? m : 0), nth = divide(col, a.group);
+        const int qhead = head * a.group.d + col - nth * a.group.d;
+        const int token0 = several ? (a.starts ? a.starts[lo + nth] : lo + nth) : p.start + nth;
+        const int place = several ? info[lo + nth].length - 1 : p.end + p.rows + nth;
+        const int from = sees_from(a, place);
+        if (tid < kCols) {
+            s.out[tid] = (int64_t)token0 * a.out.token_stride + (int64_t)qhead * a.out.head_stride;
+            s.lse[tid] = token0 * a.heads + qhead;
+        }
         {
-            const char* q = a.q.data + ((int64_t)at.token * a.q.token_stride +
-                                        (int64_t)at.head * a.q.head_stride) * Elem<DT>::SIZE;
+            const char* q = a.q.data + ((int64_t)token0 * a.q.token_stride +
+                                        (int64_t)qhead * a.q.head_stride) * Elem<DT>::SIZE;
             for (int k = wave; k < KC; k += NW) {
                 const int d0 = k * 64 + g * 16;
                 Frag f[2][QP];
@@ -285,7 +287,8 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
         }
         /* places that all queries see */
         int all_from = from, all_to = place;
-        if (p.rows > 1 || p.count > 1)
+        const bool multi = several || p.rows < -1;
+        if (multi)
             for (int d = 1; d < kCols; d <<= 1) {
                 const int f = __shfl_xor(all_from, d), t = __shfl_xor(all_to, d);
                 all_from = f > all_from ? f : all_from;
@@ -293,33 +296,32 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             }
         all_from = __builtin_amdgcn_readfirstlane(all_from);
         all_to = __builtin_amdgcn_readfirstlane(all_to);
-        const bool multi = p.rows > 1 || p.count > 1;
-        /* the part's tiles: the first `shared` of them with the same pages for all rows */
-        const int t0 = (p.first + u0) * UNIT > p.from ? (p.first + u0) * UNIT : p.from;
-        const int t1 = (int64_t)(p.first + u1) * UNIT < p.end ? (p.first + u1) * UNIT : p.end;
-        const int a0 = t0 / TT, a1 = t1 > t0 ? (t1 + TT - 1) / TT : a0;
+        /* the part's tiles: those before a_shared have the same pages for all rows */
+        const int t0 = (first + u0) * UNIT > p.from ? (first + u0) * UNIT : p.from;
+        const int t1 = (uint32_t)(first + u1) * UNIT < (uint32_t)p.end ? (first + u1) * UNIT : p.end;
+        const int a0 = t0 / TT, a1 = t1 > t0 ? (int)((uint32_t)(t1 + TT - 1) / TT) : a0;
         int a_shared = a1;
-        int ref = p.row; /* the longest row, whose table has every place */
-        if (p.rows > 1) {
+        int ref = lo; /* the longest row, whose table has every place */
+        if (several) {
             for (int i = 1; i < p.rows; ++i)
-                if (info[p.row + i].length > info[ref].length) ref = p.row + i;
+                if (info[lo + i].length > info[ref].length) ref = lo + i;
             ref = __builtin_amdgcn_readfirstlane(ref);
             if (tid == 0) s.differs = p.end;
-            __syncthreads();
+            lds_barrier();
             const int s0 = divide(t0, a.pool.page_tokens), s1 = divide(t1 - 1, a.pool.page_tokens);
-            for (int i = tid; i < (s1 - s0 + 1) * p.rows; i += NW * 64) {
-                const int slot = s0 + i / p.rows, row = p.row + i % p.rows;
-                const int last = info[row].length - 1;
+            for (int slot = s0 + (tid >> 4); slot <= s1; slot += NW * 4) {
+                if (m >= p.rows) break;
+                const int last = info[lo + m].length - 1;
                 if (slot < divide(sees_from(a, last), a.pool.page_tokens) ||
                     slot > divide(last, a.pool.page_tokens))
                     continue;
-                if (a.table[(int64_t)row * a.pool.max_slots + slot] !=
+                if (a.table[(int64_t)(lo + m) * a.pool.max_slots + slot] !=
                     a.table[(int64_t)ref * a.pool.max_slots + slot])
                     atomicMin(&s.differs, slot);
             }
         }
-        __syncthreads();
-        if (p.rows > 1) {
+        lds_barrier();
+        if (several) {
             const int64_t t = (int64_t)s.differs * a.pool.page_tokens.d;
             const int n = t < p.end ? (int)t / TT : a1;
             a_shared = __builtin_amdgcn_readfirstlane(n < a0 ? a0 : n < a1 ? n : a1);
@@ -351,7 +353,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
                     ++t.tile;
                 }
                 if (t.tile >= a1) return;
-                t.last = __builtin_amdgcn_readfirstlane(info[p.row + t.row].length - 1);
+                t.last = __builtin_amdgcn_readfirstlane(info[lo + t.row].length - 1);
                 t.first = sees_from(a, t.last);
                 if (t.tile * TT <= t.last && t.tile * TT + TT > t.first) return;
             }
@@ -371,7 +373,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             return i < t.first ? t.first : i > t.last ? t.last : i;
         };
         auto find_page = [&](const Step& t) {
-            const int row = t.row >= 0 ? p.row + t.row : ref;
+            const int row = t.row >= 0 ? lo + t.row : ref;
             return a.table[(int64_t)row * a.pool.max_slots + divide(token(t), a.pool.page_tokens)];
         };
         const char* const keys = a.k_plane + (int64_t)head * a.pool.part_bytes;
@@ -402,13 +404,13 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
                 s.scale[wave][b][0][lane] = scale.k;
                 s.scale[wave][b][1][lane] = scale.v;
             } else {
-                s.scale[wave][b][lane >> 5][lane & 31] = scale.k;
+                s.scale[wave][b][lane >> 5][lane & (TT - 1)] = scale.k;
             }
         };
         /* (dims behind head_dim, whose queries are 0 and whose sums are not kept, are read in
          * the last ones' place) */
         const int last_key = a.pool.head_dim - 16, last_value = a.pool.head_dim - 4 * VL;
-        uint32_t kw[NB][KC][4], vw[NH][8][VW];
+        uint32_t kw[NB][KC][4], vw[NH][NJ][VW];
         auto load_keys = [&](int b) {
 #pragma unroll
             for (int h = 0; h < NB; ++h) {
@@ -424,7 +426,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
 #pragma unroll
             for (int h = 0; h < NH; ++h)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < NJ; ++j) {
                     const char* from = values + s.offset[wave][b][h * 32 + (j & 4) * 4 + g * 4 + (j & 3)];
 #pragma unroll
                     for (int i = 0; i < VW; i += VL) {
@@ -445,12 +447,13 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
         if (now.tile < a1) {
             Scales scale;
             bad = locate(now, find_page(now), 0, scale);
-            keep_scales(0, scale);
             wave_fence();
             load_keys(0);
             load_values(0);
             next = advance(now);
             if (next.tile < a1) page = find_page(next);
+            keep_scales(0, scale);
+            wave_fence();
         }
         while (now.tile < a1) {
             const bool more = next.tile < a1;
@@ -465,25 +468,43 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             }
 
             f32x4 sc[NB];
+            float ks[NB];
 #pragma unroll
             for (int h = 0; h < NB; ++h) {
-                const float ks = s.scale[wave][buf][0][h * 16 + m];
+                ks[h] = s.scale[wave][buf][0][h * 16 + m];
                 sc[h] = f32x4{0, 0, 0, 0};
+            }
 #pragma unroll
-                for (int k = 0; k < KC; ++k) {
+            for (int k = 0; k < KC; ++k) {
+                Frag q[2][QP];
+#pragma unroll
+                for (int b = 0; b < QP; ++b) {
+                    q[0][b] = s.q[k][0][b][lane];
+                    q[1][b] = s.q[k][1][b][lane];
+                }
+#pragma unroll
+                for (int h = 0; h < NB; ++h) {
                     Frag f[2];
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
-                        f[w >> 1].w[(w & 1) * 2] = widen2<false>(kw[h][k][w], ks);
-                        f[w >> 1].w[(w & 1) * 2 + 1] = widen2<true>(kw[h][k][w], ks);
+                        f[w >> 1].w[(w & 1) * 2] = widen2<false>(kw[h][k][w], ks[h]);
+                        f[w >> 1].w[(w & 1) * 2 + 1] = widen2<true>(kw[h][k][w], ks[h]);
                     }
 #pragma unroll
                     for (int b = QP - 1; b >= 0; --b) {
-                        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0].v, s.q[k][0][b][lane].v, sc[h], 0, 0, 0);
-                        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1].v, s.q[k][1][b][lane].v, sc[h], 0, 0, 0);
+                        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[0].v, q[0][b].v, sc[h], 0, 0, 0);
+                        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[1].v, q[1][b].v, sc[h], 0, 0, 0);
                     }
                 }
             }
+            /* one chunk's queries are read ahead (all of them at once would take the registers) */
+            __builtin_amdgcn_sched_group_barrier(0x100, NB + 2 * QP, 0);
+#pragma unroll
+            for (int k = 1; k < KC; ++k) {
+                __builtin_amdgcn_sched_group_barrier(0x100, 2 * QP, 0);
+                __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NB, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * QP * NB, 0);
             if (more) load_keys(buf ^ 1);
             /* y[j] of half h: token h * 32 + (j & 4) * 4 + g * 4 + (j & 3) */
             const int tile0 = now.tile * TT;
@@ -491,7 +512,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             const bool partly = bad_now != 0 || tile0 < all_from || tile0 + TT - 1 > all_to || alone;
             bool nan_v = false;
             if (partly) {
-                const bool mine = !alone || member == now.row;
+                const bool mine = !alone || nth == now.row;
 #pragma unroll
                 for (int h = 0; h < NB; ++h)
 #pragma unroll
@@ -505,7 +526,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
 #pragma unroll
                     for (int h = 0; h < NH; ++h)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
+                        for (int j = 0; j < NJ; ++j)
 #pragma unroll
                             for (int w = 0; w < VW; ++w) any |= nan_codes(vw[h][j][w]);
                     nan_v = __any(any != 0);
@@ -542,57 +563,59 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
                         f[1].w[w] = pack_bf16(e0 - __uint_as_float(f[0].w[w] << 16),
                                               e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
                 }
+            if (nan_v) {
+                /* a NaN that some queries see and others do not (0 times NaN is NaN): the products
+                 * go without it, and whoever sees one, counted by a product too, gets NaN */
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-                float vs[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    vs[j] = s.scale[wave][buf][1][h * 32 + (j & 4) * 4 + g * 4 + (j & 3)];
-                if (nan_v) {
-                    /* a NaN that some queries see and others do not (0 times NaN is NaN): the
-                     * products go without it, and whoever sees one, counted by a product too,
-                     * gets NaN */
+                for (int h = 0; h < NH; ++h) {
                     Frag see;
 #pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
+                    for (int j = 0; j < NJ; j += 2) {
                         const f32x4 y = sc[h * 2 + (j >> 2)];
                         see.w[j >> 1] = (y[j & 3] == -inf32() ? 0u : 0x3F80u) |
                                         (y[(j & 3) + 1] == -inf32() ? 0u : 0x3F800000u);
                     }
-                    const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+                    float one[NJ];
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) one[j] = 1.0f;
 #pragma unroll
                     for (int w = 0; w < VW; ++w) {
-                        uint32_t is[8];
+                        uint32_t is[NJ];
                         Frag f[4];
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) {
+                        for (int j = 0; j < NJ; ++j) {
                             is[j] = nan_codes(vw[h][j][w]) * 0x38u; /* the code of 1 */
                             vw[h][j][w] = without_nan(vw[h][j][w]);
                         }
-                        value_frags(is, one, f);
+                        value_frags<NJ>(is, one, f);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const f32x4 n = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                f[i].v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
+                            const f32x4 n = multiply<NJ>(f[i], see, f32x4{0, 0, 0, 0});
 #pragma unroll
                             for (int r = 0; r < 4; ++r)
                                 o[w * 4 + i][r] = nan_where(o[w * 4 + i][r], n[r]);
                         }
                     }
                 }
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+                float vs[NJ];
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+                    vs[j] = s.scale[wave][buf][1][h * 32 + (j & 4) * 4 + g * 4 + (j & 3)];
 #pragma unroll
                 for (int w = 0; w < VW; ++w) {
-                    uint32_t word[8];
+                    uint32_t word[NJ];
                     Frag f[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) word[j] = vw[h][j][w];
-                    value_frags(word, vs, f);
+                    for (int j = 0; j < NJ; ++j) word[j] = vw[h][j][w];
+                    value_frags<NJ>(word, vs, f);
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int b = PP - 1; b >= 0; --b)
-                            o[w * 4 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                f[i].v, pw[h][b].v, o[w * 4 + i], 0, 0, 0);
+                            o[w * 4 + i] = multiply<NJ>(f[i], pw[h][b], o[w * 4 + i]);
                 }
             }
             if (more) {
@@ -612,114 +635,138 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 1) void attend_rows_kernel
             s.m[wave][m] = top == -inf32() ? top : top * c;
             s.l[wave][m] = sum;
         }
-        __syncthreads();
+        const bool whole = u0 == 0 && u1 == units;
+        const int slot = 2 * (int)blockIdx.x + (u0 == 0);
+        lds_barrier();
         if (tid < kCols) {
             float best = s.m[0][tid];
+#pragma unroll
             for (int w = 1; w < NW; ++w) best = fmaxf(best, s.m[w][tid]);
             float all = 0.0f;
+#pragma unroll
             for (int w = 0; w < NW; ++w) {
                 const float f = s.m[w][tid] == -inf32() ? 0.0f : __builtin_amdgcn_exp2f(s.m[w][tid] - best);
                 all += s.l[w][tid] * f;
                 s.l[w][tid] = f;
             }
-            const bool bad_row = p.rows == 1 && info[p.row].length < 0;
-            s.top[tid] = bad_row ? nan32() : best;
-            s.sum[tid] = bad_row ? nan32() : all;
+            const bool bad_row = !several && info[lo].length < 0;
+            best = bad_row ? nan32() : best;
+            all = bad_row ? nan32() : all;
+            s.top[tid] = best;
+            s.sum[tid] = all;
+            if (!whole && tid < cols)
+                st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot * kCols + tid) * 2),
+                       (uint64_t)__float_as_uint(best) | (uint64_t)__float_as_uint(all) << 32);
         }
-        const bool whole = u0 == 0 && u1 == p.units;
-        const int slot = 2 * (int)blockIdx.x + (u0 == 0);
-        for (int pass = 0; pass < (D + kPass - 1) / kPass; ++pass) {
-            /* lanes with dims of this pass */
+        constexpr int PD = D < kPass ? D : kPass; /* dims of a pass */
+#pragma unroll 1
+        for (int pass = 0; pass < D / PD; ++pass) {
+            /* lanes with dims of this pass: a lane has DB in each of four rows */
+            if (pass > 0) lds_barrier();
+            constexpr int GP = PD / (4 * DB); /* lane groups of a pass */
+            if (g / GP == pass && m < cols) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int d0 = DB * (g * 4 + r) - pass * kPass;
-                if (d0 >= 0 && d0 < kPass) {
+                for (int r = 0; r < 4; ++r)
 #pragma unroll
                     for (int i = 0; i < DB; i += 4)
-                        *reinterpret_cast<f32x4*>(&s.o[wave][m][d0 + i]) =
+                        *reinterpret_cast<f32x4*>(&s.o[wave][m][DB * ((g % GP) * 4 + r) + i]) =
                             f32x4{o[i][r], o[i + 1][r], o[i + 2][r], o[i + 3][r]};
-                }
             }
-            __syncthreads();
-            constexpr int Q4 = (D < kPass ? D : kPass) / 4;
-            for (int i = tid; i < cols * Q4; i += NW * 64) {
-                const int k = i / Q4, d0 = i % Q4 * 4, dim = pass * kPass + d0;
+            lds_barrier();
+            for (int i = tid; i < cols * (PD / 4); i += NW * 64) {
+                const int k = i / (PD / 4), d0 = i % (PD / 4) * 4, dim = pass * PD + d0;
                 f32x4 v = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int w = 0; w < NW; ++w)
                     v += *reinterpret_cast<const f32x4*>(&s.o[w][k][d0]) * s.l[w][k];
-                if (whole) {
-                    const Column to = column(a, info, p, head, col0 + k);
-                    put<DT>(a, to.token, to.head, dim, v, s.top[k], s.sum[k]);
-                } else {
+                if (whole)
+                    put<DT>(a, s.out[k], s.lse[k], dim, v, s.top[k], s.sum[k]);
+                else
                     st_dev4(space, (uint32_t)((slot * kCols + k) * D + dim) * 4, v);
-                }
             }
-            if (pass == 0 && tid < cols && !whole)
-                st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot * kCols + tid) * 2),
-                       (uint64_t)__float_as_uint(s.top[tid]) | (uint64_t)__float_as_uint(s.sum[tid]) << 32);
-            __syncthreads();
         }
-        if (whole) continue;
-        const int w_first = unit_group(item_first, total, groups);
-        const int parts = unit_group(item_first + p.units - 1, total, groups) - w_first + 1;
-        if (joins && parts * cols * D * 4 > kJoinBytes) {
-            if (tid == 0 && u0 == 0)
-                a.ws.records[blockIdx.x] = AttendRecord{parts, cols, col0, head * a.group.d, p.row,
-                                                        p.rows > 1 ? -1 : p.start};
-            continue;
-        }
-        /* the last of the workgroups that have a part of this item joins them */
-        if (!elect_last(&a.ws.tickets[w_first], (uint32_t)parts, &s.flag)) continue;
-        for (int i = tid; i < cols * (D / 4); i += NW * 64) {
-            const int k = i / (D / 4), dim = i % (D / 4) * 4;
-            if (dim >= a.pool.head_dim) continue;
-            Joined j;
-            constexpr int N = 8; /* parts in flight */
-            for (int w0 = 0; w0 < parts; w0 += N) {
-                float2 st[N];
-                f32x4 part[N];
+        if (!whole) {
+            const int w_first = unit_group(item_first, total, groups);
+            const int parts = unit_group(item_first + units - 1, total, groups) - w_first + 1;
+            if (joins && parts * cols * D * 4 > kJoinBytes) {
+                if (tid == 0 && u0 == 0)
+                    a.ws.records[blockIdx.x] = AttendRecord{parts, cols, col0, head * a.group.d, lo,
+                                                            several ? -1 : p.start};
+            } else if (elect_last(&a.ws.tickets[w_first], (uint32_t)parts, &s.flag)) {
+                /* the last of the workgroups that have a part of this item joins them */
+                for (int i = tid; i < cols * (D / 4); i += NW * 64) {
+                    const int k = i / (D / 4), dim = i % (D / 4) * 4;
+                    if (dim >= a.pool.head_dim) continue;
+                    Joined j;
+                    constexpr int N = 8; /* parts in flight */
+                    for (int w0 = 0; w0 < parts; w0 += N) {
+                        float2 st[N];
+                        f32x4 part[N];
 #pragma unroll
-                for (int w = 0; w < N; ++w) {
-                    const int n = w0 + w < parts ? w0 + w : parts - 1;
-                    const int slot = 2 * (w_first + n) + (n == 0);
-                    const uint64_t u = ld_dev(reinterpret_cast<const uint64_t*>(a.ws.stats + (slot * kCols + k) * 2));
-                    st[w] = make_float2(__uint_as_float((uint32_t)u), __uint_as_float((uint32_t)(u >> 32)));
-                    part[w] = ld_dev4(space, (uint32_t)((slot * kCols + k) * D + dim) * 4);
+                        for (int w = 0; w < N; ++w) {
+                            const int n = w0 + w < parts ? w0 + w : parts - 1;
+                            const int from = (2 * (w_first + n) + (n == 0)) * kCols + k;
+                            const uint64_t u = ld_dev(reinterpret_cast<const uint64_t*>(a.ws.stats + from * 2));
+                            st[w] = make_float2(__uint_as_float((uint32_t)u),
+                                                __uint_as_float((uint32_t)(u >> 32)));
+                            part[w] = ld_dev4(space, (uint32_t)(from * D + dim) * 4);
+                        }
+                        join(j, parts - w0, st, part);
+                    }
+                    put<DT>(a, s.out[k], s.lse[k], dim, j.v, j.top, j.sum);
                 }
-                join(j, parts - w0, st, part);
             }
-            const Column to = column(a, info, p, head, col0 + k);
-            put<DT>(a, to.token, to.head, dim, j.v, j.top, j.sum);
         }
-        __syncthreads();
+        lds_barrier(); /* the next part's columns and queries take the place of these */
     }
 }
 
-/* The parts that are left to it, joined: four dims of a column a thread. */
+/* The parts that are left to it, joined: two columns a workgroup, four dims a thread, the parts dealt
+ * out to as many threads as there are. */
+constexpr int kJoinCols = 2;
 template <int DT, int D>
 __global__ __launch_bounds__(kB) void join_rows_kernel(AttendArgs a)
 {
+    constexpr int QUADS = kJoinCols * D / 4, DEAL = kB > QUADS ? kB / QUADS : 1;
+    __shared__ f32x4 s_v[DEAL][QUADS];
+    __shared__ float2 s_st[DEAL][QUADS];
     const AttendRecord r = a.ws.records[blockIdx.x];
-    const int i = blockIdx.y * kB + threadIdx.x, k = i / (D / 4), dim = i % (D / 4) * 4;
-    if (r.parts == 0 || k >= r.cols || dim >= a.pool.head_dim) return;
+    const int deal = threadIdx.x / QUADS, i = threadIdx.x % QUADS;
+    const int k = blockIdx.y * kJoinCols + i / (D / 4), dim = i % (D / 4) * 4;
+    if (r.parts == 0 || (int)blockIdx.y * kJoinCols >= r.cols) return;
     Joined j;
     constexpr int N = 8; /* parts in flight */
-    for (int w0 = 0; w0 < r.parts; w0 += N) {
+    const int col = k < r.cols ? k : 0;
+    for (int w0 = deal; w0 < r.parts; w0 += N * DEAL) {
         float2 st[N];
         f32x4 part[N];
 #pragma unroll
         for (int w = 0; w < N; ++w) {
-            const int n = w0 + w < r.parts ? w0 + w : r.parts - 1;
+            const int n = w0 + w * DEAL < r.parts ? w0 + w * DEAL : r.parts - 1;
             const int slot = 2 * ((int)blockIdx.x + n) + (n == 0);
-            st[w] = *reinterpret_cast<const float2*>(a.ws.stats + (slot * kCols + k) * 2);
-            part[w] = *reinterpret_cast<const f32x4*>(a.ws.sums + (int64_t)(slot * kCols + k) * D + dim);
+            st[w] = *reinterpret_cast<const float2*>(a.ws.stats + (slot * kCols + col) * 2);
+            part[w] = *reinterpret_cast<const f32x4*>(a.ws.sums + (int64_t)(slot * kCols + col) * D + dim);
         }
-        join(j, r.parts - w0, st, part);
+        join(j, (r.parts - w0 + DEAL - 1) / DEAL, st, part);
     }
-    const int col = r.col0 + k, nth = divide(col, a.group);
+    s_v[deal][i] = j.v;
+    s_st[deal][i] = make_float2(j.top, j.sum);
+    __syncthreads();
+    if (deal > 0 || k >= r.cols) return;
+    Joined all;
+    float2 st[DEAL];
+    f32x4 part[DEAL];
+#pragma unroll
+    for (int w = 0; w < DEAL; ++w) {
+        st[w] = s_st[w][i];
+        part[w] = s_v[w][i];
+    }
+    join(all, DEAL, st, part);
+    const int c = r.col0 + k, nth = divide(c, a.group);
     const int token = r.start >= 0 ? r.start + nth : a.starts ? a.starts[r.row + nth] : r.row + nth;
-    put<DT>(a, token, r.head0 + col - nth * a.group.d, dim, j.v, j.top, j.sum);
+    const int head = r.head0 + c - nth * a.group.d;
+    put<DT>(a, (int64_t)token * a.out.token_stride + (int64_t)head * a.out.head_stride,
+            (int64_t)token * a.heads + head, dim, all.v, all.top, all.sum);
 }
 
 template <int DT, int D>
@@ -727,11 +774,11 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
 {
     constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT, UNIT = NW * TT;
     const size_t lds = ((sizeof(Shared<DT, D, NW, TT>) + 15) & ~(size_t)15) + ((size_t)a.rows + 1) * 8 +
-                       (size_t)a.rows * sizeof(RowInfo);
+                       (size_t)a.rows * (sizeof(RowInfo) + sizeof(Group));
     /* no more workgroups than the rows can have use for */
     const int64_t blocks = (a.group.d + kCols - 1) / kCols;
     const int64_t units = (cache_room(a.pool) + UNIT - 1) / UNIT + 1;
-    const int64_t most = ((int64_t)a.rows * a.kv_heads * blocks * units + kUnits - 1) / kUnits;
+    const int64_t most = ((int64_t)a.rows * a.kv_heads * blocks * units + Shape<DT, D>::UNITS - 1) / Shape<DT, D>::UNITS;
     const int groups = most < a.ws.groups ? (int)most : a.ws.groups;
     /* the most that can be left to be joined of one item: a launch of its own is enqueued only
      * where it may have something to do */
@@ -740,7 +787,7 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
     const int joins = parts * cols * D * 4 > kJoinBytes;
     hipError_t e = launch(attend_rows_kernel<DT, D>, groups, NW * 64, lds, stream, a, joins);
     if (e != hipSuccess || !joins) return e;
-    return launch(join_rows_kernel<DT, D>, dim3((unsigned)groups, (unsigned)(kCols * D / 4 / kB)), kB, 0,
+    return launch(join_rows_kernel<DT, D>, dim3((unsigned)groups, (unsigned)(kCols / kJoinCols)), kB, 0,
                   stream, a);
 }
 
@@ -767,7 +814,7 @@ int32_t attend_width(int32_t head_dim)
     return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512;
 }
 
-int32_t attend_groups(int32_t ncu) { return ncu; }
+int32_t attend_groups(int32_t ncu) { return 2 * ncu; }
 
 hipError_t attend_init_launch(const AttendSpace& ws, hipStream_t stream)
 {

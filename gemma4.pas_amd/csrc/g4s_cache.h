@@ -167,13 +167,14 @@ struct AttendRecord {
 
 /* Workspace of the attention: what several workgroups found for the same columns. */
 struct AttendSpace {
-    float* sums;       /* kAttendSums for each workgroup */
+    float* sums;       /* kAttendSums for each workgroup of the rows' kernel */
     float* stats;      /* kAttendStats */
     uint32_t* tickets; /* one; 0 between calls */
     AttendRecord* records; /* one: what the rows' kernel leaves to be joined */
-    int32_t groups;    /* workgroups with parts of columns in a launch at most */
+    int32_t groups;    /* workgroups of the rows' kernel at most; of the prompts' kernel half as
+                          many, with twice the space, split the tokens */
 };
-constexpr int kAttendSums = 32768, kAttendStats = 512;
+constexpr int kAttendSums = 16384, kAttendStats = 256;
 
 struct AttendArgs {
     CachePool pool;

@@ -94,6 +94,7 @@ __device__ __forceinline__ int again(int x)
     return x;
 }
 
+constexpr int kSlotSums = 2 * kAttendSums, kSlotStats = 2 * kAttendStats;
 constexpr int kJoin = 256; /* threads of a joining workgroup */
 
 template <int D, int KT>
@@ -132,7 +133,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     constexpr int THREADS = NW * 64;
     constexpr int KL = (KT * D / 16 + THREADS - 1) / THREADS; /* 16-code loads of a thread */
     constexpr int VL = (KT * D / 16 + THREADS - 1) / THREADS; /* 4 x 4-code loads */
-    static_assert(CB * D <= kAttendSums && CB * 2 <= kAttendStats, "a slot a workgroup");
+    static_assert(CB * D <= kSlotSums && CB * 2 <= kSlotStats, "a slot a workgroup");
     extern __shared__ char lds[];
     auto& s = *reinterpret_cast<Shared<D, KT>*>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -443,11 +444,11 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             continue;
         }
         const int64_t slot = (x * gridDim.x + head) * splits + part;
-        float* to = a.ws.sums + slot * kAttendSums + (int64_t)k * D;
+        float* to = a.ws.sums + slot * kSlotSums + (int64_t)k * D;
 #pragma unroll
         for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[t][i];
         if (g == 0)
-            *reinterpret_cast<float2*>(a.ws.stats + slot * kAttendStats + k * 2) =
+            *reinterpret_cast<float2*>(a.ws.stats + slot * kSlotStats + k * 2) =
                 make_float2(base, sum[t]);
     }
 }
@@ -464,8 +465,8 @@ __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int s
     const int i = blockIdx.z * kJoin + threadIdx.x, k = i / (D / 4), dim = i % (D / 4) * 4;
     if (k >= b.cols || dim >= a.pool.head_dim) return;
     const int64_t slot = (x * gridDim.x + head) * splits;
-    const float* stats = a.ws.stats + slot * kAttendStats + k * 2;
-    const float* sums = a.ws.sums + slot * kAttendSums + (int64_t)k * D + dim;
+    const float* stats = a.ws.stats + slot * kSlotStats + k * 2;
+    const float* sums = a.ws.sums + slot * kSlotSums + (int64_t)k * D + dim;
     Joined j;
     constexpr int N = 8; /* parts in flight */
     for (int w0 = 0; w0 < b.parts; w0 += N) {
@@ -474,8 +475,8 @@ __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int s
 #pragma unroll
         for (int w = 0; w < N; ++w) {
             const int64_t n = w0 + w < b.parts ? w0 + w : b.parts - 1;
-            st[w] = *reinterpret_cast<const float2*>(stats + n * kAttendStats);
-            p[w] = *reinterpret_cast<const f32x4*>(sums + n * kAttendSums);
+            st[w] = *reinterpret_cast<const float2*>(stats + n * kSlotStats);
+            p[w] = *reinterpret_cast<const f32x4*>(sums + n * kSlotSums);
         }
         join(j, b.parts - w0, st, p);
     }
@@ -490,7 +491,7 @@ hipError_t prompts_launch(const AttendArgs& a, hipStream_t stream)
     constexpr int CB = NW * NT * 16;
     const int64_t slots = (int64_t)a.tokens * a.group.d / CB + a.rows;
     const int64_t items = slots * a.kv_heads;
-    int64_t splits = a.ws.groups / items;
+    int64_t splits = a.ws.groups / 2 / items;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)slots, (unsigned)splits);
     const hipError_t e = launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64,
