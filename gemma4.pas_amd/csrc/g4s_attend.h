@@ -28,6 +28,22 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
 
+/* Bit i: whether token tile0 + shift + i is one of first .. last. */
+__device__ __forceinline__ uint64_t seen_bits(int tile0, int first, int last, int shift)
+{
+    const int lo = first - tile0, hi = last - tile0; /* as places of the tile */
+    const uint64_t from = lo <= 0 ? ~(uint64_t)0 : lo > 63 ? 0 : ~(uint64_t)0 << lo;
+    const uint64_t to = hi >= 63 ? ~(uint64_t)0 : hi < 0 ? 0 : ~(uint64_t)0 >> (63 - hi);
+    return (from & to) >> shift;
+}
+/* x where bit i is set, `other` where it is not. */
+__device__ __forceinline__ float where_bit(uint64_t bits, int i, float x, float other)
+{
+    const uint32_t w = i < 32 ? (uint32_t)bits : (uint32_t)(bits >> 32);
+    const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)w, i & 31, 1);
+    return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
+}
+
 /* Eight bf16 of a matrix operand. */
 union Frag {
     uint32_t w[4];

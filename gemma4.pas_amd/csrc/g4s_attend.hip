@@ -332,37 +332,38 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
         float top = -inf32(), sum = 0.0f;
 
-        /* steps, every NW-th of them the wave's: a tile for all rows (row -1), behind those a tile
-         * for each row that sees it */
+        /* steps, every NW-th of them the wave's: a tile for all rows, and behind those (i >= 0) a
+         * tile for each row that sees it, tile by tile */
         struct Step {
-            int tile, row, first, last; /* first and last place that is read */
+            int tile, i, row; /* row: the table that is read */
+            int first, last;  /* first and last place that is read */
         };
+        const uint32_t by_rows = several ? 0xFFFFFFFFu / (uint32_t)p.rows + 1u : 0u; /* i / rows = high(i * it) */
         auto settle = [&](Step& t) {
-            if (t.row < 0) {
-                if (t.tile < a_shared) {
-                    t.first = p.from;
-                    t.last = p.end - 1;
-                    return;
-                }
-                t.row = t.tile - a_shared;
-                t.tile = a_shared;
+            if (t.i < 0) {
+                t.row = ref;
+                t.first = p.from;
+                t.last = p.end - 1;
+                if (t.tile < a_shared) return;
+                t.i = t.tile - a_shared;
+                t.tile = a1;
+                if (!several) return;
             }
-            for (;; t.row += NW) {
-                while (t.row >= p.rows && t.tile < a1) {
-                    t.row -= p.rows;
-                    ++t.tile;
-                }
+            for (;; t.i += NW) {
+                const uint32_t q = __umulhi((uint32_t)t.i, by_rows);
+                t.tile = a_shared + (int)q;
                 if (t.tile >= a1) return;
-                t.last = __builtin_amdgcn_readfirstlane(info[lo + t.row].length - 1);
+                t.row = lo + t.i - (int)q * p.rows;
+                t.last = __builtin_amdgcn_readfirstlane(info[t.row].length - 1);
                 t.first = sees_from(a, t.last);
                 if (t.tile * TT <= t.last && t.tile * TT + TT > t.first) return;
             }
         };
         auto advance = [&](Step t) {
-            if (t.row < 0)
+            if (t.i < 0)
                 t.tile += NW;
             else
-                t.row += NW;
+                t.i += NW;
             settle(t);
             return t;
         };
@@ -373,8 +374,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
             return i < t.first ? t.first : i > t.last ? t.last : i;
         };
         auto find_page = [&](const Step& t) {
-            const int row = t.row >= 0 ? lo + t.row : ref;
-            return a.table[(int64_t)row * a.pool.max_slots + divide(token(t), a.pool.page_tokens)];
+            return a.table[(int64_t)t.row * a.pool.max_slots + divide(token(t), a.pool.page_tokens)];
         };
         const char* const keys = a.k_plane + (int64_t)head * a.pool.part_bytes;
         const char* const values = a.v_plane + (int64_t)head * a.pool.part_bytes;
@@ -439,7 +439,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
                 }
         };
 
-        Step now{a0 + wave, -1, 0, 0};
+        Step now{a0 + wave, -1, 0, 0, 0};
         settle(now);
         Step next = now;
         int buf = 0, page = 0;
@@ -508,19 +508,27 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
             if (more) load_keys(buf ^ 1);
             /* y[j] of half h: token h * 32 + (j & 4) * 4 + g * 4 + (j & 3) */
             const int tile0 = now.tile * TT;
-            const bool alone = now.row >= 0;
+            const bool alone = now.i >= 0;
             const bool partly = bad_now != 0 || tile0 < all_from || tile0 + TT - 1 > all_to || alone;
             bool nan_v = false;
             if (partly) {
-                const bool mine = !alone || nth == now.row;
+                /* (bits, as a comparison for each score would hold a mask of lanes for each) */
+                const bool mine = !alone || lo + nth == now.row;
+                uint64_t seen = seen_bits(tile0, from, place, g * 4);
+                seen = mine ? seen : 0;
 #pragma unroll
                 for (int h = 0; h < NB; ++h)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int i = h * 16 + g * 4 + j, t = tile0 + i;
-                        if (bad_now >> i & 1) sc[h][j] = nan32();
-                        if (t < from || t > place || !mine) sc[h][j] = -inf32();
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        sc[h][j] = where_bit(seen, h * 16 + j, sc[h][j], -inf32());
+                if (bad_now != 0) {
+                    const uint64_t wrong = (bad_now >> (g * 4)) & seen;
+#pragma unroll
+                    for (int h = 0; h < NB; ++h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            sc[h][j] = where_bit(wrong, h * 16 + j, nan32(), sc[h][j]);
+                }
                 if (multi) {
                     uint32_t any = 0;
 #pragma unroll

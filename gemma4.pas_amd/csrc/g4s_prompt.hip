@@ -324,14 +324,20 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             for (int t = 0; t < NT; ++t) {
                 float now = -inf32();
                 if (partly) {
+                    const uint64_t seen = seen_bits(t0, from[t], place[t], g * 4);
 #pragma unroll
                     for (int b = 0; b < TB; ++b)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int in = b * 16 + g * 4 + i, at = t0 + in;
-                            if (bad >> in & 1) sc[t][b][i] = nan32();
-                            if (at < from[t] || at > place[t]) sc[t][b][i] = -inf32();
-                        }
+                        for (int i = 0; i < 4; ++i)
+                            sc[t][b][i] = where_bit(seen, b * 16 + i, sc[t][b][i], -inf32());
+                    if (bad != 0) {
+                        const uint64_t wrong = (bad >> (g * 4)) & seen;
+#pragma unroll
+                        for (int b = 0; b < TB; ++b)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                sc[t][b][i] = where_bit(wrong, b * 16 + i, nan32(), sc[t][b][i]);
+                    }
                 }
 #pragma unroll
                 for (int b = 0; b < TB; ++b)
