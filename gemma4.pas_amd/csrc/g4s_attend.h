@@ -28,6 +28,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4_4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t u32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
 
+__device__ __forceinline__ float inf32() { return __builtin_inff(); }
+__device__ __forceinline__ float nan32() { return __builtin_nanf(""); }
+
 /* Bit i: whether token tile0 + shift + i is one of first .. last. */
 __device__ __forceinline__ uint64_t seen_bits(int tile0, int first, int last, int shift)
 {
@@ -44,15 +47,20 @@ __device__ __forceinline__ float where_bit(uint64_t bits, int i, float x, float 
     return __uint_as_float((__float_as_uint(x) & m) | (__float_as_uint(other) & ~m));
 }
 
+/* Whether a softmax moves to another base (to base two; -inf: none yet): the weights may grow to
+ * 2^kSlack before it does, as moving costs a product for every sum. */
+constexpr float kSlack = 8.0f;
+__device__ __forceinline__ bool rebase(float base, float above)
+{
+    return base == -inf32() ? above > -inf32() : above > kSlack;
+}
+
 /* Eight bf16 of a matrix operand. */
 union Frag {
     uint32_t w[4];
     bf16x8 v;
     i16x4 half; /* its first four */
 };
-
-__device__ __forceinline__ float inf32() { return __builtin_inff(); }
-__device__ __forceinline__ float nan32() { return __builtin_nanf(""); }
 
 /* Two codes of a word and their scale (a power of two) as bf16, which holds every product. */
 template <bool HI>

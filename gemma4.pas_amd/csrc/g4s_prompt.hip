@@ -181,41 +181,53 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
     const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
     f32x4 o[NT][DB];
-    float top[NT], sum[NT];
+    float base[NT], sum[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        top[t] = -inf32();
+        base[t] = -inf32();
         sum[t] = 0.0f;
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[t][i] = f32x4{0, 0, 0, 0};
     }
 
+    /* Where the tokens of a tile are, found by the first wave in three steps of a tile each, so that
+     * it waits for none of them: their pages, their scales, and both to LDS. */
     const int32_t* pages = a.table + (int64_t)row * a.pool.max_slots;
-    /* tile n's tokens: where they are, by the first lanes */
-    auto locate = [&](int n) {
-        if (tid >= 64 || n >= n1) return;
-        const int i = KT == 64 ? lane : lane & (KT - 1);
-        int t = (t_first + n) * KT + i;
+    const bool locates = wave == 0;
+    int page = 0, in_page = 0;
+    float k_scale = 0.0f, v_scale = 0.0f;
+    int64_t offset = 0;
+    uint64_t wrong = 0;
+    auto find_pages = [&](int n) {
+        if (!locates || n >= n1) return;
+        int t = (t_first + n) * KT + (lane & (KT - 1));
         t = t < from0 ? from0 : t >= end0 ? end0 - 1 : t;
         const int slot = divide(t, a.pool.page_tokens);
-        const int in = t - slot * a.pool.page_tokens.d;
-        int page = pages[slot];
+        in_page = t - slot * a.pool.page_tokens.d;
+        page = pages[slot];
+    };
+    auto find_scales = [&](int n) {
+        if (!locates || n >= n1) return;
         const bool ok = page >= 0 && page < a.pool.n_pages;
-        if (!ok) page = 0;
-        const int64_t off = cache_offset(a.pool, page, in, head);
-        const int in_block = in - divide(in, a.pool.scale_tokens) * a.pool.scale_tokens.d;
-        const int64_t sc = off - (int64_t)in_block * a.pool.token_bytes + a.pool.head_dim;
-        const uint64_t bad = __ballot(!ok);
-        const int b = n % 3;
-        s.offset[b][i] = off;
-        s.scale[b][0][i] = *reinterpret_cast<const float*>(a.k_plane + sc);
-        s.scale[b][1][i] = *reinterpret_cast<const float*>(a.v_plane + sc);
-        if (lane == 0) s.bad[b] = bad;
+        offset = cache_offset(a.pool, ok ? page : 0, in_page, head);
+        const int in_block = in_page - divide(in_page, a.pool.scale_tokens) * a.pool.scale_tokens.d;
+        const int64_t at = offset - (int64_t)in_block * a.pool.token_bytes + a.pool.head_dim;
+        k_scale = *reinterpret_cast<const float*>(a.k_plane + at);
+        v_scale = *reinterpret_cast<const float*>(a.v_plane + at);
+        wrong = __ballot(!ok);
+    };
+    auto keep_places = [&](int n) {
+        if (!locates || n >= n1) return;
+        const int b = n % 3, i = lane & (KT - 1);
+        s.offset[b][i] = offset;
+        s.scale[b][0][i] = k_scale;
+        s.scale[b][1][i] = v_scale;
+        if (lane == 0) s.bad[b] = wrong;
     };
     uint32_t kw[KL][4], vw[VL][4];
     auto load = [&](int n) {
         const int b = n % 3;
-        const int tid = again(threadIdx.x);
+        const int tid = D > 128 ? again(threadIdx.x) : (int)threadIdx.x;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
             const int u = tid + i * THREADS, t = u / (D / 16), d0 = u % (D / 16) * 16;
@@ -239,7 +251,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     };
     auto store = [&](int n) {
         const int b = n % 3, to = n & 1;
-        const int tid = again(threadIdx.x);
+        const int tid = D > 128 ? again(threadIdx.x) : (int)threadIdx.x;
         uint32_t any = 0;
 #pragma unroll
         for (int i = 0; i < KL; ++i) {
@@ -286,17 +298,23 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     };
 
     if (tid < 2) s.nan[tid] = 0;
-    locate(n0);
-    locate(n0 + 1);
-    __syncthreads();
+    find_pages(n0);
+    find_scales(n0);
+    find_pages(n0 + 1);
+    keep_places(n0);
+    find_scales(n0 + 1);
+    find_pages(n0 + 2);
+    keep_places(n0 + 1);
+    lds_barrier();
     if (n0 < n1) {
         load(n0);
         store(n0);
     }
-    __syncthreads();
+    lds_barrier();
     for (int n = n0; n < n1; ++n) {
         if (n + 1 < n1) load(n + 1);
-        locate(n + 2);
+        find_scales(n + 2);
+        find_pages(n + 3);
         const int t0 = (t_first + n) * KT;
         const int buf = n & 1;
         if (busy && t0 <= w_last && t0 + KT > any_from) {
@@ -322,7 +340,6 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             Frag pw[NT][TB / 2][PP];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float now = -inf32();
                 if (partly) {
                     const uint64_t seen = seen_bits(t0, from[t], place[t], g * 4);
 #pragma unroll
@@ -331,50 +348,53 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                         for (int i = 0; i < 4; ++i)
                             sc[t][b][i] = where_bit(seen, b * 16 + i, sc[t][b][i], -inf32());
                     if (bad != 0) {
-                        const uint64_t wrong = (bad >> (g * 4)) & seen;
+                        const uint64_t none = (bad >> (g * 4)) & seen;
 #pragma unroll
                         for (int b = 0; b < TB; ++b)
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
-                                sc[t][b][i] = where_bit(wrong, b * 16 + i, nan32(), sc[t][b][i]);
+                                sc[t][b][i] = where_bit(none, b * 16 + i, nan32(), sc[t][b][i]);
                     }
                 }
+                /* exponents against the base that holds, and their largest */
+                float y[TB * 4], now = -inf32();
+                const float old = base[t] == -inf32() ? 0.0f : base[t];
 #pragma unroll
-                for (int b = 0; b < TB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now = fmaxf(now, sc[t][b][i]);
+                for (int i = 0; i < TB * 4; ++i) {
+                    y[i] = __builtin_fmaf(sc[t][i >> 2][i & 3], c, -old);
+                    now = fmaxf(now, y[i]);
+                }
                 now = fmaxf(now, __shfl_xor(now, 16));
                 now = fmaxf(now, __shfl_xor(now, 32));
-                now = fmaxf(now, top[t]);
-                if (__any(now > top[t])) {
-                    const float keep = now > top[t] ? __builtin_amdgcn_exp2f((top[t] - now) * c) : 1.0f;
+                if (__any(rebase(base[t], now))) {
+                    const bool moves = rebase(base[t], now);
+                    const float keep = moves && base[t] != -inf32() ? __builtin_amdgcn_exp2f(-now) : 1.0f;
+                    if (moves) base[t] = old + now;
                     sum[t] *= keep;
 #pragma unroll
                     for (int i = 0; i < DB; ++i) o[t][i] *= keep;
-                    top[t] = now;
+                    const float b = base[t] == -inf32() ? 0.0f : base[t];
+#pragma unroll
+                    for (int i = 0; i < TB * 4; ++i) y[i] = __builtin_fmaf(sc[t][i >> 2][i & 3], c, -b);
                 }
-                const float base = top[t] == -inf32() ? 0.0f : top[t] * c;
 #pragma unroll
-                for (int b = 0; b < TB; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; i += 2) {
-                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i], c, -base));
-                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][b][i + 1], c, -base));
-                        sum[t] += e0 + e1;
-                        Frag* f = pw[t][b >> 1];
-                        const int w = (b & 1) * 2 + (i >> 1);
-                        f[0].w[w] = pack_bf16(e0, e1);
-                        if constexpr (PP == 2)
-                            f[1].w[w] = pack_bf16(e0 - __uint_as_float(f[0].w[w] << 16),
-                                                  e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
-                    }
+                for (int i = 0; i < TB * 4; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(y[i]), e1 = __builtin_amdgcn_exp2f(y[i + 1]);
+                    sum[t] += e0 + e1;
+                    Frag* f = pw[t][i >> 3];
+                    const int w = (i & 7) >> 1;
+                    f[0].w[w] = pack_bf16(e0, e1);
+                    if constexpr (PP == 2)
+                        f[1].w[w] = pack_bf16(e0 - __uint_as_float(f[0].w[w] << 16),
+                                              e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
+                }
             }
             /* value_piece(i * 16 + m, h * 4 + g) is that of m and g, exchanged by 2 i and 4 h: few
              * addresses for all */
             const char* const v0 = reinterpret_cast<const char*>(&s.v[buf][m][0]);
             const int piece = value_piece<KT>(m, g);
             auto value = [&](int i, int h) {
-                const int p = piece ^ ((h * 4) ^ (i * 2)) & (KT / 8 - 1);
+                const int p = piece ^ (((h * 4) ^ (i * 2)) & (KT / 8 - 1));
                 Frag f;
                 f.v = *reinterpret_cast<const bf16x8*>(v0 + p * 16 + i * 16 * KT * 2);
                 return f;
@@ -430,7 +450,8 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             }
         }
         if (n + 1 < n1) store(n + 1);
-        __syncthreads();
+        keep_places(n + 2);
+        lds_barrier();
     }
 
     /* what the workgroup found */
@@ -440,13 +461,12 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
         sum[t] += __shfl_xor(sum[t], 32);
         const int k = (wave * NT + t) * 16 + m;
         if (k >= cols) continue;
-        const float base = top[t] == -inf32() ? top[t] : top[t] * c;
         if (parts == 1) {
             const Column at = column(a, r, head, col0 + k);
             const float inv = 1.0f / sum[t];
 #pragma unroll
             for (int i = 0; i < DB; ++i) put<DT>(a, r, at, i * 16 + g * 4, o[t][i] * inv);
-            if (g == 0) put_lse(a, r, at, base, sum[t]);
+            if (g == 0) put_lse(a, r, at, base[t], sum[t]);
             continue;
         }
         const int64_t slot = (x * gridDim.x + head) * splits + part;
@@ -455,7 +475,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
         for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[t][i];
         if (g == 0)
             *reinterpret_cast<float2*>(a.ws.stats + slot * kSlotStats + k * 2) =
-                make_float2(base, sum[t]);
+                make_float2(base[t], sum[t]);
     }
 }
 
@@ -512,9 +532,9 @@ hipError_t by_width(const AttendArgs& a, hipStream_t stream)
 {
     constexpr bool F32 = DT == G4S_DTYPE_F32;
     switch (attend_width(a.pool.head_dim)) {
-    case 64: return prompts_launch<DT, 64, 8, F32 ? 1 : 2, 64>(a, stream);
+    case 64: return prompts_launch<DT, 64, 4, F32 ? 1 : 2, 64>(a, stream);
     case 128: return prompts_launch<DT, 128, 8, F32 ? 1 : 2, 64>(a, stream);
-    case 256: return prompts_launch<DT, 256, F32 ? 8 : 4, F32 ? 1 : 2, 64>(a, stream);
+    case 256: return prompts_launch<DT, 256, 8, 1, 64>(a, stream);
     default: return prompts_launch<DT, 512, 4, 1, 32>(a, stream);
     }
 }
