@@ -31,6 +31,25 @@ typedef uint32_t u32x2_4 __attribute__((ext_vector_type(2), aligned(4)));
 __device__ __forceinline__ float inf32() { return __builtin_inff(); }
 __device__ __forceinline__ float nan32() { return __builtin_nanf(""); }
 
+/* The largest, and the sum, of a column's four lanes (l, l + 16, l + 32, l + 48), in each of them: rows
+ * of lanes are exchanged in registers, a shuffle through LDS takes ten times as long. */
+__device__ __forceinline__ float column_max(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1])));
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float column_sum(float x)
+{
+    const uint32_t u = __float_as_uint(x);
+    const auto a = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t v = __float_as_uint(__uint_as_float(a[0]) + __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 /* Bit i: whether token tile0 + shift + i is one of first .. last. */
 __device__ __forceinline__ uint64_t seen_bits(int tile0, int first, int last, int shift)
 {

@@ -97,14 +97,14 @@ __device__ __forceinline__ int again(int x)
 constexpr int kSlotSums = 2 * kAttendSums, kSlotStats = 2 * kAttendStats;
 constexpr int kJoin = 256; /* threads of a joining workgroup */
 
-template <int D, int KT>
+template <int D, int KT, int NV>
 struct Shared {
     alignas(16) uint16_t k[2][KT][D + 8];
-    alignas(16) uint16_t v[2][D][KT];
+    alignas(16) uint16_t v[NV][D][KT];
     int64_t offset[3][KT];
     float scale[3][2][KT];
     uint64_t bad[3];
-    int nan[2];
+    int nan; /* whether any value so far was one */
 };
 
 /* `steps` reads of a matrix operand from LDS and `each` products with it, as the compiler is to lay
@@ -131,11 +131,13 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     constexpr int CB = NW * NT * 16;
     constexpr int KS = D / 32, DB = D / 16, TB = KT / 16;
     constexpr int THREADS = NW * 64;
+    constexpr bool LATE = D <= 128; /* (where LDS holds a third tile of values) */
+    constexpr int NV = LATE ? 3 : 2;
     constexpr int KL = (KT * D / 16 + THREADS - 1) / THREADS; /* 16-code loads of a thread */
     constexpr int VL = (KT * D / 16 + THREADS - 1) / THREADS; /* 4 x 4-code loads */
     static_assert(CB * D <= kSlotSums && CB * 2 <= kSlotStats, "a slot a workgroup");
     extern __shared__ char lds[];
-    auto& s = *reinterpret_cast<Shared<D, KT>*>(lds);
+    auto& s = *reinterpret_cast<Shared<D, KT, NV>*>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int m = lane & 15, g = lane >> 4;
 
@@ -290,14 +292,84 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int dim = d0 + j, p = value_piece<KT>(dim, quad >> 1);
-                    *reinterpret_cast<uint2*>(&s.v[to][dim][p * 8 + (quad & 1) * 4]) = w[j];
+                    *reinterpret_cast<uint2*>(&s.v[n % NV][dim][p * 8 + (quad & 1) * 4]) = w[j];
                 }
             }
         }
-        if (__any(any != 0) && lane == 0) s.nan[to] = 1;
+        if (__any(any != 0) && lane == 0) s.nan = 1;
     };
 
-    if (tid < 2) s.nan[tid] = 0;
+    /* the sums of tile n's values; `nan`: some of them may be NaN, and not all queries see all of them */
+    Frag pw[NT][TB / 2][PP];
+    auto add_values = [&](int n, bool nan_v) {
+        /* value_piece(i * 16 + m, h * 4 + g) is that of m and g, exchanged by 2 i and 4 h: few
+         * addresses for all */
+        const char* const v0 = reinterpret_cast<const char*>(&s.v[n % NV][m][0]);
+        const int piece = value_piece<KT>(m, g);
+        auto value = [&](int i, int h) {
+            const int p = piece ^ (((h * 4) ^ (i * 2)) & (KT / 8 - 1));
+            Frag f;
+            f.v = *reinterpret_cast<const bf16x8*>(v0 + p * 16 + i * 16 * KT * 2);
+            return f;
+        };
+        if (!nan_v) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int h = 0; h < TB / 2; ++h) {
+                    const Frag f = value(i, h);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int p = PP - 1; p >= 0; --p)
+                            o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
+                }
+            lay_out<DB * TB / 2, NT * PP>();
+        } else {
+            /* a NaN that some queries see and others do not (0 times NaN is NaN): the
+             * products go without it, and whoever sees one, counted by a product too,
+             * gets NaN */
+#pragma unroll
+            for (int i = 0; i < DB; ++i)
+#pragma unroll
+                for (int h = 0; h < TB / 2; ++h) {
+                    Frag f = value(i, h), is;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        /* (an exponent of ones carries into the sign's bit) */
+                        const uint32_t nan = ((((f.w[w] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu;
+                        f.w[w] &= ~nan;
+                        is.w[w] = nan & 0x3F803F80u;
+                    }
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        Frag see; /* 1 for the tokens that the column sees */
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            const int at = (t_first + n) * KT + h * 32 + (w & 2) * 8 + g * 4 + (w & 1) * 2;
+                            see.w[w] = (at >= from[t] && at <= place[t] ? 0x3F80u : 0u) |
+                                       (at + 1 >= from[t] && at + 1 <= place[t] ? 0x3F800000u : 0u);
+                        }
+                        const f32x4 e = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            is.v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            o[t][i][j] = nan_where(o[t][i][j], e[j]);
+#pragma unroll
+                        for (int p = PP - 1; p >= 0; --p)
+                            o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
+                    }
+                }
+        }
+    };
+    /* Half of the waves add a tile's values while the others, on the same SIMDs, multiply the next
+     * tile's keys, and the other way round: matrix products of one beside the exponentials of the
+     * other. */
+    const bool late = LATE && wave >= NW / 2;
+    int before = -1; /* a late wave's tile whose values are still to be added */
+    bool before_nan = false;
+
+    if (tid == 0) s.nan = 0;
     find_pages(n0);
     find_scales(n0);
     find_pages(n0 + 1);
@@ -317,6 +389,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
         find_pages(n + 3);
         const int t0 = (t_first + n) * KT;
         const int buf = n & 1;
+        if (before >= 0) {
+            add_values(before, before_nan);
+            before = -1;
+        }
         if (busy && t0 <= w_last && t0 + KT > any_from) {
             f32x4 sc[NT][TB];
 #pragma unroll
@@ -336,8 +412,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             lay_out<TB * KS, NT * QP>();
             const uint64_t bad = s.bad[n % 3];
             const bool partly = bad != 0 || t0 < all_from || t0 + KT - 1 > w_first;
-            const bool nan_v = partly && s.nan[buf] != 0;
-            Frag pw[NT][TB / 2][PP];
+            const bool nan_v = partly && s.nan != 0;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 if (partly) {
@@ -364,8 +439,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                     y[i] = __builtin_fmaf(sc[t][i >> 2][i & 3], c, -old);
                     now = fmaxf(now, y[i]);
                 }
-                now = fmaxf(now, __shfl_xor(now, 16));
-                now = fmaxf(now, __shfl_xor(now, 32));
+                now = column_max(now);
                 if (__any(rebase(base[t], now))) {
                     const bool moves = rebase(base[t], now);
                     const float keep = moves && base[t] != -inf32() ? __builtin_amdgcn_exp2f(-now) : 1.0f;
@@ -389,76 +463,23 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                                               e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u));
                 }
             }
-            /* value_piece(i * 16 + m, h * 4 + g) is that of m and g, exchanged by 2 i and 4 h: few
-             * addresses for all */
-            const char* const v0 = reinterpret_cast<const char*>(&s.v[buf][m][0]);
-            const int piece = value_piece<KT>(m, g);
-            auto value = [&](int i, int h) {
-                const int p = piece ^ (((h * 4) ^ (i * 2)) & (KT / 8 - 1));
-                Frag f;
-                f.v = *reinterpret_cast<const bf16x8*>(v0 + p * 16 + i * 16 * KT * 2);
-                return f;
-            };
-            if (!nan_v) {
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int h = 0; h < TB / 2; ++h) {
-                        const Frag f = value(i, h);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int p = PP - 1; p >= 0; --p)
-                                o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
-                    }
-                lay_out<DB * TB / 2, NT * PP>();
+            if (late) {
+                before = n;
+                before_nan = nan_v;
             } else {
-                /* a NaN that some queries see and others do not (0 times NaN is NaN): the
-                 * products go without it, and whoever sees one, counted by a product too,
-                 * gets NaN */
-#pragma unroll
-                for (int i = 0; i < DB; ++i)
-#pragma unroll
-                    for (int h = 0; h < TB / 2; ++h) {
-                        Frag f = value(i, h), is;
-#pragma unroll
-                        for (int w = 0; w < 4; ++w) {
-                            /* (an exponent of ones carries into the sign's bit) */
-                            const uint32_t nan = ((((f.w[w] & 0x7F807F80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xFFFFu;
-                            f.w[w] &= ~nan;
-                            is.w[w] = nan & 0x3F803F80u;
-                        }
-#pragma unroll
-                        for (int t = 0; t < NT; ++t) {
-                            Frag see; /* 1 for the tokens that the column sees */
-#pragma unroll
-                            for (int w = 0; w < 4; ++w) {
-                                const int at = t0 + h * 32 + (w & 2) * 8 + g * 4 + (w & 1) * 2;
-                                see.w[w] = (at >= from[t] && at <= place[t] ? 0x3F80u : 0u) |
-                                           (at + 1 >= from[t] && at + 1 <= place[t] ? 0x3F800000u : 0u);
-                            }
-                            const f32x4 e = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                                is.v, see.v, f32x4{0, 0, 0, 0}, 0, 0, 0);
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                o[t][i][j] = nan_where(o[t][i][j], e[j]);
-#pragma unroll
-                            for (int p = PP - 1; p >= 0; --p)
-                                o[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.v, pw[t][h][p].v, o[t][i], 0, 0, 0);
-                        }
-                    }
+                add_values(n, nan_v);
             }
         }
         if (n + 1 < n1) store(n + 1);
         keep_places(n + 2);
         lds_barrier();
     }
+    if (before >= 0) add_values(before, before_nan);
 
     /* what the workgroup found */
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        sum[t] += __shfl_xor(sum[t], 16);
-        sum[t] += __shfl_xor(sum[t], 32);
+        sum[t] = column_sum(sum[t]);
         const int k = (wave * NT + t) * 16 + m;
         if (k >= cols) continue;
         if (parts == 1) {
@@ -521,7 +542,7 @@ hipError_t prompts_launch(const AttendArgs& a, hipStream_t stream)
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)slots, (unsigned)splits);
     const hipError_t e = launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64,
-                                sizeof(Shared<D, KT>), stream, a, (int)splits);
+                                sizeof(Shared<D, KT, (D <= 128 ? 3 : 2)>), stream, a, (int)splits);
     if (e != hipSuccess || splits == 1) return e;
     const dim3 join((unsigned)a.kv_heads, (unsigned)slots, (unsigned)(CB * D / 4 / kJoin));
     return launch(join_prompts_kernel<DT, D, CB, KT>, join, kJoin, 0, stream, a, (int)splits);
