@@ -72,7 +72,7 @@ __device__ __forceinline__ Group find_group(const AttendArgs& a, const RowInfo* 
         if (p.rows > 1) return p;
     }
     const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
-    p.rows = is_prompt(r.count, a.group.d) ? 0 : -r.count;
+    p.rows = is_prompt(r.count, a.group.d, a.few) ? 0 : -r.count;
     p.start = r.start;
     p.end = r.length;
     p.from = sees_from(a, r.length - r.count);

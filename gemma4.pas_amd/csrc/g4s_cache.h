@@ -190,6 +190,7 @@ struct AttendArgs {
     int32_t window;
     int32_t heads, kv_heads;
     Divisor group;
+    int32_t few; /* kFewCols, or 0: all rows are prompts */
     AttendSpace ws;
 };
 
@@ -199,12 +200,12 @@ hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream)
 hipError_t attend_rows_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t attend_prompts_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 
-/* Rows with more than one token and more than kFewCols columns (tokens x heads of a key head)
+/* Rows with more than one token and more than `few` columns (tokens x heads of a key head)
  * are the prompts' kernel's, the others the rows' kernel's. */
 constexpr int kFewCols = 16;
-G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group)
+G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group, int32_t few)
 {
-    return count > 1 && (int64_t)count * group > kFewCols;
+    return (int64_t)count * group > few && (count > 1 || few == 0);
 }
 
 int32_t attend_groups(int32_t ncu);

@@ -383,9 +383,13 @@ G4S_API int g4s_cache_attend(g4s_cache* h, const g4s_page_state* state, int32_t 
     a.kv_heads = c.kv_heads;
     a.group = g4s::divisor(c.heads / c.kv_heads);
     a.ws = h->ws;
-    /* rows of one token each have no prompts among them */
-    hipError_t e = g4s::attend_rows_launch(a, dtype, h->stream);
-    if (e == hipSuccess && d_starts) e = g4s::attend_prompts_launch(a, dtype, h->stream);
+    /* Which rows have how many tokens is known on the device alone, so a call of ragged ones
+     * enqueues both kernels, but for those that cannot have prompts and the one row that is one. */
+    const bool prompts = d_starts && (int64_t)tokens * a.group.d > g4s::kFewCols;
+    a.few = prompts && rows == 1 ? 0 : g4s::kFewCols;
+    hipError_t e = hipSuccess;
+    if (a.few > 0) e = g4s::attend_rows_launch(a, dtype, h->stream);
+    if (e == hipSuccess && prompts) e = g4s::attend_prompts_launch(a, dtype, h->stream);
     if (e != hipSuccess) return fail(h, G4S_ERR_HIP, "attention launch: %s", hipGetErrorString(e));
     return G4S_OK;
 }

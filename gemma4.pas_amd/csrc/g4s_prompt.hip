@@ -47,7 +47,7 @@ __device__ __forceinline__ Block find_block(const AttendArgs& a, int64_t x, int 
     b.r = row_tokens(a.starts, a.lengths, b.row, a.tokens, cache_room(a.pool));
     const int64_t block = x - share_begin(a.starts, b.row, a.group.d, unit, 1);
     const int64_t all = (int64_t)b.r.count * a.group.d;
-    if (!is_prompt(b.r.count, a.group.d) || block < 0 || block * unit >= all) return b;
+    if (!is_prompt(b.r.count, a.group.d, a.few) || block < 0 || block * unit >= all) return b;
     b.col0 = (int)(block * unit);
     b.cols = all - b.col0 < unit ? (int)(all - b.col0) : unit;
     const int before = b.r.length - b.r.count;
@@ -134,7 +134,10 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     constexpr bool LATE = D <= 128; /* (where LDS holds a third tile of values) */
     constexpr int NV = LATE ? 3 : 2;
     constexpr int KL = (KT * D / 16 + THREADS - 1) / THREADS; /* 16-code loads of a thread */
-    constexpr int VL = (KT * D / 16 + THREADS - 1) / THREADS; /* 4 x 4-code loads */
+    /* values: units of 8 tokens x 4 codes, or of 4 where that would leave threads without any */
+    constexpr int VT = KT * D / 32 >= THREADS ? 8 : 4;
+    constexpr int VU = KT * D / 4 / VT;
+    constexpr int VL = (VU + THREADS - 1) / THREADS;
     static_assert(CB * D <= kSlotSums && CB * 2 <= kSlotStats, "a slot a workgroup");
     extern __shared__ char lds[];
     auto& s = *reinterpret_cast<Shared<D, KT, NV>*>(lds);
@@ -226,7 +229,9 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
         s.scale[b][1][i] = v_scale;
         if (lane == 0) s.bad[b] = wrong;
     };
-    uint32_t kw[KL][4], vw[VL][4];
+    /* a unit's first token */
+    auto unit_token = [](int i) { return VT == 8 ? i / 4 * 32 + i % 4 * 4 : i * 4; };
+    uint32_t kw[KL][4], vw[VL][VT];
     auto load = [&](int n) {
         const int b = n % 3;
         const int tid = D > 128 ? again(threadIdx.x) : (int)threadIdx.x;
@@ -242,12 +247,13 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
         }
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-            const int u = tid + i * THREADS, t = u / (D / 4) * 4, d0 = u % (D / 4) * 4;
-            if (KT * D / 16 % THREADS == 0 || u < KT * D / 16) {
+            const int u = tid + i * THREADS, d0 = u % (D / 4) * 4;
+            if (VU % THREADS == 0 || u < VU) {
+                const int64_t* at = &s.offset[b][unit_token(u / (D / 4))];
+                const char* from = a.v_plane + (d0 < a.pool.head_dim ? d0 : 0);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    vw[i][j] = *reinterpret_cast<const uint32_t*>(
-                        a.v_plane + s.offset[b][t + j] + (d0 < a.pool.head_dim ? d0 : 0));
+                for (int j = 0; j < VT; ++j)
+                    vw[i][j] = *reinterpret_cast<const uint32_t*>(from + at[(j & 4) * 4 + (j & 3)]);
             }
         }
     };
@@ -270,29 +276,26 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                 at[1] = hi;
             }
         }
+        /* piece 4 h + g of a dim: tokens 4 g .. 4 g + 3 of 32 h and those 16 behind them, in the order
+         * that a lane of the second product takes them */
 #pragma unroll
         for (int i = 0; i < VL; ++i) {
-            const int u = tid + i * THREADS, t = u / (D / 4) * 4, d0 = u % (D / 4) * 4;
-            if (KT * D / 16 % THREADS == 0 || u < KT * D / 16) {
-                uint32_t lo[4], hi[4];
+            const int u = tid + i * THREADS, d0 = u % (D / 4) * 4, t = unit_token(u / (D / 4));
+            if (VU % THREADS == 0 || u < VU) {
+                float vs[VT];
+                Frag f[4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float vs = s.scale[b][1][t + j];
-                    lo[j] = widen2<false>(vw[i][j], vs);
-                    hi[j] = widen2<true>(vw[i][j], vs);
+                for (int j = 0; j < VT; ++j) {
+                    vs[j] = s.scale[b][1][t + (j & 4) * 4 + (j & 3)];
                     any |= nan_codes(vw[i][j]);
                 }
-                /* tokens 4 k .. 4 k + 3 of 32 (k = 0 .. 7) at quads 2 (k % 4) + k / 4: in the order that a
-                 * lane of the second product takes them */
-                const int k = t / 4 % 8, quad = t / 32 * 8 + (k & 3) * 2 + (k >> 2);
-                const uint2 w[4] = {make_uint2(lows(lo[0], lo[1]), lows(lo[2], lo[3])),
-                                    make_uint2(highs(lo[0], lo[1]), highs(lo[2], lo[3])),
-                                    make_uint2(lows(hi[0], hi[1]), lows(hi[2], hi[3])),
-                                    make_uint2(highs(hi[0], hi[1]), highs(hi[2], hi[3]))};
+                value_frags<VT>(vw[i], vs, f);
+                const int piece = t / 32 * 4 + t % 16 / 4;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int dim = d0 + j, p = value_piece<KT>(dim, quad >> 1);
-                    *reinterpret_cast<uint2*>(&s.v[n % NV][dim][p * 8 + (quad & 1) * 4]) = w[j];
+                    uint16_t* to = &s.v[n % NV][d0 + j][value_piece<KT>(d0 + j, piece) * 8 + t % 32 / 16 * 4];
+                    if constexpr (VT == 8) *reinterpret_cast<bf16x8*>(to) = f[j].v;
+                    else *reinterpret_cast<uint2*>(to) = make_uint2(f[j].w[0], f[j].w[1]);
                 }
             }
         }
