@@ -97,15 +97,24 @@ __device__ __forceinline__ int again(int x)
 constexpr int kSlotSums = 2 * kAttendSums, kSlotStats = 2 * kAttendStats;
 constexpr int kJoin = 256; /* threads of a joining workgroup */
 
-template <int D, int KT, int NV>
+template <int D, int NW, int KT, int NV, int HALVES>
 struct Shared {
     alignas(16) uint16_t k[2][KT][D + 8];
     alignas(16) uint16_t v[NV][D][KT];
+    f32x4 part[HALVES == 2 ? NW : 0][KT / 16][64]; /* products of keys with half of the dims */
     int64_t offset[3][KT];
     float scale[3][2][KT];
     uint64_t bad[3];
     int nan; /* whether any value so far was one */
 };
+
+/* Waves that share columns, each with a part of their dims: one wave's registers do not hold the
+ * queries and sums of 512. */
+template <int D>
+constexpr int kHalves = D > 256 ? 2 : 1;
+/* LDS holds a third tile of values, so that waves may be a phase apart. */
+template <int D>
+constexpr bool kLate = D <= 128;
 
 /* `steps` reads of a matrix operand from LDS and `each` products with it, as the compiler is to lay
  * them out: kAhead reads ahead of their products.  Left to itself it reads everything first
@@ -124,14 +133,15 @@ __device__ __forceinline__ void lay_out()
 }
 
 template <int DT, int D, int NW, int NT, int KT>
-__global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a, int splits)
+__global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_kernel(AttendArgs a, int splits)
 {
     constexpr int QP = DT == G4S_DTYPE_F32 ? 3 : 1;
     constexpr int PP = DT == G4S_DTYPE_F32 ? 2 : 1;
-    constexpr int CB = NW * NT * 16;
-    constexpr int KS = D / 32, DB = D / 16, TB = KT / 16;
+    constexpr int HALVES = kHalves<D>, COLW = NW / HALVES, DW = D / HALVES; /* a wave's dims */
+    constexpr int CB = COLW * NT * 16;
+    constexpr int KS = DW / 32, DB = DW / 16, TB = KT / 16;
     constexpr int THREADS = NW * 64;
-    constexpr bool LATE = D <= 128; /* (where LDS holds a third tile of values) */
+    constexpr bool LATE = kLate<D>;
     constexpr int NV = LATE ? 3 : 2;
     constexpr int KL = (KT * D / 16 + THREADS - 1) / THREADS; /* 16-code loads of a thread */
     /* values: units of 8 tokens x 4 codes, or of 4 where that would leave threads without any */
@@ -140,8 +150,9 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     constexpr int VL = (VU + THREADS - 1) / THREADS;
     static_assert(CB * D <= kSlotSums && CB * 2 <= kSlotStats, "a slot a workgroup");
     extern __shared__ char lds[];
-    auto& s = *reinterpret_cast<Shared<D, KT, NV>*>(lds);
+    auto& s = *reinterpret_cast<Shared<D, NW, KT, NV, HALVES>*>(lds);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int colw = wave % COLW, dim0 = wave / COLW * DW;
     const int m = lane & 15, g = lane >> 4;
 
     /* heads side by side; the last columns of a row, which see most, first */
@@ -160,7 +171,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     Frag q[NT][KS][QP];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        const int c = (wave * NT + t) * 16 + m;
+        const int c = (colw * NT + t) * 16 + m;
         const bool has = c < cols;
         const Column at = column(a, r, head, col0 + (has ? c : 0));
         place[t] = at.place;
@@ -169,14 +180,14 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                                      (int64_t)at.head * a.q.head_stride) * Elem<DT>::SIZE;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
-            const int d0 = k * 32 + g * 8;
+            const int d0 = dim0 + k * 32 + g * 8;
             const bool in = d0 < a.pool.head_dim;
             load_query<DT>(q0 + (int64_t)(in ? d0 : 0) * Elem<DT>::SIZE, has && in, a.scale < 0.0f,
                            q[t][k]);
         }
     }
     /* places that any and that all of the wave's queries see */
-    const int wcol0 = wave * NT * 16;
+    const int wcol0 = colw * NT * 16;
     const int wcol1 = wcol0 + NT * 16 < cols ? wcol0 + NT * 16 : cols;
     const bool busy = wcol0 < cols;
     const int w_first = r.length - r.count + divide(col0 + (busy ? wcol0 : 0), a.group);
@@ -307,7 +318,7 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
     auto add_values = [&](int n, bool nan_v) {
         /* value_piece(i * 16 + m, h * 4 + g) is that of m and g, exchanged by 2 i and 4 h: few
          * addresses for all */
-        const char* const v0 = reinterpret_cast<const char*>(&s.v[n % NV][m][0]);
+        const char* const v0 = reinterpret_cast<const char*>(&s.v[n % NV][dim0 + m][0]);
         const int piece = value_piece<KT>(m, g);
         auto value = [&](int i, int h) {
             const int p = piece ^ (((h * 4) ^ (i * 2)) & (KT / 8 - 1));
@@ -396,15 +407,16 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
             add_values(before, before_nan);
             before = -1;
         }
-        if (busy && t0 <= w_last && t0 + KT > any_from) {
-            f32x4 sc[NT][TB];
+        const bool sees = busy && t0 <= w_last && t0 + KT > any_from;
+        f32x4 sc[NT][TB];
+        if (sees) {
 #pragma unroll
             for (int b = 0; b < TB; ++b) {
 #pragma unroll
                 for (int t = 0; t < NT; ++t) sc[t][b] = f32x4{0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < KS; ++k) {
-                    const bf16x8 f = *reinterpret_cast<const bf16x8*>(&s.k[buf][b * 16 + m][k * 32 + g * 8]);
+                    const bf16x8 f = *reinterpret_cast<const bf16x8*>(&s.k[buf][b * 16 + m][dim0 + k * 32 + g * 8]);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -413,6 +425,18 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
                 }
             }
             lay_out<TB * KS, NT * QP>();
+        }
+        if constexpr (HALVES == 2) {
+            static_assert(NT == 1, "one block of columns a wave");
+            if (sees)
+#pragma unroll
+                for (int b = 0; b < TB; ++b) s.part[wave][b][lane] = sc[0][b];
+            lds_barrier();
+            if (sees)
+#pragma unroll
+                for (int b = 0; b < TB; ++b) sc[0][b] += s.part[wave ^ COLW][b][lane];
+        }
+        if (sees) {
             const uint64_t bad = s.bad[n % 3];
             const bool partly = bad != 0 || t0 < all_from || t0 + KT - 1 > w_first;
             const bool nan_v = partly && s.nan != 0;
@@ -483,21 +507,21 @@ __global__ __launch_bounds__(NW * 64, 1) void attend_prompts_kernel(AttendArgs a
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         sum[t] = column_sum(sum[t]);
-        const int k = (wave * NT + t) * 16 + m;
+        const int k = (colw * NT + t) * 16 + m;
         if (k >= cols) continue;
         if (parts == 1) {
             const Column at = column(a, r, head, col0 + k);
             const float inv = 1.0f / sum[t];
 #pragma unroll
-            for (int i = 0; i < DB; ++i) put<DT>(a, r, at, i * 16 + g * 4, o[t][i] * inv);
-            if (g == 0) put_lse(a, r, at, base[t], sum[t]);
+            for (int i = 0; i < DB; ++i) put<DT>(a, r, at, dim0 + i * 16 + g * 4, o[t][i] * inv);
+            if (g == 0 && dim0 == 0) put_lse(a, r, at, base[t], sum[t]);
             continue;
         }
         const int64_t slot = (x * gridDim.x + head) * splits + part;
         float* to = a.ws.sums + slot * kSlotSums + (int64_t)k * D;
 #pragma unroll
-        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + i * 16 + g * 4) = o[t][i];
-        if (g == 0)
+        for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + dim0 + i * 16 + g * 4) = o[t][i];
+        if (g == 0 && dim0 == 0)
             *reinterpret_cast<float2*>(a.ws.stats + slot * kSlotStats + k * 2) =
                 make_float2(base[t], sum[t]);
     }
@@ -538,14 +562,14 @@ __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int s
 template <int DT, int D, int NW, int NT, int KT>
 hipError_t prompts_launch(const AttendArgs& a, hipStream_t stream)
 {
-    constexpr int CB = NW * NT * 16;
+    constexpr int CB = NW / kHalves<D> * NT * 16;
     const int64_t slots = (int64_t)a.tokens * a.group.d / CB + a.rows;
     const int64_t items = slots * a.kv_heads;
     int64_t splits = a.ws.groups / 2 / items;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
     const dim3 grid((unsigned)a.kv_heads, (unsigned)slots, (unsigned)splits);
     const hipError_t e = launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64,
-                                sizeof(Shared<D, KT, (D <= 128 ? 3 : 2)>), stream, a, (int)splits);
+                                sizeof(Shared<D, NW, KT, (kLate<D> ? 3 : 2), kHalves<D>>), stream, a, (int)splits);
     if (e != hipSuccess || splits == 1) return e;
     const dim3 join((unsigned)a.kv_heads, (unsigned)slots, (unsigned)(CB * D / 4 / kJoin));
     return launch(join_prompts_kernel<DT, D, CB, KT>, join, kJoin, 0, stream, a, (int)splits);
@@ -559,7 +583,7 @@ hipError_t by_width(const AttendArgs& a, hipStream_t stream)
     case 64: return prompts_launch<DT, 64, 4, F32 ? 1 : 2, 64>(a, stream);
     case 128: return prompts_launch<DT, 128, 8, F32 ? 1 : 2, 64>(a, stream);
     case 256: return prompts_launch<DT, 256, 8, 1, 64>(a, stream);
-    default: return prompts_launch<DT, 512, 4, 1, 32>(a, stream);
+    default: return prompts_launch<DT, 512, 8, 1, 32>(a, stream);
     }
 }
 
