@@ -330,7 +330,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         f32x4 o[DB];
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
-        float top = -inf32(), sum = 0.0f;
+        float base = -inf32(), sum = 0.0f;
 
         /* steps, every NW-th of them the wave's: a tile for all rows, and behind those (i >= 0) a
          * tile for each row that sees it, tile by tile */
@@ -540,29 +540,37 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
                     nan_v = __any(any != 0);
                 }
             }
-            float best = sc[0][0];
+            /* exponents against the base that holds, and their largest */
+            float y[NB][4], most = -inf32();
+            const float old = base == -inf32() ? 0.0f : base;
 #pragma unroll
             for (int h = 0; h < NB; ++h)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) best = fmaxf(best, sc[h][j]);
-            best = fmaxf(best, __shfl_xor(best, 16));
-            best = fmaxf(best, __shfl_xor(best, 32));
-            best = fmaxf(best, top);
-            if (__any(best > top)) {
-                const float keep = best > top ? __builtin_amdgcn_exp2f((top - best) * c) : 1.0f;
+                for (int j = 0; j < 4; ++j) {
+                    y[h][j] = __builtin_fmaf(sc[h][j], c, -old);
+                    most = fmaxf(most, y[h][j]);
+                }
+            most = column_max(most);
+            if (__any(rebase(base, most))) {
+                const bool moves = rebase(base, most);
+                const float keep = moves && base != -inf32() ? __builtin_amdgcn_exp2f(-most) : 1.0f;
+                if (moves) base = old + most;
                 sum *= keep;
 #pragma unroll
                 for (int i = 0; i < DB; ++i) o[i] *= keep;
-                top = best;
+                const float b = base == -inf32() ? 0.0f : base;
+#pragma unroll
+                for (int h = 0; h < NB; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[h][j] = __builtin_fmaf(sc[h][j], c, -b);
             }
-            const float base = top == -inf32() ? 0.0f : top * c;
             Frag pw[NH][PP];
 #pragma unroll
             for (int h = 0; h < NB; ++h)
 #pragma unroll
                 for (int j = 0; j < 4; j += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j], c, -base));
-                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[h][j + 1], c, -base));
+                    const float e0 = __builtin_amdgcn_exp2f(y[h][j]);
+                    const float e1 = __builtin_amdgcn_exp2f(y[h][j + 1]);
                     sum += e0 + e1;
                     Frag* f = pw[h >> 1];
                     const int w = (h & 1) * 2 + (j >> 1);
@@ -637,10 +645,9 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         }
 
         /* the waves join */
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
+        sum = column_sum(sum);
         if (g == 0) {
-            s.m[wave][m] = top == -inf32() ? top : top * c;
+            s.m[wave][m] = base;
             s.l[wave][m] = sum;
         }
         const bool whole = u0 == 0 && u1 == units;
@@ -790,7 +797,7 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
     const int groups = most < a.ws.groups ? (int)most : a.ws.groups;
     /* the most that can be left to be joined of one item: a launch of its own is enqueued only
      * where it may have something to do */
-    const int64_t cols = (int64_t)a.rows * a.group.d < kCols ? (int64_t)a.rows * a.group.d : kCols;
+    const int64_t cols = (int64_t)a.tokens * a.group.d < kCols ? (int64_t)a.tokens * a.group.d : kCols;
     const int64_t share = groups / a.kv_heads + 2, parts = units < share ? units : share;
     const int joins = parts * cols * D * 4 > kJoinBytes;
     hipError_t e = launch(attend_rows_kernel<DT, D>, groups, NW * 64, lds, stream, a, joins);
