@@ -30,6 +30,7 @@ constexpr int kJoinBytes = 96 << 10;
  * together with others (-1: none). */
 struct RowInfo {
     int length, key;
+    int differs; /* about the first slot whose page is not that of the row it is compared with */
 };
 
 /* The rows that begin with a row and are taken together, and the places that any of their
@@ -39,7 +40,9 @@ struct Group {
                   without tokens, or the prompts' kernel's) */
     int start; /* a single row's first token */
     int from, end;
+    int shared; /* units of tokens of several rows that are likely to have the same pages */
 };
+constexpr int kNone = 0x7FFFFFFF;
 
 __device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
 {
@@ -54,22 +57,35 @@ __device__ __forceinline__ int group_rows(const AttendArgs& a)
     return n >= 16 ? 16 : n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
 }
 
+template <int UNIT>
+__device__ __forceinline__ int last_unit(const Group& p)
+{
+    return (int)(((uint32_t)p.end + UNIT - 1) / UNIT);
+}
+template <int UNIT>
 __device__ __forceinline__ Group find_group(const AttendArgs& a, const RowInfo* info, int row)
 {
-    Group p{0, 0, 0, 0};
+    Group p{0, 0, 0, 0, 0};
     const int key = info[row].key, most = group_rows(a), in = row & (most - 1);
     if (key >= 0) {
         if (in > 0 && info[row - 1].key == key) return p;
         p.rows = 1;
         p.end = info[row].length;
         p.from = sees_from(a, p.end - 1);
+        int differs = info[row].differs;
         for (int i = 1; in + i < most && row + i < a.rows && info[row + i].key == key; ++i) {
             const int n = info[row + i].length, f = sees_from(a, n - 1);
             p.end = n > p.end ? n : p.end;
             p.from = f < p.from ? f : p.from;
+            differs = info[row + i].differs < differs ? info[row + i].differs : differs;
             ++p.rows;
         }
-        if (p.rows > 1) return p;
+        if (p.rows > 1) {
+            const int64_t t = (int64_t)differs * a.pool.page_tokens.d;
+            const int n = t < p.end ? (int)t / UNIT : last_unit<UNIT>(p);
+            p.shared = n > p.from / UNIT ? n - p.from / UNIT : 0;
+            return p;
+        }
     }
     const RowTokens r = row_tokens(a.starts, a.lengths, row, a.tokens, cache_room(a.pool));
     p.rows = is_prompt(r.count, a.group.d, a.few) ? 0 : -r.count;
@@ -80,7 +96,8 @@ __device__ __forceinline__ Group find_group(const AttendArgs& a, const RowInfo* 
 }
 
 /* Query columns (tokens x heads of a key head) of a group, and units of UNIT tokens of each of
- * its blocks of them: one at least, for the output. */
+ * its blocks of them: one at least, for the output.  Tokens whose pages several rows share
+ * count once, the others for each row. */
 __device__ __forceinline__ int group_cols(const AttendArgs& a, const Group& p)
 {
     return (p.rows < 0 ? -p.rows : p.rows) * a.group.d;
@@ -88,7 +105,52 @@ __device__ __forceinline__ int group_cols(const AttendArgs& a, const Group& p)
 template <int UNIT>
 __device__ __forceinline__ int group_units(const Group& p)
 {
-    return p.end > p.from ? (int)(((uint32_t)p.end + UNIT - 1) / UNIT) - p.from / UNIT : 1;
+    if (p.end <= p.from) return 1;
+    const int n = last_unit<UNIT>(p) - p.from / UNIT;
+    return p.rows > 1 ? p.shared + (n - p.shared) * p.rows : n;
+}
+
+/* Where the pages of rows that may be taken together part from those of the longest of them, in
+ * the slots that both see: a search that takes one of EACH + 1 stretches a step by the
+ * pages at their ends, EACH lanes a row.  It finds the slot if pages that have parted never
+ * meet again, and otherwise some slot; it only decides how work is shared out. */
+template <int NW, int EACH>
+__device__ __forceinline__ void find_partings(const AttendArgs& a, RowInfo* info)
+{
+    const int lane = threadIdx.x & (EACH - 1), most = group_rows(a);
+    for (int r0 = 0; r0 < a.rows; r0 += NW * 64 / EACH) {
+        const int r = r0 + (int)threadIdx.x / EACH;
+        const int key = r < a.rows ? info[r].key : -1;
+        int ref = r;
+        if (key >= 0) {
+            for (int i = r - 1; i >= (r & -most) && info[i].key == key; --i)
+                if (info[i].length >= info[ref].length) ref = i;
+            for (int i = r + 1; i < a.rows && (i & (most - 1)) != 0 && info[i].key == key; ++i)
+                if (info[i].length > info[ref].length) ref = i;
+        }
+        int lo = 0, hi = 0; /* the first that differs is one of lo .. hi, hi meaning none */
+        if (ref != r) {
+            lo = divide(sees_from(a, info[ref].length - 1), a.pool.page_tokens);
+            hi = divide(info[r].length - 1, a.pool.page_tokens) + 1;
+        }
+        const int end = hi;
+        const int32_t* mine = a.table + (int64_t)(r < a.rows ? r : 0) * a.pool.max_slots;
+        const int32_t* other = a.table + (int64_t)(ref < a.rows ? ref : 0) * a.pool.max_slots;
+        while (__any(lo < hi)) {
+            const int n = (hi - lo + EACH) / (EACH + 1); /* slots lo + n i - 1 are looked at */
+            const int at = lo + n * (lane + 1) - 1;
+            const bool differs = lo < hi && (at >= hi || mine[at] != other[at]);
+            const uint32_t found = (uint32_t)(__ballot(differs) >> ((threadIdx.x & 63) & -EACH)) &
+                                   ((1u << EACH) - 1);
+            if (lo < hi) {
+                const int k = found ? __builtin_ctz(found) : EACH;
+                const int top = lo + n * (k + 1) - 1;
+                if (found && top < hi) hi = top;
+                lo += n * k;
+            }
+        }
+        if (lane == 0 && key >= 0) info[r].differs = lo < end ? lo : kNone;
+    }
 }
 
 /* info and groups [0 .. rows - 1], and the work of the groups before each row, in units,
@@ -103,16 +165,23 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, Gr
     for (int r = tid; r < a.rows; r += NW * 64) {
         const int page = a.table[(int64_t)r * a.pool.max_slots];
         const RowTokens t = row_tokens(a.starts, a.lengths, r, a.tokens, room);
-        RowInfo i{t.bad ? -1 : t.length, -1};
+        RowInfo i{t.bad ? -1 : t.length, -1, kNone};
         if (t.count == 1 && t.length > 0 && page >= 0 && page < a.pool.n_pages) i.key = page;
         info[r] = i;
     }
     lds_barrier();
+    if (a.rows > 1 && group_rows(a) > 1) {
+        if (a.rows <= NW * 4)
+            find_partings<NW, 16>(a, info);
+        else
+            find_partings<NW, 4>(a, info);
+        lds_barrier();
+    }
     int64_t sum = 0;
     for (int i = 0; i < each; ++i) {
         const int r = tid * each + i;
         if (r >= a.rows) break;
-        const Group p = find_group(a, info, r);
+        const Group p = find_group<UNIT>(a, info, r);
         const int blocks = (group_cols(a, p) + kCols - 1) / kCols;
         groups[r] = p;
         before[r + 1] = (int64_t)(blocks * a.kv_heads) * group_units<UNIT>(p);
@@ -244,6 +313,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         p.start = __builtin_amdgcn_readfirstlane(p.start);
         p.from = __builtin_amdgcn_readfirstlane(p.from);
         p.end = __builtin_amdgcn_readfirstlane(p.end);
+        p.shared = __builtin_amdgcn_readfirstlane(p.shared);
         const bool several = p.rows > 1; /* rows */
         const int all_cols = group_cols(a, p), blocks = (all_cols + kCols - 1) / kCols;
         const int units = group_units<UNIT>(p), first = p.from / UNIT;
@@ -296,9 +366,13 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
             }
         all_from = __builtin_amdgcn_readfirstlane(all_from);
         all_to = __builtin_amdgcn_readfirstlane(all_to);
-        /* the part's tiles: those before a_shared have the same pages for all rows */
-        const int t0 = (first + u0) * UNIT > p.from ? (first + u0) * UNIT : p.from;
-        const int t1 = (uint32_t)(first + u1) * UNIT < (uint32_t)p.end ? (first + u1) * UNIT : p.end;
+        /* the part's tiles: first those of all rows, of which the ones before a_shared have the
+         * same pages for all, and then units v0 .. v1 - 1 of single rows' tiles */
+        const int once = several ? p.shared : units;
+        const int s0 = u0 < once ? u0 : once, s1 = u1 < once ? u1 : once;
+        const int v0 = u0 - s0, v1 = u1 - s1;
+        const int t0 = (first + s0) * UNIT > p.from ? (first + s0) * UNIT : p.from;
+        const int t1 = (uint32_t)(first + s1) * UNIT < (uint32_t)p.end ? (first + s1) * UNIT : p.end;
         const int a0 = t0 / TT, a1 = t1 > t0 ? (int)((uint32_t)(t1 + TT - 1) / TT) : a0;
         int a_shared = a1;
         int ref = lo; /* the longest row, whose table has every place */
@@ -308,8 +382,9 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
             ref = __builtin_amdgcn_readfirstlane(ref);
             if (tid == 0) s.differs = p.end;
             lds_barrier();
-            const int s0 = divide(t0, a.pool.page_tokens), s1 = divide(t1 - 1, a.pool.page_tokens);
-            for (int slot = s0 + (tid >> 4); slot <= s1; slot += NW * 4) {
+            const int begin = t0 < t1 ? divide(t0, a.pool.page_tokens) : 0;
+            const int end = t0 < t1 ? divide(t1 - 1, a.pool.page_tokens) + 1 : 0;
+            for (int slot = begin + (tid >> 4); slot < end; slot += NW * 4) {
                 if (m >= p.rows) break;
                 const int last = info[lo + m].length - 1;
                 if (slot < divide(sees_from(a, last), a.pool.page_tokens) ||
@@ -332,13 +407,14 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         for (int i = 0; i < DB; ++i) o[i] = f32x4{0, 0, 0, 0};
         float base = -inf32(), sum = 0.0f;
 
-        /* steps, every NW-th of them the wave's: a tile for all rows, and behind those (i >= 0) a
-         * tile for each row that sees it, tile by tile */
+        /* steps, every NW-th of them the wave's: a tile for all rows, behind those (i >= 0) a tile
+         * for each row that sees it, tile by tile, and then the single rows' units */
         struct Step {
             int tile, i, row; /* row: the table that is read */
             int first, last;  /* first and last place that is read */
         };
         const uint32_t by_rows = several ? 0xFFFFFFFFu / (uint32_t)p.rows + 1u : 0u; /* i / rows = high(i * it) */
+        const int mixed = several ? ((a1 - a_shared) * p.rows + NW - 1) & -NW : 0;
         auto settle = [&](Step& t) {
             if (t.i < 0) {
                 t.row = ref;
@@ -346,14 +422,21 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
                 t.last = p.end - 1;
                 if (t.tile < a_shared) return;
                 t.i = t.tile - a_shared;
-                t.tile = a1;
+                t.tile = kNone;
                 if (!several) return;
             }
             for (;; t.i += NW) {
-                const uint32_t q = __umulhi((uint32_t)t.i, by_rows);
-                t.tile = a_shared + (int)q;
-                if (t.tile >= a1) return;
-                t.row = lo + t.i - (int)q * p.rows;
+                const int v = t.i < mixed ? t.i : v0 + (t.i - mixed) / NW;
+                const int q = (int)__umulhi((uint32_t)v, by_rows);
+                if (t.i < mixed) {
+                    t.tile = a_shared + q;
+                    if (t.tile >= a1) continue;
+                } else {
+                    t.tile = kNone;
+                    if (v >= v1) return;
+                    t.tile = (first + once + q) * NW + t.i % NW;
+                }
+                t.row = lo + v - q * p.rows;
                 t.last = __builtin_amdgcn_readfirstlane(info[t.row].length - 1);
                 t.first = sees_from(a, t.last);
                 if (t.tile * TT <= t.last && t.tile * TT + TT > t.first) return;
@@ -444,19 +527,19 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         Step next = now;
         int buf = 0, page = 0;
         uint64_t bad = 0;
-        if (now.tile < a1) {
+        if (now.tile != kNone) {
             Scales scale;
             bad = locate(now, find_page(now), 0, scale);
             wave_fence();
             load_keys(0);
             load_values(0);
             next = advance(now);
-            if (next.tile < a1) page = find_page(next);
+            if (next.tile != kNone) page = find_page(next);
             keep_scales(0, scale);
             wave_fence();
         }
-        while (now.tile < a1) {
-            const bool more = next.tile < a1;
+        while (now.tile != kNone) {
+            const bool more = next.tile != kNone;
             const uint64_t bad_now = bad;
             Scales scale{0.0f, 0.0f};
             Step after = next;
@@ -464,7 +547,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
                 bad = locate(next, page, buf ^ 1, scale);
                 wave_fence();
                 after = advance(next);
-                if (after.tile < a1) page = find_page(after);
+                if (after.tile != kNone) page = find_page(after);
             }
 
             f32x4 sc[NB];
@@ -793,12 +876,13 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
     /* no more workgroups than the rows can have use for */
     const int64_t blocks = (a.group.d + kCols - 1) / kCols;
     const int64_t units = (cache_room(a.pool) + UNIT - 1) / UNIT + 1;
+    const int64_t together = kCols / a.group.d < 1 ? 1 : kCols / a.group.d < a.rows ? kCols / a.group.d : a.rows;
     const int64_t most = ((int64_t)a.rows * a.kv_heads * blocks * units + Shape<DT, D>::UNITS - 1) / Shape<DT, D>::UNITS;
     const int groups = most < a.ws.groups ? (int)most : a.ws.groups;
     /* the most that can be left to be joined of one item: a launch of its own is enqueued only
      * where it may have something to do */
     const int64_t cols = (int64_t)a.tokens * a.group.d < kCols ? (int64_t)a.tokens * a.group.d : kCols;
-    const int64_t share = groups / a.kv_heads + 2, parts = units < share ? units : share;
+    const int64_t share = groups / a.kv_heads + 2, parts = units * together < share ? units * together : share;
     const int joins = parts * cols * D * 4 > kJoinBytes;
     hipError_t e = launch(attend_rows_kernel<DT, D>, groups, NW * 64, lds, stream, a, joins);
     if (e != hipSuccess || !joins) return e;
