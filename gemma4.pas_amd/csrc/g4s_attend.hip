@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kB = 256;
 constexpr int kCols = 16;  /* query columns of a workgroup's part */
-constexpr int kPass = 128; /* dims that the waves join at once */
 /* Bytes of parts that their last workgroup joins by itself: more are left to a launch of
  * their own. */
 constexpr int kJoinBytes = 96 << 10;
@@ -206,11 +205,15 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, Gr
     lds_barrier();
 }
 
+/* Dims that the waves join at once (LDS also holds 40 bytes for each of up to 2048 rows). */
+template <int D, int NW>
+constexpr int kPass = D * NW < 512 ? D : 512 / NW;
+
 template <int DT, int D, int NW, int TT>
 struct Shared {
     union {
         Frag q[D / 64][2][DT == G4S_DTYPE_F32 ? 3 : 1][64]; /* the queries, as lanes take them */
-        float o[NW][kCols][kPass + 4];                      /* the waves' sums */
+        float o[NW][kCols][kPass<D, NW> + 4];               /* the waves' sums */
     };
     int64_t offset[NW][2][TT];
     float scale[NW][2][2][TT];
@@ -252,13 +255,14 @@ __device__ __forceinline__ void put(const AttendArgs& a, int64_t out, int64_t ls
 }
 
 /* How a kernel is made for a width of heads: tokens of a wave's step, as many as its registers
- * hold beside the sums (16, 32 or 64). */
-constexpr int kWaves = 4;
+ * hold beside the sums (16, 32 or 64); waves, of which eight are a CU's; and units that a workgroup
+ * takes at least where there are enough of them. */
+constexpr int kResident = 8;
 template <int DT, int D>
 struct Shape {
-    static constexpr int NW = kWaves;
+    static constexpr int NW = D <= 128 ? 8 : 4;
     static constexpr int TT = D <= 128 ? 64 : D <= 256 ? 32 : 16;
-    static constexpr int UNITS = D <= 128 ? 2 : 4; /* of a workgroup at least, where there are few */
+    static constexpr int UNITS = D <= 128 ? 1 : D <= 256 ? 2 : 4;
 };
 
 template <int DT, int D>
@@ -287,10 +291,12 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
     if (joins && tid == 0) a.ws.records[blockIdx.x].parts = 0;
     scan_rows<NW, UNIT>(a, info, group, before, s.wave);
     const int64_t total = before[a.rows];
+    /* one unit a workgroup while that leaves CUs without any, and UNITS at least of each otherwise */
     constexpr int UNITS = Shape<DT, D>::UNITS;
-    const int64_t least = (total + UNITS - 1) / UNITS;
-    const int groups = least < gridDim.x ? (int)least : (int)gridDim.x;
-    if ((int)blockIdx.x >= groups) return;
+    const int64_t one_each = total < a.ws.groups / 2 ? total : a.ws.groups / 2;
+    int64_t groups = (total + UNITS - 1) / UNITS;
+    groups = groups < one_each ? one_each : groups < gridDim.x ? groups : gridDim.x;
+    if (blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
     const int64_t x_end = first_unit(total, blockIdx.x + 1, groups);
     /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
@@ -756,7 +762,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
                 st_dev(reinterpret_cast<uint64_t*>(a.ws.stats + (slot * kCols + tid) * 2),
                        (uint64_t)__float_as_uint(best) | (uint64_t)__float_as_uint(all) << 32);
         }
-        constexpr int PD = D < kPass ? D : kPass; /* dims of a pass */
+        constexpr int PD = kPass<D, NW>;
 #pragma unroll 1
         for (int pass = 0; pass < D / PD; ++pass) {
             /* lanes with dims of this pass: a lane has DB in each of four rows */
@@ -877,8 +883,9 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
     const int64_t blocks = (a.group.d + kCols - 1) / kCols;
     const int64_t units = (cache_room(a.pool) + UNIT - 1) / UNIT + 1;
     const int64_t together = kCols / a.group.d < 1 ? 1 : kCols / a.group.d < a.rows ? kCols / a.group.d : a.rows;
-    const int64_t most = ((int64_t)a.rows * a.kv_heads * blocks * units + Shape<DT, D>::UNITS - 1) / Shape<DT, D>::UNITS;
-    const int groups = most < a.ws.groups ? (int)most : a.ws.groups;
+    const int64_t most = (int64_t)a.rows * a.kv_heads * blocks * units;
+    const int resident = a.ws.groups / 2 * (kResident / NW);
+    const int groups = most < resident ? (int)most : resident;
     /* the most that can be left to be joined of one item: a launch of its own is enqueued only
      * where it may have something to do */
     const int64_t cols = (int64_t)a.tokens * a.group.d < kCols ? (int64_t)a.tokens * a.group.d : kCols;
