@@ -23,9 +23,9 @@ namespace {
 constexpr int kB = 256;
 constexpr int kTile = 16;  /* places of a workgroup, or one block where that is longer */
 constexpr int kChunk = 8;  /* dims of a thread */
-constexpr int kStep = 16;  /* tokens whose angles are in LDS at once */
-constexpr int kPairs = 2048; /* .. as long as they have no more pairs than this */
-constexpr int kQueryHeads = 8, kKeyHeads = 2; /* of a workgroup, where there are several tokens */
+constexpr int kPairs = 2048; /* angles in LDS at once */
+constexpr int kQueryHeads = 8; /* of a workgroup at least, where there are several tokens */
+constexpr int kFill = 768;     /* workgroups, three a CU */
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -71,19 +71,28 @@ __device__ __forceinline__ const char* element(const CacheView& v, int64_t token
     return v.data + (token * v.token_stride + head * v.head_stride + dim) * Elem<DT>::SIZE;
 }
 
-/* kChunk elements, 16-byte aligned. */
+/* kChunk elements as they are stored, 16-byte aligned. */
 template <int DT>
-__device__ __forceinline__ void load_chunk(const char* p, float (&x)[kChunk])
+struct Words {
+    uint4 x[DT == G4S_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Words<DT> load_words(const char* p)
+{
+    Words<DT> w;
+    w.x[0] = reinterpret_cast<const uint4*>(p)[0];
+    if constexpr (DT == G4S_DTYPE_F32) w.x[1] = reinterpret_cast<const uint4*>(p)[1];
+    return w;
+}
+template <int DT>
+__device__ __forceinline__ void widen(const Words<DT>& v, float (&x)[kChunk])
 {
     if constexpr (DT == G4S_DTYPE_F32) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0];
-        const float4 b = reinterpret_cast<const float4*>(p)[1];
-        const float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        const uint32_t w[8] = {v.x[0].x, v.x[0].y, v.x[0].z, v.x[0].w, v.x[1].x, v.x[1].y, v.x[1].z, v.x[1].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = v[i];
+        for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(w[i]);
     } else {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        const uint32_t w[4] = {v.x[0].x, v.x[0].y, v.x[0].z, v.x[0].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             x[2 * i] = __uint_as_float(w[i] << 16);
@@ -153,19 +162,29 @@ struct Tile {
 enum Mode { kHalves, kNeighbours, kAny };
 
 /* Chunk `c` of a head of one token: what is in it, and what is paired with it. */
+template <int DT, int MODE>
 struct Chunk {
-    float x[kChunk], o[kChunk];
+    Words<DT> x, o;
+};
+template <int DT>
+struct Chunk<DT, kNeighbours> {
+    Words<DT> x;
+};
+template <int DT>
+struct Chunk<DT, kAny> {
+    Words<DT> x;
+    float o[kChunk];
 };
 template <int DT, int MODE>
 __device__ __forceinline__ void read_chunk(const AppendArgs& a, const CacheView& view, int64_t token,
-                                           int head, int c, bool rotate, Chunk& w)
+                                           int head, int c, bool rotate, Chunk<DT, MODE>& w)
 {
     const int d0 = c * kChunk, half = a.rotary_dims >> 1;
-    load_chunk<DT>(element<DT>(view, token, head, d0), w.x);
+    w.x = load_words<DT>(element<DT>(view, token, head, d0));
     if (!rotate || d0 >= a.rotary_dims) return;
-    if (MODE == kHalves)
-        load_chunk<DT>(element<DT>(view, token, head, d0 < half ? d0 + half : d0 - half), w.o);
-    if (MODE == kAny) {
+    if constexpr (MODE == kHalves)
+        w.o = load_words<DT>(element<DT>(view, token, head, d0 < half ? d0 + half : d0 - half));
+    if constexpr (MODE == kAny) {
         for (int i = 0; i < kChunk; ++i) {
             const int d = d0 + i;
             const int pair = a.rotary_pairs == G4S_ROTARY_NEIGHBOURS ? d ^ 1 : d < half ? d + half : d - half;
@@ -204,15 +223,17 @@ __device__ __forceinline__ void read_turn(const AppendArgs& a, int c, const doub
         }
     }
 }
-template <int MODE>
-__device__ __forceinline__ void rotate(const AppendArgs& a, const Chunk& w, int c, const Turn& r,
-                                       double (&y)[kChunk])
+template <int DT, int MODE>
+__device__ __forceinline__ void rotate(const AppendArgs& a, const Chunk<DT, MODE>& w, int c,
+                                       const Turn& r, double (&y)[kChunk])
 {
     const int d0 = c * kChunk, half = a.rotary_dims >> 1;
+    float x[kChunk];
+    widen(w.x, x);
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) y[i] = (double)w.x[i];
+    for (int i = 0; i < kChunk; ++i) y[i] = (double)x[i];
     if (d0 >= a.rotary_dims) return;
-    if (MODE == kNeighbours) {
+    if constexpr (MODE == kNeighbours) {
 #pragma unroll
         for (int i = 0; i < kChunk; i += 2) {
             const double u = y[i], v = y[i + 1];
@@ -220,12 +241,15 @@ __device__ __forceinline__ void rotate(const AppendArgs& a, const Chunk& w, int 
             y[i + 1] = __builtin_fma(v, r.t[i].x, u * r.t[i].y);
         }
     } else {
+        float o[kChunk];
+        if constexpr (MODE == kHalves) widen(w.o, o);
 #pragma unroll
         for (int i = 0; i < kChunk; ++i) {
+            if constexpr (MODE == kAny) o[i] = w.o[i];
             const bool low = MODE == kHalves ? d0 < half
                              : a.rotary_pairs == G4S_ROTARY_NEIGHBOURS ? (i & 1) == 0
                                                                       : d0 + i < half;
-            const double v = (double)w.o[i] * r.t[i].y;
+            const double v = (double)o[i] * r.t[i].y;
             y[i] = __builtin_fma(y[i], r.t[i].x, low ? -v : v);
         }
     }
@@ -284,16 +308,6 @@ __device__ __forceinline__ bool find_tile(const AppendArgs& a, int64_t x, int ti
 
 /* The largest finite magnitude of a chunk, as the bits of a binary32, which are in order.
  * (to_odd keeps a value on its side of 448 * 2^e, whose last bit is even.) */
-__device__ __forceinline__ uint32_t top_of(const double (&y)[kChunk])
-{
-    double m = 0.0;
-#pragma unroll
-    for (int i = 0; i < kChunk; ++i) {
-        const double v = __builtin_fabs(y[i]);
-        m = v > m && v < __builtin_inf() ? v : m;
-    }
-    return __float_as_uint(to_odd(m));
-}
 __device__ __forceinline__ uint32_t top_of(const float (&x)[kChunk])
 {
     float m = 0.0f;
@@ -324,17 +338,29 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t m, int chunks)
     return m;
 }
 
-/* Values are exact in binary32, and so are their products with a scale's inverse. */
-__device__ __forceinline__ void store_codes(char* at, bool value, const Chunk& w,
-                                            const double (&y)[kChunk], float scale)
+/* What of a chunk is stored: a value as it is, a rotated key as the odd binary32 next to it,
+ * whose product with a scale's inverse (a power of two) is exact and rounds to the code that the key
+ * itself has. */
+template <int DT, int MODE>
+__device__ __forceinline__ void stored(const AppendArgs& a, const Chunk<DT, MODE>& w, int c, bool value,
+                                       const Turn& r, float (&x)[kChunk])
+{
+    widen(w.x, x);
+    if (value || c * kChunk >= a.rotary_dims) return;
+    double y[kChunk];
+    rotate(a, w, c, r, y);
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) x[i] = to_odd(y[i]);
+}
+__device__ __forceinline__ void store_codes(char* at, const float (&x)[kChunk], float scale)
 {
     const float inv = 1.0f / scale;
-    float x[kChunk];
+    float q[kChunk];
 #pragma unroll
-    for (int i = 0; i < kChunk; ++i) x[i] = value ? w.x[i] * inv : to_odd(y[i] * (double)inv);
+    for (int i = 0; i < kChunk; ++i) q[i] = x[i] * inv;
     uint32_t* to = reinterpret_cast<uint32_t*>(at);
-    to[0] = codes4(x);
-    to[1] = codes4(x + 4);
+    to[0] = codes4(q);
+    to[1] = codes4(q + 4);
 }
 
 /* ------------------------------------------------------- a token for each row */
@@ -357,8 +383,8 @@ __global__ __launch_bounds__(kB) void append_step_kernel(AppendArgs a, int queri
     const int item = vector - queries;
     const bool value = !query && item >= a.kv_heads;
     const int head = query ? vector : value ? item - a.kv_heads : item;
-    Chunk w;
-    if (in) read_chunk<DT, MODE>(a, query ? a.q : value ? a.v : a.k, row, head, c, !value, w);
+    Chunk<DT, MODE> w;
+    if (in) read_chunk(a, query ? a.q : value ? a.v : a.k, row, head, c, !value, w);
     const float freq = tid < half ? a.freqs[tid] : 0.0f;
     const int position = a.positions ? a.positions[row] : 0;
     const int length = a.lengths[row];
@@ -381,16 +407,20 @@ __global__ __launch_bounds__(kB) void append_step_kernel(AppendArgs a, int queri
         turn[i] = make_double2(t, s);
     }
     __syncthreads();
-    double y[kChunk];
-    if (in && !value) {
-        Turn t;
-        read_turn<MODE>(a, c, turn, t);
-        rotate<MODE>(a, w, c, t, y);
-    }
-    if (in && query)
-        store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, row, head, c * kChunk)), y);
+    float x[kChunk];
     uint32_t top = 0;
-    if (in && !query) top = value ? top_of(w.x) : top_of(y);
+    if (in) {
+        Turn t;
+        if (!value) read_turn<MODE>(a, c, turn, t);
+        if (query) {
+            double y[kChunk];
+            rotate(a, w, c, t, y);
+            store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, row, head, c * kChunk)), y);
+        } else {
+            stored(a, w, c, value, t, x);
+            top = top_of(x);
+        }
+    }
     if ((chunks & (chunks - 1)) == 0) {
         top = lanes_max(top, chunks);
     } else {
@@ -401,7 +431,7 @@ __global__ __launch_bounds__(kB) void append_step_kernel(AppendArgs a, int queri
     if (off < 0) return;
     float grown;
     const float scale = block_scale(top, before > 0, old, grown);
-    store_codes(block + (int64_t)before * a.pool.token_bytes + c * kChunk, value, w, y, scale);
+    store_codes(block + (int64_t)before * a.pool.token_bytes + c * kChunk, x, scale);
     if (c == 0) *scale_at = scale;
     if (grown == 1.0f) return;
     for (int j = 0; j < before; ++j) {
@@ -465,102 +495,175 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, const Tile& 
         for (int j = l.token; j < n; j += l.tokens) {
             Turn r;
             read_turn<MODE>(a, l.c, turn + j * half, r);
-#pragma unroll 2
-            for (int h = head0; h < end; ++h) {
-                Chunk w;
-                read_chunk<DT, MODE>(a, a.q, token0 + j, h, l.c, true, w);
-                double y[kChunk];
-                rotate<MODE>(a, w, l.c, r, y);
-                store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, token0 + j, h, l.c * kChunk)), y);
+            constexpr int HELD = DT == G4S_DTYPE_F32 ? 2 : 4;
+            for (int h = head0; h < end; h += HELD) {
+                Chunk<DT, MODE> w[HELD];
+#pragma unroll
+                for (int k = 0; k < HELD; ++k)
+                    if (h + k < end) read_chunk(a, a.q, token0 + j, h + k, l.c, true, w[k]);
+#pragma unroll
+                for (int k = 0; k < HELD; ++k) {
+                    if (h + k >= end) break;
+                    double y[kChunk];
+                    rotate(a, w[k], l.c, r, y);
+                    store_chunk<DT>(const_cast<char*>(element<DT>(a.q_out, token0 + j, h + k, l.c * kChunk)), y);
+                }
             }
         }
     }
 }
 
-/* Keys, or values, of `heads` heads. */
-template <int DT, int MODE, bool VALUE>
+/* What a workgroup does between the two looks at a group of heads' vectors: scales of its blocks in the
+ * place of their magnitudes, and the codes of earlier tokens under scales that grew. */
+__device__ __forceinline__ void settle_scales(const AppendArgs& a, const Tile& t, const Places& places,
+                                              char* plane, int head0, int heads, uint32_t* top,
+                                              float* ratio)
+{
+    const int B = a.pool.scale_tokens.d, tid = threadIdx.x;
+    const int first_block = divide(t.first, a.pool.scale_tokens);
+    const int blocks = divide(t.end - 1, a.pool.scale_tokens) - first_block + 1;
+    __syncthreads();
+    for (int i = tid; i < blocks * heads; i += kB) {
+        const int b = i / heads, k = i - b * heads;
+        const int64_t off = place_offset(a, places, (first_block + b) * B, head0 + k);
+        const bool earlier = b == 0 && t.before > 0 && off >= 0;
+        float* at = reinterpret_cast<float*>(plane + off + a.pool.head_dim);
+        float grown;
+        const float scale = block_scale(top[i], earlier, earlier ? *at : 0.0f, grown);
+        if (off >= 0) *at = scale;
+        top[i] = __float_as_uint(scale);
+        if (b == 0) ratio[k] = grown;
+    }
+    __syncthreads();
+    if (t.before == 0) return;
+    const int words = a.pool.head_dim / 4;
+    for (int i = tid; i < heads * t.before * words; i += kB) {
+        const int v = i / words, k = v / t.before, j = v - k * t.before;
+        if (ratio[k] == 1.0f) continue;
+        const int64_t off = place_offset(a, places, first_block * B + j, head0 + k);
+        if (off < 0) continue;
+        uint32_t* at = reinterpret_cast<uint32_t*>(plane + off) + (i - v * words);
+        *at = regrown(*at, ratio[k]);
+    }
+}
+
+/* Keys, or values, of `heads` heads.  HELD: a thread keeps its vectors of a group of heads, HELD
+ * tokens' of each, in registers from the first look to the second; 0: of tiles with more tokens,
+ * whose vectors are read twice. */
+constexpr int kHeld = 4;
+/* Keeps what follows behind what came before: the angles of one vector, in binary64, are as many
+ * registers as there is room for. */
+__device__ __forceinline__ void one_by_one()
+{
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+/* Heads at once. */
+constexpr int group_heads(int held) { return held > 0 ? kHeld / held : kHeld; }
+template <int DT, int MODE, bool VALUE, int HELD>
 __device__ __forceinline__ void append_heads(const AppendArgs& a, const Tile& t, int head0, int heads,
                                              int step, double2* turn, uint32_t* top, float* ratio)
 {
-    const int half = a.rotary_dims >> 1, B = a.pool.scale_tokens.d, tid = threadIdx.x;
+    constexpr int GROUP = group_heads(HELD);
+    const int half = a.rotary_dims >> 1, tid = threadIdx.x;
     const CacheView& view = VALUE ? a.v : a.k;
     char* const plane = VALUE ? a.v_plane : a.k_plane;
     const Places places = places_of(a, t.row, t.first);
-    const int first_block = t.first / B;
-    const int blocks = (t.end - 1) / B - first_block + 1;
+    const int first_block = divide(t.first, a.pool.scale_tokens);
+    const int blocks = divide(t.end - 1, a.pool.scale_tokens) - first_block + 1;
     const int end = head0 + heads < a.kv_heads ? head0 + heads : a.kv_heads;
-    heads = end - head0;
     const Lanes l = lanes_of(a.pool.head_dim / kChunk);
     const bool pow2 = (l.chunks & (l.chunks - 1)) == 0;
-    for (int i = tid; i < blocks * heads; i += kB) top[i] = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int s0 = t.first; s0 < t.end; s0 += step) {
-            const int n = t.end - s0 < step ? t.end - s0 : step;
-            const int64_t token0 = t.token + (s0 - t.first);
-            if (pass == 0 || t.end - t.first > step) {
-                __syncthreads();
-                if (!VALUE) fill_turns(a, t, s0, n, turn);
-                __syncthreads();
+    auto raise = [&](int at, bool in, uint32_t m) {
+        if (pow2) m = lanes_max(m, l.chunks);
+        if (in && (!pow2 || l.c == 0)) atomicMax(&top[at], m);
+    };
+    for (int h0 = head0; h0 < end; h0 += GROUP) {
+        const int n_heads = end - h0 < GROUP ? end - h0 : GROUP;
+        if constexpr (HELD > 0) {
+            /* (lanes without a token take the first one, and keep nothing) */
+            Chunk<DT, MODE> w[HELD][GROUP];
+            float x[HELD][GROUP][kChunk];
+            bool in[HELD];
+            int at[HELD], turn_at[HELD];
+            int64_t off[HELD];
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                int j = i * l.tokens + l.token;
+                in[i] = l.token < l.tokens && t.first + j < t.end;
+                j = in[i] ? j : 0;
+                turn_at[i] = j * half;
+                at[i] = (divide(t.first + j, a.pool.scale_tokens) - first_block) * n_heads;
+#pragma unroll
+                for (int k = 0; k < GROUP; ++k)
+                    read_chunk(a, view, t.token + j, h0 + (k < n_heads ? k : 0), l.c, !VALUE, w[i][k]);
+                off[i] = place_offset(a, places, t.first + j, h0);
             }
-            for (int j0 = 0; j0 < n; j0 += l.tokens) {
-                const int j = j0 + l.token;
-                const bool in = l.token < l.tokens && j < n;
-                const int place = s0 + j;
+            __syncthreads(); /* (the group before has read its scales) */
+            for (int i = tid; i < blocks * n_heads; i += kB) top[i] = 0;
+            if (!VALUE && h0 == head0) fill_turns(a, t, t.first, t.end - t.first, turn);
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
                 Turn r;
-                if (!VALUE && in) read_turn<MODE>(a, l.c, turn + j * half, r);
-                const int64_t off = pass == 1 && in ? place_offset(a, places, place, head0) : -1;
-                const int at = in ? (place / B - first_block) * heads : 0;
-#pragma unroll 2
-                for (int k = 0; k < heads; ++k) {
-                    Chunk w;
-                    double y[kChunk];
-                    if (in) {
-                        read_chunk<DT, MODE>(a, view, token0 + j, head0 + k, l.c, !VALUE, w);
-                        if (!VALUE) rotate<MODE>(a, w, l.c, r, y);
-                    }
-                    if (pass == 0) {
-                        uint32_t m = 0;
-                        if (in) m = VALUE ? top_of(w.x) : top_of(y);
-                        if (pow2) m = lanes_max(m, l.chunks);
-                        if (in && (!pow2 || l.c == 0)) atomicMax(&top[at + k], m);
-                    } else if (off >= 0) {
-                        store_codes(plane + off + (int64_t)k * a.pool.part_bytes + l.c * kChunk, VALUE,
-                                    w, y, __uint_as_float(top[at + k]));
+                if (!VALUE) read_turn<MODE>(a, l.c, turn + turn_at[i], r);
+#pragma unroll
+                for (int k = 0; k < GROUP; ++k) {
+                    stored(a, w[i][k], l.c, VALUE, r, x[i][k]);
+                    if (k < n_heads) raise(at[i] + k, in[i], in[i] ? top_of(x[i][k]) : 0);
+                }
+                one_by_one();
+            }
+            settle_scales(a, t, places, plane, h0, n_heads, top, ratio);
+#pragma unroll
+            for (int i = 0; i < HELD; ++i) {
+                if (!in[i] || off[i] < 0) continue;
+#pragma unroll
+                for (int k = 0; k < GROUP; ++k)
+                    if (k < n_heads)
+                        store_codes(plane + off[i] + (int64_t)k * a.pool.part_bytes + l.c * kChunk, x[i][k],
+                                    __uint_as_float(top[at[i] + k]));
+            }
+        } else {
+            __syncthreads();
+            for (int i = tid; i < blocks * n_heads; i += kB) top[i] = 0;
+            for (int pass = 0; pass < 2; ++pass) {
+                for (int s0 = t.first; s0 < t.end; s0 += step) {
+                    const int n = t.end - s0 < step ? t.end - s0 : step;
+                    __syncthreads();
+                    if (!VALUE) fill_turns(a, t, s0, n, turn);
+                    __syncthreads();
+                    for (int j0 = 0; j0 < n; j0 += l.tokens) {
+                        const int j = j0 + l.token, place = s0 + j;
+                        const bool in = l.token < l.tokens && j < n;
+                        Turn r;
+                        if (!VALUE && in) read_turn<MODE>(a, l.c, turn + j * half, r);
+                        const int64_t off = pass == 1 && in ? place_offset(a, places, place, h0) : -1;
+                        const int at = in ? (divide(place, a.pool.scale_tokens) - first_block) * n_heads : 0;
+                        for (int k = 0; k < n_heads; ++k) {
+                            Chunk<DT, MODE> w;
+                            float x[kChunk];
+                            if (in) {
+                                read_chunk(a, view, t.token + (place - t.first), h0 + k, l.c, !VALUE, w);
+                                stored(a, w, l.c, VALUE, r, x);
+                            }
+                            if (pass == 0)
+                                raise(at + k, in, in ? top_of(x) : 0);
+                            else if (off >= 0)
+                                store_codes(plane + off + (int64_t)k * a.pool.part_bytes + l.c * kChunk, x,
+                                            __uint_as_float(top[at + k]));
+                        }
                     }
                 }
+                if (pass == 0) settle_scales(a, t, places, plane, h0, n_heads, top, ratio);
             }
-        }
-        if (pass == 1) break;
-        __syncthreads();
-        /* scales in the place of the magnitudes */
-        for (int i = tid; i < blocks * heads; i += kB) {
-            const int b = i / heads, k = i - b * heads;
-            const int64_t off = place_offset(a, places, (first_block + b) * B, head0 + k);
-            const bool earlier = b == 0 && t.before > 0 && off >= 0;
-            float* at = reinterpret_cast<float*>(plane + off + a.pool.head_dim);
-            float grown;
-            const float scale = block_scale(top[i], earlier, earlier ? *at : 0.0f, grown);
-            if (off >= 0) *at = scale;
-            top[i] = __float_as_uint(scale);
-            if (b == 0) ratio[k] = grown;
-        }
-        __syncthreads();
-        if (t.before == 0) continue;
-        const int words = a.pool.head_dim / 4;
-        for (int i = tid; i < heads * t.before * words; i += kB) {
-            const int v = i / words, k = v / t.before, j = v - k * t.before;
-            if (ratio[k] == 1.0f) continue;
-            const int64_t off = place_offset(a, places, first_block * B + j, head0 + k);
-            if (off < 0) continue;
-            uint32_t* at = reinterpret_cast<uint32_t*>(plane + off) + (i - v * words);
-            *at = regrown(*at, ratio[k]);
         }
     }
 }
 
 /* Workgroups of queries, of keys and of values, one behind the other in y. */
-template <int DT, int MODE>
-__global__ __launch_bounds__(kB, 4) void append_tiles_kernel(AppendArgs a, int tile, int step,
+template <int DT, int MODE, int HELD>
+__global__ __launch_bounds__(kB, 3) void append_tiles_kernel(AppendArgs a, int tile, int step,
                                                              int q_heads, int q_slices, int kv_heads,
                                                              int kv_slices)
 {
@@ -569,23 +672,32 @@ __global__ __launch_bounds__(kB, 4) void append_tiles_kernel(AppendArgs a, int t
     if (!find_tile(a, blockIdx.x, tile, t)) return;
     double2* turn = reinterpret_cast<double2*>(lds); /* [step][rotary_dims / 2] */
     const int blocks = (tile + a.pool.scale_tokens.d - 1) / a.pool.scale_tokens.d;
-    uint32_t* top = reinterpret_cast<uint32_t*>(turn + step * (a.rotary_dims >> 1)); /* [blocks][heads] */
-    float* ratio = reinterpret_cast<float*>(top + blocks * kv_heads);                /* [heads] */
+    uint32_t* top = reinterpret_cast<uint32_t*>(turn + step * (a.rotary_dims >> 1)); /* [blocks][kHeld] */
+    float* ratio = reinterpret_cast<float*>(top + blocks * kHeld);                   /* [kHeld] */
     const int y = blockIdx.y;
     if (y < q_slices)
         append_queries<DT, MODE>(a, t, y * q_heads, q_heads, step, turn);
     else if (y < q_slices + kv_slices)
-        append_heads<DT, MODE, false>(a, t, (y - q_slices) * kv_heads, kv_heads, step, turn, top, ratio);
+        append_heads<DT, MODE, false, HELD>(a, t, (y - q_slices) * kv_heads, kv_heads, step, turn, top, ratio);
     else
-        append_heads<DT, MODE, true>(a, t, (y - q_slices - kv_slices) * kv_heads, kv_heads, step, turn,
-                                     top, ratio);
+        append_heads<DT, MODE, true, HELD>(a, t, (y - q_slices - kv_slices) * kv_heads, kv_heads, step, turn,
+                                           top, ratio);
+}
+
+/* Heads of a workgroup: the more, the fewer angles are computed again; but as few as `unit` where
+ * there would not be kFill workgroups otherwise. */
+int32_t heads_each(int32_t heads, int32_t unit, int64_t tiles)
+{
+    int32_t each = unit;
+    while (each < heads && tiles * ((heads + 2 * each - 1) / (2 * each)) >= kFill) each *= 2;
+    return each < heads ? each : heads;
 }
 
 template <int DT, int MODE>
 hipError_t launch_mode(const AppendArgs& a, hipStream_t stream)
 {
+    const int at_once = kB / 64 * (64 / (a.pool.head_dim / kChunk)); /* vectors of a workgroup */
     if (!a.starts) {
-        const int at_once = kB / 64 * (64 / (a.pool.head_dim / kChunk));
         const int queries = a.q.data ? a.heads : 0;
         const int vectors = queries + (a.k.data ? 2 * a.kv_heads : 0);
         const dim3 grid((unsigned)a.rows, (unsigned)((vectors + at_once - 1) / at_once));
@@ -593,19 +705,24 @@ hipError_t launch_mode(const AppendArgs& a, hipStream_t stream)
     }
     const int B = a.pool.scale_tokens.d, half = a.rotary_dims / 2;
     const int tile = B > kTile ? B : kTile / B * B;
-    int step = half > 0 ? kPairs / half : kStep;
-    step = step > kStep ? kStep : step;
+    int step = half > 0 ? kPairs / half : tile;
     step = step > tile ? tile : step;
-    const int q_heads = a.heads < kQueryHeads ? a.heads : kQueryHeads;
-    const int kv_heads = a.kv_heads < kKeyHeads ? a.kv_heads : kKeyHeads;
+    /* tokens of a thread that it can keep, if it has the angles of all of a tile's */
+    const int tokens = (tile + at_once - 1) / at_once;
+    const int held = step < tile || tokens > kHeld ? 0 : tokens == 3 ? 4 : tokens;
+    const int64_t tiles = (int64_t)a.tokens / tile + 2 * (int64_t)a.rows;
+    const int q_heads = heads_each(a.heads, kQueryHeads, tiles);
+    const int kv_heads = heads_each(a.kv_heads, group_heads(held), tiles);
     const int q_slices = a.q.data ? (a.heads + q_heads - 1) / q_heads : 0;
     const int kv_slices = a.k.data ? (a.kv_heads + kv_heads - 1) / kv_heads : 0;
-    const int64_t tiles = (int64_t)a.tokens / tile + 2 * (int64_t)a.rows;
     const size_t lds = (size_t)step * half * sizeof(double2) +
-                       ((size_t)(tile + B - 1) / B + 1) * kv_heads * sizeof(uint32_t);
+                       ((size_t)(tile + B - 1) / B + 1) * kHeld * sizeof(uint32_t);
     const dim3 grid((unsigned)tiles, (unsigned)(q_slices + 2 * kv_slices));
-    return launch(append_tiles_kernel<DT, MODE>, grid, kB, lds, stream, a, tile, step, q_heads,
-                  q_slices, kv_heads, kv_slices);
+    auto kernel = held == 1   ? append_tiles_kernel<DT, MODE, 1>
+                  : held == 2 ? append_tiles_kernel<DT, MODE, 2>
+                  : held == 4 ? append_tiles_kernel<DT, MODE, 4>
+                              : append_tiles_kernel<DT, MODE, 0>;
+    return launch(kernel, grid, kB, lds, stream, a, tile, step, q_heads, q_slices, kv_heads, kv_slices);
 }
 
 template <int DT>
