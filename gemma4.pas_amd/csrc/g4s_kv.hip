@@ -63,11 +63,11 @@ int check_view(g4s_cache* h, const char* name, const g4s_cache_view* v, int32_t 
     if (!v->data) return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s->data is NULL", name);
     const int64_t d = h->config.head_dim;
     const int64_t ts = tokens > 1 ? v->token_stride : 0, hs = heads > 1 ? v->head_stride : 0;
+    if (ts < 0 || hs < 0 || ts > kMaxElements / tokens || hs > kMaxElements / heads)
+        return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s: a stride is negative or too large", name);
     if (((uintptr_t)v->data & 15) || ((ts * esize) & 15) || ((hs * esize) & 15))
         return fail(h, G4S_ERR_INVALID_ARGUMENT,
                     "%s: data and strides must be multiples of 16 bytes", name);
-    if (ts < 0 || hs < 0 || ts > kMaxElements / tokens || hs > kMaxElements / heads)
-        return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s: a stride is negative or too large", name);
     const int64_t head_end = (heads - 1) * hs + d, token_end = (tokens - 1) * ts + d;
     /* heads within a token, or tokens within a head, none on another */
     const bool a = (heads == 1 || hs >= d) && (tokens == 1 || ts >= head_end);
@@ -200,6 +200,9 @@ G4S_API int g4s_cache_create(g4s_cache** out, const g4s_page_geometry* geometry,
                     "(head_dim + 4 = %d), strides %lld and %lld (multiples of 4)",
                     g.planes, g.parts, c.kv_heads, (long long)g.token_bytes, c.head_dim + 4,
                     (long long)g.plane_stride, (long long)g.page_stride);
+    if ((int64_t)g.max_slots * g.page_tokens > G4S_CACHE_MAX_CONTEXT)
+        return fail(none, G4S_ERR_INVALID_ARGUMENT, "geometry: max_slots %d of %d tokens, a row holds at most %d",
+                    g.max_slots, g.page_tokens, G4S_CACHE_MAX_CONTEXT);
     int device = 0;
     auto refuse = [&](int code, auto... a) { return fail(none, code, a...); };
     int ncu = 0;

@@ -156,8 +156,9 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
     const int m = lane & 15, g = lane >> 4;
 
     /* heads side by side; the last columns of a row, which see most, first */
-    const int head = blockIdx.x, part = blockIdx.z;
-    const int64_t x = (int64_t)gridDim.y - 1 - blockIdx.y;
+    const int slots = (int)(gridDim.x / (uint32_t)a.kv_heads);
+    const int head = (int)(blockIdx.x % (uint32_t)a.kv_heads), part = blockIdx.z;
+    const int64_t x = slots - 1 - (int)(blockIdx.x / (uint32_t)a.kv_heads);
     const Block b = find_block(a, x, CB, KT, splits);
     if (b.cols == 0 || part >= b.parts) return;
     const RowTokens r = b.r;
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
             if (g == 0 && dim0 == 0) put_lse(a, r, at, base[t], sum[t]);
             continue;
         }
-        const int64_t slot = (x * gridDim.x + head) * splits + part;
+        const int64_t slot = (x * a.kv_heads + head) * splits + part;
         float* to = a.ws.sums + slot * kSlotSums + (int64_t)k * D;
 #pragma unroll
         for (int i = 0; i < DB; ++i) *reinterpret_cast<f32x4*>(to + dim0 + i * 16 + g * 4) = o[t][i];
@@ -532,13 +533,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
 template <int DT, int D, int CB, int KT>
 __global__ __launch_bounds__(kJoin) void join_prompts_kernel(AttendArgs a, int splits)
 {
-    const int head = blockIdx.x;
-    const int64_t x = blockIdx.y;
+    const int head = (int)(blockIdx.x % (uint32_t)a.kv_heads);
+    const int64_t x = blockIdx.x / (uint32_t)a.kv_heads;
     const Block b = find_block(a, x, CB, KT, splits);
     if (b.cols == 0 || b.parts == 1) return;
     const int i = blockIdx.z * kJoin + threadIdx.x, k = i / (D / 4), dim = i % (D / 4) * 4;
     if (k >= b.cols || dim >= a.pool.head_dim) return;
-    const int64_t slot = (x * gridDim.x + head) * splits;
+    const int64_t slot = (x * a.kv_heads + head) * splits;
     const float* stats = a.ws.stats + slot * kSlotStats + k * 2;
     const float* sums = a.ws.sums + slot * kSlotSums + (int64_t)k * D + dim;
     Joined j;
@@ -567,11 +568,12 @@ hipError_t prompts_launch(const AttendArgs& a, hipStream_t stream)
     const int64_t items = slots * a.kv_heads;
     int64_t splits = a.ws.groups / 2 / items;
     splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
-    const dim3 grid((unsigned)a.kv_heads, (unsigned)slots, (unsigned)splits);
+    /* (in x, as the other two hold 2^16 - 1 each) */
+    const dim3 grid((unsigned)items, 1, (unsigned)splits);
     const hipError_t e = launch(attend_prompts_kernel<DT, D, NW, NT, KT>, grid, NW * 64,
                                 sizeof(Shared<D, NW, KT, (kLate<D> ? 3 : 2), kHalves<D>>), stream, a, (int)splits);
     if (e != hipSuccess || splits == 1) return e;
-    const dim3 join((unsigned)a.kv_heads, (unsigned)slots, (unsigned)(CB * D / 4 / kJoin));
+    const dim3 join((unsigned)items, 1, (unsigned)(CB * D / 4 / kJoin));
     return launch(join_prompts_kernel<DT, D, CB, KT>, join, kJoin, 0, stream, a, (int)splits);
 }
 

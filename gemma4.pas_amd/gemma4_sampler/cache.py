@@ -17,6 +17,7 @@ MAX_GROUP = 64
 MAX_HEAD_DIM = 512
 MAX_SCALE_TOKENS = 256
 MAX_TOKENS = 1048576
+MAX_CONTEXT = 1073741824
 
 ROTARY = {"halves": 0, "neighbours": 1}
 

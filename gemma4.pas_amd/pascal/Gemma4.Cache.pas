@@ -28,6 +28,7 @@ const
   G4S_CACHE_MAX_HEAD_DIM = 512;
   G4S_CACHE_MAX_SCALE_TOKENS = 256;
   G4S_CACHE_MAX_TOKENS = 1048576;
+  G4S_CACHE_MAX_CONTEXT = 1073741824;
 
   G4S_ROTARY_HALVES = 0;
   G4S_ROTARY_NEIGHBOURS = 1;

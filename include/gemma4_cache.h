@@ -29,13 +29,14 @@ extern "C" {
 #endif
 
 /* Most heads of queries and of keys, query heads of one key head, dims of a head, tokens that
- * share a scale, and tokens of a call. */
+ * share a scale, tokens of a call, and tokens that a row has slots for. */
 #define G4S_CACHE_MAX_HEADS 512
 #define G4S_CACHE_MAX_KV_HEADS 64
 #define G4S_CACHE_MAX_GROUP 64
 #define G4S_CACHE_MAX_HEAD_DIM 512
 #define G4S_CACHE_MAX_SCALE_TOKENS 256
 #define G4S_CACHE_MAX_TOKENS 1048576
+#define G4S_CACHE_MAX_CONTEXT 1073741824
 
 /* Which dims of a head the rotation pairs, j = 0 .. rotary_dims / 2 - 1. */
 #define G4S_ROTARY_HALVES 0     /* j and j + rotary_dims / 2 */
@@ -127,9 +128,9 @@ int g4s_cache_append(g4s_cache* cache, const g4s_page_state* state, int32_t rows
  *   rows, d_starts, tokens, dtype   as for g4s_cache_append (q and out)
  *   d_lse      device [tokens * heads], or NULL
  * A query that sees nothing (a row that has ended) gets zeros and -inf.  A
- * query that is not finite, one that sees a NaN, or a page outside the pool,
- * gets NaN, and so does every query of a row whose length is outside the
- * table.  What a query does not see does not count, whatever it is.  Queries that no
+ * query that is not finite, one that sees a NaN among the keys, or a page outside the
+ * pool, gets NaN, and so does every query of a row whose length is outside the
+ * table; a NaN among the values gives one in its dim.  What a query does not see does not count, whatever it is.  Queries that no
  * row has are left alone.  An output that overlaps another array of the call is
  * refused.  Stream-ordered; the same call gives the same bits. */
 int g4s_cache_attend(g4s_cache* cache, const g4s_page_state* state, int32_t rows,

@@ -50,7 +50,8 @@ def test_config_limits(change):
     dict(planes=1), dict(planes=0), dict(parts=1), dict(parts=3), dict(token_bytes=64),
     dict(token_bytes=72), dict(page_stride=16 * 2 * 68 + 2),
     dict(plane_stride=16 * 2 * 68 * 8 + 1), dict(n_pages=0), dict(page_tokens=18),
-    dict(max_slots=0), dict(page_stride=100)])
+    dict(max_slots=0), dict(page_stride=100),
+    dict(page_tokens=65536, max_slots=16385, n_pages=1)])
 def test_geometry_limits(change):
     with pytest.raises(native.SamplerError) as e:
         cache.KvCache(geo(**change), **GOOD)
@@ -113,7 +114,7 @@ def test_pascal_and_python_constants_match_the_header(unit):
     want = {n: int(v) for n, v in re.findall(r"#define\s+(G4S_\w+)\s+(\d+)", shared._c(HEADER))}
     got = {n: int(v) for n, v in re.findall(r"\b(G4S_\w+)\s*=\s*(\d+)\s*;", shared._pascal())}
     assert got == want
-    for name in ("HEADS", "KV_HEADS", "GROUP", "HEAD_DIM", "SCALE_TOKENS", "TOKENS"):
+    for name in ("HEADS", "KV_HEADS", "GROUP", "HEAD_DIM", "SCALE_TOKENS", "TOKENS", "CONTEXT"):
         assert getattr(cache, "MAX_" + name) == want["G4S_CACHE_MAX_" + name]
     assert cache.ROTARY == {"halves": want["G4S_ROTARY_HALVES"],
                             "neighbours": want["G4S_ROTARY_NEIGHBOURS"]}
