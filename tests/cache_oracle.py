@@ -179,10 +179,10 @@ def limits(to, dim, dtype):
     A score is a sum of dim products (exact) in 32 bits, scaled and taken to base two: it is off by
     at most (dim + 8) / 2^24 of `size`, and so is the maximum under it.  A sum over the tokens
     seen, with a rounding each and a few for the exponential and the joining: seen + 16 steps
-    of 2^-23.  Weights are rounded to bf16 (2^-8), or to two bf16 pieces (2^-16)."""
+    of 2^-23.  Weights are rounded to bf16 (2^-8) for bf16 outputs alone."""
     score = (dim + 8) * 2.0 ** -24 * to.size
     sums = (to.seen + 16) * 2.0 ** -23
-    weight, half = (2.0 ** -16, 2.0 ** -24) if dtype == "f32" else (2.0 ** -8, 2.0 ** -8)
+    weight, half = (0.0, 2.0 ** -24) if dtype == "f32" else (2.0 ** -8, 2.0 ** -8)
     rel = 2 * score + sums + weight
     out = rel[..., None] * to.mass + half * np.abs(to.out) + 1e-37
     lse = score + sums + 2.0 ** -23 * np.abs(np.where(np.isfinite(to.lse), to.lse, 0.0))
