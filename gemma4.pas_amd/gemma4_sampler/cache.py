@@ -8,7 +8,7 @@ a failing call raises native.SamplerError.
 import ctypes
 
 from . import native
-from .beam import PageCache, PageGeometry, PageState, _ref, _stream  # noqa: F401
+from .beam import PageCache, PageGeometry, PageState, _stream  # noqa: F401
 from .native import DTYPE_BF16, DTYPE_F32, G4S_OK, SamplerError, _ptr  # noqa: F401
 
 MAX_HEADS = 512
@@ -37,6 +37,7 @@ class View(ctypes.Structure):
     def __init__(self, data, token_stride, head_stride):
         super().__init__(_ptr(data), int(token_stride), int(head_stride))
         self._owners = (data,)
+        self._at = ctypes.addressof(self)
 
 
 def geometry(page_tokens, n_pages, max_rows, max_slots, kv_heads, head_dim, planes=2,
@@ -49,6 +50,16 @@ def geometry(page_tokens, n_pages, max_rows, max_slots, kv_heads, head_dim, plan
     plane_stride = page_stride * int(n_pages) if plane_stride is None else int(plane_stride)
     return PageGeometry(int(page_tokens), int(n_pages), int(max_rows), int(max_slots),
                         int(planes), int(kv_heads), token, plane_stride, page_stride)
+
+
+def _address(x):
+    """What a pointer argument takes, without a new object for most: a step's calls are as
+    long on the host as on the GPU."""
+    if x is None or type(x) is int:
+        return x
+    if type(x) is View:
+        return x._at
+    return ctypes.byref(x) if isinstance(x, ctypes.Structure) else _ptr(x)
 
 
 _bound = False
@@ -77,7 +88,7 @@ class KvCache:
 
     def __init__(self, geometry, heads, kv_heads, head_dim, scale_tokens=1, rotary_dims=None,
                  rotary_pairs="halves", stream=None):
-        self.h = None
+        self.h = self._at = None
         L = load()
         rotary = int(head_dim) if rotary_dims is None else int(rotary_dims)
         self.geometry = geometry
@@ -89,6 +100,7 @@ class KvCache:
         if rc != G4S_OK:
             raise SamplerError(rc, L.g4s_cache_last_error(None).decode())
         self.h = h
+        self._at, self._append, self._attend = h.value, L.g4s_cache_append, L.g4s_cache_attend
 
     def last_error(self):
         return load().g4s_cache_last_error(self.h).decode()
@@ -100,23 +112,26 @@ class KvCache:
     def append(self, state, rows, tokens, dtype, d_pool=None, k_plane=0, v_plane=1, q=None, k=None,
                v=None, q_out=None, d_starts=None, d_positions=None, d_freqs=None):
         """g4s_cache_append (stream-ordered); q, k, v and q_out are Views"""
-        self._check(load().g4s_cache_append(
-            self.h, _ref(state), int(rows), _ptr(d_starts), int(tokens), int(dtype), _ref(q),
-            _ref(k), _ref(v), _ref(q_out), _ptr(d_positions), _ptr(d_freqs), _ptr(d_pool),
-            int(k_plane), int(v_plane)))
+        rc = self._append(self._at, _address(state), int(rows), _address(d_starts), int(tokens),
+                          int(dtype), _address(q), _address(k), _address(v), _address(q_out),
+                          _address(d_positions), _address(d_freqs), _address(d_pool),
+                          int(k_plane), int(v_plane))
+        if rc:
+            self._check(rc)
 
     def attend(self, state, rows, tokens, dtype, d_pool, k_plane, v_plane, q, out, scale, window=0,
                d_starts=None, d_lse=None):
         """g4s_cache_attend (stream-ordered); q and out are Views"""
-        self._check(load().g4s_cache_attend(
-            self.h, _ref(state), int(rows), _ptr(d_starts), int(tokens), int(dtype), _ref(q),
-            _ptr(d_pool), int(k_plane), int(v_plane), float(scale), int(window), _ref(out),
-            _ptr(d_lse)))
+        rc = self._attend(self._at, _address(state), int(rows), _address(d_starts), int(tokens),
+                          int(dtype), _address(q), _address(d_pool), int(k_plane), int(v_plane),
+                          float(scale), int(window), _address(out), _address(d_lse))
+        if rc:
+            self._check(rc)
 
     def close(self):
         if self.h is not None and self.h.value:
             load().g4s_cache_destroy(self.h)
-        self.h = None
+        self.h = self._at = None
 
     def __del__(self):
         try:
