@@ -893,11 +893,15 @@ hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
     const int64_t most = (int64_t)a.rows * a.kv_heads * blocks * units;
     const int resident = a.ws.groups / 2 * (kResident / NW);
     const int groups = most < resident ? (int)most : resident;
-    /* the most that can be left to be joined of one item: a launch of its own is enqueued only
-     * where it may have something to do */
+    /* the most that can be left to be joined of one item, of one row's tokens or of rows that are taken
+     * together: a launch of its own is enqueued only where it may have something to do */
     const int64_t cols = (int64_t)a.tokens * a.group.d < kCols ? (int64_t)a.tokens * a.group.d : kCols;
-    const int64_t share = groups / a.kv_heads + 2, parts = units * together < share ? units * together : share;
-    const int joins = parts * cols * D * 4 > kJoinBytes;
+    const int64_t share = groups / a.kv_heads + 2;
+    const int64_t parts = units < share ? units : share;
+    const int64_t parts_of_all = units * together < share ? units * together : share;
+    const int64_t cols_of_all = together * a.group.d < kCols ? together * a.group.d : kCols;
+    const int64_t one = parts * cols, all = parts_of_all * cols_of_all;
+    const int joins = (one > all ? one : all) * D * 4 > kJoinBytes;
     hipError_t e = launch(attend_rows_kernel<DT, D>, groups, NW * 64, lds, stream, a, joins);
     if (e != hipSuccess || !joins) return e;
     return launch(join_rows_kernel<DT, D>, dim3((unsigned)groups, (unsigned)(kCols / kJoinCols)), kB, 0,
