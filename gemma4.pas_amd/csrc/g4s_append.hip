@@ -3,14 +3,20 @@
  * rotated by their positions on the way, and the queries rotated beside
  * them, on gfx950.
  *
- * A workgroup takes up to `tile` places of one row, whole blocks of tokens that share a
- * scale, so that a scale and the codes under it have one writer, and some of the heads: of
- * queries, or of keys and values.  Those it goes over twice, for the largest
- * magnitude of each block and head, and to store them (the second time they come
- * from registers where a thread has one vector, from the caches otherwise).
- * Keys are rotated in binary64 and rounded once: next to a border between two codes a
- * rounding in between would choose the other one.  Cosines and sines are computed once per
- * token and pair, in LDS for all heads of the workgroup.
+ * A code is x / scale with a scale that depends on all of a block's new values, so the vectors are looked
+ * at twice: for the largest magnitude of each block and head, and to store them.  A
+ * workgroup takes up to `tile` places of one row, whole blocks of tokens that share a scale, so that
+ * a scale and the codes under it have one writer, and some of the heads: of queries, or of keys
+ * and values.  A thread keeps its vectors in registers between the looks where a tile has no more than
+ * four tokens for it (read twice, from the caches, they took 174 instead of 115 us for seven prompts of
+ * 2,000 tokens, 32 and 8 heads of 128 dims).  Keys are rotated in binary64 and rounded once: next to a
+ * border between two codes a rounding in between would choose the other one.  Cosines and sines
+ * are computed once per token and pair, in LDS for all heads of the workgroup.
+ *
+ * One token a row: 4.0 us for a row and 4.9 for 192, the latency of a launch and of lengths, page, scale
+ * and vectors one after the other.  The seven prompts: 115 us for 361 MB (3.1 TB/s, a copy 4.9): queries alone
+ * 66, keys and values alone 57, of which the angles are 16; the vector units' issue (binary64) next to
+ * memory that two to three workgroups a CU keep waiting.
  */
 #include "g4s_cache.h"
 #include "g4s_device.h"
@@ -558,7 +564,8 @@ __device__ __forceinline__ void one_by_one()
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
 }
-/* Heads at once. */
+/* Heads at once: as many vectors as a thread holds (one head each where it holds two tokens: 133 us for the
+ * prompts instead of 123). */
 constexpr int group_heads(int held) { return held > 0 ? kHeld / held : kHeld; }
 template <int DT, int MODE, bool VALUE, int HELD>
 __device__ __forceinline__ void append_heads(const AppendArgs& a, const Tile& t, int head0, int heads,
@@ -663,7 +670,8 @@ __device__ __forceinline__ void append_heads(const AppendArgs& a, const Tile& t,
 
 /* Workgroups of queries, of keys and of values, one behind the other in y. */
 template <int DT, int MODE, int HELD>
-__global__ __launch_bounds__(kB, 3) void append_tiles_kernel(AppendArgs a, int tile, int step,
+__global__ __launch_bounds__(kB, 3) /* (123 us for the prompts; 2: 144, 4: 143, which spills) */
+void append_tiles_kernel(AppendArgs a, int tile, int step,
                                                              int q_heads, int q_slices, int kv_heads,
                                                              int kv_slices)
 {
@@ -685,7 +693,8 @@ __global__ __launch_bounds__(kB, 3) void append_tiles_kernel(AppendArgs a, int t
 }
 
 /* Heads of a workgroup: the more, the fewer angles are computed again; but as few as `unit` where
- * there would not be kFill workgroups otherwise. */
+ * there would not be kFill workgroups otherwise (the prompts' queries: 67 us with 768, 66 with 400, 83
+ * with 1,500; keys without angles 80, 69 and 98). */
 int32_t heads_each(int32_t heads, int32_t unit, int64_t tiles)
 {
     int32_t each = unit;

@@ -6,11 +6,19 @@
  * with one prompt) are taken together, as far as 16 query columns hold them: as long as
  * their pages are the same a tile of keys and values is read once for all, from the first
  * page on that differs each row's tiles by themselves.  The work of a launch, counted in units of
- * NW x 32 tokens of one such group and key head, is shared out evenly over the
+ * NW x TT tokens of one such group and key head, is shared out evenly over the
  * workgroups, whatever the lengths; every workgroup finds its share from them by itself.  A wave
- * takes 32 tokens of each unit with a softmax of its own; the waves join in LDS, and where several
+ * takes TT tokens of each unit with a softmax of its own; the waves join in LDS, and where several
  * workgroups have parts of one group and head, the one that ends last joins those, in their
- * order, so that results do not depend on who that is.
+ * order, so that results do not depend on who that is; many parts are joined by a launch of their own.
+ *
+ * Scores are products of the widened codes (exact in bf16) with the queries as matrix operands, K Q^T,
+ * so that a lane holds scores of one column and multiplies them, as weights, with V^T without
+ * an exchange.  All that is read is read once, one step ahead of its use: 131,071 tokens of 8 heads of 128
+ * dims 60 us (4.5 TB/s; this card reads 6.1 at most), 64 rows of 3,000 to 5,000 tokens 99 us (4.7
+ * TB/s; 5.4 between start and end).  What is left is the start (lengths and tables 2 to 8 us, queries 1 to 6, page, scales
+ * and codes one behind the other 2 to 8) and the joins (3 to 8 us, 4 to 11 in their own launch): 12
+ * searches of 4 beams over 3,800 tokens, 512 dims in binary32, 84 us, of which the steps are 26.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -22,7 +30,8 @@ namespace {
 constexpr int kB = 256;
 constexpr int kCols = 16;  /* query columns of a workgroup's part */
 /* Bytes of parts that their last workgroup joins by itself: more are left to a launch of
- * their own. */
+ * their own (the 12 searches of 512 dims: 86 us, 100 without it; 192 rows with windows of 512: 38.5 and, all
+ * joined by it, 41). */
 constexpr int kJoinBytes = 96 << 10;
 
 /* What the scan keeps of a row: its length (bad: -1), and the first page of one that may be taken
@@ -255,8 +264,10 @@ __device__ __forceinline__ void put(const AttendArgs& a, int64_t out, int64_t ls
 }
 
 /* How a kernel is made for a width of heads: tokens of a wave's step, as many as its registers
- * hold beside the sums (16, 32 or 64); waves, of which eight are a CU's; and units that a workgroup
- * takes at least where there are enough of them. */
+ * hold beside the sums (16, 32 or 64); waves, of which eight are a CU's (131,071 tokens of 128 dims: 60 us with
+ * workgroups of eight, which have half the parts to join, and 64 of four; 12 rows of 3,800 of 512 dims 82 and
+ * 67, as their units are then twice as long); and units that a workgroup takes at least where there are enough of
+ * them (1, 2 and 4 of them: 49, 39 and 44 us for the windows of 256 dims, 89, 88 and 83 for the searches of 512). */
 constexpr int kResident = 8;
 template <int DT, int D>
 struct Shape {
@@ -291,7 +302,8 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
     if (joins && tid == 0) a.ws.records[blockIdx.x].parts = 0;
     scan_rows<NW, UNIT>(a, info, group, before, s.wave);
     const int64_t total = before[a.rows];
-    /* one unit a workgroup while that leaves CUs without any, and UNITS at least of each otherwise */
+    /* one unit a workgroup while that leaves CUs without any, and UNITS at least of each otherwise (501
+     * tokens of 256 dims: 11 us, 15 with UNITS) */
     constexpr int UNITS = Shape<DT, D>::UNITS;
     const int64_t one_each = total < a.ws.groups / 2 ? total : a.ws.groups / 2;
     int64_t groups = (total + UNITS - 1) / UNITS;

@@ -5,9 +5,18 @@
  * A workgroup takes NW x NT x 16 query columns (tokens x heads of one key head) and goes over the
  * tokens that they see in tiles of KT: all its threads widen the next tile's codes into LDS, keys as
  * [token][dim] and values as [dim][token], while its waves multiply the present one, each
- * for NT x 16 columns of its own with the softmax in registers.  Where there are fewer columns than
+ * for NT x 16 columns of its own with the softmax in registers: K Q^T leaves a lane scores of one column,
+ * which are an operand of V^T P^T as they are.  The exponents' base moves only when a score passes it
+ * by 2^8, so that the sums are seldom multiplied.  Where there are fewer columns than
  * workgroups the tokens are split too, and a second launch joins what the parts of a block
  * found, in their order.
+ *
+ * Four prompts of 4,000 tokens, 32 and 8 heads of 128 dims: 750 us, 784 TFLOP/s of the 1,260 that a large
+ * bf16 product reaches here; bound by the vector units' issue (exponentials, weights, widened
+ * codes) beside the products.  256 tokens behind 7,844, 8 and 2 heads of 256 dims: 50 us (333 TFLOP/s), of which the joining
+ * launch is 8 and start and end 10: a wave's 16 columns are all that its registers hold beside their sums, so
+ * that LDS is read once for each 16 (1.7 us of a tile's 2.7).  Binary32 costs three times the products: the first
+ * prompts 1.58 ms.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -109,10 +118,11 @@ struct Shared {
 };
 
 /* Waves that share columns, each with a part of their dims: one wave's registers do not hold the
- * queries and sums of 512. */
+ * queries and sums of 512 (256 tokens behind 7,844: 112 us and, binary32, 140; alone 169 and 425). */
 template <int D>
 constexpr int kHalves = D > 256 ? 2 : 1;
-/* LDS holds a third tile of values, so that waves may be a phase apart. */
+/* LDS holds a third tile of values, so that waves may be a phase apart (the four prompts: 752 us, 779 in
+ * step; with 64 dims 605 and 637). */
 template <int D>
 constexpr bool kLate = D <= 128;
 
@@ -588,6 +598,8 @@ template <int DT>
 hipError_t by_width(const AttendArgs& a, hipStream_t stream)
 {
     constexpr bool F32 = DT == G4S_DTYPE_F32;
+    /* (32 columns a wave where they fit: with 256 dims, in four waves or tiles of 32, they took 74 and 128
+     * us for the chunk instead of 54; 64 dims in eight waves 609 us, in four 605) */
     switch (attend_width(a.pool.head_dim)) {
     case 64: return prompts_launch<DT, 64, 4, F32 ? 1 : 2, 64>(a, stream);
     case 128: return prompts_launch<DT, 128, 8, F32 ? 1 : 2, 64>(a, stream);
