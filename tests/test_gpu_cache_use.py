@@ -421,6 +421,17 @@ def test_one_row_with_fewer_tokens_than_views(news):
     rig.attend(window=30)
 
 
+@pytest.mark.parametrize("length", [-1, 7 * 16 + 1])
+@pytest.mark.parametrize("news", [None, [1], [40]])
+def test_one_row_whose_length_is_none(length, news):
+    """NaN for all of its queries, and nothing appended."""
+    rig = Rig([90], news=news, kv=1, group=4)
+    rig.lengths[0] = length
+    rig.upload()
+    rig.append()
+    rig.attend()
+
+
 @pytest.mark.parametrize("d", [512, 128, 16])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_most_rows(d, dtype):
