@@ -202,9 +202,10 @@ hipError_t attend_prompts_launch(const AttendArgs& a, int32_t dtype, hipStream_t
 
 /* Rows with more than one token and more than `few` columns (tokens x heads of a key head)
  * are the prompts' kernel's, the others the rows' kernel's, which takes 16 columns a pass over the
- * tokens.  Eight rows of 3,500 tokens, 4 heads of 128 dims (2 binary32 groups of 4, of 256) a key head:
- * 32 columns 49 (44) us by rows and 74 (57) by prompts, 64 columns 100 (94) and 77 (65). */
-constexpr int kFewCols = 32;
+ * tokens.  Eight rows of some 3,500 tokens, 8 key heads with 4 heads of 128 dims (2 of 256, binary32):
+ * 24 columns a row 45 (41) us by rows and 59 (54) by prompts, 48 columns 63 (48) and 74 (59).  Rows on
+ * both sides cost both kernels, one behind the other: 99 (79) us. */
+constexpr int kFewCols = 48;
 G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group, int32_t few)
 {
     return (int64_t)count * group > few && (count > 1 || few == 0);
