@@ -50,6 +50,13 @@ __device__ __forceinline__ float column_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+/* The first place that a query at `place` (which may be negative) sees. */
+__device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
+{
+    const int from = a.window > 0 ? (int)((uint32_t)place - (uint32_t)a.window + 1u) : 0;
+    return from > 0 && a.window <= place ? from : 0;
+}
+
 /* Bit i: whether token tile0 + shift + i is one of first .. last. */
 __device__ __forceinline__ uint64_t seen_bits(int tile0, int first, int last, int shift)
 {

@@ -52,12 +52,6 @@ struct Group {
 };
 constexpr int kNone = 0x7FFFFFFF;
 
-__device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
-{
-    const int from = a.window > 0 ? (int)((uint32_t)place - (uint32_t)a.window + 1u) : 0;
-    return from > 0 && a.window <= place ? from : 0;
-}
-
 /* Rows that are taken together at most: a power of two, of rows that begin at a multiple of it. */
 __device__ __forceinline__ int group_rows(const AttendArgs& a)
 {

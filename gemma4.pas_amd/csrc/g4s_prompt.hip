@@ -43,11 +43,6 @@ struct Block {
     int first, tiles; /* tiles of them */
     int parts;        /* workgroups that share the tiles */
 };
-__device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
-{
-    const int64_t f = a.window > 0 ? (int64_t)place - a.window + 1 : 0;
-    return f > 0 ? (int)f : 0;
-}
 __device__ __forceinline__ Block find_block(const AttendArgs& a, int64_t x, int unit, int tile,
                                             int splits)
 {
