@@ -28,7 +28,6 @@ namespace g4s {
 namespace {
 
 constexpr int kB = 256;
-constexpr int kCols = 16;  /* query columns of a workgroup's part */
 /* Bytes of parts that their last workgroup joins by itself: more are left to a launch of
  * their own (the 12 searches of 512 dims: 86 us, 100 without it; 192 rows with windows of 512: 38.5 and, all
  * joined by it, 41). */
@@ -107,8 +106,7 @@ __device__ __forceinline__ int group_cols(const AttendArgs& a, const Group& p)
 template <int UNIT>
 __device__ __forceinline__ int group_units(const Group& p)
 {
-    if (p.end <= p.from) return 1;
-    const int n = last_unit<UNIT>(p) - p.from / UNIT;
+    const int n = place_units(p.from, p.end, UNIT);
     return p.rows > 1 ? p.shared + (n - p.shared) * p.rows : n;
 }
 
@@ -184,7 +182,7 @@ __device__ __forceinline__ void scan_rows(const AttendArgs& a, RowInfo* info, Gr
         const int r = tid * each + i;
         if (r >= a.rows) break;
         const Group p = find_group<UNIT>(a, info, r);
-        const int blocks = (group_cols(a, p) + kCols - 1) / kCols;
+        const int blocks = column_blocks(group_cols(a, p));
         groups[r] = p;
         before[r + 1] = (int64_t)(blocks * a.kv_heads) * group_units<UNIT>(p);
         sum += before[r + 1];
@@ -257,24 +255,18 @@ __device__ __forceinline__ void put(const AttendArgs& a, int64_t out, int64_t ls
     if (dim == 0 && a.lse) a.lse[lse] = none ? -inf32() : (top + __builtin_amdgcn_logf(sum)) * kLn2;
 }
 
-/* How a kernel is made for a width of heads: tokens of a wave's step, as many as its registers
- * hold beside the sums (16, 32 or 64); waves, of which eight are a CU's (131,071 tokens of 128 dims: 60 us with
- * workgroups of eight, which have half the parts to join, and 64 of four; 12 rows of 3,800 of 512 dims 82 and
- * 67, as their units are then twice as long); and units that a workgroup takes at least where there are enough of
- * them (1, 2 and 4 of them: 49, 39 and 44 us for the windows of 256 dims, 89, 88 and 83 for the searches of 512). */
+/* rows_shape: tokens of a wave's step, as many as its registers hold beside the sums (16, 32 or 64); waves, of
+ * which eight are a CU's (131,071 tokens of 128 dims: 60 us with workgroups of eight, which have half the
+ * parts to join, and 64 of four; 12 rows of 3,800 of 512 dims 82 and 67, as their units are then twice as long);
+ * and units that a workgroup takes at least where there are enough of them (1, 2 and 4 of them: 49, 39 and 44 us
+ * for the windows of 256 dims, 89, 88 and 83 for the searches of 512). */
 constexpr int kResident = 8;
-template <int DT, int D>
-struct Shape {
-    static constexpr int NW = D <= 128 ? 8 : 4;
-    static constexpr int TT = D <= 128 ? 64 : D <= 256 ? 32 : 16;
-    static constexpr int UNITS = D <= 128 ? 1 : D <= 256 ? 2 : 4;
-};
 
 template <int DT, int D>
-__global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel(AttendArgs a, int joins)
+__global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kernel(AttendArgs a, int joins)
 {
-    constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT;
-    constexpr int UNIT = NW * TT;
+    constexpr int NW = rows_shape(D).waves, TT = rows_shape(D).tokens;
+    constexpr int UNIT = rows_shape(D).unit();
     constexpr int NB = TT / 16;                     /* blocks of 16 tokens of a step */
     constexpr int NJ = TT < 32 ? 4 : 8;             /* tokens of a lane in a product with V .. */
     constexpr int NH = TT / (4 * NJ);               /* .. of which a step has so many */
@@ -296,13 +288,8 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
     if (joins && tid == 0) a.ws.records[blockIdx.x].parts = 0;
     scan_rows<NW, UNIT>(a, info, group, before, s.wave);
     const int64_t total = before[a.rows];
-    /* one unit a workgroup while that leaves CUs without any, and UNITS at least of each otherwise (501
-     * tokens of 256 dims: 11 us, 15 with UNITS) */
-    constexpr int UNITS = Shape<DT, D>::UNITS;
-    const int64_t one_each = total < a.ws.groups / 2 ? total : a.ws.groups / 2;
-    int64_t groups = (total + UNITS - 1) / UNITS;
-    groups = groups < one_each ? one_each : groups < gridDim.x ? groups : gridDim.x;
-    if (blockIdx.x >= groups) return;
+    const int groups = sharing_groups(total, rows_shape(D).units, a.ws.groups / 2, (int)gridDim.x);
+    if ((int)blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
     const int64_t x_end = first_unit(total, blockIdx.x + 1, groups);
     /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
@@ -327,7 +314,7 @@ __global__ __launch_bounds__((Shape<DT, D>::NW * 64), 2) void attend_rows_kernel
         p.end = __builtin_amdgcn_readfirstlane(p.end);
         p.shared = __builtin_amdgcn_readfirstlane(p.shared);
         const bool several = p.rows > 1; /* rows */
-        const int all_cols = group_cols(a, p), blocks = (all_cols + kCols - 1) / kCols;
+        const int all_cols = group_cols(a, p), blocks = column_blocks(all_cols);
         const int units = group_units<UNIT>(p), first = p.from / UNIT;
         const int64_t in_group = x - before[lo];
         const int item = __builtin_amdgcn_readfirstlane((int)quotient(in_group, units));
@@ -889,14 +876,14 @@ __global__ __launch_bounds__(kB) void join_rows_kernel(AttendArgs a)
 template <int DT, int D>
 hipError_t rows_launch(const AttendArgs& a, hipStream_t stream)
 {
-    constexpr int NW = Shape<DT, D>::NW, TT = Shape<DT, D>::TT, UNIT = NW * TT;
+    constexpr int NW = rows_shape(D).waves, TT = rows_shape(D).tokens, UNIT = rows_shape(D).unit();
     const size_t lds = ((sizeof(Shared<DT, D, NW, TT>) + 15) & ~(size_t)15) + ((size_t)a.rows + 1) * 8 +
                        (size_t)a.rows * (sizeof(RowInfo) + sizeof(Group));
     /* no more workgroups than the rows can have use for */
-    const int64_t blocks = (a.group.d + kCols - 1) / kCols;
+    const int64_t most = most_units(a.rows, a.tokens, a.starts, a.kv_heads, a.group.d, a.few,
+                                    cache_room(a.pool), UNIT);
     const int64_t units = (cache_room(a.pool) + UNIT - 1) / UNIT + 1;
     const int64_t together = kCols / a.group.d < 1 ? 1 : kCols / a.group.d < a.rows ? kCols / a.group.d : a.rows;
-    const int64_t most = (int64_t)a.rows * a.kv_heads * blocks * units;
     const int resident = a.ws.groups / 2 * (kResident / NW);
     const int groups = most < resident ? (int)most : resident;
     /* the most that can be left to be joined of one item, of one row's tokens or of rows that are taken
@@ -931,11 +918,6 @@ __global__ void attend_init_kernel(uint32_t* tickets, int n)
 }
 
 }  // namespace
-
-int32_t attend_width(int32_t head_dim)
-{
-    return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512;
-}
 
 int32_t attend_groups(int32_t ncu) { return 2 * ncu; }
 

@@ -109,6 +109,62 @@ G4S_PAGE_HD int32_t unit_group(int64_t x, int64_t total, int32_t groups)
     return (int32_t)quotient((x + 1) * groups - 1, total);
 }
 
+/* Dims that the attention's kernels are made for, at least head_dim. */
+G4S_PAGE_HD int32_t attend_width(int32_t head_dim)
+{
+    return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : head_dim <= 256 ? 256 : 512;
+}
+
+/* Query columns (tokens x heads of a key head) that the rows' kernel takes in a pass over the tokens, and how it is
+ * made for a width of heads: waves of a workgroup, tokens of a wave's step, and units of `waves` steps
+ * that a workgroup takes at least where there are enough of them. */
+constexpr int kCols = 16;
+struct RowsShape {
+    int32_t waves, tokens, units;
+    G4S_PAGE_HD constexpr int32_t unit() const { return waves * tokens; }
+};
+G4S_PAGE_HD constexpr RowsShape rows_shape(int32_t width)
+{
+    return width <= 128 ? RowsShape{8, 64, 1} : width <= 256 ? RowsShape{4, 32, 2} : RowsShape{4, 16, 4};
+}
+
+/* Rows with more than one token and more than `few` columns (tokens x heads of a key head)
+ * are the prompts' kernel's, the others the rows' kernel's, which takes 16 columns a pass over the
+ * tokens.  Eight rows of some 3,500 tokens, 8 key heads with 4 heads of 128 dims (2 of 256, binary32):
+ * 24 columns a row 45 (41) us by rows and 59 (54) by prompts, 48 columns 63 (48) and 74 (59).  Rows on
+ * both sides cost both kernels, one behind the other: 99 (79) us. */
+constexpr int kFewCols = 48;
+G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group, int32_t few)
+{
+    return (int64_t)count * group > few && (count > 1 || few == 0);
+}
+
+/* Units of `unit` tokens that places from .. end - 1 lie in: one at least, for the output. */
+G4S_PAGE_HD int32_t place_units(int32_t from, int32_t end, int32_t unit)
+{
+    return end > from ? (int32_t)(((uint32_t)end + unit - 1) / unit) - from / unit : 1;
+}
+G4S_PAGE_HD int32_t column_blocks(int32_t cols) { return (cols + kCols - 1) / kCols; }
+
+/* The most units of a call's rows: each block of a row's columns, for each key head, goes over the row's places.  A
+ * row of the rows' kernel has one token, or (with d_starts) as many as `few` columns hold; rows that
+ * are taken together have no more than each by itself. */
+G4S_PAGE_HD int64_t most_units(int32_t rows, int32_t tokens, bool starts, int32_t kv_heads, int32_t group,
+                               int32_t few, int64_t room, int32_t unit)
+{
+    int64_t cols = (int64_t)tokens * group < few ? (int64_t)tokens * group : few;
+    cols = starts && cols > group ? cols : group;
+    return (int64_t)rows * kv_heads * column_blocks((int32_t)cols) * ((room + unit - 1) / unit + 1);
+}
+/* Workgroups, of a grid, that share `total` units: one unit each while that leaves CUs without any, and
+ * `units` at least of each otherwise (501 tokens of 256 dims: 11 us, 15 with two at least). */
+G4S_PAGE_HD int32_t sharing_groups(int64_t total, int32_t units, int32_t ncu, int32_t grid)
+{
+    const int64_t one_each = total < ncu ? total : ncu, several = (total + units - 1) / units;
+    const int64_t groups = several < one_each ? one_each : several;
+    return (int32_t)(groups < grid ? groups : grid);
+}
+
 /* Where a row's slots of a grid begin: `times` columns a token, `unit` columns a slot.  A row of
  * n tokens has floor(n * times / unit) + extra slots at least. */
 G4S_PAGE_HD int64_t share_begin(const int32_t* starts, int32_t row, int32_t times, int32_t unit,
@@ -200,20 +256,7 @@ hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream)
 hipError_t attend_rows_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t attend_prompts_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 
-/* Rows with more than one token and more than `few` columns (tokens x heads of a key head)
- * are the prompts' kernel's, the others the rows' kernel's, which takes 16 columns a pass over the
- * tokens.  Eight rows of some 3,500 tokens, 8 key heads with 4 heads of 128 dims (2 of 256, binary32):
- * 24 columns a row 45 (41) us by rows and 59 (54) by prompts, 48 columns 63 (48) and 74 (59).  Rows on
- * both sides cost both kernels, one behind the other: 99 (79) us. */
-constexpr int kFewCols = 48;
-G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group, int32_t few)
-{
-    return (int64_t)count * group > few && (count > 1 || few == 0);
-}
-
 int32_t attend_groups(int32_t ncu);
-/* Dims that the kernels are made for, at least head_dim. */
-int32_t attend_width(int32_t head_dim);
 hipError_t attend_init_launch(const AttendSpace& ws, hipStream_t stream);
 
 #endif

@@ -72,4 +72,43 @@ int t_units_shared(int64_t total, int32_t groups)
     }
     return 1;
 }
+/* The rows' kernel's share of a call (rows of `counts` tokens, none taken together; those with more columns
+ * than kFewCols are the prompts' kernel's): 0, or what is wrong with it.  1: more units than
+ * the grid is made for, 2: work is shared among workgroups that the grid does not have, 3: units that are
+ * no workgroup's, 4: an item whose parts are not those that its last workgroup waits for. */
+int t_rows_share(int32_t head_dim, int32_t kv_heads, int32_t group, int32_t rows, int32_t tokens,
+                 const int32_t* counts, int starts, const int32_t* lengths, int64_t room, int32_t window,
+                 int32_t ncu)
+{
+    const RowsShape shape = rows_shape(attend_width(head_dim));
+    const int32_t unit = shape.unit(), resident = ncu * (8 / shape.waves);
+    const int64_t most = most_units(rows, tokens, starts, kv_heads, group, kFewCols, room, unit);
+    const int32_t grid = most < resident ? (int32_t)most : resident;
+    int64_t total = 0;
+    for (int32_t r = 0; r < rows; ++r) {
+        if (is_prompt(counts[r], group, kFewCols)) continue;
+        const int32_t first = lengths[r] - counts[r], from = first - window + 1;
+        total += (int64_t)column_blocks(counts[r] * group) * kv_heads *
+                 place_units(window > 0 && from > 0 ? from : 0, lengths[r], unit);
+    }
+    if (total > most) return 1;
+    const int32_t groups = sharing_groups(total, shape.units, ncu, grid);
+    if (groups > grid) return 2;
+    if (total == 0) return groups != 0;
+    if (first_unit(total, 0, groups) != 0 || first_unit(total, groups, groups) != total) return 3;
+    int64_t first = 0;
+    for (int32_t r = 0; r < rows; ++r) {
+        if (is_prompt(counts[r], group, kFewCols)) continue;
+        const int32_t at = lengths[r] - counts[r] - window + 1;
+        const int64_t units = place_units(window > 0 && at > 0 ? at : 0, lengths[r], unit);
+        for (int32_t i = 0; i < column_blocks(counts[r] * group) * kv_heads; ++i, first += units) {
+            const int32_t a = unit_group(first, total, groups);
+            const int32_t b = unit_group(first + units - 1, total, groups);
+            if (a < 0 || b < a || b >= grid || first_unit(total, a, groups) > first ||
+                first_unit(total, b + 1, groups) < first + units)
+                return 4;
+        }
+    }
+    return 0;
+}
 }

@@ -202,3 +202,43 @@ def test_units_are_shared_out_whole(host):
     for groups in (1, 2, 3, 255, 256, 512):
         for total in (groups, groups + 1, 2 * groups - 1, 1000 * groups + 7, (1 << 43) + 5):
             assert host.t_units_shared(total, groups) == 1
+
+
+def _share(host, d, kv, group, counts, lengths, room, window=0, ncu=256, spare=0):
+    counts, lengths = np.asarray(counts, np.int32), np.asarray(lengths, np.int32)
+    starts = bool((counts != 1).any()) or spare > 0
+    host.t_rows_share.argtypes = [ctypes.c_int32] * 5 + [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                                         ctypes.c_int64, ctypes.c_int32, ctypes.c_int32]
+    return host.t_rows_share(d, kv, group, len(counts), int(counts.sum()) + spare, counts.ctypes.data,
+                             starts, lengths.ctypes.data, room, window, ncu)
+
+
+@pytest.mark.parametrize("d, kv, group, new, length, room", [
+    (256, 2, 4, 6, 8100, 8192), (256, 2, 4, 10, 3000, 8192), (256, 1, 8, 3, 8100, 8192),
+    (512, 1, 8, 4, 8100, 8192), (256, 1, 4, 10, 64, 64), (256, 2, 4, 8, 5000, 8192),
+    (256, 1, 1, 48, 128, 128), (512, 2, 4, 8, 500, 520)])
+def test_rows_of_several_blocks_of_columns_are_shared_out_whole(host, d, kv, group, new, length, room):
+    """One row of 17 to 48 columns in a table that it fills: three blocks go over its tokens."""
+    assert _share(host, d, kv, group, [new], [length], room) == 0
+
+
+def test_no_unit_is_left_to_workgroups_that_are_not_there(host):
+    for d in (64, 128, 192, 256, 272, 512):
+        for kv, group in ((1, 1), (1, 3), (2, 4), (1, 16), (3, 17), (8, 4), (1, 64), (64, 8)):
+            for cols in (1, 15, 16, 17, 24, 31, 32, 33, 47, 48, 49, 200):
+                new = max(1, cols // group)
+                for room in (1, 16, 64, 127, 128, 129, 1024, 8192, 131072, 1 << 30):
+                    for ncu in (1, 64, 256):
+                        for rows in (1, 3, 40):
+                            length = [max(0, room - r * 7 % (room + 1)) for r in range(rows)]
+                            got = _share(host, d, kv, group, [new] * rows, length, room, ncu=ncu,
+                                         window=0 if rows < 40 else 100)
+                            assert got == 0, (d, kv, group, new, room, ncu, rows, got)
+    rng = random.Random(2)
+    for _ in range(3000):
+        rows, room = rng.randrange(1, 70), int(2 ** rng.uniform(0, 14))
+        got = _share(host, rng.randrange(1, 33) * 16, rng.choice([1, 2, 3, 8]), rng.choice([1, 2, 4, 5, 16, 40]),
+                     [rng.choice([0, 1, 1, 2, 5, 9, 17, 48, 90]) for _ in range(rows)],
+                     [rng.randrange(room + 1) for _ in range(rows)], room,
+                     rng.choice([0, 0, 1, 33, 512]), rng.choice([1, 32, 256]), rng.choice([0, 3]))
+        assert got == 0
