@@ -463,7 +463,7 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
         /* where its tokens are, a token a lane, and the keys' and values' scales (by halves of the
          * lanes where there are 32) */
         struct Scales {
-            float k, v;
+            float k = 0.0f, v = 0.0f;
         };
         auto locate = [&](const Step& t, int page, int b, Scales& scale) {
             const int i = token(t);
@@ -481,12 +481,19 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
             }
             return (uint64_t)__ballot(!ok);
         };
-        auto keep_scales = [&](int b, const Scales& scale) {
+        /* A token whose page or scale is none is widened under 1, and NaN for who sees it: `bad` with
+         * those of the scales. */
+        auto keep_scales = [&](int b, const Scales& scale, uint64_t bad) {
+            const bool ok = !(bad >> lane & 1) && scale_ok(__float_as_uint(scale.k)) &&
+                            (TT < 64 || scale_ok(__float_as_uint(scale.v)));
             if constexpr (TT == 64) {
-                s.scale[wave][b][0][lane] = scale.k;
-                s.scale[wave][b][1][lane] = scale.v;
+                s.scale[wave][b][0][lane] = ok ? scale.k : 1.0f;
+                s.scale[wave][b][1][lane] = ok ? scale.v : 1.0f;
+                return bad | (uint64_t)__ballot(!ok);
             } else {
-                s.scale[wave][b][lane >> 5][lane & (TT - 1)] = scale.k;
+                s.scale[wave][b][lane >> 5][lane & (TT - 1)] = ok ? scale.k : 1.0f;
+                const uint64_t none = __ballot(!ok);
+                return bad | none | none >> 32;
             }
         };
         /* (dims behind head_dim, whose queries are 0 and whose sums are not kept, are read in
@@ -534,13 +541,13 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
             load_values(0);
             next = advance(now);
             if (next.tile != kNone) page = find_page(next);
-            keep_scales(0, scale);
+            bad = keep_scales(0, scale, bad);
             wave_fence();
         }
         while (now.tile != kNone) {
             const bool more = next.tile != kNone;
             const uint64_t bad_now = bad;
-            Scales scale{0.0f, 0.0f};
+            Scales scale;
             Step after = next;
             if (more) {
                 bad = locate(next, page, buf ^ 1, scale);
@@ -725,7 +732,7 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
             }
             if (more) {
                 load_values(buf ^ 1);
-                keep_scales(buf ^ 1, scale);
+                bad = keep_scales(buf ^ 1, scale, bad);
             }
             wave_fence(); /* before what comes after the next tile takes the place of this one */
             buf ^= 1;

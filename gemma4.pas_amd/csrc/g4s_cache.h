@@ -90,6 +90,10 @@ G4S_PAGE_HD int32_t scale_exponent(double top)
     return e > kScaleHigh ? kScaleHigh : e;
 }
 
+/* Whether these bits are those of a scale, a number from 0 to 2^kScaleHigh.  Any code times that is finite in
+ * bf16; what is not would be NaN after a product with a weight of 0, for queries that do not see it, too. */
+G4S_PAGE_HD bool scale_ok(uint32_t bits) { return bits <= (uint32_t)(127 + kScaleHigh) << 23; }
+
 /* n / d (n >= 0, d > 0), in 32 bits where they hold both. */
 G4S_PAGE_HD int64_t quotient(int64_t n, int64_t d)
 {

@@ -241,10 +241,14 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
     auto keep_places = [&](int n) {
         if (!locates || n >= n1) return;
         const int b = n % 3, i = lane & (KT - 1);
+        /* (a token whose page or scale is none is widened under 1, and NaN for who sees it) */
+        const bool ok = !(wrong >> lane & 1) && scale_ok(__float_as_uint(k_scale)) &&
+                        scale_ok(__float_as_uint(v_scale));
         s.offset[b][i] = offset;
-        s.scale[b][0][i] = k_scale;
-        s.scale[b][1][i] = v_scale;
-        if (lane == 0) s.bad[b] = wrong;
+        s.scale[b][0][i] = ok ? k_scale : 1.0f;
+        s.scale[b][1][i] = ok ? v_scale : 1.0f;
+        const uint64_t bad = __ballot(!ok);
+        if (lane == 0) s.bad[b] = bad;
     };
     /* a unit's first token */
     auto unit_token = [](int i) { return VT == 8 ? i / 4 * 32 + i % 4 * 4 : i * 4; };

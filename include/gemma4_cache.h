@@ -128,9 +128,9 @@ int g4s_cache_append(g4s_cache* cache, const g4s_page_state* state, int32_t rows
  *   rows, d_starts, tokens, dtype   as for g4s_cache_append (q and out)
  *   d_lse      device [tokens * heads], or NULL
  * A query that sees nothing (a row that has ended) gets zeros and -inf.  A
- * query that is not finite, one that sees a NaN among the keys, or a page outside the
- * pool, gets NaN, and so does every query of a row whose length is outside the
- * table; a NaN among the values gives one in its dim.  What a query does not see does not count, whatever it is.  Queries that no
+ * query that is not finite, one that sees a NaN among the keys, a page outside the
+ * pool, or a scale that is no number from 0 to 2^119, gets NaN, and so does every query of a row whose
+ * length is outside the table; a NaN among the values gives one in its dim.  What a query does not see does not count, whatever it is.  Queries that no
  * row has are left alone.  An output that overlaps another array of the call is
  * refused.  Stream-ordered; the same call gives the same bits. */
 int g4s_cache_attend(g4s_cache* cache, const g4s_page_state* state, int32_t rows,

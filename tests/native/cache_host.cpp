@@ -42,6 +42,7 @@ int64_t t_cache_offset(int64_t page_stride, int32_t part_bytes, int32_t token_by
     p.token_bytes = token_bytes;
     return cache_offset(p, page, in_page, head);
 }
+int t_scale_ok(uint32_t bits) { return scale_ok(bits); }
 int32_t t_scale_exponent(double top) { return scale_exponent(top); }
 /* Tiles of a row of `count` tokens from place `from` on that find no slot in the grid
  * of the append (rows one behind the other from token `start` on): 0. */

@@ -181,6 +181,13 @@ def test_scale_exponent(host):
         assert host.t_scale_exponent(top) == e, top
 
 
+def test_which_bits_are_a_scale(host):
+    for x, want in ((0.0, 1), (1e-45, 1), (2.0 ** -100, 1), (1.0, 1), (2.0 ** 119, 1), (1.5 * 2.0 ** 119, 0),
+                    (2.0 ** 120, 0), (2.0 ** 127, 0), (math.inf, 0), (math.nan, 0), (-1.0, 0), (-math.inf, 0)):
+        bits = int(np.array([x], np.float32).view(np.uint32)[0])
+        assert host.t_scale_ok(ctypes.c_uint32(bits)) == want, x
+
+
 def test_every_tile_of_a_row_has_a_slot(host):
     for tile in (1, 2, 3, 16, 15, 64, 256):
         for start in (0, 1, tile - 1, tile, tile + 1, 1000):

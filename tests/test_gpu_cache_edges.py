@@ -3,6 +3,8 @@ of query columns, and the calls that follow on the same handle."""
 import numpy as np
 import pytest
 
+import cache_oracle as co
+
 from test_gpu_cache import Rig
 
 pytestmark = pytest.mark.gpu
@@ -39,3 +41,95 @@ def test_few_new_tokens_behind_long_contexts(kv, group, new, length, d, dtype):
     single_tokens(rig)
     for _ in range(2):
         rig.attend()
+
+
+# ----------------------------------------------- what a query does not see
+
+SCALES = [0xFFFFFFFF, 0x7F800000, 0x7F000000, 0xFF800000, 0x7FC00000]
+
+
+def cells(rig):
+    return rig.pool.reshape(3, rig.geo.n_pages, rig.kv, rig.P, rig.d + 4)
+
+
+def unwritten_first_page(rig, bits):
+    """Page 0 becomes no row's, with codes that are numbers and scales that are none."""
+    c = cells(rig)
+    spare = next(p for p in range(1, rig.geo.n_pages) if p not in rig.table)
+    c[:, spare] = c[:, 0]
+    rig.table[rig.table == 0] = spare
+    c[:, 0, ..., :rig.d] = co.encode(rig.rng.standard_normal(c[:, 0, ..., :rig.d].shape) * 100)
+    c[:, 0, ..., rig.d:] = np.full(c.shape[2:4] + (1,), bits, np.uint32).view(np.uint8)
+    rig.d_pool.upload(rig.pool)
+
+
+def scales_that_are_none_give_nan(monkeypatch, rig):
+    """The oracle's values under a scale that is no number from 0 to 2^119, in either plane."""
+    plain = co.Cache.value
+
+    def value(self, plane, table, row, t, head):
+        at = self.place(table, row, t)
+        if at is not None:
+            page, o = at
+            for p in rig.planes:
+                if not 0 <= self.scales[p, page, head, o - o % self.block] <= 2.0 ** 119:
+                    return np.full(self.d, np.nan)
+        return plain(self, plane, table, row, t, head)
+    monkeypatch.setattr(co.Cache, "value", value)
+
+
+@pytest.mark.parametrize("bits", SCALES)
+@pytest.mark.parametrize("shape, bad", [
+    (dict(lengths=[70, 53], news=[40, 10], group=4), [(0, 3), (1, 3)]),
+    (dict(lengths=[53, 30], news=[10, 1], group=1, d=256), [(0, 3)]),
+    (dict(lengths=[90, 90, 91, 92], group=2, d=512, share=(4, 3)), [(1, 4), (3, 3)]),
+    (dict(lengths=[150], news=[100], kv=1, group=1, d=512), [(0, 5)]),
+    (dict(lengths=[150], news=[120], kv=1, group=1, d=256), [(0, 5)])])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pages_outside_the_pool_and_an_unwritten_first_page(dtype, shape, bad, bits):
+    """Whoever does not see the page is not touched by what stands in another one."""
+    rig = Rig(dtype=dtype, **shape)
+    unwritten_first_page(rig, bits)
+    for row, slot in bad:
+        rig.table[row, slot] = -1 if slot % 2 else rig.geo.n_pages
+    rig.upload()
+    rig.attend()
+    rig.attend(window=20)
+
+
+@pytest.mark.parametrize("bits", SCALES)
+@pytest.mark.parametrize("plane", [0, 1])
+@pytest.mark.parametrize("shape, at", [
+    (dict(lengths=[70, 53], news=[40, 10], group=4), [(0, 50), (1, 50)]),
+    (dict(lengths=[53, 30], news=[10, 1], group=1, d=256), [(0, 48)]),
+    (dict(lengths=[90, 90, 91, 92], group=2, d=512, share=(4, 3)), [(1, 70), (3, 91)]),
+    (dict(lengths=[100, 40], group=2, d=64), [(0, 99), (1, 0)]),
+    (dict(lengths=[150], news=[100], kv=1, group=1, d=512), [(0, 90)])])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.filterwarnings("ignore:invalid value")
+def test_scales_that_are_none(monkeypatch, dtype, shape, at, plane, bits):
+    """NaN for who sees a token under such a scale, nobody else."""
+    rig = Rig(dtype=dtype, **shape)
+    c = cells(rig)
+    for row, t in at:
+        t -= t % rig.B
+        c[rig.planes[plane], rig.table[row, t // rig.P], 0, t % rig.P, rig.d:] = \
+            np.full(1, bits, np.uint32).view(np.uint8)
+    rig.d_pool.upload(rig.pool)
+    scales_that_are_none_give_nan(monkeypatch, rig)
+    rig.attend()
+    rig.attend(window=20)
+
+
+@pytest.mark.parametrize("bits", SCALES)
+@pytest.mark.parametrize("group, d, dtype", [(4, 64, "bf16"), (2, 256, "f32"), (1, 512, "bf16")])
+@pytest.mark.filterwarnings("ignore:invalid value")
+def test_slots_that_the_window_has_left_behind(group, d, dtype, bits):
+    """Rows of one first page and different lengths: slots between their windows name an
+    unwritten page."""
+    rig = Rig([60, 400, 399, 250], group=group, d=d, dtype=dtype, share=(4, 1))
+    unwritten_first_page(rig, bits)
+    for row, length in enumerate(rig.lengths):
+        rig.table[row, 1:(length - 20) // rig.P] = 0 if row % 2 else -1
+    rig.upload()
+    rig.attend(window=20)
