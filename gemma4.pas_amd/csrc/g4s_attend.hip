@@ -271,7 +271,7 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
     constexpr int NJ = TT < 32 ? 4 : 8;             /* tokens of a lane in a product with V .. */
     constexpr int NH = TT / (4 * NJ);               /* .. of which a step has so many */
     constexpr int QP = DT == G4S_DTYPE_F32 ? 3 : 1; /* pieces of a query */
-    constexpr int PP = DT == G4S_DTYPE_F32 ? 3 : 1; /* and of a weight */
+    constexpr int PP = DT == G4S_DTYPE_F32 ? 3 : 2; /* and of a weight */
     constexpr int KC = D / 64;                      /* 16-dim chunks of a lane of K and Q */
     constexpr int VW = D / 64;                      /* words of a lane of V */
     constexpr int VL = VW < 4 ? VW : 4;             /* of one load */
@@ -664,13 +664,13 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
                     Frag* f = pw[h >> 1];
                     const int w = (h & 1) * 2 + (j >> 1);
                     f[0].w[w] = pack_bf16(e0, e1);
-                    /* (bf16 as they are: rounded by 2^-9 at most, which next to an output's own
-                     * rounding is small and costs one product instead of three; binary32 in three
-                     * pieces, as two were off by 2^-17, more than all else together) */
+                    /* (pieces of eight bits: three are the weight, two are off by 2^-16 at most, which a
+                     * bf16 output's own rounding hides and which costs a product less; a
+                     * single one is off by 2^-8, as much as that rounding) */
+                    const float r0 = e0 - __uint_as_float(f[0].w[w] << 16);
+                    const float r1 = e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u);
+                    f[1].w[w] = pack_bf16(r0, r1);
                     if constexpr (PP == 3) {
-                        const float r0 = e0 - __uint_as_float(f[0].w[w] << 16);
-                        const float r1 = e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u);
-                        f[1].w[w] = pack_bf16(r0, r1);
                         f[2].w[w] = pack_bf16(r0 - __uint_as_float(f[1].w[w] << 16),
                                               r1 - __uint_as_float(f[1].w[w] & 0xFFFF0000u));
                     }

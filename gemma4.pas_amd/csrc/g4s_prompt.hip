@@ -141,7 +141,7 @@ template <int DT, int D, int NW, int NT, int KT>
 __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_kernel(AttendArgs a, int splits)
 {
     constexpr int QP = DT == G4S_DTYPE_F32 ? 3 : 1;
-    constexpr int PP = DT == G4S_DTYPE_F32 ? 3 : 1;
+    constexpr int PP = DT == G4S_DTYPE_F32 ? 3 : 2;
     constexpr int HALVES = kHalves<D>, COLW = NW / HALVES, DW = D / HALVES; /* a wave's dims */
     constexpr int CB = COLW * NT * 16;
     constexpr int KS = DW / 32, DB = DW / 16, TB = KT / 16;
@@ -495,13 +495,13 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
                     Frag* f = pw[t][i >> 3];
                     const int w = (i & 7) >> 1;
                     f[0].w[w] = pack_bf16(e0, e1);
-                    /* (bf16 as they are: rounded by 2^-9 at most, which next to an output's own
-                     * rounding is small and costs one product instead of three; binary32 in three
-                     * pieces, as two were off by 2^-17, more than all else together) */
+                    /* (pieces of eight bits: three are the weight, two are off by 2^-16 at most, which a
+                     * bf16 output's own rounding hides and which costs a product less; a
+                     * single one is off by 2^-8, as much as that rounding) */
+                    const float r0 = e0 - __uint_as_float(f[0].w[w] << 16);
+                    const float r1 = e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u);
+                    f[1].w[w] = pack_bf16(r0, r1);
                     if constexpr (PP == 3) {
-                        const float r0 = e0 - __uint_as_float(f[0].w[w] << 16);
-                        const float r1 = e1 - __uint_as_float(f[0].w[w] & 0xFFFF0000u);
-                        f[1].w[w] = pack_bf16(r0, r1);
                         f[2].w[w] = pack_bf16(r0 - __uint_as_float(f[1].w[w] << 16),
                                               r1 - __uint_as_float(f[1].w[w] & 0xFFFF0000u));
                     }

@@ -122,8 +122,8 @@ int g4s_cache_append(g4s_cache* cache, const g4s_page_state* state, int32_t rows
  * head h / (heads / kv_heads):
  *   s(j) = scale * dot(q, key(j))
  *   lse = log(sum of exp(s(j)))      out = sum of exp(s(j) - lse) * value(j)
- * Sums and exponentials in 32 bits.  For bf16 outputs the weights exp(s) are rounded to
- * bf16 before they meet the values; those of fp32 outputs, keys, values and queries
+ * Sums and exponentials in 32 bits.  For bf16 outputs the weights exp(s) are off by
+ * 2^-16 at most where they meet the values; those of fp32 outputs, keys, values and queries
  * are not rounded.
  *   rows, d_starts, tokens, dtype   as for g4s_cache_append (q and out)
  *   d_lse      device [tokens * heads], or NULL

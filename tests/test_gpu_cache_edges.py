@@ -133,3 +133,31 @@ def test_slots_that_the_window_has_left_behind(group, d, dtype, bits):
         rig.table[row, 1:(length - 20) // rig.P] = 0 if row % 2 else -1
     rig.upload()
     rig.attend(window=20)
+
+
+# ------------------------------------------------- roundings of bf16 outputs
+
+
+def two_pieces(to, dim, dtype):
+    """cache_oracle.limits where the weights of bf16 outputs are kept in two bf16 pieces: what
+    the first one leaves is at most 2^-8 of a weight, and the second is off by 2^-8 of that."""
+    out, lse = plain_limits(to, dim, dtype)
+    return out - (2.0 ** -8 - 2.0 ** -16) * to.mass, lse
+
+
+plain_limits = co.limits
+
+
+@pytest.mark.parametrize("window", [0, 33])
+@pytest.mark.parametrize("shape", [
+    dict(lengths=[501], d=256, B=1), dict(lengths=[1500, 3, 700], d=128, kv=1, group=3),
+    dict(lengths=[150, 150, 151, 149], d=512, group=2, share=(4, 6)), dict(lengths=[90] * 5, share=(5, 3)),
+    dict(lengths=[200], news=[160], P=64, B=64, kv=1, group=8, d=128),
+    dict(lengths=[129, 140], news=[129, 11], P=9, B=3, kv=3, group=1, d=80),
+    dict(lengths=[300, 17], news=[90, 1], kv=1, group=2, d=64),
+    dict(lengths=[333, 64], news=[70, 1], kv=2, group=1, d=256),
+    dict(lengths=[219, 34], news=[55, 3], d=512, kv=1, group=3, B=16)])
+def test_weights_of_bf16_outputs(monkeypatch, shape, window):
+    """Outputs near zero under values that are not: the weights are not rounded to bf16."""
+    monkeypatch.setattr(co, "limits", two_pieces)
+    Rig(dtype="bf16", **shape).attend(window, size=0.5)
