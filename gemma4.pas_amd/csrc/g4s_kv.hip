@@ -147,6 +147,15 @@ Inputs inputs(const g4s_cache* h, const g4s_page_state* state, int32_t rows,
     return in;
 }
 
+/* Integers and floats: scalar loads take no notice of an address' last two bits. */
+int check_alignment(g4s_cache* h, const Inputs& in)
+{
+    for (int i = 0; i < in.n; ++i)
+        if ((uintptr_t)in.at[i].at & 3)
+            return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s must be 4-byte aligned", in.at[i].name);
+    return G4S_OK;
+}
+
 int refuse_overlap(g4s_cache* h, const char* a, const char* b)
 {
     return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s overlaps %s", a, b);
@@ -290,6 +299,8 @@ G4S_API int g4s_cache_append(g4s_cache* h, const g4s_page_state* state, int32_t 
     Inputs in = inputs(h, state, rows, d_starts);
     in.add("d_positions", d_positions, (int64_t)tokens * 4);
     in.add("d_freqs", d_freqs, (int64_t)c.rotary_dims / 2 * 4);
+    rc = check_alignment(h, in);
+    if (rc) return rc;
     const Span pool{"d_pool", k ? d_pool : nullptr, g4s::pool_extent(h->geo)};
     for (int i = 0; i < in.n; ++i) {
         if (overlap(span(co), in.at[i])) return refuse_overlap(h, "q_out", in.at[i].name);
@@ -358,6 +369,8 @@ G4S_API int g4s_cache_attend(g4s_cache* h, const g4s_page_state* state, int32_t 
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "d_lse must be 4-byte aligned");
     Inputs in = inputs(h, state, rows, d_starts);
     in.add("d_pool", d_pool, g4s::pool_extent(h->geo));
+    rc = check_alignment(h, in);
+    if (rc) return rc;
     const Span lse{"d_lse", d_lse, (int64_t)tokens * c.heads * 4};
     for (int i = 0; i < in.n; ++i) {
         if (overlap(span(co), in.at[i])) return refuse_overlap(h, "out", in.at[i].name);

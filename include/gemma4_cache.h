@@ -14,7 +14,7 @@
  * message of the last failure kept per handle (with a NULL handle that of the
  * thread's last failed call without one), one handle = one HIP stream, a
  * handle is not thread-safe, device pointers are memory of the handle's device
- * (which need not be the current one).  Only g4s_cache_create allocates;
+ * (which need not be the current one), those of integers and floats 4-byte aligned.  Only g4s_cache_create allocates;
  * append and attend are kernel launches alone and may be captured into a
  * hipGraph.  A graph that attends uses its handle's workspace: it is
  * replayed on one stream at a time with the handle's other calls.

@@ -4,8 +4,9 @@ import numpy as np
 import pytest
 
 import cache_oracle as co
-
+from gemma4_sampler import beam, native
 from test_gpu_cache import Rig
+from test_gpu_cache_use import Calls
 
 pytestmark = pytest.mark.gpu
 
@@ -161,3 +162,31 @@ def test_weights_of_bf16_outputs(monkeypatch, shape, window):
     """Outputs near zero under values that are not: the weights are not rounded to bf16."""
     monkeypatch.setattr(co, "limits", two_pieces)
     Rig(dtype="bf16", **shape).attend(window, size=0.5)
+
+
+# ------------------------------------------------------------------ refusals
+
+
+@pytest.fixture(scope="module")
+def calls():
+    return Calls()
+
+
+def refused(call, **change):
+    with pytest.raises(native.SamplerError) as e:
+        call(**change)
+    assert e.value.code == native.G4S_ERR_INVALID_ARGUMENT
+    return str(e.value)
+
+
+@pytest.mark.parametrize("by", [1, 2, 3])
+def test_addresses_between_integers(calls, by):
+    r = calls.rig
+    for name, change in (
+            ("table", dict(state=beam.PageState(r.d_table.offset(by), r.d_lengths, None))),
+            ("lengths", dict(state=beam.PageState(r.d_table, r.d_lengths.offset(by), None))),
+            ("d_starts", dict(d_starts=r.d_starts.offset(by)))):
+        for call in (calls.append, calls.attend):
+            assert name in refused(call, **change)
+    assert "d_positions" in refused(calls.append, d_positions=calls.positions.offset(by))
+    assert "d_freqs" in refused(calls.append, d_freqs=r.d_freqs.offset(by))
