@@ -50,6 +50,13 @@ __device__ __forceinline__ float column_sum(float x)
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+/* What products are multiplied by, to base two (the scale's sign is in the queries).  Never 0, as what is
+ * masked stays -inf; the least number in its place makes 2^-21 of the largest product. */
+__device__ __forceinline__ float base_two(float scale)
+{
+    return fmaxf(__builtin_fabsf(scale * kLog2e), 0x1p-149f);
+}
+
 /* The first place that a query at `place` (which may be negative) sees. */
 __device__ __forceinline__ int sees_from(const AttendArgs& a, int place)
 {

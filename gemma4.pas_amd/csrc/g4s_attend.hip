@@ -292,8 +292,7 @@ __global__ __launch_bounds__(rows_shape(D).waves * 64, 2) void attend_rows_kerne
     if ((int)blockIdx.x >= groups) return;
     int64_t x = first_unit(total, blockIdx.x, groups);
     const int64_t x_end = first_unit(total, blockIdx.x + 1, groups);
-    /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
-    const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
+    const float c = base_two(a.scale);
     const __amdgpu_buffer_rsrc_t space = shared_space(a.ws.sums, (uint32_t)a.ws.groups * kAttendSums * 4);
 
     while (x < x_end) {

@@ -356,8 +356,8 @@ G4S_API int g4s_cache_attend(g4s_cache* h, const g4s_page_state* state, int32_t 
     if (rc) return rc;
     const g4s_cache_config& c = h->config;
     if (!q || !out) return fail(h, G4S_ERR_INVALID_ARGUMENT, "q and out must be non-NULL");
-    if (!std::isfinite(scale))
-        return fail(h, G4S_ERR_INVALID_ARGUMENT, "scale %g is not finite", scale);
+    if (!(std::fabs(scale) <= 0x1p127f)) /* (times log2(e) it is a number) */
+        return fail(h, G4S_ERR_INVALID_ARGUMENT, "scale %g is not within +-2^127", scale);
     if (window < 0) return fail(h, G4S_ERR_INVALID_ARGUMENT, "window %d is negative", window);
     const int64_t esize = dtype_size(dtype);
     Checked cq, co;

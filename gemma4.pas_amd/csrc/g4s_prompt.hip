@@ -200,8 +200,7 @@ __global__ __launch_bounds__(NW * 64, NW == 4 ? 2 : NW / 4) void attend_prompts_
     const int w_last = r.length - r.count + divide(col0 + (busy ? wcol1 - 1 : 0), a.group);
     const int any_from = sees_from(a, w_first), all_from = sees_from(a, w_last);
 
-    /* to base two, and never 0: what is masked stays -inf.  (The scale's sign is in the queries.) */
-    const float c = fmaxf(__builtin_fabsf(a.scale * kLog2e), 1e-37f);
+    const float c = base_two(a.scale);
     f32x4 o[NT][DB];
     float base[NT], sum[NT];
 #pragma unroll

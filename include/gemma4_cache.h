@@ -126,6 +126,7 @@ int g4s_cache_append(g4s_cache* cache, const g4s_page_state* state, int32_t rows
  * 2^-16 at most where they meet the values; those of fp32 outputs, keys, values and queries
  * are not rounded.
  *   rows, d_starts, tokens, dtype   as for g4s_cache_append (q and out)
+ *   scale      within +-2^127
  *   d_lse      device [tokens * heads], or NULL
  * A query that sees nothing (a row that has ended) gets zeros and -inf.  A
  * query that is not finite, one that sees a NaN among the keys, a page outside the

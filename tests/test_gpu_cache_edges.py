@@ -190,3 +190,25 @@ def test_addresses_between_integers(calls, by):
             assert name in refused(call, **change)
     assert "d_positions" in refused(calls.append, d_positions=calls.positions.offset(by))
     assert "d_freqs" in refused(calls.append, d_freqs=r.d_freqs.offset(by))
+
+
+# ---------------------------------------------------------- scales of scores
+
+
+@pytest.mark.parametrize("news", [None, [60, 1]])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, -3e-38, 1e-40])
+def test_small_scales_of_large_products(scale, dtype, news):
+    """Products of queries and keys next to the largest number: a scale of 0 is one, and a
+    tiny one is not rounded up."""
+    Rig([100, 7], news=news, dtype=dtype).attend(scale=scale, size=2e35)
+
+
+@pytest.mark.parametrize("news", [None, [60, 1]])
+def test_largest_scale(news):
+    Rig([100, 7], news=news).attend(scale=2.0 ** 127, size=0.0)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, -3e38])
+def test_scales_that_are_too_large_to_base_two(calls, scale):
+    assert "scale" in refused(calls.attend, scale=scale)
