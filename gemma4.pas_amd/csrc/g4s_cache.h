@@ -177,6 +177,48 @@ G4S_PAGE_HD int64_t share_begin(const int32_t* starts, int32_t row, int32_t time
     return (int64_t)(starts ? starts[row] : row) * times / unit + (int64_t)extra * row;
 }
 
+/* Vectors of `vec` bytes for tokens and heads, at `at` and strides in bytes, where heads lie within a
+ * token's stride or tokens within a head's (strides of dimensions with one vector are 0). */
+struct Vectors {
+    uint64_t at;
+    int64_t tokens, heads, token_stride, head_stride, vec;
+    G4S_PAGE_HD int64_t head_end() const { return (heads - 1) * head_stride + vec; }
+    G4S_PAGE_HD int64_t end() const { return (tokens - 1) * token_stride + head_end(); }
+};
+/* Whether two of them (of vectors as long) share memory.  Views of the same strides, as parts of each token's record
+ * or of each head's, do where a vector of one does with a vector of the other; those of one token stride
+ * and different head strides where their heads do; others where they begin and end say so. */
+G4S_PAGE_HD bool vectors_meet(const Vectors& a, const Vectors& b)
+{
+    if (!a.at || !b.at || a.at >= b.at + (uint64_t)b.end() || b.at >= a.at + (uint64_t)a.end()) return false;
+    const int64_t ts = a.tokens > 1 ? a.token_stride : b.token_stride;
+    const int64_t hs = a.heads > 1 ? a.head_stride : b.head_stride;
+    const bool same_ts = b.tokens == 1 || b.token_stride == ts, same_hs = b.heads == 1 || b.head_stride == hs;
+    const int64_t gap = (int64_t)(b.at - a.at);
+    if (same_ts && same_hs) {
+        /* gap + (tokens apart) ts + (heads apart) hs, next to 0 in the outer stride, then in the inner one */
+        const bool by_token = ts >= hs;
+        const int64_t outer = by_token ? ts : hs, inner = by_token ? hs : ts;
+        const int64_t out_a = by_token ? a.tokens : a.heads, out_b = by_token ? b.tokens : b.heads;
+        const int64_t in_a = by_token ? a.heads : a.tokens, in_b = by_token ? b.heads : b.tokens;
+        const int64_t o0 = outer ? -gap / outer : 0;
+        for (int64_t o = o0 - 1; o <= o0 + 1; ++o) {
+            if (o <= -out_a || o >= out_b) continue;
+            const int64_t rest = gap + o * outer, i0 = inner ? -rest / inner : 0;
+            for (int64_t i = i0 - 1; i <= i0 + 1; ++i) {
+                const int64_t apart = rest + i * inner;
+                if (i > -in_a && i < in_b && apart < a.vec && apart > -a.vec) return true;
+            }
+        }
+        return false;
+    }
+    if (same_ts && ts > 0 && a.head_end() <= ts && b.head_end() <= ts) {
+        const int64_t r = (gap % ts + ts) % ts;
+        return r < a.head_end() || ts - r < b.head_end();
+    }
+    return true;
+}
+
 #if defined(__HIPCC__)
 
 /* The row whose share holds slot x: the last one that begins at or before it.  Every lane

@@ -46,19 +46,17 @@ constexpr int64_t kMaxElements = (int64_t)1 << 50;
 
 int64_t dtype_size(int32_t dtype) { return dtype == G4S_DTYPE_F32 ? 4 : 2; }
 
-/* A view of `heads` heads as checked: where it begins and ends, in bytes. */
+/* A view as checked: as the kernels take it, and its bytes. */
 struct Checked {
     const char* name;
     CacheView view;
-    int64_t bytes;   /* from the first to behind the last */
-    int64_t heads;   /* of one token's heads */
-    int64_t stride;  /* of a token; 0: one token */
+    g4s::Vectors vectors;
 };
 
 int check_view(g4s_cache* h, const char* name, const g4s_cache_view* v, int32_t heads,
                int32_t tokens, int64_t esize, Checked* out)
 {
-    *out = Checked{name, CacheView{}, 0, 0, 0};
+    *out = Checked{name, CacheView{}, g4s::Vectors{}};
     if (!v) return G4S_OK;
     if (!v->data) return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s->data is NULL", name);
     const int64_t d = h->config.head_dim;
@@ -76,26 +74,12 @@ int check_view(g4s_cache* h, const char* name, const g4s_cache_view* v, int32_t 
         return fail(h, G4S_ERR_INVALID_ARGUMENT, "%s: vectors of head_dim %d overlap", name,
                     h->config.head_dim);
     out->view = CacheView{static_cast<char*>(v->data), ts, hs};
-    out->bytes = ((tokens - 1) * ts + head_end) * esize;
-    out->heads = head_end * esize;
-    out->stride = a ? ts * esize : 0;
+    out->vectors = g4s::Vectors{(uint64_t)(uintptr_t)v->data, tokens, heads, ts * esize, hs * esize, d * esize};
     return G4S_OK;
 }
 
-Span span(const Checked& c) { return Span{c.name, c.view.data, c.bytes}; }
-
-/* Whether two views share memory.  Views of one token stride whose heads lie within
- * it (queries, keys and values side by side) are apart where their heads are. */
-bool overlap(const Checked& a, const Checked& b)
-{
-    if (!overlap(span(a), span(b))) return false;
-    if (a.stride > 0 && a.stride == b.stride && a.heads <= a.stride && b.heads <= a.stride) {
-        int64_t gap = (int64_t)((intptr_t)b.view.data - (intptr_t)a.view.data) % a.stride;
-        if (gap < 0) gap += a.stride;
-        return gap < a.heads || a.stride - gap < b.heads;
-    }
-    return true;
-}
+Span span(const Checked& c) { return Span{c.name, c.view.data, c.view.data ? c.vectors.end() : 0}; }
+bool overlap(const Checked& a, const Checked& b) { return vectors_meet(a.vectors, b.vectors); }
 
 int check_call(g4s_cache* h, const g4s_page_state* state, int32_t rows, const int32_t* d_starts,
                int32_t tokens, int32_t dtype)

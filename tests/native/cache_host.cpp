@@ -73,6 +73,11 @@ int t_units_shared(int64_t total, int32_t groups)
     }
     return 1;
 }
+int t_vectors_meet(const int64_t* a, const int64_t* b)
+{
+    return vectors_meet(Vectors{(uint64_t)a[0], a[1], a[2], a[3], a[4], a[5]},
+                        Vectors{(uint64_t)b[0], b[1], b[2], b[3], b[4], b[5]});
+}
 /* The rows' kernel's share of a call (rows of `counts` tokens, none taken together; those with more columns
  * than kFewCols are the prompts' kernel's): 0, or what is wrong with it.  1: more units than
  * the grid is made for, 2: work is shared among workgroups that the grid does not have, 3: units that are

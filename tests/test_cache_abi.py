@@ -249,3 +249,67 @@ def test_no_unit_is_left_to_workgroups_that_are_not_there(host):
                      [rng.randrange(room + 1) for _ in range(rows)], room,
                      rng.choice([0, 0, 1, 33, 512]), rng.choice([1, 32, 256]), rng.choice([0, 3]))
         assert got == 0
+
+
+# ---------------------------------------------------- views that lie together
+
+
+def _bytes_of(v):
+    at, tokens, heads, ts, hs, vec = v
+    return {at + i * ts + h * hs + x for i in range(tokens) for h in range(heads) for x in range(vec)}
+
+
+def _meet(host, a, b):
+    got = [host.t_vectors_meet((ctypes.c_int64 * 6)(*x), (ctypes.c_int64 * 6)(*y))
+           for x, y in ((a, b), (b, a))]
+    assert got[0] == got[1]
+    return bool(got[0])
+
+
+def test_parts_of_each_heads_record_are_apart(host):
+    """Queries, keys, values and rotated queries of a head side by side, head by head."""
+    d, heads, tokens = 8, 4, 5
+    for order in ("tokens", "heads"):
+        hs = 4 * d if order == "tokens" else 4 * d * tokens
+        ts = 4 * d * heads if order == "tokens" else 4 * d
+        parts = [(1000 + i * d, tokens, heads, ts, hs, d) for i in range(4)]
+        for i, a in enumerate(parts):
+            for j, b in enumerate(parts):
+                assert _meet(host, a, b) == (i == j)
+            assert _meet(host, a, (1000 + i * d + 4,) + a[1:])
+    # keys of one head beside queries of several
+    assert not _meet(host, (1000, 5, 4, 100, 16, 8), (1008, 5, 1, 100, 0, 8))
+    assert not _meet(host, (1000, 1, 4, 0, 16, 8), (1008, 1, 4, 0, 16, 8))
+    assert _meet(host, (1000, 1, 4, 0, 16, 8), (1012, 1, 4, 0, 16, 8))
+
+
+def test_views_meet_where_their_bytes_do(host):
+    """Views of the same strides: exactly.  Others: never apart where they are not."""
+    rng = random.Random(3)
+    exact = met = 0
+    for _ in range(30000):
+        vec, shape = 4, []
+        tokens = rng.randrange(1, 5)
+        strides = None
+        for _ in range(2):
+            heads = rng.randrange(1, 5)
+            if strides is None or rng.random() < 0.4:
+                inner = vec * rng.randrange(1, 4)
+                if rng.random() < 0.5:
+                    strides = ("tokens", inner, inner * 4 + vec * rng.randrange(3))
+                else:
+                    strides = ("heads", inner, inner * 4 + vec * rng.randrange(3))
+            kind, s, big = strides
+            ts, hs = (big, s) if kind == "tokens" else (s, big)
+            shape.append((1000 + rng.randrange(60), tokens, heads, ts if tokens > 1 else 0,
+                          hs if heads > 1 else 0, vec))
+        a, b = shape
+        want, got = bool(_bytes_of(a) & _bytes_of(b)), _meet(host, a, b)
+        assert got or not want, (a, b)
+        one = [(x[3], x[4]) for x in shape]
+        if one[0] == one[1]:
+            assert got == want, (a, b)
+            exact += 1
+            met += want
+    assert exact > 5000 and 1000 < met < exact - 1000
+    assert not _meet(host, (0, 1, 1, 0, 0, 4), (0, 1, 1, 0, 0, 4))  # (no view)

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 import cache_oracle as co
-from gemma4_sampler import beam, native
-from test_gpu_cache import Rig
+from gemma4_sampler import beam, cache, hip, native
+from test_gpu_cache import Rig, Vectors
 from test_gpu_cache_use import Calls
 
 pytestmark = pytest.mark.gpu
@@ -212,3 +212,33 @@ def test_largest_scale(news):
 @pytest.mark.parametrize("scale", [2.4e38, -3e38])
 def test_scales_that_are_too_large_to_base_two(calls, scale):
     assert "scale" in refused(calls.attend, scale=scale)
+
+
+# --------------------------------------------------- parts of a head's record
+
+
+def test_views_that_lie_side_by_side_in_each_head():
+    """Keys, values and queries of each head one behind the other, queries rotated in place: taken, and
+    what views of their own give."""
+    r = Rig([20, 9, 30], news=[5, 9, 2], kv=3, group=1, d=64)
+    n, d = r.tokens, r.d
+    x = r.rng.standard_normal((n, 3, 3, d))  # token, head, part
+    qkv = Vectors(x.reshape(n, 9, d), "bf16")
+    parts = [cache.View(qkv.buf.offset(2 * d * i), 9 * d, 3 * d) for i in range(3)]
+    apart = [Vectors(x[:, :, i], "bf16") for i in range(3)]
+    pools = []
+    for k, v, q in (parts, [a.view for a in apart]):
+        r.d_pool.upload(r.pool)
+        r.cache.append(r.state, r.rows, n, native.DTYPE_BF16, r.d_pool, *r.planes, q=q, k=k, v=v, q_out=q,
+                       d_starts=r.d_starts, d_freqs=r.d_freqs)
+        hip.synchronize()
+        pools.append(r.d_pool.download(np.uint8))
+    assert np.array_equal(*pools) and not np.array_equal(pools[0], r.pool)
+    got = qkv.download().reshape(n, 3, 3, d)
+    for i in range(3):
+        assert np.array_equal(got[:, :, i], apart[i].download()), i
+    beside = cache.View(qkv.buf.offset(2 * d + 16), 9 * d, 3 * d)
+    assert "overlaps" in refused(r.cache.append, state=r.state, rows=r.rows, tokens=n,
+                                 dtype=native.DTYPE_BF16, d_pool=r.d_pool, k_plane=2, v_plane=0,
+                                 q=parts[2], k=parts[0], v=parts[1], q_out=beside,
+                                 d_starts=r.d_starts, d_freqs=r.d_freqs)
