@@ -297,7 +297,6 @@ struct AttendArgs {
 };
 
 hipError_t append_launch(const AppendArgs& a, int32_t dtype, hipStream_t stream);
-hipError_t attend_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 
 hipError_t attend_rows_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
 hipError_t attend_prompts_launch(const AttendArgs& a, int32_t dtype, hipStream_t stream);
