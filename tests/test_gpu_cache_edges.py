@@ -242,3 +242,123 @@ def test_views_that_lie_side_by_side_in_each_head():
                                  dtype=native.DTYPE_BF16, d_pool=r.d_pool, k_plane=2, v_plane=0,
                                  q=parts[2], k=parts[0], v=parts[1], q_out=beside,
                                  d_starts=r.d_starts, d_freqs=r.d_freqs)
+
+
+# ------------------------------------------------------------- largest sizes
+
+
+def page_values(rng, P, d, size):
+    """A page of one head: its cells, and what its tokens stand for."""
+    codes = co.encode(rng.standard_normal((P, d)) * size)
+    cells = np.zeros((P, d + 4), np.uint8)
+    cells[:, :d] = codes
+    cells[:, d:] = np.full((P, 1), 2.0 ** -5, np.float32).view(np.uint8)
+    return cells, co.E4M3[codes] * 2.0 ** -5
+
+
+@pytest.mark.parametrize("rows, new, window", [(1, 1, 0), (4, 1, 0), (1, 1, 70000), (4, 1, 70000),
+                                               (1, 300, 70000), (2, 40, 1 << 30), (1, 300, 1 << 30),
+                                               (1, 1, (1 << 31) - 1)])
+def test_longest_context(rows, new, window):
+    """Rows of 2^30 tokens, all in the pages that their tables name over and over: a
+    full page and, behind it, one of each row's own."""
+    P, d, slots = 65536, 16, 16384
+    if window == 1 << 30:
+        slots = 1024  # (several tokens that see all of 2^26)
+    rng = np.random.default_rng(rows + new)
+    pages = [[page_values(rng, P, d, 40) for _ in range(rows + 1)] for _ in range(2)]
+    pool = np.stack([np.stack([c for c, _ in plane]) for plane in pages])
+    geo = cache.geometry(P, rows + 1, rows, slots, 1, d)
+    length = slots * P - np.arange(rows) * 100
+    table = np.zeros((rows, slots), np.int32)
+    table[:, -1] = np.arange(rows) + 1
+    q = rng.standard_normal((rows * new, 1, d))
+    vq, out = Vectors(q, "f32"), Vectors(q, "f32")
+    lse = hip.Buffer(rows * new * 4)
+    starts = None if new == 1 else hip.Buffer.from_array((np.arange(rows + 1) * new).astype(np.int32))
+    d_pool = hip.Buffer.from_array(pool.reshape(-1))
+    bufs = [hip.Buffer.from_array(x) for x in (table, length.astype(np.int32))]
+    h = cache.KvCache(geo, 1, 1, d, 64, 0)
+    h.attend(beam.PageState(*bufs, None), rows, rows * new, native.DTYPE_F32, d_pool, 0, 1, vq.view,
+             out.view, 0.25, window, starts, lse)
+    hip.synchronize()
+    got, got_lse = out.download()[:, 0], lse.download(np.float32)
+    x = vq.values()[:, 0]
+    for r in range(rows):
+        for i in range(0, new, 37):
+            at = length[r] - new + i  # its place
+            lo = max(0, at - window + 1) if window else 0
+            count = np.zeros((2, P))  # how often it sees each token of the two pages
+            first, last = lo // P, at // P
+            for slot in range(first, last + 1) if last - first < 4 else (first, last):
+                c = count[int(slot == slots - 1)]
+                a, b = max(lo - slot * P, 0), min(at - slot * P + 1, P)
+                c[a:b] += 1
+            if last - first >= 4:
+                count[0] += last - first - 1
+            k, v = (np.concatenate([plane[0][1], plane[r + 1][1]]) for plane in pages)
+            s, n = 0.25 * (k @ x[r * new + i]), count.reshape(-1)
+            m = s.max()
+            w = n * np.exp(s - m)
+            want = m + np.log(w.sum())
+            # sums of as many terms as a lane adds one by one: 2^30 / (256 x 8 x 64) steps of 16, or
+            # 2^26 / (64 x 64) of 16 where a prompt's tokens are split 64 ways
+            off = 262144 * 2.0 ** -24
+            assert abs(got_lse[r * new + i] - want) <= off + 1e-5 * abs(want), (r, i)
+            mass = (w @ np.abs(v)) / w.sum()
+            assert (np.abs(got[r * new + i] - (w @ v) / w.sum()) <= 2 * off * mass).all(), (r, i)
+    h.close()
+
+
+@pytest.mark.parametrize("rows", [1, 2048])
+def test_most_tokens(rows):
+    """A call of 2^20 tokens: appended and attended over with a window, compared at some of them."""
+    N, P, B, d, window = cache.MAX_TOKENS, 256, 16, 16, 40
+    rng = np.random.default_rng(rows)
+    news = np.full(rows, N // rows)
+    news[-1] += N - news.sum()
+    starts = np.concatenate([[0], np.cumsum(news)]).astype(np.int32)
+    used = -(-news // P)
+    slots, n_pages = int(used.max()), int(used.sum())
+    table = np.full((rows, slots), -1, np.int32)
+    order, at = rng.permutation(n_pages), 0
+    for r in range(rows):
+        table[r, :used[r]] = order[at:at + used[r]]
+        at += used[r]
+    geo = cache.geometry(P, n_pages, rows, slots, 1, d)
+    x = rng.standard_normal((3, N, 1, d)).astype(np.float32)
+    q, k, v = (Vectors(a, "bf16") for a in x)
+    out = Vectors(x[0], "bf16")
+    d_pool = hip.Buffer(2 * geo.plane_stride)
+    d_pool.zero()
+    bufs = [hip.Buffer.from_array(a) for a in (table, news.astype(np.int32), starts)]
+    state = beam.PageState(bufs[0], bufs[1], None)
+    h = cache.KvCache(geo, 1, 1, d, B, 0)
+    h.append(state, rows, N, native.DTYPE_BF16, d_pool, 0, 1, q=q.view, k=k.view, v=v.view, q_out=q.view,
+             d_starts=bufs[2])
+    h.attend(state, rows, N, native.DTYPE_BF16, d_pool, 0, 1, q.view, out.view, 0.25, window, bufs[2])
+    hip.synchronize()
+    got = out.download()[:, 0]
+    assert np.array_equal(q.download(), q.values())
+    kv = [a.values()[:, 0] for a in (k, v)]
+    picks = np.unique(np.concatenate([rng.integers(0, N, 300), starts[:-1], starts[1:] - 1]))
+    for i in picks[rng.permutation(len(picks))[:600]]:
+        r = int(np.searchsorted(starts, i, side="right")) - 1
+        t = i - starts[r]
+        lo = max(0, t - window + 1)
+        seen = []
+        for y in kv:
+            vals = []
+            for b in range(lo // B, t // B + 1):
+                blk = y[starts[r] + b * B:min(starts[r] + b * B + B, starts[r + 1])]
+                s = co.scale_of(np.abs(blk).max())
+                c = co.encode(blk / s)
+                vals.append(np.where(c >= 128, -1.0, 1.0) * co.E4M3[c & 127] * s)
+            seen.append(np.concatenate(vals)[lo - lo // B * B:t - lo // B * B + 1])
+        s = 0.25 * (seen[0] @ q.values()[i, 0])
+        w = np.exp(s - s.max())
+        w /= w.sum()
+        mass, want = w @ np.abs(seen[1]), w @ seen[1]
+        # (2^-16 of the weights; 2 x 24 x 2^-24 of scores' size, some 20; 56 x 2^-23 of sums)
+        assert (np.abs(got[i] - want) <= 2.0 ** -8 * np.abs(want) + 1e-4 * mass).all(), i
+    h.close()
