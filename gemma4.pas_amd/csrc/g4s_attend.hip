@@ -15,10 +15,10 @@
  * Scores are products of the widened codes (exact in bf16) with the queries as matrix operands, K Q^T,
  * so that a lane holds scores of one column and multiplies them, as weights, with V^T without
  * an exchange.  All that is read is read once, one step ahead of its use: 131,071 tokens of 8 heads of 128
- * dims 60 us (4.5 TB/s; this card reads 6.1 at most), 64 rows of 3,000 to 5,000 tokens 99 us (4.7
+ * dims 61 us (4.4 TB/s; this card reads 6.1 at most), 64 rows of 3,000 to 5,000 tokens 100 us (4.7
  * TB/s; 5.4 between start and end).  What is left is the start (lengths and tables 2 to 8 us, queries 1 to 6, page, scales
  * and codes one behind the other 2 to 8) and the joins (3 to 8 us, 4 to 11 in their own launch): 12
- * searches of 4 beams over 3,800 tokens, 512 dims in binary32, 84 us, of which the steps are 26.
+ * searches of 4 beams over 3,800 tokens, 512 dims in binary32, 85 us, of which the steps are 26.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -256,8 +256,8 @@ __device__ __forceinline__ void put(const AttendArgs& a, int64_t out, int64_t ls
 }
 
 /* rows_shape: tokens of a wave's step, as many as its registers hold beside the sums (16, 32 or 64); waves, of
- * which eight are a CU's (131,071 tokens of 128 dims: 60 us with workgroups of eight, which have half the
- * parts to join, and 64 of four; 12 rows of 3,800 of 512 dims 82 and 67, as their units are then twice as long);
+ * which eight are a CU's (131,071 tokens of 128 dims: 61 us with workgroups of eight, which have half the
+ * parts to join, and 65 of four; 12 rows of 3,800 of 512 dims 82 and 67, as their units are then twice as long);
  * and units that a workgroup takes at least where there are enough of them (1, 2 and 4 of them: 49, 39 and 44 us
  * for the windows of 256 dims, 89, 88 and 83 for the searches of 512). */
 constexpr int kResident = 8;

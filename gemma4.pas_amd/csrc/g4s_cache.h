@@ -135,8 +135,9 @@ G4S_PAGE_HD constexpr RowsShape rows_shape(int32_t width)
 /* Rows with more than one token and more than `few` columns (tokens x heads of a key head)
  * are the prompts' kernel's, the others the rows' kernel's, which takes 16 columns a pass over the
  * tokens.  Eight rows of some 3,500 tokens, 8 key heads with 4 heads of 128 dims (2 of 256, binary32):
- * 24 columns a row 45 (41) us by rows and 59 (54) by prompts, 48 columns 63 (48) and 74 (59).  Rows on
- * both sides cost both kernels, one behind the other: 99 (79) us. */
+ * 24 to 28 columns a row 48 (42) us by rows and 69 (53) by prompts, 32 to 36 columns 50 (44) and 87 (58).  Rows
+ * on both sides (48 to 60 columns) cost both kernels, one behind the other: 111 (82) us, 88 (59) by
+ * prompts alone. */
 constexpr int kFewCols = 48;
 G4S_PAGE_HD bool is_prompt(int32_t count, int32_t group, int32_t few)
 {

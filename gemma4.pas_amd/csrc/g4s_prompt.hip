@@ -11,12 +11,14 @@
  * workgroups the tokens are split too, and a second launch joins what the parts of a block
  * found, in their order.
  *
- * Four prompts of 4,000 tokens, 32 and 8 heads of 128 dims: 750 us, 784 TFLOP/s of the 1,260 that a large
- * bf16 product reaches here; bound by the vector units' issue (exponentials, weights, widened
- * codes) beside the products.  256 tokens behind 7,844, 8 and 2 heads of 256 dims: 50 us (333 TFLOP/s), of which the joining
- * launch is 8 and start and end 10: a wave's 16 columns are all that its registers hold beside their sums, so
- * that LDS is read once for each 16 (1.7 us of a tile's 2.7).  Binary32 costs three times the products: the first
- * prompts 1.58 ms.
+ * Four prompts of 4,000 tokens, 32 and 8 heads of 128 dims: 910 us, 646 TFLOP/s of the 1,260 that a large
+ * bf16 product reaches here (three products for two, as the weights are in two pieces: 747 us with one).  No single
+ * unit is the bound: vector instructions (exponentials, weights, widened codes) are issued in 57% of the cycles,
+ * the matrix units work in 42%, LDS in 39% (18% of all on bank conflicts), and they hardly overlap.  256 tokens
+ * behind 7,844, 8 and 2 heads of 256 dims: 53 us (314 TFLOP/s), of which the joining launch is 8 and start and
+ * end 10: a wave's 16 columns are all that its registers hold beside their sums, so that LDS, busy in 51% of the
+ * cycles (22% of all on conflicts), is read once for each 16.  Binary32 costs three times the products: the first
+ * prompts 1.60 ms.  Dims between head_dim and the width that a kernel is made for are multiplied too.
  */
 #include "g4s_attend.h"
 #include "g4s_launch.h"
@@ -113,11 +115,12 @@ struct Shared {
 };
 
 /* Waves that share columns, each with a part of their dims: one wave's registers do not hold the
- * queries and sums of 512 (256 tokens behind 7,844: 112 us and, binary32, 140; alone 169 and 425). */
+ * queries and sums of 512 (256 tokens behind 7,844, weights in one piece: 112 us and, binary32, 140; alone 169
+ * and 425.  Now 118 and 146). */
 template <int D>
 constexpr int kHalves = D > 256 ? 2 : 1;
-/* LDS holds a third tile of values, so that waves may be a phase apart (the four prompts: 752 us, 779 in
- * step; with 64 dims 605 and 637). */
+/* LDS holds a third tile of values, so that waves may be a phase apart (the four prompts: 910 us, 950 in
+ * step; binary32 1,596 and 1,669; with 64 dims 736 and 715, binary32 947 and 976). */
 template <int D>
 constexpr bool kLate = D <= 128;
 
@@ -596,8 +599,8 @@ template <int DT>
 hipError_t by_width(const AttendArgs& a, hipStream_t stream)
 {
     constexpr bool F32 = DT == G4S_DTYPE_F32;
-    /* (32 columns a wave where they fit: with 256 dims, in four waves or tiles of 32, they took 74 and 128
-     * us for the chunk instead of 54; 64 dims in eight waves 609 us, in four 605) */
+    /* (32 columns a wave where they fit: with 256 dims, in four waves, they take 146 us for the chunk instead of
+     * 54; 64 dims in eight waves 742 us, in four 736) */
     switch (attend_width(a.pool.head_dim)) {
     case 64: return prompts_launch<DT, 64, 4, F32 ? 1 : 2, 64>(a, stream);
     case 128: return prompts_launch<DT, 128, 8, F32 ? 1 : 2, 64>(a, stream);
