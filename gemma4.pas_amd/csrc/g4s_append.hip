@@ -13,7 +13,7 @@
  * border between two codes a rounding in between would choose the other one.  Cosines and sines
  * are computed once per token and pair, in LDS for all heads of the workgroup.
  *
- * One token a row: 4.0 us for a row and 4.9 for 192, the latency of a launch and of lengths, page, scale
+ * One token a row: 4.0 us for a row and 4.4 for 192, the latency of a launch and of lengths, page, scale
  * and vectors one after the other.  The seven prompts: 115 us for 361 MB (3.1 TB/s, a copy 4.9): queries alone
  * 66, keys and values alone 57, of which the angles are 16.  Vector instructions (binary64 most of
  * them) are issued in 54% of the cycles, and two to three workgroups a CU do not have the memory's latency behind
